@@ -238,6 +238,57 @@ int tpf_trimul_bwd_stages(const void* d_out, const void* z, const float* mask,
                    void* workspace, int64_t workspace_bytes, int64_t rows_per_batch, int stages,
                    void* dx_cm, void* da_cm, void* db_cm, void* stream);
 
+/* ---- row-wise operators (no counterparts in the reference, which uses torch's LayerNorm and Linear) ----------
+ * Element types of rows and parameters. */
+#define TPF_F32 0
+#define TPF_BF16 1
+#define TPF_F16 2
+
+/* Layer norm of rows: y = (x - mean) / sqrt(var + eps) * weight + bias, statistics and sums in fp32.
+ *   x        [rows, cols] of `type`, row pitch x_pitch elements (0: one row for all); 1 <= cols <= 8192; any alignment
+ *            (rows that start on 16-byte boundaries, 32 in fp32, with cols a multiple of 8 are accessed by vectors)
+ *   weight, bias  [cols] of their own types, or NULL (ones, zeros)
+ *   y        [rows, cols] of `type`, contiguous
+ *   codes, scales  NULL, or where x is kept in the 8-bit format of tpf_int8_pack
+ *   mean, rstd     fp32 [rows] for the backward pass, or NULL */
+int tpf_layer_norm_fwd(const void* x, int64_t x_pitch, int type, const void* weight, int weight_type, const void* bias,
+                       int bias_type, void* y, void* codes, float* scales, float* mean, float* rstd, int64_t rows,
+                       int64_t cols, float eps, void* stream);
+
+/* Its backward pass: dx (of `type`, contiguous, may be NULL), dweight and dbias [cols] (of their types, may be NULL; zeros
+ * for no rows).  dy is contiguous.  x is taken from codes and scales when they are given (x may be NULL then).
+ * Deterministic: fixed summation orders.  workspace: 4-byte aligned, needed for dweight and dbias only. */
+int64_t tpf_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t cols);
+int tpf_layer_norm_bwd(const void* dy, const void* x, int64_t x_pitch, const void* codes, const float* scales, int type,
+                       const float* mean, const float* rstd, const void* weight, int weight_type, void* dx, void* dweight,
+                       int dweight_type, void* dbias, int dbias_type, void* workspace, int64_t workspace_bytes,
+                       int64_t rows, int64_t cols, void* stream);
+
+/* Activations in 8 bits.  Groups of 128 consecutive elements of a row (the last one ragged) share a scale: with a = max |x|,
+ * code = rint(x * fl32(127 / a)), scale = fl32(a / 127), value = code * scale.  Groups with a < 2^-119 are kept as zeros;
+ * the scale of a group that holds an infinity or a NaN is NaN and its codes are 0.
+ *   codes int8 [rows, cols] contiguous, scales fp32 [rows, ceil(cols / 128)]; fewer than 2^31 groups.
+ * tpf_int8_unpack writes x contiguous. */
+int tpf_int8_pack(const void* x, int64_t x_pitch, int type, void* codes, float* scales, int64_t rows, int64_t cols,
+                  void* stream);
+int tpf_int8_unpack(const void* codes, const float* scales, int type, void* x, int64_t rows, int64_t cols, void* stream);
+
+/* Normalised projection out = layer_norm(x) weight^T: x bf16 [rows, cols] (16-byte aligned rows), weight bf16 [outs, cols],
+ * out bf16 [rows, outs], cols and outs multiples of 8, cols <= 8192.  The norm's arguments are those of tpf_layer_norm_fwd
+ * and _bwd.  d_weight is [outs, cols] of its own type; gradients whose pointer is NULL are not computed. */
+int64_t tpf_norm_linear_fwd_workspace_bytes(int64_t rows, int64_t cols, int64_t outs);
+int64_t tpf_norm_linear_bwd_workspace_bytes(int64_t rows, int64_t cols, int64_t outs);
+int tpf_norm_linear_fwd(const void* x, int64_t x_pitch, const void* norm_weight, int norm_weight_type,
+                        const void* norm_bias, int norm_bias_type, const void* weight, void* out, void* codes,
+                        float* scales, float* mean, float* rstd, void* workspace, int64_t workspace_bytes, int64_t rows,
+                        int64_t cols, int64_t outs, float eps, void* stream);
+int tpf_norm_linear_bwd(const void* d_out, const void* x, int64_t x_pitch, const void* codes, const float* scales,
+                        const float* mean, const float* rstd, const void* norm_weight, int norm_weight_type,
+                        const void* norm_bias, int norm_bias_type, const void* weight, void* dx, void* d_norm_weight,
+                        int d_norm_weight_type, void* d_norm_bias, int d_norm_bias_type, void* d_weight,
+                        int d_weight_type, void* workspace, int64_t workspace_bytes, int64_t rows, int64_t cols,
+                        int64_t outs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

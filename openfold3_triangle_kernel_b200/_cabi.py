@@ -42,10 +42,23 @@ SIGNATURES = {
     "tpf_trimul_bwd_stages": [_P] * 9 + [_i, _I, _I, _I] + [_P] * 21 + [_I, _I, _i, _P, _P, _P, _P],
     "tpf_trimul_fwd": [_P] * 10 + [_i, _I, _I, _I] + [_P] * 12 + [_I, _P],
     "tpf_trimul_bwd": [_P] * 9 + [_i, _I, _I, _I] + [_P] * 21 + [_I, _P],
+    "tpf_layer_norm_fwd": [_P, _I, _i, _P, _i, _P, _i, _P, _P, _P, _P, _P, _I, _I, _f, _P],
+    "tpf_layer_norm_bwd_workspace_bytes": [_I, _I],
+    "tpf_layer_norm_bwd": [_P, _P, _I, _P, _P, _i, _P, _P, _P, _i, _P, _P, _i, _P, _i, _P, _I, _I, _I, _P],
+    "tpf_int8_pack": [_P, _I, _i, _P, _P, _I, _I, _P],
+    "tpf_int8_unpack": [_P, _P, _i, _P, _I, _I, _P],
+    "tpf_norm_linear_fwd_workspace_bytes": [_I, _I, _I],
+    "tpf_norm_linear_bwd_workspace_bytes": [_I, _I, _I],
+    "tpf_norm_linear_fwd": [_P, _I, _P, _i, _P, _i] + [_P] * 7 + [_I, _I, _I, _I, _f, _P],
+    "tpf_norm_linear_bwd": [_P, _P, _I] + [_P] * 4 + [_P, _i, _P, _i, _P, _P, _P, _i, _P, _i, _P, _i, _P, _I, _I, _I, _I,
+                                                   _P],
 }
 _RESTYPES = {"tpf_trimul_fwd_workspace_bytes": ctypes.c_int64, "tpf_trimul_bwd_workspace_bytes": ctypes.c_int64,
              "tpf_trimul_bwd_stages_workspace_bytes": ctypes.c_int64,
              "tpf_attn_bwd_workspace_bytes": ctypes.c_int64,
+             "tpf_layer_norm_bwd_workspace_bytes": ctypes.c_int64,
+             "tpf_norm_linear_fwd_workspace_bytes": ctypes.c_int64,
+             "tpf_norm_linear_bwd_workspace_bytes": ctypes.c_int64,
              "tpf_attn_bwd_static_scratch_capacity": ctypes.c_int64, "tpf_launch_count": ctypes.c_int64,
              "tpf_version": ctypes.c_char_p, "tpf_last_error_string": ctypes.c_char_p}
 

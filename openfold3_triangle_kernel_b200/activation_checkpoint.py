@@ -1,0 +1,173 @@
+"""Activations kept in 8 bits between a forward and a backward pass.
+
+Format: groups of 128 consecutive elements of a row (the last one ragged) share an fp32 scale.  With ``a`` the largest
+magnitude of a group, ``code = rint(x * fl32(127 / a))`` (ties to even, the product exact), ``scale = fl32(a / 127)`` and
+``value = code * scale``: off by half a step, ``a / 254``, at most.  Groups with ``a < 2**-119`` are kept as zeros; a group
+that holds an infinity or a NaN comes back as NaN.
+
+* :func:`pack_activation` / :func:`unpack_activation`: the two directions, for any ``[*, C]`` in bf16, fp16 or fp32.
+* :func:`int8_activations`: a context inside which autograd keeps large 16-bit activations in this format.
+* ``checkpoint="int8"`` of :func:`turbo_layer_norm` and :func:`turbo_norm_linear`, whose kernels write the codes in the
+  forward pass and read them in the backward pass, without a pass of their own.
+
+None of them is differentiated.  Unsupported inputs raise ``ValueError("... unsupported [code]: reason")``.  The reference
+has no counterpart: it keeps activations whole or computes them again (openfold3/core/utils/checkpointing.py).
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _cabi as C
+from .layer_norm import ROW_DTYPES
+from .trimul import SupportResult
+
+GROUP = 128
+_MAX_GROUPS = 2 ** 31 - 1024
+_SCALAR_TYPES = {torch.float16: 5, torch.float32: 6, torch.bfloat16: 15}  # c10::ScalarType
+
+
+def _groups(cols):
+    return -(-cols // GROUP)
+
+
+def check_pack_support(x, *, check_device=True) -> SupportResult:
+    """Metadata-only contract check of :func:`pack_activation`."""
+    if not isinstance(x, torch.Tensor):
+        return SupportResult(False, "x_type", "x must be a torch.Tensor")
+    if x.ndim < 1:
+        return SupportResult(False, "x_shape", "x must have shape [*,C]")
+    if x.dtype not in ROW_DTYPES:
+        return SupportResult(False, "x_dtype", "x must be BF16, FP16 or FP32")
+    cols = x.shape[-1]
+    rows = x.numel() // cols if cols else 0
+    if cols >= 2 ** 31 - GROUP or rows * _groups(cols) >= _MAX_GROUPS:
+        return SupportResult(False, "extent", "x must have fewer than 2^31 groups of 128 elements")
+    if check_device:
+        if not x.is_cuda:
+            return SupportResult(False, "device", "x must be a CUDA tensor")
+        if torch.cuda.get_device_capability(x.device)[0] != 10:
+            return SupportResult(False, "device_arch", "these kernels require a Blackwell sm_100a device")
+    return SupportResult(True, "ok", "supported")
+
+
+def check_unpack_support(codes, scales, dtype, *, check_device=True) -> SupportResult:
+    """Metadata-only contract check of :func:`unpack_activation`."""
+    if not isinstance(codes, torch.Tensor) or not isinstance(scales, torch.Tensor):
+        return SupportResult(False, "x_type", "codes and scales must be torch.Tensor instances")
+    if codes.dtype != torch.int8 or scales.dtype != torch.float32:
+        return SupportResult(False, "x_dtype", "codes must be int8 and scales FP32")
+    if codes.ndim < 1 or tuple(scales.shape) != tuple(codes.shape[:-1]) + (_groups(codes.shape[-1]),):
+        return SupportResult(False, "x_shape", "scales must have one entry per 128 elements of a row of codes")
+    if dtype not in ROW_DTYPES:
+        return SupportResult(False, "dtype", "dtype must be torch.bfloat16, float16 or float32")
+    if scales.device != codes.device:
+        return SupportResult(False, "device", "codes and scales must share one device")
+    if check_device:
+        if not codes.is_cuda:
+            return SupportResult(False, "device", "codes and scales must be CUDA tensors")
+        if torch.cuda.get_device_capability(codes.device)[0] != 10:
+            return SupportResult(False, "device_arch", "these kernels require a Blackwell sm_100a device")
+    return SupportResult(True, "ok", "supported")
+
+
+@torch.library.custom_op("tpf_b200::int8_pack", mutates_args=())
+def _int8_pack(x: torch.Tensor) -> list[torch.Tensor]:
+    return C.native().int8_pack_op(x)
+
+
+@_int8_pack.register_fake
+def _(x):
+    return [x.new_empty(x.shape, dtype=torch.int8),
+            x.new_empty(x.shape[:-1] + (_groups(x.shape[-1]),), dtype=torch.float32)]
+
+
+@torch.library.custom_op("tpf_b200::int8_unpack", mutates_args=())
+def _int8_unpack(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    return C.native().int8_unpack_op(codes, scales, _SCALAR_TYPES[dtype])
+
+
+@_int8_unpack.register_fake
+def _(codes, scales, dtype):
+    return codes.new_empty(codes.shape, dtype=dtype)
+
+
+def pack_activation(x):
+    """``x [*, C]`` -> ``(codes int8 [*, C], scales fp32 [*, ceil(C / 128)])``."""
+    if not torch.compiler.is_compiling():
+        res = check_pack_support(x)
+        if not res.supported:
+            raise ValueError(f"pack_activation unsupported [{res.code}]: {res.reason}")
+        packed = C.native().int8_pack(x)
+        if packed is not None:
+            return packed
+    codes, scales = torch.ops.tpf_b200.int8_pack(x.detach())
+    return codes, scales
+
+
+def unpack_activation(codes, scales, dtype=torch.bfloat16):
+    """The values that ``(codes, scales)`` of :func:`pack_activation` stand for, in ``dtype``."""
+    if not torch.compiler.is_compiling():
+        res = check_unpack_support(codes, scales, dtype)
+        if not res.supported:
+            raise ValueError(f"unpack_activation unsupported [{res.code}]: {res.reason}")
+        x = C.native().int8_unpack(codes, scales, dtype)
+        if x is not None:
+            return x
+    return torch.ops.tpf_b200.int8_unpack(codes, scales.detach(), dtype)
+
+
+class _Packed:
+    """A kept activation: its memory, flat, in 8 bits, and the size and strides to give it back with."""
+
+    __slots__ = ("codes", "scales", "dtype", "size", "stride")
+
+    def __init__(self, t):
+        flat = t.as_strided((t.numel(),), (1,))
+        self.codes, self.scales = pack_activation(flat.view(-1, GROUP) if flat.numel() % GROUP == 0 else flat)
+        self.dtype, self.size, self.stride = t.dtype, t.size(), t.stride()
+
+    def tensor(self):
+        return unpack_activation(self.codes, self.scales, self.dtype).as_strided(self.size, self.stride)
+
+
+def _is_dense(t):
+    """Do the elements fill one stretch of memory, each once, in some order of the dimensions?"""
+    expected = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz != 1):
+        if stride != expected:
+            return False
+        expected *= size
+    return True
+
+
+def _is_parameter(t):
+    base = t if t._base is None else t._base
+    return base.is_leaf and base.requires_grad
+
+
+def _packable(t, min_elements):
+    return (type(t) in (torch.Tensor, torch.nn.Parameter) and t.is_cuda and t.dtype in (torch.bfloat16, torch.float16)
+            and t.layout == torch.strided and t.numel() >= min_elements and not _is_parameter(t)
+            and not t.is_conj() and not t.is_neg() and _is_dense(t)
+            and (t.numel() % GROUP == 0 or t.numel() < 2 ** 31 - GROUP)
+            and torch.cuda.get_device_capability(t.device)[0] == 10)
+
+
+def int8_activations(min_elements=65536, keep_whole=None):
+    """Context manager: what autograd keeps inside it for the backward pass, it keeps in 8 bits and gives back as the values
+    these stand for.
+
+    That holds for bf16 and fp16 CUDA tensors of at least ``min_elements`` elements (the groups follow their memory order).
+    fp32 tensors (statistics, log-sum-exps), leaves that require gradients and views of them (parameters), tensors whose
+    elements overlap or leave gaps, and tensors for which ``keep_whole(t)`` is true are kept as they are.  An activation
+    that holds an infinity (logits behind a mask) would come back as NaN in its groups: keep such tensors whole.
+    """
+    def pack(t):
+        if not _packable(t, min_elements) or (keep_whole is not None and keep_whole(t)):
+            return t
+        return _Packed(t.detach())
+
+    def unpack(kept):
+        return kept.tensor() if isinstance(kept, _Packed) else kept
+
+    return torch.autograd.graph.saved_tensors_hooks(pack, unpack)

@@ -2,6 +2,7 @@
 #include "../../include/tpf_b200.h"
 #include "tpf_host.cuh"
 #include "tpf_internal.h"
+#include "tpf_rows.h"
 
 namespace tpf {
 
@@ -249,6 +250,69 @@ int tpf_trimul_bwd(const void* d_out, const void* z, const float* mask, const fl
                                zln, mean_in, rstd_in, a_cm, b_cm, gate, x_cm, xln, mean_out, rstd_out, d_z, d_p_in,
                                d_g_in, d_p_out, d_g_out, d_norm_in_w, d_norm_in_b, d_norm_out_w, d_norm_out_b,
                                workspace, workspace_bytes, 0, 7, nullptr, nullptr, nullptr, stream);
+}
+
+int tpf_layer_norm_fwd(const void* x, int64_t x_pitch, int type, const void* weight, int weight_type, const void* bias,
+                       int bias_type, void* y, void* codes, float* scales, float* mean, float* rstd, int64_t rows,
+                       int64_t cols, float eps, void* stream) {
+  const tpf::NormCall c{rows, cols, type, x, x_pitch, codes, scales, mean, rstd, weight, bias, weight_type, bias_type};
+  return tpf::layer_norm_fwd(c, y, eps, static_cast<cudaStream_t>(stream));
+}
+
+int64_t tpf_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t cols) {
+  return rows > 0 && cols > 0 ? tpf::layer_norm_bwd_workspace_bytes(rows, cols) : 0;
+}
+
+int tpf_layer_norm_bwd(const void* dy, const void* x, int64_t x_pitch, const void* codes, const float* scales, int type,
+                       const float* mean, const float* rstd, const void* weight, int weight_type, void* dx, void* dweight,
+                       int dweight_type, void* dbias, int dbias_type, void* workspace, int64_t workspace_bytes,
+                       int64_t rows, int64_t cols, void* stream) {
+  const tpf::NormCall c{rows, cols, type, x, x_pitch, const_cast<void*>(codes), const_cast<float*>(scales),
+                        const_cast<float*>(mean), const_cast<float*>(rstd), weight, nullptr, weight_type, 0};
+  const tpf::NormGrads g{dy, dx, dweight, dbias, dweight_type, dbias_type};
+  return tpf::layer_norm_bwd(c, g, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int tpf_int8_pack(const void* x, int64_t x_pitch, int type, void* codes, float* scales, int64_t rows, int64_t cols,
+                  void* stream) {
+  return tpf::int8_pack(x, x_pitch, type, codes, scales, rows, cols, static_cast<cudaStream_t>(stream));
+}
+
+int tpf_int8_unpack(const void* codes, const float* scales, int type, void* x, int64_t rows, int64_t cols, void* stream) {
+  return tpf::int8_unpack(codes, scales, type, x, rows, cols, static_cast<cudaStream_t>(stream));
+}
+
+static bool norm_linear_shape_ok(int64_t rows, int64_t cols, int64_t outs) { return rows > 0 && cols > 0 && outs > 0; }
+
+int64_t tpf_norm_linear_fwd_workspace_bytes(int64_t rows, int64_t cols, int64_t outs) {
+  return norm_linear_shape_ok(rows, cols, outs) ? tpf::norm_linear_fwd_workspace_bytes(rows, cols, outs) : 0;
+}
+
+int64_t tpf_norm_linear_bwd_workspace_bytes(int64_t rows, int64_t cols, int64_t outs) {
+  return norm_linear_shape_ok(rows, cols, outs) ? tpf::norm_linear_bwd_workspace_bytes(rows, cols, outs) : 0;
+}
+
+int tpf_norm_linear_fwd(const void* x, int64_t x_pitch, const void* norm_weight, int norm_weight_type,
+                        const void* norm_bias, int norm_bias_type, const void* weight, void* out, void* codes,
+                        float* scales, float* mean, float* rstd, void* workspace, int64_t workspace_bytes, int64_t rows,
+                        int64_t cols, int64_t outs, float eps, void* stream) {
+  const tpf::NormCall c{rows, cols, TPF_BF16, x, x_pitch, codes, scales, mean, rstd, norm_weight, norm_bias,
+                        norm_weight_type, norm_bias_type};
+  return tpf::norm_linear_fwd(c, weight, outs, out, eps, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int tpf_norm_linear_bwd(const void* d_out, const void* x, int64_t x_pitch, const void* codes, const float* scales,
+                        const float* mean, const float* rstd, const void* norm_weight, int norm_weight_type,
+                        const void* norm_bias, int norm_bias_type, const void* weight, void* dx, void* d_norm_weight,
+                        int d_norm_weight_type, void* d_norm_bias, int d_norm_bias_type, void* d_weight,
+                        int d_weight_type, void* workspace, int64_t workspace_bytes, int64_t rows, int64_t cols,
+                        int64_t outs, void* stream) {
+  const tpf::NormCall c{rows, cols, TPF_BF16, x, x_pitch, const_cast<void*>(codes), const_cast<float*>(scales),
+                        const_cast<float*>(mean), const_cast<float*>(rstd), norm_weight, norm_bias, norm_weight_type,
+                        norm_bias_type};
+  const tpf::NormLinearGrads g{d_out, dx, d_norm_weight, d_norm_bias, d_norm_weight_type, d_norm_bias_type, d_weight,
+                               d_weight_type};
+  return tpf::norm_linear_bwd(c, weight, outs, g, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -1,0 +1,150 @@
+// The normalised projection: out = y W^T with y = layer_norm(x), bf16, no bias.
+//
+//   forward    y = w xh + b (bf16), out = y W^T
+//   backward   dy = d_out W (bf16), the layer norm's backward on it, dW = d_out^T y~ with y~ from what was kept of x
+#include "tpf_layer_norm.cuh"
+
+namespace tpf {
+
+int bmm_bf16(const void* A, int64_t lda, int64_t bsa, int a_mn, const void* B, int64_t ldb, int64_t bsb, int b_mn,
+             void* D, int64_t ldd, int64_t bsd, int out_f32, int64_t M, int64_t N, int64_t K, int64_t batch,
+             int64_t k_per_split, int swizzle_bytes, cudaStream_t stream);
+
+namespace {
+
+// y~ = w (x - mean) rstd + b in bf16, x from the codes or as it was: eight elements a thread.
+template <bool CODES>
+__global__ void __launch_bounds__(256) renorm_kernel(const NormArgs a, bf16* __restrict__ y, FastDiv per_row, int64_t pieces) {
+  griddep_wait();
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= pieces) return;
+  const int64_t row = i / per_row.d;
+  const int c = (int)(i - row * per_row.d) * 8;
+  float x[8];
+  if constexpr (CODES) load_codes<8>(a.codes + row * a.cols + c, a.scales[row * a.groups + c / kGroup], x);
+  else load_vec<bf16, 8>(static_cast<const bf16*>(a.x) + row * a.x_pitch + c, x);
+  const float mean = a.mean[row], rstd = a.rstd[row];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = (x[e] - mean) * rstd * param_at(a.w, c + e, 1.f) + param_at(a.b, c + e, 0.f);
+  store_vec<bf16, 8>(y + row * a.cols + c, x);
+}
+
+__global__ void __launch_bounds__(256) split_fold_kernel(const float* __restrict__ part, int splits, int64_t n, ParamOut out) {
+  griddep_wait();
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float s = 0.f;
+  for (int k = 0; k < splits; ++k) s += part[k * n + i];
+  param_put(out, i, s);
+}
+
+int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
+
+struct Splits {
+  int64_t count, rows;
+};
+Splits dw_splits(int64_t rows, int64_t cols, int64_t outs) {
+  const int64_t tiles = ((outs + 127) / 128) * ((cols + 127) / 128);
+  int64_t want = (2 * sm_count() + tiles - 1) / tiles;
+  int64_t per = (rows + want - 1) / want;
+  per = (per + 63) / 64 * 64;
+  if (per < 256) per = 256;
+  return {(rows + per - 1) / per, per};
+}
+
+// What both passes ask of their arguments.  x (or its codes) is read eight elements at a time.
+int check_linear(const NormCall& c, const void* w, int64_t outs, const char* who) {
+  TPF_REQUIRE(c.type == kRowBF16, TPF_ERR_UNSUPPORTED, "%s: bf16 only", who);
+  TPF_REQUIRE(c.cols >= 8 && c.cols <= kMaxNormCols && c.cols % 8 == 0 && outs >= 8 && outs % 8 == 0, TPF_ERR_UNSUPPORTED,
+              "%s: columns and outputs must be multiples of 8, columns at most %lld", who, (long long)kMaxNormCols);
+  TPF_REQUIRE(c.rows >= 0 && c.rows < (1ll << 31) - 256 && outs < (1ll << 31) - 256, TPF_ERR_UNSUPPORTED,
+              "%s: extent too large", who);
+  TPF_REQUIRE(w != nullptr, TPF_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  TPF_REQUIRE_ALIGNED16(w, who, "weight");
+  TPF_REQUIRE(rows_vec_ok(c.x, c.x_pitch, c.type), TPF_ERR_INVALID_ARGUMENT, "%s: x must have 16-byte aligned rows", who);
+  TPF_REQUIRE((reinterpret_cast<uintptr_t>(c.codes) & 7) == 0, TPF_ERR_INVALID_ARGUMENT, "%s: codes must be 8-byte aligned",
+              who);
+  return TPF_OK;
+}
+
+}  // namespace
+
+int64_t norm_linear_fwd_workspace_bytes(int64_t rows, int64_t cols, int64_t outs) { return up256(rows * cols * 2); }
+
+int norm_linear_fwd(const NormCall& norm, const void* w, int64_t outs, void* out, float eps, void* workspace,
+                    int64_t workspace_bytes, cudaStream_t stream) {
+  const char* who = "norm_linear_fwd";
+  if (int rc = check_linear(norm, w, outs, who)) return rc;
+  if (norm.rows == 0) return TPF_OK;
+  TPF_REQUIRE(out != nullptr && norm.x != nullptr, TPF_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  TPF_REQUIRE_ALIGNED16(out, who, "out");
+  const int64_t need = norm_linear_fwd_workspace_bytes(norm.rows, norm.cols, outs);
+  TPF_REQUIRE(workspace != nullptr && workspace_bytes >= need, TPF_ERR_WORKSPACE,
+              "%s: workspace of %lld bytes required, %lld given", who, (long long)need, (long long)workspace_bytes);
+  TPF_REQUIRE_ALIGNED16(workspace, who, "workspace");
+  if (int rc = layer_norm_fwd(norm, workspace, eps, stream)) return rc;
+  return bmm_bf16(workspace, norm.cols, 0, 0, w, norm.cols, 0, 0, out, outs, 0, 0, norm.rows, outs, norm.cols, 1, 0, 128,
+                  stream);
+}
+
+int64_t norm_linear_bwd_workspace_bytes(int64_t rows, int64_t cols, int64_t outs) {
+  const Splits s = dw_splits(rows, cols, outs);
+  return up256(rows * cols * 2) + up256(layer_norm_bwd_workspace_bytes(rows, cols)) + up256(rows * cols * 2) +
+         up256(s.count * outs * cols * 4);
+}
+
+int norm_linear_bwd(const NormCall& norm, const void* w, int64_t outs, const NormLinearGrads& g, void* workspace,
+                    int64_t workspace_bytes, cudaStream_t stream) {
+  const char* who = "norm_linear_bwd";
+  if (int rc = check_linear(norm, w, outs, who)) return rc;
+  TPF_REQUIRE((norm.x != nullptr || norm.codes != nullptr || norm.rows == 0) && (g.d_out != nullptr || norm.rows == 0) &&
+                  (norm.mean != nullptr || norm.rows == 0),
+              TPF_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
+  TPF_REQUIRE_ALIGNED16(g.d_out, who, "d_out");
+  TPF_REQUIRE_ALIGNED16(g.dx, who, "dx");
+  TPF_REQUIRE(g.dw == nullptr || row_type_ok(g.dw_type), TPF_ERR_INVALID_ARGUMENT, "%s: unknown parameter type", who);
+  const int64_t need = norm_linear_bwd_workspace_bytes(norm.rows, norm.cols, outs);
+  TPF_REQUIRE(norm.rows == 0 || (workspace != nullptr && workspace_bytes >= need), TPF_ERR_WORKSPACE,
+              "%s: workspace of %lld bytes required, %lld given", who, (long long)need, (long long)workspace_bytes);
+  TPF_REQUIRE_ALIGNED16(workspace, who, "workspace");
+  const int64_t R = norm.rows, C = norm.cols;
+  char* base = static_cast<char*>(workspace);
+  const int64_t ln_bytes = layer_norm_bwd_workspace_bytes(R, C);
+  void* dy = base;
+  void* ln_ws = base + up256(R * C * 2);
+  void* y = base + up256(R * C * 2) + up256(ln_bytes);
+  float* part = reinterpret_cast<float*>(static_cast<char*>(y) + up256(R * C * 2));
+  if (g.dx != nullptr || g.dweight != nullptr || g.dbias != nullptr) {
+    if (R > 0)
+      if (int rc = bmm_bf16(g.d_out, outs, 0, 0, w, C, 0, 1, dy, C, 0, 0, R, C, outs, 1, 0, 128, stream)) return rc;
+    const NormGrads n{dy, g.dx, g.dweight, g.dbias, g.dweight_type, g.dbias_type};
+    if (int rc = layer_norm_bwd(norm, n, ln_ws, ln_bytes, stream)) return rc;
+  }
+  if (g.dw == nullptr) return TPF_OK;
+  if (R == 0) {
+    TPF_CUDA_OK(cudaMemsetAsync(g.dw, 0, outs * C * row_type_size(g.dw_type), stream));
+    return TPF_OK;
+  }
+  NormArgs a;
+  if (int rc = make_norm_args(&a, norm, who)) return rc;
+  const int64_t pieces = R * (C / 8);
+  const FastDiv per_row = FastDiv::make((uint32_t)(C / 8));
+  TPF_REQUIRE(pieces / 256 < (1ll << 31) - 1, TPF_ERR_UNSUPPORTED, "%s: extent too large", who);
+  const dim3 grid((unsigned)((pieces + 255) / 256));
+  if (norm.codes != nullptr)
+    launch_kernel(renorm_kernel<true>, grid, dim3(256), 0, stream, a, static_cast<bf16*>(y), per_row, pieces);
+  else
+    launch_kernel(renorm_kernel<false>, grid, dim3(256), 0, stream, a, static_cast<bf16*>(y), per_row, pieces);
+  TPF_LAUNCH_OK();
+  const Splits s = dw_splits(R, C, outs);
+  if (int rc = bmm_bf16(g.d_out, outs, 0, 1, y, C, 0, 1, part, C, outs * C, 1, outs, C, R, s.count, s.rows, 128, stream))
+    return rc;
+  const int64_t n = outs * C;
+  TPF_REQUIRE(n / 256 < (1ll << 31) - 1, TPF_ERR_UNSUPPORTED, "%s: extent too large", who);
+  launch_kernel(split_fold_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, part, (int)s.count, n,
+                ParamOut{g.dw, g.dw_type});
+  TPF_LAUNCH_OK();
+  return TPF_OK;
+}
+
+}  // namespace tpf

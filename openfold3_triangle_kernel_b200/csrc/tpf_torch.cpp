@@ -76,4 +76,14 @@ PYBIND11_MODULE(_native, m) {
   m.def("trimul_fwd", &tpf_torch::trimul_fwd);
   m.def("pair_block", &tpf_torch::py_pair_block);
   m.def("trimul_bwd", &tpf_torch::trimul_bwd);
+  m.def("layer_norm", &tpf_torch::py_layer_norm);
+  m.def("layer_norm_fwd", &tpf_torch::layer_norm_fwd);
+  m.def("layer_norm_bwd", &tpf_torch::layer_norm_bwd);
+  m.def("norm_linear", &tpf_torch::py_norm_linear);
+  m.def("norm_linear_fwd", &tpf_torch::norm_linear_fwd);
+  m.def("norm_linear_bwd", &tpf_torch::norm_linear_bwd);
+  m.def("int8_pack", &tpf_torch::py_int8_pack);
+  m.def("int8_unpack", &tpf_torch::py_int8_unpack);
+  m.def("int8_pack_op", &tpf_torch::int8_pack);
+  m.def("int8_unpack_op", &tpf_torch::int8_unpack);
 }

@@ -81,4 +81,21 @@ std::vector<Tensor> trimul_bwd(const Tensor& d_out, const Tensor& z, const Tenso
 py::object py_pair_block(py::handle z, py::handle mask, py::tuple tri_out, py::tuple tri_in, py::tuple start,
                          py::tuple end, int64_t heads);
 
+// ---- row-wise operators (tpf_torch_rows.cpp) ------------------------------------------------
+py::object py_layer_norm(py::handle x, py::handle w, py::handle b, double eps, bool int8);
+std::vector<Tensor> layer_norm_fwd(const Tensor& x, const std::optional<Tensor>& w, const std::optional<Tensor>& b, double eps,
+                                   bool int8);
+std::vector<Tensor> layer_norm_bwd(const Tensor& dy, const std::optional<Tensor>& x, const Tensor& stats, const Tensor& codes,
+                                   const Tensor& scales, const std::optional<Tensor>& w, const std::optional<Tensor>& b);
+py::object py_norm_linear(py::handle x, py::handle nw, py::handle nb, py::handle w, double eps, bool int8);
+std::vector<Tensor> norm_linear_fwd(const Tensor& x, const std::optional<Tensor>& nw, const std::optional<Tensor>& nb,
+                                    const Tensor& w, double eps, bool int8);
+std::vector<Tensor> norm_linear_bwd(const Tensor& d_out, const std::optional<Tensor>& x, const Tensor& stats,
+                                    const Tensor& codes, const Tensor& scales, const std::optional<Tensor>& nw,
+                                    const std::optional<Tensor>& nb, const Tensor& w);
+py::object py_int8_pack(py::handle x);
+py::object py_int8_unpack(py::handle codes, py::handle scales, py::object dtype);
+std::vector<Tensor> int8_pack(const Tensor& x);
+Tensor int8_unpack(const Tensor& codes, const Tensor& scales, int64_t type);
+
 }  // namespace tpf_torch

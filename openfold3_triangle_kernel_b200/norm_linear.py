@@ -1,0 +1,115 @@
+"""``turbo_norm_linear``: a layer norm and the bias-free Linear that follows it, on B200.
+
+    out = layer_norm(x; norm_weight, norm_bias, eps) @ weight^T
+
+Operator contract:
+
+* ``x``: bf16 ``[*, C]``, C a multiple of 8 up to 8192; ``weight``: ``[O, C]``, O a multiple of 8, bf16, fp16 or fp32
+  (rounded to bf16 inside, like the projections of :func:`turbo_trimul`); ``norm_weight``, ``norm_bias``: as in
+  :func:`turbo_layer_norm`.  Projections that share an input (q, k, v, gate) go into one weight.
+* ``checkpoint``: as in :func:`turbo_layer_norm`.  Only x is kept, whole or in 8 bits: the normalised rows are made again
+  in the backward pass, for the weight's gradient too.
+* returns bf16 ``[*, O]``; autograd for x, norm_weight, norm_bias and weight (first order only).  The normalised rows and
+  the gradient that reaches them are rounded to bf16 on their way to the tensor cores, sums are fp32.
+
+Unsupported inputs raise ``ValueError("turbo_norm_linear unsupported [code]: reason")``.  There is no counterpart among the
+reference's kernels (it calls torch's LayerNorm and Linear).
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+
+from . import _cabi as C
+from .layer_norm import CHECKPOINTS, ROW_DTYPES, check_parameter, check_rows, kept_like
+from .trimul import SupportResult
+
+
+def check_norm_linear_support(x, norm_weight, norm_bias, weight, eps=1e-5, checkpoint=None, *,
+                              check_device=True) -> SupportResult:
+    """Metadata-only contract check; returns the first failure."""
+    bad = check_rows(x, eps, checkpoint, check_device)
+    if bad is not None:
+        return bad
+    if x.dtype != torch.bfloat16:
+        return SupportResult(False, "x_dtype", "x must be BF16")
+    cols = x.shape[-1]
+    if cols % 8:
+        return SupportResult(False, "columns", f"C={cols} is not a multiple of 8")
+    if not isinstance(weight, torch.Tensor) or weight.ndim != 2 or weight.shape[1] != cols:
+        return SupportResult(False, "weight_shape", f"weight must have shape (O, {cols})")
+    if weight.shape[0] < 8 or weight.shape[0] % 8:
+        return SupportResult(False, "outputs", f"O={weight.shape[0]} is not a positive multiple of 8")
+    if weight.dtype not in ROW_DTYPES:
+        return SupportResult(False, "weight_dtype", "weight must be BF16, FP16 or FP32")
+    if weight.device != x.device:
+        return SupportResult(False, "weight_device", "weight must live on x's device")
+    for name, p in (("norm_weight", norm_weight), ("norm_bias", norm_bias)):
+        bad = check_parameter(name, p, cols, x)
+        if bad is not None:
+            return bad
+    return SupportResult(True, "ok", "supported")
+
+
+# --------------------------------------------------------------------------------------
+# custom ops: what a traced graph holds.  An eager call on plain CUDA tensors goes to `_native.norm_linear`.
+# --------------------------------------------------------------------------------------
+@torch.library.custom_op("tpf_b200::norm_linear_fwd", mutates_args=())
+def _norm_linear_fwd(x: torch.Tensor, norm_weight: Optional[torch.Tensor], norm_bias: Optional[torch.Tensor],
+                     weight: torch.Tensor, eps: float, int8: bool) -> list[torch.Tensor]:
+    return C.native().norm_linear_fwd(x, norm_weight, norm_bias, weight, eps, int8)
+
+
+@_norm_linear_fwd.register_fake
+def _(x, norm_weight, norm_bias, weight, eps, int8):
+    return [x.new_empty(x.shape[:-1] + (weight.shape[0],)), *kept_like(x, int8)]
+
+
+@torch.library.custom_op("tpf_b200::norm_linear_bwd", mutates_args=())
+def _norm_linear_bwd(d_out: torch.Tensor, x: Optional[torch.Tensor], stats: torch.Tensor, codes: torch.Tensor,
+                     scales: torch.Tensor, norm_weight: Optional[torch.Tensor], norm_bias: Optional[torch.Tensor],
+                     weight: torch.Tensor) -> list[torch.Tensor]:
+    return C.native().norm_linear_bwd(d_out, x, stats, codes, scales, norm_weight, norm_bias, weight)
+
+
+@_norm_linear_bwd.register_fake
+def _(d_out, x, stats, codes, scales, norm_weight, norm_bias, weight):
+    none = lambda: d_out.new_empty((0,), dtype=torch.float32)  # noqa: E731
+    return [d_out.new_empty(d_out.shape[:-1] + (weight.shape[1],)), weight.new_empty(weight.shape),
+            none() if norm_weight is None else norm_weight.new_empty(norm_weight.shape),
+            none() if norm_bias is None else norm_bias.new_empty(norm_bias.shape)]
+
+
+def _setup_context(ctx, inputs, output):
+    x, norm_weight, norm_bias, weight, _, int8 = inputs
+    _, stats, codes, scales = output
+    ctx.save_for_backward(None if int8 else x, stats, codes, scales, norm_weight, norm_bias, weight)
+    ctx.set_materialize_grads(False)
+
+
+def _backward(ctx, grads):
+    d_out = grads[0]
+    if d_out is None:
+        return (None,) * 6
+    x, stats, codes, scales, norm_weight, norm_bias, weight = ctx.saved_tensors
+    dx, dw, dnw, dnb = torch.ops.tpf_b200.norm_linear_bwd(d_out.to(torch.bfloat16), x, stats, codes, scales, norm_weight,
+                                                          norm_bias, weight)
+    return dx, None if norm_weight is None else dnw, None if norm_bias is None else dnb, dw, None, None
+
+
+_norm_linear_fwd.register_autograd(_backward, setup_context=_setup_context)
+
+
+def turbo_norm_linear(x, norm_weight, norm_bias, weight, *, eps=1e-5, checkpoint=None):
+    """Layer norm and Linear in one operator; see the module docstring for the contract."""
+    if not torch.compiler.is_compiling():
+        if checkpoint in CHECKPOINTS and isinstance(eps, (int, float)) and math.isfinite(eps):
+            out = C.native().norm_linear(x, norm_weight, norm_bias, weight, eps, checkpoint == "int8")
+            if out is not None:
+                return out
+        res = check_norm_linear_support(x, norm_weight, norm_bias, weight, eps, checkpoint)
+        if not res.supported:
+            raise ValueError(f"turbo_norm_linear unsupported [{res.code}]: {res.reason}")
+    return torch.ops.tpf_b200.norm_linear_fwd(x, norm_weight, norm_bias, weight, eps, checkpoint == "int8")[0]

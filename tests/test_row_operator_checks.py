@@ -1,0 +1,210 @@
+"""Refusals of the row-wise operators, none of which needs a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+import openfold3_triangle_kernel_b200 as tk
+from openfold3_triangle_kernel_b200 import _cabi as C
+from openfold3_triangle_kernel_b200.activation_checkpoint import check_pack_support, check_unpack_support
+
+ONE = ctypes.c_void_p(256)
+NULL = ctypes.c_void_p(0)
+
+
+def _codes(res):
+    return res.supported, res.code
+
+
+@pytest.mark.parametrize("kw, code", [
+    (dict(x=[1.0]), "x_type"),
+    (dict(x=torch.zeros(4, 8, dtype=torch.float64)), "x_dtype"),
+    (dict(x=torch.zeros(())), "x_shape"),
+    (dict(x=torch.zeros(4, 0)), "x_shape"),
+    (dict(x=torch.zeros(1, 8193)), "columns"),
+    (dict(x=torch.zeros(4, 8), weight=torch.zeros(7)), "weight_shape"),
+    (dict(x=torch.zeros(4, 8), bias=torch.zeros(8, 1)), "weight_shape"),
+    (dict(x=torch.zeros(4, 8), weight=torch.zeros(8, dtype=torch.float64)), "weight_dtype"),
+    (dict(x=torch.zeros(4, 8), checkpoint="fp8"), "checkpoint"),
+    (dict(x=torch.zeros(4, 8), eps=-1.0), "eps"),
+    (dict(x=torch.zeros(4, 8), eps=float("nan")), "eps"),
+])
+def test_layer_norm_support(kw, code):
+    assert _codes(tk.check_layer_norm_support(**kw, check_device=False)) == (False, code)
+
+
+def test_layer_norm_support_accepts():
+    for dt in (torch.bfloat16, torch.float16, torch.float32):
+        x = torch.zeros(2, 3, 5, dtype=dt)
+        assert tk.check_layer_norm_support(x, torch.ones(5), None, check_device=False).supported
+    assert tk.check_layer_norm_support(torch.zeros(0, 8192), check_device=False).supported
+
+
+@pytest.mark.parametrize("kw, code", [
+    (dict(x=torch.zeros(4, 16)), "x_dtype"),
+    (dict(x=torch.zeros(4, 12).bfloat16()), "columns"),
+    (dict(weight=torch.zeros(16, 8)), "weight_shape"),
+    (dict(weight=torch.zeros(16)), "weight_shape"),
+    (dict(weight=torch.zeros(12, 16)), "outputs"),
+    (dict(weight=torch.zeros(0, 16)), "outputs"),
+    (dict(weight=torch.zeros(8, 16, dtype=torch.int8)), "weight_dtype"),
+    (dict(norm_weight=torch.zeros(8)), "weight_shape"),
+    (dict(norm_bias=torch.zeros(16, dtype=torch.float64)), "weight_dtype"),
+    (dict(checkpoint=True), "checkpoint"),
+])
+def test_norm_linear_support(kw, code):
+    full = dict(x=torch.zeros(4, 16).bfloat16(), norm_weight=None, norm_bias=None, weight=torch.zeros(24, 16))
+    full.update(kw)
+    assert _codes(tk.check_norm_linear_support(**full, check_device=False)) == (False, code)
+
+
+@pytest.mark.parametrize("x, code", [
+    ("x", "x_type"), (torch.zeros(()), "x_shape"), (torch.zeros(4, dtype=torch.int8), "x_dtype"),
+    (torch.zeros(1, 1).bfloat16().expand(2 ** 31, 1), "extent"),
+    (torch.zeros(1).bfloat16().expand(2 ** 31), "extent"),
+])
+def test_pack_support(x, code):
+    assert _codes(check_pack_support(x, check_device=False)) == (False, code)
+
+
+@pytest.mark.parametrize("codes, scales, dtype, code", [
+    (torch.zeros(4, 200), torch.zeros(4, 2), torch.float32, "x_dtype"),
+    (torch.zeros(4, 200, dtype=torch.int8), torch.zeros(4, 2).half(), torch.float32, "x_dtype"),
+    (torch.zeros(4, 200, dtype=torch.int8), torch.zeros(4, 1), torch.float32, "x_shape"),
+    (torch.zeros(4, 200, dtype=torch.int8), torch.zeros(2), torch.float32, "x_shape"),
+    (torch.zeros(4, 200, dtype=torch.int8), torch.zeros(4, 2), torch.float64, "dtype"),
+])
+def test_unpack_support(codes, scales, dtype, code):
+    assert _codes(check_unpack_support(codes, scales, dtype, check_device=False)) == (False, code)
+
+
+def test_operators_refuse_cpu_tensors():
+    x = torch.zeros(4, 16)
+    with pytest.raises(ValueError, match=r"turbo_layer_norm unsupported \[device\]"):
+        tk.turbo_layer_norm(x)
+    with pytest.raises(ValueError, match=r"turbo_norm_linear unsupported \[device\]"):
+        tk.turbo_norm_linear(x.bfloat16(), None, None, torch.zeros(8, 16))
+    with pytest.raises(ValueError, match=r"pack_activation unsupported \[device\]"):
+        tk.pack_activation(x)
+    with pytest.raises(ValueError, match=r"unpack_activation unsupported \[device\]"):
+        tk.unpack_activation(x.to(torch.int8), torch.zeros(4, 1))
+
+
+def test_int8_activations_leaves_cpu_tensors_alone():
+    x = torch.randn(300, 300, requires_grad=True)
+    with tk.int8_activations(min_elements=1):
+        y = (x.bfloat16() * 2).sin().sum()
+    y.backward()
+    x2 = x.detach().clone().requires_grad_(True)
+    (x2.bfloat16() * 2).sin().sum().backward()
+    assert torch.equal(x.grad, x2.grad)
+
+
+# ---- the C entries -------------------------------------------------------------------------------
+def _ln_fwd(**kw):
+    a = dict(x=ONE, pitch=8, type=1, w=NULL, wt=0, b=NULL, bt=0, y=ONE, codes=NULL, scales=NULL, mean=NULL, rstd=NULL, rows=4,
+             cols=8, eps=1e-5, stream=NULL)
+    a.update(kw)
+    return C.call("tpf_layer_norm_fwd", *a.values())
+
+
+def _ln_bwd(**kw):
+    a = dict(dy=ONE, x=ONE, pitch=8, codes=NULL, scales=NULL, type=1, mean=ONE, rstd=ONE, w=NULL, wt=0, dx=ONE, dw=NULL, dwt=0,
+             db=NULL, dbt=0, ws=NULL, wsb=0, rows=4, cols=8, stream=NULL)
+    a.update(kw)
+    return C.call("tpf_layer_norm_bwd", *a.values())
+
+
+@pytest.mark.parametrize("kw, text", [
+    (dict(type=3), "unknown element type"), (dict(rows=-1), "rows must not be negative"), (dict(cols=0), "1 to 8192 columns"),
+    (dict(cols=8193, pitch=8193), "1 to 8192 columns"), (dict(pitch=7), "rows overlap"), (dict(codes=ONE), "come together"),
+    (dict(mean=ONE), "come together"), (dict(w=ONE, wt=5), "unknown parameter type"), (dict(x=NULL), "null pointer"),
+    (dict(y=NULL), "null pointer"),
+])
+def test_layer_norm_forward_entry_refuses(kw, text):
+    with pytest.raises(ValueError, match=text):
+        _ln_fwd(**kw)
+
+
+@pytest.mark.parametrize("kw, text", [
+    (dict(x=NULL), "null pointer"), (dict(mean=NULL, rstd=NULL), "null pointer"), (dict(dy=NULL), "null pointer"),
+    (dict(dw=ONE, dwt=9), "unknown parameter type"), (dict(cols=9000, pitch=9000), "1 to 8192 columns"),
+])
+def test_layer_norm_backward_entry_refuses(kw, text):
+    with pytest.raises(ValueError, match=text):
+        _ln_bwd(**kw)
+
+
+def test_layer_norm_backward_entry_wants_a_workspace():
+    with pytest.raises(C.TpfError, match="workspace of"):
+        _ln_bwd(dw=ONE)
+    lib = C.load()
+    assert lib.tpf_layer_norm_bwd_workspace_bytes(4, 8) == 4 * 2 * 8 * 4
+    assert lib.tpf_layer_norm_bwd_workspace_bytes(0, 8) == 0
+    assert lib.tpf_layer_norm_bwd_workspace_bytes(10 ** 6, 128) <= 8 * 160 * 2 * 128 * 4
+
+
+def test_no_rows_is_no_launch():
+    before = C.load().tpf_launch_count()
+    _ln_fwd(rows=0, x=NULL, y=NULL)
+    _ln_bwd(rows=0, x=NULL, dy=NULL, mean=NULL, rstd=NULL)
+    C.call("tpf_int8_pack", NULL, 8, 1, NULL, NULL, 0, 8, NULL)
+    C.call("tpf_int8_unpack", NULL, NULL, 1, NULL, 4, 0, NULL)
+    assert C.load().tpf_launch_count() == before
+
+
+@pytest.mark.parametrize("args, text", [
+    ((ONE, 8, 7, ONE, ONE, 4, 8, NULL), "unknown element type"), ((NULL, 8, 1, ONE, ONE, 4, 8, NULL), "null pointer"),
+    ((ONE, 7, 1, ONE, ONE, 4, 8, NULL), "rows overlap"), ((ONE, 8, 1, ONE, ONE, -4, 8, NULL), "must not be negative"),
+    ((ONE, 8, 1, ONE, ONE, 1 << 31, 8, NULL), "2\\^31"), ((ONE, 1 << 31, 1, ONE, ONE, 1, 1 << 31, NULL), "2\\^31"),
+])
+def test_pack_entry_refuses(args, text):
+    with pytest.raises(ValueError, match=text):
+        C.call("tpf_int8_pack", *args)
+
+
+def _nl_fwd(**kw):
+    a = dict(x=ONE, pitch=16, nw=NULL, nwt=0, nb=NULL, nbt=0, w=ONE, out=ONE, codes=NULL, scales=NULL, mean=NULL, rstd=NULL,
+             ws=ONE, wsb=1 << 20, rows=4, cols=16, outs=8, eps=1e-5, stream=NULL)
+    a.update(kw)
+    return C.call("tpf_norm_linear_fwd", *a.values())
+
+
+@pytest.mark.parametrize("kw, text", [
+    (dict(cols=12, pitch=12), "multiples of 8"), (dict(outs=12), "multiples of 8"), (dict(outs=0), "multiples of 8"),
+    (dict(w=NULL), "null pointer"), (dict(x=NULL), "null pointer"), (dict(out=NULL), "null pointer"),
+    (dict(w=ctypes.c_void_p(264)), "weight must be 16-byte aligned"), (dict(out=ctypes.c_void_p(264)), "out must be 16-byte"),
+    (dict(x=ctypes.c_void_p(258)), "x must"), (dict(pitch=20), "x must"), (dict(rows=1 << 31), "too large"),
+])
+def test_norm_linear_forward_entry_refuses(kw, text):
+    with pytest.raises(ValueError, match=text):
+        _nl_fwd(**kw)
+
+
+def _nl_bwd(**kw):
+    a = dict(d_out=ONE, x=ONE, pitch=16, codes=NULL, scales=NULL, mean=ONE, rstd=ONE, nw=NULL, nwt=0, nb=NULL, nbt=0, w=ONE,
+             dx=ONE, dnw=NULL, dnwt=0, dnb=NULL, dnbt=0, dw=NULL, dwt=1, ws=ONE, wsb=1 << 30, rows=4, cols=16, outs=8,
+             stream=NULL)
+    a.update(kw)
+    return C.call("tpf_norm_linear_bwd", *a.values())
+
+
+@pytest.mark.parametrize("kw, text", [
+    (dict(d_out=NULL), "null pointer"), (dict(x=NULL), "null pointer"), (dict(d_out=ctypes.c_void_p(264)), "16-byte aligned"),
+    (dict(dx=ctypes.c_void_p(264)), "16-byte aligned"), (dict(dw=ONE, dwt=4), "unknown parameter type"),
+    (dict(outs=4), "multiples of 8"), (dict(x=ctypes.c_void_p(258)), "x must"),
+    (dict(codes=ctypes.c_void_p(260), scales=ONE), "codes must"),
+])
+def test_norm_linear_backward_entry_refuses(kw, text):
+    with pytest.raises(ValueError, match=text):
+        _nl_bwd(**kw)
+
+
+def test_norm_linear_entries_want_workspaces():
+    with pytest.raises(C.TpfError, match="workspace of"):
+        _nl_fwd(rows=1000, wsb=0, ws=NULL)
+    with pytest.raises(C.TpfError, match="workspace of"):
+        _nl_bwd(wsb=8)
+    lib = C.load()
+    assert lib.tpf_norm_linear_fwd_workspace_bytes(0, 16, 8) == 0
+    assert lib.tpf_norm_linear_bwd_workspace_bytes(1000, 16, 8) % 256 == 0
