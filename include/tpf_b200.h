@@ -249,7 +249,8 @@ int tpf_trimul_bwd_stages(const void* d_out, const void* z, const float* mask,
  *            (rows that start on 16-byte boundaries, 32 in fp32, with cols a multiple of 8 are accessed by vectors)
  *   weight, bias  [cols] of their own types, or NULL (ones, zeros)
  *   y        [rows, cols] of `type`, contiguous
- *   codes, scales  NULL, or where x is kept in the 8-bit format of tpf_int8_pack
+ *   codes, scales  NULL, or where x is kept in the 8-bit format of tpf_int8_pack, rows of codes at a pitch of cols rounded up
+ *            to a multiple of 16 (what lies between is left as it was)
  *   mean, rstd     fp32 [rows] for the backward pass, or NULL */
 int tpf_layer_norm_fwd(const void* x, int64_t x_pitch, int type, const void* weight, int weight_type, const void* bias,
                        int bias_type, void* y, void* codes, float* scales, float* mean, float* rstd, int64_t rows,

@@ -160,6 +160,10 @@ struct PerDeviceOnce {
   std::atomic<bool> done[kMaxDevices];
 };
 
+struct PerDeviceInt {
+  std::atomic<int> v[kMaxDevices];
+};
+
 // cudaFuncAttributeMaxDynamicSharedMemorySize for `kern` on the current device, once per device.  `base_align`: what a
 // kernel without room to align its dynamic shared memory by hand relies on.  That memory starts behind the part of the
 // block's shared memory that the system keeps and the kernel's static variables (their padding included).

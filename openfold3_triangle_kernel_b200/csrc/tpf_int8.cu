@@ -21,104 +21,161 @@ struct Int8Args {
 };
 
 struct GroupPos {
-  int64_t row;
-  int first, count;  // columns
+  int64_t x, code;  // offsets of the group's first element
+  int count;        // its columns
 };
+// FLAT: contiguous rows of a multiple of 128 columns, groups of all rows lie one after the other.
+template <bool FLAT>
 __device__ __forceinline__ GroupPos locate(const Int8Args& a, int64_t g) {
+  if constexpr (FLAT) return {g * kGroup, g * kGroup, kGroup};
   const uint32_t row = a.per_row.div((uint32_t)g);
   const int first = (int)((uint32_t)g - row * a.per_row.d) * kGroup;
-  return {row, first, min(kGroup, a.cols - first)};
+  return {row * a.x_pitch + first, (int64_t)row * a.cols + first, min(kGroup, a.cols - first)};
 }
 
 constexpr int kUnroll = 4;  // groups a team works on at once, their loads issued before the first use
 
 // VEC = 8: LANES lanes with eight elements each; the last piece of a row whose width is no multiple of eight (only possible
 // in a single row) element by element.  VEC = 1: 32 lanes, four elements each, 32 apart.
-template <typename T, int VEC, int LANES, bool PACK>
+// A lane whose columns do not exist, or not all of them, loads the group's first ones instead and ignores them.
+template <typename T, int VEC, int LANES, bool FLAT, bool PACK>
 __global__ void __launch_bounds__(256) int8_kernel(const Int8Args a) {
   griddep_wait();
   constexpr int TEAMS = 256 / LANES, STRIDE = VEC == 8 ? 1 : 32;  // distance of a lane's elements
   static_assert(VEC == 8 || LANES == 32, "");
-  constexpr int E = VEC == 8 ? 8 : 4;
+  constexpr int E = VEC == 8 ? 8 : 4, PIECES = E / VEC;
   const int lane = threadIdx.x % LANES;
   const int64_t g0 = ((int64_t)blockIdx.x * TEAMS + threadIdx.x / LANES) * kUnroll;
-  float x[kUnroll][E], down[kUnroll];
-  uint2 w[kUnroll];
-  GroupPos pos[kUnroll];
   const int c0 = VEC == 8 ? lane * 8 : lane;
+  GroupPos pos[kUnroll];
+  bool live[kUnroll];
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    pos[u] = g0 + u < a.groups ? locate(a, g0 + u) : GroupPos{0, 0, 0};
-    const int left = pos[u].count - c0;  // columns of this lane and those behind it
-    const T* src = static_cast<const T*>(a.x) + pos[u].row * a.x_pitch + pos[u].first + c0;
-    const int8_t* code = a.codes + pos[u].row * a.cols + pos[u].first + c0;
-    if constexpr (PACK) {
-      if (VEC == 8 && left >= 8) {
-        load_vec<T, 8>(src, x[u]);
-      } else {
+    live[u] = g0 + u < a.groups;
+    pos[u] = locate<FLAT>(a, live[u] ? g0 + u : a.groups - 1);
+  }
+  // the column a lane loads its piece from
+  auto column = [&](int u, int e) {
+    const int c = c0 + e * STRIDE;
+    return FLAT || c + VEC <= pos[u].count ? c : 0;
+  };
+  auto whole = [&](int u) { return VEC == 8 && (FLAT || c0 + 8 <= pos[u].count); };
+  auto loadable = [&](int u) { return FLAT || VEC == 1 || pos[u].count >= 8; };
+  if constexpr (PACK) {
+    Piece<T, VEC> raw[kUnroll][PIECES];
+    float amax[kUnroll], up[kUnroll];
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[u][e] = e * STRIDE < left ? to_f32(src[e * STRIDE]) : 0.f;
-      }
-    } else {
-      down[u] = pos[u].count > 0 ? a.scales[g0 + u] : 0.f;
-      if (VEC == 8 && left >= 8) {
-        w[u] = *reinterpret_cast<const uint2*>(code);
-      } else {
-        w[u] = make_uint2(0u, 0u);
+    for (int u = 0; u < kUnroll; ++u) {
+      const T* src = static_cast<const T*>(a.x) + pos[u].x;
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (e * STRIDE < left) (e < 4 ? w[u].x : w[u].y) |= (uint32_t)(uint8_t)code[e * STRIDE] << (8 * (e & 3));
+      for (int e = 0; e < PIECES; ++e) {
+        if (loadable(u)) raw[u][e].load(src + column(u, e));
+        else raw[u][e].zero();
       }
     }
-  }
+    float tail[kUnroll][FLAT || VEC == 1 ? 1 : 8];  // the ragged end of a single row
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    const int left = pos[u].count - c0;
-    if constexpr (PACK) {
+    for (int u = 0; u < kUnroll; ++u) {
       float m = 0.f;
+      if constexpr (VEC == 1) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) m = max_nan(m, fabsf(x[u][e]));
+        for (int e = 0; e < PIECES; ++e) {
+          if (c0 + e * STRIDE >= pos[u].count) raw[u][e].zero();
+          m = max_nan(m, raw[u][e].amax());
+        }
+      } else if (whole(u)) {
+        m = raw[u][0].amax();
+      } else if constexpr (!FLAT) {
+        const T* src = static_cast<const T*>(a.x) + pos[u].x + c0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          tail[u][e] = c0 + e < pos[u].count ? to_f32(src[e]) : 0.f;
+          m = max_nan(m, fabsf(tail[u][e]));
+        }
+      }
 #pragma unroll
       for (int off = LANES / 2; off > 0; off >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, off));
-      const GroupScale s = group_scale(m);
-      int8_t* code = a.codes + pos[u].row * a.cols + pos[u].first + c0;
-      if (VEC == 8 && left >= 8) {
-        store_codes<VEC>(code, x[u], s);
-      } else {
+      amax[u] = m;
+    }
+    const float down = group_scales<kUnroll, LANES>(amax, up);
+    if (lane < kUnroll && g0 + lane < a.groups) a.scales[g0 + lane] = down;
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (e * STRIDE < left) code[e * STRIDE] = code_of(x[u][e], s);
+    for (int u = 0; u < kUnroll; ++u) {
+      if (!live[u]) continue;
+      int8_t* code = a.codes + pos[u].code + c0;
+      if constexpr (VEC == 1) {
+#pragma unroll
+        for (int e = 0; e < PIECES; ++e) {
+          float x;
+          raw[u][e].get(&x);
+          if (c0 + e * STRIDE < pos[u].count) code[e * STRIDE] = code_of(x, up[u]);
+        }
+      } else if (whole(u)) {
+        float x[8];
+        raw[u][0].get(x);
+        const uint64_t f = f2_dup(up[u]);
+        const bool good = up[u] == up[u];
+        *reinterpret_cast<uint2*>(code) = make_uint2(pack_codes(f2_pack(x[0], x[1]), f2_pack(x[2], x[3]), f, good),
+                                                     pack_codes(f2_pack(x[4], x[5]), f2_pack(x[6], x[7]), f, good));
+      } else if constexpr (!FLAT) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c0 + e < pos[u].count) code[e] = code_of(tail[u][e], up[u]);
       }
-      if (lane == 0 && pos[u].count > 0) a.scales[g0 + u] = s.down;
-    } else {
-      unpack_codes(w[u].x, down[u], x[u]);
-      if constexpr (E == 8) unpack_codes(w[u].y, down[u], x[u] + 4);
-      T* dst = static_cast<T*>(const_cast<void*>(a.x)) + pos[u].row * a.x_pitch + pos[u].first + c0;
-      if (VEC == 8 && left >= 8) {
-        store_vec<T, VEC>(dst, x[u]);
-      } else {
+    }
+  } else {
+    using Raw = std::conditional_t<VEC == 1, int8_t, uint2>;
+    Raw raw[kUnroll][PIECES];
+    float down[kUnroll];
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (e * STRIDE < left) dst[e * STRIDE] = from_f32<T>(x[u][e]);
+    for (int u = 0; u < kUnroll; ++u) {
+      const int8_t* code = a.codes + pos[u].code;
+      down[u] = a.scales[live[u] ? g0 + u : a.groups - 1];
+#pragma unroll
+      for (int e = 0; e < PIECES; ++e)
+        raw[u][e] = loadable(u) ? *reinterpret_cast<const Raw*>(code + column(u, e)) : Raw{};
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      if (!live[u]) continue;
+      T* dst = static_cast<T*>(const_cast<void*>(a.x)) + pos[u].x + c0;
+      if constexpr (VEC == 1) {
+#pragma unroll
+        for (int e = 0; e < PIECES; ++e)
+          if (c0 + e * STRIDE < pos[u].count) dst[e * STRIDE] = from_f32<T>((float)raw[u][e] * down[u]);
+      } else if (whole(u)) {
+        uint64_t p[4];
+        unpack_codes(raw[u][0].x, p);
+        unpack_codes(raw[u][0].y, p + 2);
+        float x[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f2_unpack(f2_mul(p[k], f2_dup(down[u])), x[2 * k], x[2 * k + 1]);
+        store_vec<T, VEC>(dst, x);
+      } else if constexpr (!FLAT) {
+        const int8_t* code = a.codes + pos[u].code + c0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c0 + e < pos[u].count) dst[e] = from_f32<T>((float)code[e] * down[u]);
       }
     }
   }
 }
 
-template <typename T, int VEC, int LANES, bool PACK>
+template <typename T, int VEC, int LANES, bool FLAT, bool PACK>
 int int8_launch(const Int8Args& a, cudaStream_t stream) {
   constexpr int per_block = 256 / LANES * kUnroll;
-  launch_kernel(int8_kernel<T, VEC, LANES, PACK>, dim3((unsigned)((a.groups + per_block - 1) / per_block)), dim3(256), 0,
-                stream, a);
+  launch_kernel(int8_kernel<T, VEC, LANES, FLAT, PACK>, dim3((unsigned)((a.groups + per_block - 1) / per_block)), dim3(256),
+                0, stream, a);
   TPF_LAUNCH_OK();
   return TPF_OK;
 }
 template <typename T, bool PACK>
 int int8_by_width(const Int8Args& a, bool vec, cudaStream_t stream) {
-  if (!vec) return int8_launch<T, 1, 32, PACK>(a, stream);
-  if (a.cols <= 32) return int8_launch<T, 8, 4, PACK>(a, stream);
-  if (a.cols <= 64) return int8_launch<T, 8, 8, PACK>(a, stream);
-  return int8_launch<T, 8, 16, PACK>(a, stream);
+  if (!vec) return int8_launch<T, 1, 32, false, PACK>(a, stream);
+  if (a.cols % kGroup == 0 && a.x_pitch == a.cols) return int8_launch<T, 8, 16, true, PACK>(a, stream);
+  if (a.cols <= 32) return int8_launch<T, 8, 4, false, PACK>(a, stream);
+  if (a.cols <= 64) return int8_launch<T, 8, 8, false, PACK>(a, stream);
+  return int8_launch<T, 8, 16, false, PACK>(a, stream);
 }
 
 template <bool PACK>
@@ -134,7 +191,7 @@ int int8_run(const char* who, const void* x, int64_t pitch, int type, void* code
   TPF_REQUIRE(rows == 1 || pitch >= cols || (PACK && pitch == 0), TPF_ERR_INVALID_ARGUMENT, "%s: rows overlap", who);
   const bool vec = vec_ok(x, type) && (reinterpret_cast<uintptr_t>(codes) & 7) == 0 &&
                    (rows == 1 || (cols % 8 == 0 && pitch % 8 == 0));
-  const Int8Args a{x, pitch, static_cast<int8_t*>(codes), scales, per_row * rows, FastDiv::make((uint32_t)per_row),
+  const Int8Args a{x, rows == 1 ? cols : pitch, static_cast<int8_t*>(codes), scales, per_row * rows, FastDiv::make((uint32_t)per_row),
                    (int)cols};
   if (type == kRowF32) return int8_by_width<float, PACK>(a, vec, stream);
   if (type == kRowBF16) return int8_by_width<bf16, PACK>(a, vec, stream);

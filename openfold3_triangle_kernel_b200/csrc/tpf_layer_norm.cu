@@ -16,94 +16,153 @@ namespace tpf {
 
 namespace {
 
-// ROWS rows a team at a time, all their loads issued before the first use.
+// A CTA walks the row groups blockIdx.x, + gridDim.x, ..., ROWS rows a team at a time; the next rows are loaded while these
+// are worked on, and the parameters stay in registers.
 template <typename T, class Tm, int ROWS, bool KEEP>
-__global__ void __launch_bounds__(Tm::BLOCK) norm_fwd_kernel(const NormArgs a, T* __restrict__ y, float eps) {
+__global__ void __launch_bounds__(Tm::MAXB, min_ctas<Tm, false>()) norm_fwd_kernel(const NormArgs a, T* __restrict__ y, float eps) {
   griddep_wait();
-  constexpr int E = Tm::E, VEC = Tm::VEC;
-  __shared__ float red[Tm::TS > 32 ? 2 * Tm::WARPS * ROWS : 1];
+  constexpr int E = Tm::E, P = E / 2, ITEMS = Tm::ITEMS;
+  __shared__ __align__(8) float red[Tm::BLOCK ? 2 * 64 : 1];
   const Tm tm;
   int turn = 0;
-  const int64_t row0 = ((int64_t)blockIdx.x * Tm::TEAMS + tm.index) * ROWS;
-  float x[ROWS][E];
+  int at[ITEMS];
+  bool on[ITEMS], ragged = false;
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r)
+  for (int i = 0; i < ITEMS; ++i) {
+    on[i] = tm.column(i) < a.cols;
+    at[i] = on[i] ? tm.column(i) : 0;
+    ragged |= !on[i];
+  }
+  // (BLOCK) columns of this warp; only the last warp of the team has fewer than 32 E
+  const float warp_inv = 1.f / (float)min(32 * E, a.cols - (int)(threadIdx.x >> 5) * 32 * E);
+  const int64_t step = (int64_t)gridDim.x * Tm::TEAMS * ROWS;
+  int64_t base = (int64_t)blockIdx.x * Tm::TEAMS * ROWS;
+  Frag<T, Tm> raw[ROWS];
+  auto load = [&](const RowSet<ROWS>& rows) {
+    const T* src = static_cast<const T*>(a.x) + rows.first * a.x_pitch;
 #pragma unroll
-    for (int i = 0; i < Tm::ITEMS; ++i) {
-      const int c = tm.column(i);
-      if (row0 + r < a.rows && c < a.cols)
-        load_vec<T, VEC>(static_cast<const T*>(a.x) + (row0 + r) * a.x_pitch + c, &x[r][i * VEC]);
-      else
+    for (int r = 0; r < ROWS; ++r) raw[r].load(src + rows.at(r) * a.x_pitch, at);
+  };
+  RowSet<ROWS> next(base + tm.index * ROWS, a.rows);
+  load(next);
+  uint64_t w[P], b[P];
+  {
+    float f[E], g[E];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) x[r][i * VEC + e] = 0.f;
+    for (int i = 0; i < ITEMS; ++i) {
+      param_load<Tm::VEC, 1>(a.w, tm.column(i), a.cols, 1.f, f + i * Tm::VEC);
+      param_load<Tm::VEC, 1>(a.b, tm.column(i), a.cols, 0.f, g + i * Tm::VEC);
     }
-  if constexpr (KEEP) {
-    constexpr int NG = VEC == 8 ? Tm::ITEMS : (Tm::ITEMS + 3) / 4;
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+      w[k] = f2_pack(f[2 * k], f[2 * k + 1]);
+      b[k] = f2_pack(g[2 * k], g[2 * k + 1]);
+    }
+  }
+  // every team of a block makes the same number of rounds: the sums over a team are converged
+  for (; base < a.rows; base += step) {
+    const RowSet<ROWS> rows = next;
+    uint64_t x[ROWS][P];
+    constexpr int NG = Groups<Tm>::N, N = ROWS * NG;
+    float amax[KEEP ? N : 1];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-      float amax[NG];
-      group_amax<Tm>(x[r], amax);
-#pragma unroll
-      for (int i = 0; i < Tm::ITEMS; ++i) {
-        const int c = tm.column(i);
-        const GroupScale s = group_scale(amax[VEC == 8 ? i : i / 4]);
-        if (row0 + r < a.rows && c < a.cols) {
-          store_codes<VEC>(a.codes + (row0 + r) * a.cols + c, &x[r][i * VEC], s);
-          if (c % kGroup == 0) a.scales[(row0 + r) * a.groups + c / kGroup] = s.down;
-        }
-      }
+      if (ragged) raw[r].mask(on);
+      raw[r].get(x[r]);
+      if constexpr (KEEP) raw[r].amax(amax + r * NG);
     }
-  }
-  float sum[ROWS], mean[ROWS];
-#pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
-    sum[r] = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) sum[r] += x[r][e];
-  }
-  team_sum<Tm, ROWS>(sum, red, turn);
-#pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
-    mean[r] = sum[r] * a.inv_cols;
-    sum[r] = 0.f;
-#pragma unroll
-    for (int i = 0; i < Tm::ITEMS; ++i) {
-      const bool on = tm.column(i) < a.cols;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        float& v = x[r][i * VEC + e];
-        v = on ? v - mean[r] : 0.f;
-        sum[r] += v * v;
-      }
+    if (base + step < a.rows) {
+      next = RowSet<ROWS>(base + step + tm.index * ROWS, a.rows);
+      load(next);
     }
-  }
-  team_sum<Tm, ROWS>(sum, red, turn);
-  float rstd[ROWS];
+    if constexpr (KEEP) {
+      float up[N];
+      const float down = group_scales<N, Groups<Tm>::LANES>(amax, up);
+      int8_t* codes = a.codes + rows.first * a.code_pitch;
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
-    rstd[r] = rsqrtf(sum[r] * a.inv_cols + eps);
-    if (a.mean != nullptr && tm.t == 0 && row0 + r < a.rows) {
-      a.mean[row0 + r] = mean[r];
-      a.rstd[row0 + r] = rstd[r];
+      for (int r = 0; r < ROWS; ++r)
+        if (r < rows.count) store_codes<Tm>(codes + r * (int64_t)a.code_pitch, x[r], up + r * NG, at, on);
+      // of the lanes that hold a group, number n (mod N) has the scale of group n
+      const int mine = threadIdx.x & (N - 1), first = threadIdx.x & (Groups<Tm>::LANES - 1);
+      const int r = mine / NG, g = mine % NG;
+      const int c0 = tm.column(0) + (Tm::VEC == 8 ? g * 32 * 8 - first * 8 : g * 128 - first);  // first column of the group
+      if (first == mine && r < rows.count && c0 < a.cols) a.scales[(rows.first + r) * a.groups + c0 / kGroup] = down;
     }
-  }
+    float sum[ROWS], mean[ROWS];
 #pragma unroll
-  for (int i = 0; i < Tm::ITEMS; ++i) {
-    const int c = tm.column(i);
-    if (c >= a.cols) continue;
-    float w[VEC], b[VEC];
+    for (int r = 0; r < ROWS; ++r) {
+      uint64_t s = x[r][0];
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      w[e] = param_at(a.w, c + e, 1.f);
-      b[e] = param_at(a.b, c + e, 0.f);
+      for (int k = 1; k < P; ++k) s = f2_add(s, x[r][k]);
+      sum[r] = f2_sum(s);
+    }
+    if constexpr (!Tm::BLOCK) {
+      team_sum<Tm, ROWS>(sum, red, turn);
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) mean[r] = sum[r] * a.inv_cols;
+    } else {
+      // each warp about its own mean; the warps' means and sums of squares are put together below
+      warp_sum(sum);
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) mean[r] = sum[r] * warp_inv;
     }
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-      if (row0 + r >= a.rows) continue;
-      float o[VEC];
+      const uint64_t m = f2_dup(-mean[r]);
+      uint64_t s = 0;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) o[e] = x[r][i * VEC + e] * rstd[r] * w[e] + b[e];
-      store_vec<T, VEC>(y + (row0 + r) * a.cols + c, o);
+      for (int k = 0; k < P; ++k) x[r][k] = f2_add(x[r][k], m);
+      if (ragged) mask_pairs<Tm>(x[r], on);
+#pragma unroll
+      for (int k = 0; k < P; ++k) s = f2_fma(x[r][k], x[r][k], s);
+      sum[r] = f2_sum(s);
+    }
+    if constexpr (!Tm::BLOCK) {
+      team_sum<Tm, ROWS>(sum, red, turn);
+    } else {
+      // n values with mean m and sum of squares q about it, and others: q + q' + n (m - M)^2 + n' (m' - M)^2 about the
+      // common mean M (Chan, Golub and LeVeque, "Updating formulae", 1979): one barrier for both statistics
+      using X = CrossWarp<Tm, ROWS>;
+      warp_sum(sum);
+      float2* m = reinterpret_cast<float2*>(red) + turn * 32;
+      turn ^= 1;
+      const int lane = threadIdx.x & 31, warps = blockDim.x >> 5, k = lane & (X::W - 1);
+      if (lane == 0)
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) m[r * X::W + (threadIdx.x >> 5)] = make_float2(mean[r], sum[r]);
+      __syncthreads();
+      const bool exists = X::exists() && lane < ROWS * X::W;
+      const float2 part = exists ? m[lane] : make_float2(0.f, 0.f);
+      const float n = exists ? (float)(k + 1 < warps ? 32 * E : a.cols - k * 32 * E) : 0.f;
+      const float all = X::sum(part.x * (n * a.inv_cols)), d = part.x - all;
+      const float sq = X::sum(fmaf(d * n, d, part.y));
+      float own[ROWS];
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        own[r] = mean[r];
+        mean[r] = __shfl_sync(0xffffffffu, all, r * X::W);
+        sum[r] = __shfl_sync(0xffffffffu, sq, r * X::W);
+      }
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        const uint64_t shift = f2_dup(own[r] - mean[r]);
+#pragma unroll
+        for (int k = 0; k < P; ++k) x[r][k] = f2_add(x[r][k], shift);
+      }
+    }
+    T* dst = y + rows.first * a.cols;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const float rstd = rsqrtf(fmaf(sum[r], a.inv_cols, eps));
+      if (r >= rows.count) continue;
+      if (a.mean != nullptr && tm.t == 0) {
+        a.mean[rows.first + r] = mean[r];
+        a.rstd[rows.first + r] = rstd;
+      }
+      const uint64_t rs = f2_dup(rstd);
+#pragma unroll
+      for (int k = 0; k < P; ++k) x[r][k] = f2_fma(f2_mul(x[r][k], rs), w[k], b[k]);
+      store_row<T, Tm>(dst + r * (int64_t)a.cols, x[r], at, on);
     }
   }
 }
@@ -113,17 +172,39 @@ struct FwdLaunch {
   void* y;
   float eps;
   cudaStream_t stream;
+  // The team for rows of `cols` elements.  vec: eight elements at a time are possible.
+  template <typename T>
+  int by_width(int cols, bool vec) const {
+    if (vec) {
+      if (cols <= 32) return run<T, Team<8, 4, 1>>();
+      if (cols <= 64) return run<T, Team<8, 8, 1>>();
+      if (cols <= 128) return run<T, Team<8, 16, 1>>();
+      if (cols <= 256) return run<T, Team<8, 32, 1>>();
+      if (cols <= 512) return run<T, Team<8, 32, 2>>();
+      if (cols <= 1024) return run<T, Team<8, 0, 1, 128>>();
+      if (cols <= 4096) return run<T, Team<8, 0, 2, 256>>();
+      return run<T, Team<8, 0, 4, 256>>();
+    }
+    if (cols <= 128) return run<T, Team<1, 32, 4>>();
+    if (cols <= 256) return run<T, Team<1, 32, 8>>();
+    if (cols <= 2048) return run<T, Team<1, 0, 8, 256>>();
+    if (cols <= 4096) return run<T, Team<1, 0, 8, 512>>();
+    return run<T, Team<1, 0, 16, 512>>();
+  }
   template <typename T, class Tm>
   int run() const {
-    constexpr int ROWS = rows_in_flight<Tm>();
-    const int64_t blocks = (a.rows + Tm::TEAMS * ROWS - 1) / (Tm::TEAMS * ROWS);
-    TPF_REQUIRE(blocks < (1ll << 31), TPF_ERR_INVALID_ARGUMENT, "layer norm: too many rows");
-    if (a.codes != nullptr)
-      launch_kernel(norm_fwd_kernel<T, Tm, ROWS, true>, dim3((unsigned)blocks), dim3(Tm::BLOCK), 0, stream, a,
-                    static_cast<T*>(y), eps);
-    else
-      launch_kernel(norm_fwd_kernel<T, Tm, ROWS, false>, dim3((unsigned)blocks), dim3(Tm::BLOCK), 0, stream, a,
-                    static_cast<T*>(y), eps);
+    return a.codes != nullptr ? go<T, Tm, true>() : go<T, Tm, false>();
+  }
+  template <typename T, class Tm, bool KEEP>
+  int go() const {
+    constexpr int ROWS = rows_in_flight<T, Tm, false>();
+    static PerDeviceInt regs;
+    const auto kern = norm_fwd_kernel<T, Tm, ROWS, KEEP>;
+    const int threads = Tm::threads(a.cols);
+    int fit = 1;
+    if (int rc = resident_ctas(kern, threads, regs, &fit)) return rc;
+    const int64_t want = (a.rows + Tm::TEAMS * ROWS - 1) / (Tm::TEAMS * ROWS), most = (int64_t)fit * sm_count();
+    launch_kernel(kern, dim3((unsigned)(want < most ? want : most)), dim3(threads), 0, stream, a, static_cast<T*>(y), eps);
     TPF_LAUNCH_OK();
     return TPF_OK;
   }
@@ -137,7 +218,7 @@ int layer_norm_fwd(const NormCall& c, void* y, float eps, cudaStream_t stream) {
   if (c.rows == 0) return TPF_OK;
   TPF_REQUIRE(c.x != nullptr && y != nullptr, TPF_ERR_INVALID_ARGUMENT, "layer_norm_fwd: null pointer");
   const bool vec = c.cols % 8 == 0 && rows_vec_ok(c.x, c.x_pitch, c.type) && vec_ok(y, c.type) &&
-                   (reinterpret_cast<uintptr_t>(c.codes) & 7) == 0;
+                   (reinterpret_cast<uintptr_t>(c.codes) & 15) == 0;
   return by_type(FwdLaunch{a, y, eps, stream}, c.type, a.cols, vec);
 }
 

@@ -5,95 +5,136 @@ namespace tpf {
 
 namespace {
 
-// A CTA walks the row groups blockIdx.x, + gridDim.x, ...; partials: [gridDim.x][2][cols], the CTA's sums of dy xh and dy.
+// A CTA walks the row groups blockIdx.x, + gridDim.x, ... as in the forward; partials: [gridDim.x][2][cols], the CTA's sums
+// of dy xh and dy.  From codes xh = code (s rstd) - mean rstd, one FMA, off by three roundings of what it subtracts; from x
+// itself the mean is taken off first, where it may be large.
 template <typename T, class Tm, int ROWS, bool CODES>
-__global__ void __launch_bounds__(Tm::BLOCK) norm_bwd_kernel(const NormArgs a, const T* __restrict__ dy, T* __restrict__ dx,
-                                                             float* __restrict__ partials) {
+__global__ void __launch_bounds__(Tm::MAXB, min_ctas<Tm, true>())
+    norm_bwd_kernel(const NormArgs a, const T* __restrict__ dy, T* __restrict__ dx, float* __restrict__ partials) {
   griddep_wait();
-  constexpr int E = Tm::E, VEC = Tm::VEC;
-  __shared__ float red[Tm::TS > 32 ? 2 * Tm::WARPS * 2 * ROWS : 2 * Tm::COLS];
+  constexpr int E = Tm::E, P = E / 2, ITEMS = Tm::ITEMS, NG = Groups<Tm>::N;
+  __shared__ float red[Tm::BLOCK ? 2 * 32 : 2 * Tm::COLS];
   const Tm tm;
   int turn = 0;
-  float w[E], aw[E], ab[E];
+  int at[ITEMS];
+  bool on[ITEMS], ragged = false;
 #pragma unroll
-  for (int i = 0; i < Tm::ITEMS; ++i)
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) {
-      const int c = tm.column(i);
-      w[i * VEC + e] = c < a.cols ? param_at(a.w, c + e, 1.f) : 0.f;
-      aw[i * VEC + e] = ab[i * VEC + e] = 0.f;
-    }
+  for (int i = 0; i < ITEMS; ++i) {
+    on[i] = tm.column(i) < a.cols;
+    at[i] = on[i] ? tm.column(i) : 0;
+    ragged |= !on[i];
+  }
   const int64_t step = (int64_t)gridDim.x * Tm::TEAMS * ROWS;
-  // every team of a block makes the same number of rounds: the sums over a team are converged
-  for (int64_t base = (int64_t)blockIdx.x * Tm::TEAMS * ROWS; base < a.rows; base += step) {
-    const int64_t row0 = base + tm.index * ROWS;
-    float d[ROWS][E], xh[ROWS][E], rstd[ROWS];
+  int64_t base = (int64_t)blockIdx.x * Tm::TEAMS * ROWS;
+  Frag<T, Tm> dy_raw[ROWS], x_raw[CODES ? 1 : ROWS];
+  CodeFrag<Tm> c_raw[CODES ? ROWS : 1];
+  float down[CODES ? ROWS : 1][NG], mean[ROWS], rstd[ROWS];
+  auto request = [&](int64_t row0) {
+    const RowSet<ROWS> rows(row0, a.rows);
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-      const int64_t row = row0 + r;
-      const bool live = row < a.rows;
-      const float mean = live ? a.mean[row] : 0.f;
-      rstd[r] = live ? a.rstd[row] : 0.f;
+      const int64_t row = rows.first + rows.at(r);
+      dy_raw[r].load(dy + row * a.cols, at);
+      if constexpr (CODES) {
+        c_raw[r].load(a.codes + row * a.code_pitch, at);
+        const float* s = a.scales + row * a.groups;
 #pragma unroll
-      for (int i = 0; i < Tm::ITEMS; ++i) {
-        const int c = tm.column(i);
-        if (live && c < a.cols) {
-          load_vec<T, VEC>(dy + row * a.cols + c, &d[r][i * VEC]);
-          if constexpr (CODES)
-            load_codes<VEC>(a.codes + row * a.cols + c, a.scales[row * a.groups + c / kGroup], &xh[r][i * VEC]);
-          else
-            load_vec<T, VEC>(static_cast<const T*>(a.x) + row * a.x_pitch + c, &xh[r][i * VEC]);
+        for (int g = 0; g < NG; ++g) down[r][g] = s[at[g * (ITEMS / NG)] / kGroup];
+      } else {
+        x_raw[r].load(static_cast<const T*>(a.x) + row * a.x_pitch, at);
+      }
+      mean[r] = a.mean[row];
+      rstd[r] = a.rstd[row];
+    }
+  };
+  request(base + tm.index * ROWS);
+  uint64_t w[P], aw[P], ab[P];
+  {
+    float f[E];
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) xh[r][i * VEC + e] = (xh[r][i * VEC + e] - mean) * rstd[r];
-        } else {
+    for (int i = 0; i < ITEMS; ++i) param_load<Tm::VEC, 1>(a.w, tm.column(i), a.cols, 1.f, f + i * Tm::VEC);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) d[r][i * VEC + e] = xh[r][i * VEC + e] = 0.f;
+    for (int k = 0; k < P; ++k) {
+      w[k] = f2_pack(f[2 * k], f[2 * k + 1]);
+      aw[k] = ab[k] = 0;
+    }
+  }
+  // every team of a block makes the same number of rounds: the sums over a team are converged
+  for (; base < a.rows; base += step) {
+    const RowSet<ROWS> rows(base + tm.index * ROWS, a.rows);
+    uint64_t d[ROWS][P], xh[ROWS][P];
+    float rs[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      rs[r] = rstd[r];
+      if (ragged) dy_raw[r].mask(on);
+      dy_raw[r].get(d[r]);
+      if (r >= rows.count)
+#pragma unroll
+        for (int k = 0; k < P; ++k) d[r][k] = 0;
+      if constexpr (CODES) {
+        c_raw[r].get(xh[r]);
+        const uint64_t g = f2_dup(-mean[r] * rstd[r]);
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          const uint64_t f = f2_dup(down[r][n] * rstd[r]);
+#pragma unroll
+          for (int k = n * (P / NG); k < (n + 1) * (P / NG); ++k) xh[r][k] = f2_fma(xh[r][k], f, g);
         }
+      } else {
+        if (ragged) x_raw[r].mask(on);
+        x_raw[r].get(xh[r]);
+        const uint64_t m = f2_dup(-mean[r]), f = f2_dup(rstd[r]);
+#pragma unroll
+        for (int k = 0; k < P; ++k) xh[r][k] = f2_mul(f2_add(xh[r][k], m), f);
       }
     }
+    if (base + step < a.rows) request(base + step + tm.index * ROWS);
     float s[2 * ROWS];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-      s[2 * r] = s[2 * r + 1] = 0.f;
+      uint64_t s1 = 0, s2 = 0;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float wd = w[e] * d[r][e];
-        s[2 * r] += wd;
-        s[2 * r + 1] += wd * xh[r][e];
-        aw[e] += d[r][e] * xh[r][e];
-        ab[e] += d[r][e];
+      for (int k = 0; k < P; ++k) {
+        aw[k] = f2_fma(d[r][k], xh[r][k], aw[k]);
+        ab[k] = f2_add(ab[k], d[r][k]);
+        d[r][k] = f2_mul(d[r][k], w[k]);
+        s1 = f2_add(s1, d[r][k]);
+        s2 = f2_fma(d[r][k], xh[r][k], s2);
       }
+      s[2 * r] = f2_sum(s1);
+      s[2 * r + 1] = f2_sum(s2);
     }
     team_sum<Tm, 2 * ROWS>(s, red, turn);
     if (dx != nullptr) {
+      T* dst = dx + rows.first * a.cols;
 #pragma unroll
       for (int r = 0; r < ROWS; ++r) {
-        const float m1 = s[2 * r] * a.inv_cols, m2 = s[2 * r + 1] * a.inv_cols;
+        if (r >= rows.count) continue;
+        const uint64_t m1 = f2_dup(-s[2 * r] * a.inv_cols), m2 = f2_dup(-s[2 * r + 1] * a.inv_cols), f = f2_dup(rs[r]);
 #pragma unroll
-        for (int i = 0; i < Tm::ITEMS; ++i) {
-          const int c = tm.column(i);
-          float o[VEC];
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const int k = i * VEC + e;
-            o[e] = rstd[r] * (w[k] * d[r][k] - m1 - xh[r][k] * m2);
-          }
-          if (row0 + r < a.rows && c < a.cols) store_vec<T, VEC>(dx + (row0 + r) * a.cols + c, o);
-        }
+        for (int k = 0; k < P; ++k) d[r][k] = f2_mul(f2_fma(xh[r][k], m2, f2_add(d[r][k], m1)), f);
+        store_row<T, Tm>(dst + r * (int64_t)a.cols, d[r], at, on);
       }
     }
   }
   if (partials == nullptr) return;
-  float* pw = partials + (int64_t)blockIdx.x * 2 * a.cols;
-  if constexpr (Tm::TS > 32) {
+  float fw[E], fb[E];
 #pragma unroll
-    for (int i = 0; i < Tm::ITEMS; ++i) {
+  for (int k = 0; k < P; ++k) {
+    f2_unpack(aw[k], fw[2 * k], fw[2 * k + 1]);
+    f2_unpack(ab[k], fb[2 * k], fb[2 * k + 1]);
+  }
+  float* pw = partials + (int64_t)blockIdx.x * 2 * a.cols;
+  if constexpr (Tm::BLOCK) {
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
       const int c = tm.column(i);
       if (c < a.cols)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          pw[c + e] = aw[i * VEC + e];
-          pw[a.cols + c + e] = ab[i * VEC + e];
+        for (int e = 0; e < Tm::VEC; ++e) {
+          pw[c + e] = fw[i * Tm::VEC + e];
+          pw[a.cols + c + e] = fb[i * Tm::VEC + e];
         }
     }
   } else {
@@ -102,80 +143,110 @@ __global__ void __launch_bounds__(Tm::BLOCK) norm_bwd_kernel(const NormArgs a, c
     for (int k = 0; k < E; ++k)
 #pragma unroll
       for (int off = Tm::TS; off < 32; off <<= 1) {
-        aw[k] += __shfl_xor_sync(0xffffffffu, aw[k], off);
-        ab[k] += __shfl_xor_sync(0xffffffffu, ab[k], off);
+        fw[k] += __shfl_xor_sync(0xffffffffu, fw[k], off);
+        fb[k] += __shfl_xor_sync(0xffffffffu, fb[k], off);
       }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int turn_of = 0; turn_of < Tm::WARPS; ++turn_of) {
-      if (warp == turn_of && lane < Tm::TS) {
+    for (int now = 0; now < Tm::MAXB / 32; ++now) {
+      if (warp == now && lane < Tm::TS) {
 #pragma unroll
-        for (int i = 0; i < Tm::ITEMS; ++i)
+        for (int i = 0; i < ITEMS; ++i)
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const int c = tm.column(i) + e, k = i * VEC + e;
-            red[c] = turn_of == 0 ? aw[k] : red[c] + aw[k];
-            red[Tm::COLS + c] = turn_of == 0 ? ab[k] : red[Tm::COLS + c] + ab[k];
+          for (int e = 0; e < Tm::VEC; ++e) {
+            const int c = tm.column(i) + e, k = i * Tm::VEC + e;
+            red[c] = now == 0 ? fw[k] : red[c] + fw[k];
+            red[Tm::COLS + c] = now == 0 ? fb[k] : red[Tm::COLS + c] + fb[k];
           }
       }
       __syncthreads();
     }
-    for (int c = threadIdx.x; c < a.cols; c += Tm::BLOCK) {
+    for (int c = threadIdx.x; c < a.cols; c += Tm::MAXB) {
       pw[c] = red[c];
       pw[a.cols + c] = red[Tm::COLS + c];
     }
   }
 }
 
-// out[j] = sum over terms of partials[term][j], j < 2 cols.  A CTA owns 32 columns; eight threads of each add a contiguous
-// range of the terms (eight loads in flight), then their sums are added in range order.
+// out[j] = sum over terms of partials[term][j], j < 2 cols.  A CTA owns eight columns (a sector of each term), 32 threads
+// of each add a contiguous range of the terms (eight loads in flight), and their sums are added in a fixed tree.  With 32
+// columns a CTA and eight threads for each the chain of loads took 9 us at 444 terms of 256 columns.
 __global__ void __launch_bounds__(256) norm_fold_kernel(const float* __restrict__ partials, int terms, int cols, ParamOut dw,
                                                         ParamOut db) {
   griddep_wait();
-  __shared__ float red[256];
-  const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
-  const int j = blockIdx.x * 32 + lane;
-  const int per = (terms + 7) / 8, k0 = g * per, k1 = min(terms, k0 + per);
-  const bool first = j < cols;
-  const ParamOut& out = first ? dw : db;
+  __shared__ float red[8][8];
+  const int lane = threadIdx.x & 7, g = threadIdx.x >> 3;
+  const int j = blockIdx.x * 8 + lane;
+  const int per = (terms + 31) / 32, k0 = g * per, k1 = min(terms, k0 + per);
+  const bool on = j < 2 * cols;
   float s = 0.f;
-  if (j < 2 * cols && out.p != nullptr)
-    for (int k = k0; k < k1; k += 8) {
-      float v[8];
+  for (int k = k0; k < k1; k += 8) {
+    float v[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) v[u] = k + u < k1 ? partials[(int64_t)(k + u) * 2 * cols + j] : 0.f;
+    for (int u = 0; u < 8; ++u) v[u] = on && k + u < k1 ? partials[(int64_t)(k + u) * 2 * cols + j] : 0.f;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) s += v[u];
-    }
-  red[threadIdx.x] = s;
+    for (int u = 0; u < 8; ++u) s += v[u];
+  }
+  s += __shfl_xor_sync(0xffffffffu, s, 8);
+  s += __shfl_xor_sync(0xffffffffu, s, 16);
+  if ((threadIdx.x & 31) < 8) red[threadIdx.x >> 5][lane] = s;
   __syncthreads();
-  if (g == 0 && j < 2 * cols && out.p != nullptr) {
-    for (int w = 1; w < 8; ++w) s += red[w * 32 + lane];
-    param_put(out, first ? j : j - cols, s);
+  if (threadIdx.x < 8 && on) {
+    s = red[0][lane];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) s += red[w][lane];
+    const ParamOut& out = j < cols ? dw : db;
+    if (out.p != nullptr) param_put(out, j < cols ? j : j - cols, s);
   }
 }
 
-constexpr int kMaxCtasPerSm = 8;
+constexpr int kMaxCtasPerSm = 8;  // each leaves a term of the parameter gradients
 
 struct BwdLaunch {
   const NormArgs& a;
   const NormGrads& g;
   float* partials;
   cudaStream_t stream;
+  // The team for rows of `cols` elements.  vec: eight elements at a time are possible.  Sixteen elements a thread in narrow
+  // rows, where the sums over a team and what is done once a row weigh most (66049 rows of 96 fp32 channels: 15.9 us, 18.3
+  // with eight); eight from 512 to 1024 columns (4099 rows of 1024 from codes: 12.5 us, 21.7 with sixteen, 16.4 with a warp
+  // a row).
+  template <typename T>
+  int by_width(int cols, bool vec) const {
+    if (vec) {
+      if (cols <= 32) return run<T, Team<8, 4, 1>>();
+      if (cols <= 64) return run<T, Team<8, 4, 2>>();
+      if (cols <= 128) return run<T, Team<8, 8, 2>>();
+      if (cols <= 256) return run<T, Team<8, 16, 2>>();
+      if (cols <= 512) return run<T, Team<8, 32, 2>>();
+      if (cols <= 1024) return run<T, Team<8, 0, 1, 128>>();
+      if (cols <= 4096) return run<T, Team<8, 0, 2, 256>>();
+      return run<T, Team<8, 0, 4, 256>>();
+    }
+    if (cols <= 128) return run<T, Team<1, 32, 4>>();
+    if (cols <= 256) return run<T, Team<1, 32, 8>>();
+    if (cols <= 2048) return run<T, Team<1, 0, 8, 256>>();
+    if (cols <= 4096) return run<T, Team<1, 0, 8, 512>>();
+    return run<T, Team<1, 0, 16, 512>>();
+  }
   template <typename T, class Tm>
   int run() const {
-    constexpr int ROWS = rows_in_flight<Tm>();
+    return a.codes != nullptr ? go<T, Tm, true>() : go<T, Tm, false>();
+  }
+  template <typename T, class Tm, bool CODES>
+  int go() const {
+    constexpr int ROWS = rows_in_flight<T, Tm, true>();
+    static PerDeviceInt regs;
+    const auto kern = norm_bwd_kernel<T, Tm, ROWS, CODES>;
+    const int threads = Tm::threads(a.cols);
+    int fit = 1;
+    if (int rc = resident_ctas(kern, threads, regs, &fit)) return rc;
     const int64_t want = (a.rows + Tm::TEAMS * ROWS - 1) / (Tm::TEAMS * ROWS);
-    const int64_t most = (int64_t)sm_count() * (Tm::BLOCK >= 512 ? 2 : Tm::BLOCK >= 256 ? 3 : kMaxCtasPerSm);
+    const int64_t most = (int64_t)(fit < kMaxCtasPerSm ? fit : kMaxCtasPerSm) * sm_count();
     const int blocks = (int)(want < most ? want : most);
-    const T* dy = static_cast<const T*>(g.dy);
-    T* dx = static_cast<T*>(g.dx);
-    if (a.codes != nullptr)
-      launch_kernel(norm_bwd_kernel<T, Tm, ROWS, true>, dim3(blocks), dim3(Tm::BLOCK), 0, stream, a, dy, dx, partials);
-    else
-      launch_kernel(norm_bwd_kernel<T, Tm, ROWS, false>, dim3(blocks), dim3(Tm::BLOCK), 0, stream, a, dy, dx, partials);
+    launch_kernel(kern, dim3(blocks), dim3(threads), 0, stream, a, static_cast<const T*>(g.dy), static_cast<T*>(g.dx), partials);
     TPF_LAUNCH_OK();
     if (partials == nullptr) return TPF_OK;
-    launch_kernel(norm_fold_kernel, dim3((2 * a.cols + 31) / 32), dim3(256), 0, stream, partials, blocks, a.cols,
+    launch_kernel(norm_fold_kernel, dim3((2 * a.cols + 7) / 8), dim3(256), 0, stream, partials, blocks, a.cols,
                   ParamOut{g.dweight, g.dweight_type}, ParamOut{g.dbias, g.dbias_type});
     TPF_LAUNCH_OK();
     return TPF_OK;
@@ -212,7 +283,7 @@ int layer_norm_bwd(const NormCall& c, const NormGrads& g, void* workspace, int64
   TPF_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 3) == 0, TPF_ERR_INVALID_ARGUMENT,
               "layer_norm_bwd: misaligned workspace");
   const bool from_codes = c.codes != nullptr;
-  const bool vec = c.cols % 8 == 0 && (from_codes ? (reinterpret_cast<uintptr_t>(c.codes) & 7) == 0
+  const bool vec = c.cols % 8 == 0 && (from_codes ? (reinterpret_cast<uintptr_t>(c.codes) & 15) == 0
                                                   : rows_vec_ok(c.x, c.x_pitch, c.type)) &&
                    vec_ok(g.dy, c.type) && (g.dx == nullptr || vec_ok(g.dx, c.type));
   return by_type(BwdLaunch{a, g, params ? static_cast<float*>(workspace) : nullptr, stream}, c.type, a.cols, vec);

@@ -21,11 +21,25 @@ __global__ void __launch_bounds__(256) renorm_kernel(const NormArgs a, bf16* __r
   const int64_t row = i / per_row.d;
   const int c = (int)(i - row * per_row.d) * 8;
   float x[8];
-  if constexpr (CODES) load_codes<8>(a.codes + row * a.cols + c, a.scales[row * a.groups + c / kGroup], x);
-  else load_vec<bf16, 8>(static_cast<const bf16*>(a.x) + row * a.x_pitch + c, x);
-  const float mean = a.mean[row], rstd = a.rstd[row];
+  if constexpr (CODES) {
+    const uint2 u = *reinterpret_cast<const uint2*>(a.codes + row * a.code_pitch + c);
+    uint64_t p[4];
+    unpack_codes(u.x, p);
+    unpack_codes(u.y, p + 2);
+    const float down = a.scales[row * a.groups + c / kGroup];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = (x[e] - mean) * rstd * param_at(a.w, c + e, 1.f) + param_at(a.b, c + e, 0.f);
+    for (int e = 0; e < 4; ++e) f2_unpack(f2_mul(p[e], f2_dup(down)), x[2 * e], x[2 * e + 1]);
+  } else {
+    Piece<bf16, 8> raw;
+    raw.load(static_cast<const bf16*>(a.x) + row * a.x_pitch + c);
+    raw.get(x);
+  }
+  const float mean = a.mean[row], rstd = a.rstd[row];
+  float w[8], b[8];
+  param_load<8, 1>(a.w, c, a.cols, 1.f, w);
+  param_load<8, 1>(a.b, c, a.cols, 0.f, b);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = (x[e] - mean) * rstd * w[e] + b[e];
   store_vec<bf16, 8>(y + row * a.cols + c, x);
 }
 
@@ -62,8 +76,7 @@ int check_linear(const NormCall& c, const void* w, int64_t outs, const char* who
   TPF_REQUIRE(w != nullptr, TPF_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
   TPF_REQUIRE_ALIGNED16(w, who, "weight");
   TPF_REQUIRE(rows_vec_ok(c.x, c.x_pitch, c.type), TPF_ERR_INVALID_ARGUMENT, "%s: x must have 16-byte aligned rows", who);
-  TPF_REQUIRE((reinterpret_cast<uintptr_t>(c.codes) & 7) == 0, TPF_ERR_INVALID_ARGUMENT, "%s: codes must be 8-byte aligned",
-              who);
+  TPF_REQUIRE_ALIGNED16(c.codes, who, "codes");
   return TPF_OK;
 }
 

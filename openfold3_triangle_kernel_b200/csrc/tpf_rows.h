@@ -6,12 +6,15 @@
 
 namespace tpf {
 
+// Codes of a layer norm: rows start on 16-byte boundaries.
+inline int64_t code_pitch(int64_t cols) { return (cols + 15) / 16 * 16; }
+
 struct NormCall {
   int64_t rows, cols;
   int type;               // of x, y, dy and dx: RowType
   const void* x;          // [rows, cols], row pitch x_pitch elements; may be nullptr in a backward pass from codes
   int64_t x_pitch;
-  void* codes;            // int8 [rows, cols], or nullptr
+  void* codes;            // int8 [rows, code_pitch(cols)], or nullptr
   float* scales;          // [rows, ceil(cols / 128)]
   float *mean, *rstd;     // [rows]; may be nullptr in a forward that keeps nothing
   const void *weight, *bias;  // [cols] or nullptr

@@ -79,7 +79,8 @@ tpf::NormCall norm_call(const Rows& x, const Tensor& w, const Tensor& b) {
   return c;
 }
 
-// What a forward keeps beside or in place of x: mean and rstd [2, rows]; codes [rows, cols] and scales [rows, groups].
+// What a forward keeps beside or in place of x: mean and rstd [2, rows]; codes [rows, code_pitch(cols)] and scales
+// [rows, groups].
 struct Kept {
   Tensor stats, codes, scales;
 };
@@ -90,7 +91,7 @@ Kept make_kept(tpf::NormCall& c, const Tensor& like, bool save, bool int8) {
   c.mean = fptr(k.stats);
   c.rstd = c.mean + c.rows;
   if (int8) {
-    k.codes = at::empty({c.rows, c.cols}, like.options().dtype(at::kChar));
+    k.codes = at::empty({c.rows, tpf::code_pitch(c.cols)}, like.options().dtype(at::kChar));
     k.scales = empty_f32({c.rows, (c.cols + 127) / 128}, like);
     c.codes = k.codes.data_ptr();
     c.scales = fptr(k.scales);

@@ -86,7 +86,7 @@ def kept_like(x, int8):
     cols = x.shape[-1]
     rows = math.prod(x.shape[:-1])
     return [x.new_empty((2, rows), dtype=torch.float32),
-            x.new_empty((rows, cols) if int8 else (0,), dtype=torch.int8),
+            x.new_empty((rows, -(-cols // 16) * 16) if int8 else (0,), dtype=torch.int8),
             x.new_empty((rows, -(-cols // 128)) if int8 else (0,), dtype=torch.float32)]
 
 
