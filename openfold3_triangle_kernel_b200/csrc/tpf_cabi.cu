@@ -44,6 +44,8 @@ int attn_bwd_static_scratch(const void* q, const void* k, const void* v, const v
                             int64_t O, int64_t H, int64_t N, int64_t D, float scale, cudaStream_t stream);
 int pair_attn_status_fetch_and_clear(int* out);
 int selftest_status_fetch_and_clear(int* out);
+int norm_linear_dw_status_fetch_and_clear(int* out);
+int norm_linear_bwd_status_fetch_and_clear(int* out);
 int selftest_bounded_wait(unsigned int* report, cudaStream_t stream);
 
 int trimul_status_fetch_and_clear(int* out);
@@ -89,6 +91,10 @@ int tpf_device_status(int* status) {
   if ((rc = tpf::trimul_fwd_status_fetch_and_clear(&v))) return rc;
   total |= v;
   if ((rc = tpf::pair_attn_status_fetch_and_clear(&v))) return rc;
+  total |= v;
+  if ((rc = tpf::norm_linear_dw_status_fetch_and_clear(&v))) return rc;
+  total |= v;
+  if ((rc = tpf::norm_linear_bwd_status_fetch_and_clear(&v))) return rc;
   total |= v;
   if ((rc = tpf::selftest_status_fetch_and_clear(&v))) return rc;
   total |= v;

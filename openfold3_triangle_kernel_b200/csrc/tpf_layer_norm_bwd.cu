@@ -246,14 +246,19 @@ struct BwdLaunch {
     launch_kernel(kern, dim3(blocks), dim3(threads), 0, stream, a, static_cast<const T*>(g.dy), static_cast<T*>(g.dx), partials);
     TPF_LAUNCH_OK();
     if (partials == nullptr) return TPF_OK;
-    launch_kernel(norm_fold_kernel, dim3((2 * a.cols + 7) / 8), dim3(256), 0, stream, partials, blocks, a.cols,
-                  ParamOut{g.dweight, g.dweight_type}, ParamOut{g.dbias, g.dbias_type});
-    TPF_LAUNCH_OK();
-    return TPF_OK;
+    return norm_fold(partials, blocks, a.cols, g.dweight, g.dweight_type, g.dbias, g.dbias_type, stream);
   }
 };
 
 }  // namespace
+
+int norm_fold(const float* terms, int count, int cols, void* dweight, int dweight_type, void* dbias, int dbias_type,
+              cudaStream_t stream) {
+  launch_kernel(norm_fold_kernel, dim3((2 * cols + 7) / 8), dim3(256), 0, stream, terms, count, cols,
+                ParamOut{dweight, dweight_type}, ParamOut{dbias, dbias_type});
+  TPF_LAUNCH_OK();
+  return TPF_OK;
+}
 
 int64_t layer_norm_bwd_workspace_bytes(int64_t rows, int64_t cols) {
   const int64_t most = (int64_t)sm_count() * kMaxCtasPerSm;

@@ -2,7 +2,7 @@
 //
 //   forward    y = w xh + b (bf16), out = y W^T
 //   backward   dy = d_out W (bf16), the layer norm's backward on it, dW = d_out^T y~ with y~ from what was kept of x
-#include "tpf_layer_norm.cuh"
+#include "tpf_norm_linear.cuh"
 
 namespace tpf {
 
@@ -12,59 +12,7 @@ int bmm_bf16(const void* A, int64_t lda, int64_t bsa, int a_mn, const void* B, i
 
 namespace {
 
-// y~ = w (x - mean) rstd + b in bf16, x from the codes or as it was: eight elements a thread.
-template <bool CODES>
-__global__ void __launch_bounds__(256) renorm_kernel(const NormArgs a, bf16* __restrict__ y, FastDiv per_row, int64_t pieces) {
-  griddep_wait();
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= pieces) return;
-  const int64_t row = i / per_row.d;
-  const int c = (int)(i - row * per_row.d) * 8;
-  float x[8];
-  if constexpr (CODES) {
-    const uint2 u = *reinterpret_cast<const uint2*>(a.codes + row * a.code_pitch + c);
-    uint64_t p[4];
-    unpack_codes(u.x, p);
-    unpack_codes(u.y, p + 2);
-    const float down = a.scales[row * a.groups + c / kGroup];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) f2_unpack(f2_mul(p[e], f2_dup(down)), x[2 * e], x[2 * e + 1]);
-  } else {
-    Piece<bf16, 8> raw;
-    raw.load(static_cast<const bf16*>(a.x) + row * a.x_pitch + c);
-    raw.get(x);
-  }
-  const float mean = a.mean[row], rstd = a.rstd[row];
-  float w[8], b[8];
-  param_load<8, 1>(a.w, c, a.cols, 1.f, w);
-  param_load<8, 1>(a.b, c, a.cols, 0.f, b);
-#pragma unroll
-  for (int e = 0; e < 8; ++e) x[e] = (x[e] - mean) * rstd * w[e] + b[e];
-  store_vec<bf16, 8>(y + row * a.cols + c, x);
-}
-
-__global__ void __launch_bounds__(256) split_fold_kernel(const float* __restrict__ part, int splits, int64_t n, ParamOut out) {
-  griddep_wait();
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  float s = 0.f;
-  for (int k = 0; k < splits; ++k) s += part[k * n + i];
-  param_put(out, i, s);
-}
-
 int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
-
-struct Splits {
-  int64_t count, rows;
-};
-Splits dw_splits(int64_t rows, int64_t cols, int64_t outs) {
-  const int64_t tiles = ((outs + 127) / 128) * ((cols + 127) / 128);
-  int64_t want = (2 * sm_count() + tiles - 1) / tiles;
-  int64_t per = (rows + want - 1) / want;
-  per = (per + 63) / 64 * 64;
-  if (per < 256) per = 256;
-  return {(rows + per - 1) / per, per};
-}
 
 // What both passes ask of their arguments.  x (or its codes) is read eight elements at a time.
 int check_linear(const NormCall& c, const void* w, int64_t outs, const char* who) {
@@ -76,6 +24,7 @@ int check_linear(const NormCall& c, const void* w, int64_t outs, const char* who
   TPF_REQUIRE(w != nullptr, TPF_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
   TPF_REQUIRE_ALIGNED16(w, who, "weight");
   TPF_REQUIRE(rows_vec_ok(c.x, c.x_pitch, c.type), TPF_ERR_INVALID_ARGUMENT, "%s: x must have 16-byte aligned rows", who);
+  TPF_REQUIRE(c.x == nullptr || c.x_pitch >= c.cols, TPF_ERR_INVALID_ARGUMENT, "%s: rows overlap", who);
   TPF_REQUIRE_ALIGNED16(c.codes, who, "codes");
   return TPF_OK;
 }
@@ -101,9 +50,9 @@ int norm_linear_fwd(const NormCall& norm, const void* w, int64_t outs, void* out
 }
 
 int64_t norm_linear_bwd_workspace_bytes(int64_t rows, int64_t cols, int64_t outs) {
-  const Splits s = dw_splits(rows, cols, outs);
-  return up256(rows * cols * 2) + up256(layer_norm_bwd_workspace_bytes(rows, cols)) + up256(rows * cols * 2) +
-         up256(s.count * outs * cols * 4);
+  if (norm_linear_narrow(cols, outs)) return norm_linear_narrow_bwd_workspace_bytes(rows, cols, outs);
+  return up256(rows * cols * 2) + up256(layer_norm_bwd_workspace_bytes(rows, cols)) +
+         up256(norm_linear_dw_workspace_bytes(rows, cols, outs));
 }
 
 int norm_linear_bwd(const NormCall& norm, const void* w, int64_t outs, const NormLinearGrads& g, void* workspace,
@@ -122,11 +71,15 @@ int norm_linear_bwd(const NormCall& norm, const void* w, int64_t outs, const Nor
   TPF_REQUIRE_ALIGNED16(workspace, who, "workspace");
   const int64_t R = norm.rows, C = norm.cols;
   char* base = static_cast<char*>(workspace);
+  NormArgs a;
+  if (int rc = make_norm_args(&a, norm, who)) return rc;
+  TPF_REQUIRE((g.dweight == nullptr || row_type_ok(g.dweight_type)) && (g.dbias == nullptr || row_type_ok(g.dbias_type)),
+              TPF_ERR_INVALID_ARGUMENT, "%s: unknown parameter type", who);
+  if (R > 0 && norm_linear_narrow(C, outs)) return norm_linear_narrow_bwd(a, w, outs, g, workspace, stream);
   const int64_t ln_bytes = layer_norm_bwd_workspace_bytes(R, C);
   void* dy = base;
   void* ln_ws = base + up256(R * C * 2);
-  void* y = base + up256(R * C * 2) + up256(ln_bytes);
-  float* part = reinterpret_cast<float*>(static_cast<char*>(y) + up256(R * C * 2));
+  void* dw_ws = base + up256(R * C * 2) + up256(ln_bytes);
   if (g.dx != nullptr || g.dweight != nullptr || g.dbias != nullptr) {
     if (R > 0)
       if (int rc = bmm_bf16(g.d_out, outs, 0, 0, w, C, 0, 1, dy, C, 0, 0, R, C, outs, 1, 0, 128, stream)) return rc;
@@ -138,26 +91,7 @@ int norm_linear_bwd(const NormCall& norm, const void* w, int64_t outs, const Nor
     TPF_CUDA_OK(cudaMemsetAsync(g.dw, 0, outs * C * row_type_size(g.dw_type), stream));
     return TPF_OK;
   }
-  NormArgs a;
-  if (int rc = make_norm_args(&a, norm, who)) return rc;
-  const int64_t pieces = R * (C / 8);
-  const FastDiv per_row = FastDiv::make((uint32_t)(C / 8));
-  TPF_REQUIRE(pieces / 256 < (1ll << 31) - 1, TPF_ERR_UNSUPPORTED, "%s: extent too large", who);
-  const dim3 grid((unsigned)((pieces + 255) / 256));
-  if (norm.codes != nullptr)
-    launch_kernel(renorm_kernel<true>, grid, dim3(256), 0, stream, a, static_cast<bf16*>(y), per_row, pieces);
-  else
-    launch_kernel(renorm_kernel<false>, grid, dim3(256), 0, stream, a, static_cast<bf16*>(y), per_row, pieces);
-  TPF_LAUNCH_OK();
-  const Splits s = dw_splits(R, C, outs);
-  if (int rc = bmm_bf16(g.d_out, outs, 0, 1, y, C, 0, 1, part, C, outs * C, 1, outs, C, R, s.count, s.rows, 128, stream))
-    return rc;
-  const int64_t n = outs * C;
-  TPF_REQUIRE(n / 256 < (1ll << 31) - 1, TPF_ERR_UNSUPPORTED, "%s: extent too large", who);
-  launch_kernel(split_fold_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, part, (int)s.count, n,
-                ParamOut{g.dw, g.dw_type});
-  TPF_LAUNCH_OK();
-  return TPF_OK;
+  return norm_linear_dw(a, g.d_out, outs, g.dw, g.dw_type, dw_ws, stream);
 }
 
 }  // namespace tpf

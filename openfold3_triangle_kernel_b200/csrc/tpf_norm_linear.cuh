@@ -1,0 +1,19 @@
+// The parts of the normalised projection (tpf_norm_linear.cu).
+#pragma once
+
+#include "tpf_layer_norm.cuh"
+
+namespace tpf {
+
+int64_t norm_linear_dw_workspace_bytes(int64_t rows, int64_t cols, int64_t outs);
+// dw [outs, cols] = d_out^T y~; y~ from norm.codes where they are given, else from norm.x.
+int norm_linear_dw(const NormArgs& norm, const void* d_out, int64_t outs, void* dw, int dw_type, void* workspace,
+                   cudaStream_t stream);
+
+// The backward for narrow rows (tpf_norm_linear_bwd.cu): is it one, scratch, all gradients that g asks for.
+bool norm_linear_narrow(int64_t cols, int64_t outs);
+int64_t norm_linear_narrow_bwd_workspace_bytes(int64_t rows, int64_t cols, int64_t outs);
+int norm_linear_narrow_bwd(const NormArgs& norm, const void* w, int64_t outs, const NormLinearGrads& g, void* workspace,
+                           cudaStream_t stream);
+
+}  // namespace tpf

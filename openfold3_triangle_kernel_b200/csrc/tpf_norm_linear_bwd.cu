@@ -1,0 +1,637 @@
+// Backward of the normalised projection for narrow rows (up to 128 columns, a weight that stays in shared memory), in one
+// kernel that reads d_out from memory once.
+//
+//   dx: dy = d_out W, then the layer norm's backward on the rows of dy while they are in TMEM
+//   G = d_out^T xh~ and s = d_out^T 1, from what was kept of x
+//
+// The parameters' gradients all follow from G and s:
+//   dW = G diag(w) + s b^T,   dw_c = sum_r dy_rc xh~_rc = sum_o W_oc G_oc,   db_c = sum_r dy_rc = sum_o W_oc s_o,
+// so that nothing is summed over the rows of dy.  xh~ is rounded to bf16 for the tensor cores, sums are fp32.
+//
+// Both products need the same d_out, one as rows and one as columns, and neither fits beside the other: G takes the whole
+// of TMEM, W most of shared memory.  So CTAs of the two kinds work side by side through the same ranges of rows, and what
+// one of them brought from memory the others find in L2.  A range has `tiles` CTAs for G (256 outputs each, or 128) and as
+// many for dx (every tiles-th 128 rows).
+#include "tpf_gemm_host.cuh"
+#include "tpf_norm_linear.cuh"
+
+namespace tpf {
+
+namespace {
+
+__device__ int g_nl_bwd_status;
+
+constexpr int kRows = 64;         // of a stage of G
+constexpr int kWarps = 10;        // TMA, UMMA, eight that work on elements
+constexpr int kChunk = kRows * 128;  // 64 rows of 64 bf16 columns
+constexpr int kSmemMax = 227 * 1024;
+
+struct BwdArgs {
+  NormArgs norm;
+  int64_t rows_per_range;
+  int outs, tiles, g_ctas, dx_ctas;  // of a range (0: not wanted)
+  int w_blocks;    // blocks of 64 outputs
+  int col_blocks;  // blocks of 64 columns: 1 or 2
+  float* g;        // [ranges][outs][cols]
+  float* s;        // [ranges][outs]
+};
+
+// Everything in dynamic shared memory, which then starts on a 1024-byte boundary.
+struct Shared {
+  uint64_t full[8], empty[8], second_full[2], second_empty[2], w_full, done;
+  uint32_t tmem;
+  volatile int abort_flag;
+};
+constexpr int kSharedBytes = 1024;
+static_assert(sizeof(Shared) <= 512, "");  // the other 512 bytes: the norm's weight
+
+// ---- G and s -------------------------------------------------------------------------------------
+template <int MT, bool CODES>
+struct GradConfig {
+  static constexpr int A_BYTES = MT * 2 * kChunk, RAW_BYTES = CODES ? kChunk : 2 * kChunk, STAGE = A_BYTES + RAW_BYTES;
+  static constexpr int B_BYTES = 3 * kChunk;  // up to 128 columns of xh~, a block whose first column is ones
+  static constexpr int FIT = (kSmemMax - kSharedBytes - 2 * B_BYTES) / STAGE, STAGES = FIT > 6 ? 6 : FIT;
+  static constexpr int SMEM = kSharedBytes + 2 * B_BYTES + STAGES * STAGE;
+  static constexpr int TMEM = MT == 2 ? 512 : 256;  // 256 columns a tile: 128 and 16 are used
+};
+
+template <int MT, bool CODES>
+__device__ __forceinline__ void grad_role(uint8_t* smem, Shared* sh, const WaitCtx& wctx, const CUtensorMap& tm_cols,
+                                          const CUtensorMap& tm_x, const BwdArgs& a, int tile, int range) {
+  using Cfg = GradConfig<MT, CODES>;
+  constexpr int STAGES = Cfg::STAGES;
+  uint8_t* b_buf = smem;
+  uint8_t* ring = smem + 2 * Cfg::B_BYTES;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  const int m0 = tile * (MT * 128);
+  const int64_t row_begin = range * a.rows_per_range;
+  const int64_t row_end = min(a.norm.rows, row_begin + a.rows_per_range);
+  const int steps = (int)((row_end - row_begin + kRows - 1) / kRows);
+  const int ones = a.col_blocks;  // block of the ones
+
+  if (warp == 0) {
+    const uint32_t el = elect_one();
+    int s = 0;
+    uint32_t ph = 1;
+    for (int k = 0; k < steps; ++k) {
+      warp_wait(&sh->empty[s], ph, wctx);
+      mbar_expect_tx(el, &sh->full[s], Cfg::STAGE);
+      uint8_t* dst = ring + s * Cfg::STAGE;
+      const int row = (int)(row_begin + (int64_t)k * kRows);
+#pragma unroll
+      for (int c = 0; c < MT * 2; ++c) tma_load_3d(el, dst + c * kChunk, &tm_cols, &sh->full[s], m0 + c * 64, row, 0);
+#pragma unroll
+      for (int c = 0; c < (CODES ? 1 : 2); ++c)
+        tma_load_3d(el, dst + Cfg::A_BYTES + c * kChunk, &tm_x, &sh->full[s], c * 64, row, 0);
+      if (++s == STAGES) {
+        s = 0;
+        ph ^= 1;
+      }
+    }
+  } else if (warp == 1) {
+    const uint32_t el = elect_one();
+    const uint32_t idesc = make_idesc_bf16(128, ones * 64 + 16, true, true);
+    const uint64_t a_desc = make_smem_desc(smem_u32(ring), kChunk, 1024, swizzle_mode_for_bytes(128));
+    const uint64_t b_desc = make_smem_desc(smem_u32(b_buf), kChunk, 1024, swizzle_mode_for_bytes(128));
+    const uint32_t tmem = sh->tmem;
+    int s = 0;
+    uint32_t ph = 0;
+    for (int k = 0; k < steps; ++k) {
+      const int b = k & 1;
+      warp_wait2(&sh->full[s], ph, &sh->second_full[b], (k >> 1) & 1, wctx);
+      tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const uint64_t ad = a_desc + ((s * Cfg::STAGE + i * 2 * kChunk) >> 4), bd = b_desc + ((b * Cfg::B_BYTES) >> 4);
+#pragma unroll
+        for (int j = 0; j < kRows / 16; ++j)
+          umma_ss(el, tmem + i * 256, ad + j * (16 * 128 >> 4), bd + j * (16 * 128 >> 4), idesc, (k | j) != 0 ? 1u : 0u);
+      }
+      umma_commit(el, &sh->empty[s]);
+      umma_commit(el, &sh->second_empty[b]);
+      if (++s == STAGES) {
+        s = 0;
+        ph ^= 1;
+      }
+    }
+    umma_commit(el, &sh->done);
+  } else {
+    // A lane makes 16 consecutive columns of a row at a time: 8 lanes a row, two rows a stage.
+    const int w8 = warp - 2, piece = lane & 7, sub = lane >> 3;
+    // the block of ones: its first column is 1, the rest 0, in both buffers and for good
+    for (int i = threadIdx.x - 64; i < 2 * kRows * 8; i += 256) {
+      const int b = i >= kRows * 8, r = (i >> 3) & (kRows - 1), q = i & 7;
+      *reinterpret_cast<uint4*>(b_buf + b * Cfg::B_BYTES + ones * kChunk + r * 128 + ((q ^ (r & 7)) << 4)) =
+          make_uint4(q == 0 ? 0x3f80u : 0u, 0u, 0u, 0u);
+    }
+    const bool mine = piece < 4 * ones;  // (64 columns or fewer: the lanes of the second block have nothing to write)
+    float mean[2], rstd[2], down[2];
+    auto stats = [&](int k) {  // of the rows, one stage ahead
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const int64_t row = min(row_begin + (int64_t)k * kRows + w8 * 8 + p * 4 + sub, a.norm.rows - 1);
+        mean[p] = a.norm.mean[row];
+        rstd[p] = a.norm.rstd[row];
+        down[p] = CODES ? a.norm.scales[row] : 1.f;
+      }
+    };
+    stats(0);
+    int s = 0;
+    uint32_t ph = 0;
+    for (int k = 0; k < steps; ++k) {
+      const int b = k & 1;
+      uint64_t f2[2], m2[2];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        f2[p] = f2_dup(CODES ? down[p] * rstd[p] : rstd[p]);
+        m2[p] = f2_dup(CODES ? -mean[p] * rstd[p] : -mean[p]);
+      }
+      if (k + 1 < steps) stats(k + 1);
+      warp_wait2(&sh->full[s], ph, &sh->second_empty[b], ((k >> 1) & 1) ^ 1, wctx);
+      const uint8_t* raw = ring + s * Cfg::STAGE + Cfg::A_BYTES;
+      uint8_t* dst = b_buf + b * Cfg::B_BYTES + (piece >> 2) * kChunk;
+      uint4 u[2][CODES ? 1 : 2];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const int r = w8 * 8 + p * 4 + sub;
+        if constexpr (CODES) {
+          u[p][0] = *reinterpret_cast<const uint4*>(raw + r * 128 + piece * 16);
+        } else {
+          const uint4* src = reinterpret_cast<const uint4*>(raw + (piece >> 2) * kChunk + r * 128 + (piece & 3) * 32);
+          u[p][0] = src[0];
+          u[p][1] = src[1];
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const int r = w8 * 8 + p * 4 + sub;
+        uint64_t x[8];
+        if constexpr (CODES) {
+          unpack_codes(u[p][0].x, x);
+          unpack_codes(u[p][0].y, x + 2);
+          unpack_codes(u[p][0].z, x + 4);
+          unpack_codes(u[p][0].w, x + 6);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = f2_fma(x[e], f2[p], m2[p]);
+        } else {
+          const uint32_t v[8] = {u[p][0].x, u[p][0].y, u[p][0].z, u[p][0].w, u[p][1].x, u[p][1].y, u[p][1].z, u[p][1].w};
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            x[e] = f2_mul(f2_add(f2_pack_bits(v[e] << 16, v[e] & 0xffff0000u), m2[p]), f2[p]);
+        }
+        uint32_t o[8];
+        const bool live = row_begin + (int64_t)k * kRows + r < row_end;  // (where d_out is zero: a NaN must not meet it)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float lo, hi;
+          f2_unpack(x[e], lo, hi);
+          o[e] = live ? pack_bf16x2(lo, hi) : 0u;
+        }
+        uint8_t* row = dst + r * 128;
+        const int q = (piece & 3) * 2, sw = r & 7;
+        if (mine) {
+          *reinterpret_cast<uint4*>(row + ((q ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(row + (((q + 1) ^ sw) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+        }
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&sh->second_full[b]);
+        mbar_arrive(&sh->empty[s]);
+      }
+      if (++s == STAGES) {
+        s = 0;
+        ph ^= 1;
+      }
+    }
+    // the sums: two warps a lane quarter, a tile each or half the columns
+    warp_wait(&sh->done, 0, wctx);
+    tc_fence_after();
+    const int quarter = warp & 3, half = w8 >> 2;
+    const int o = m0 + (MT == 2 ? half * 128 : 0) + quarter * 32 + lane;
+    const uint32_t t = tmem_addr(sh->tmem, quarter * 32, MT == 2 ? half * 256 : 0);
+    float* g = a.g + ((int64_t)range * a.outs + o) * a.norm.cols;
+#pragma unroll 1
+    for (int c = MT == 2 ? 0 : half * 32; c < a.norm.cols; c += MT == 2 ? 32 : 64) {
+      uint32_t v[32];
+      tmem_ld32(t + c, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int e = 0; e < 32; e += 4)
+        if (o < a.outs && c + e < a.norm.cols)
+          *reinterpret_cast<uint4*>(g + c + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+      __syncwarp();
+    }
+    if (MT == 2 || half == 0) {
+      uint32_t v[8];
+      tmem_ld8(t + ones * 64, v);
+      tmem_ld_wait();
+      if (o < a.outs) a.s[(int64_t)range * a.outs + o] = __uint_as_float(v[0]);
+    }
+  }
+}
+
+// ---- dx ------------------------------------------------------------------------------------------
+constexpr int kWBytes = 128 * 1024;      // most of the weight
+constexpr int kATile = 128 * 128;        // 128 rows of 64 outputs
+constexpr int kDxStages = 5;
+constexpr int kDxSmem = kSharedBytes + kWBytes + kDxStages * kATile + 8 * 2048;
+static_assert(kDxSmem <= kSmemMax, "");
+
+// Columns 64 h .. 64 h + 63 of 128 rows (32 h .. where a row has 64 at most): a thread has a row's part of them.
+template <bool CODES>
+struct KeptRow {
+  uint4 u[CODES ? 4 : 8];
+  float mean, rstd, down;
+  __device__ __forceinline__ void load(const NormArgs& n, int64_t row, int c0, int width) {
+    const int64_t r = row < n.rows ? row : n.rows - 1;
+    mean = n.mean[r];
+    rstd = n.rstd[r];
+    down = CODES ? n.scales[r] : 1.f;
+#pragma unroll
+    for (int i = 0; i < (CODES ? 4 : 8); ++i) {
+      const int c = c0 + i * (CODES ? 16 : 8);
+      const bool in = i * (CODES ? 16 : 8) < width && c < n.cols;  // (codes: rows have room up to a multiple of 16)
+      if constexpr (CODES) u[i] = in ? *reinterpret_cast<const uint4*>(n.codes + r * n.code_pitch + c) : make_uint4(0u, 0u, 0u, 0u);
+      else
+        u[i] = in ? *reinterpret_cast<const uint4*>(static_cast<const bf16*>(n.x) + r * n.x_pitch + c)
+                  : make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+  // xh of the pairs 8 i .. 8 i + 7 (sixteen columns)
+  __device__ __forceinline__ void get(int i, uint64_t f, uint64_t m, uint64_t (&x)[8]) const {
+    if constexpr (CODES) {
+      unpack_codes(u[i].x, x);
+      unpack_codes(u[i].y, x + 2);
+      unpack_codes(u[i].z, x + 4);
+      unpack_codes(u[i].w, x + 6);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = f2_fma(x[e], f, m);
+    } else {
+      const uint32_t v[8] = {u[2 * i].x, u[2 * i].y, u[2 * i].z, u[2 * i].w,
+                             u[2 * i + 1].x, u[2 * i + 1].y, u[2 * i + 1].z, u[2 * i + 1].w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = f2_mul(f2_add(f2_pack_bits(v[e] << 16, v[e] & 0xffff0000u), m), f);
+    }
+  }
+};
+
+template <bool CODES>
+__device__ __forceinline__ void dx_role(uint8_t* smem, Shared* sh, const WaitCtx& wctx, const CUtensorMap& tm_rows,
+                                        const CUtensorMap& tm_w, const CUtensorMap& tm_dx, const BwdArgs& a, int part,
+                                        int range) {
+  uint8_t* w_buf = smem;
+  uint8_t* ring = smem + kWBytes;
+  uint8_t* staging = ring + kDxStages * kATile;
+  float* w_norm = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(sh) + 512);
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  const int64_t range_begin = range * a.rows_per_range;
+  const int64_t range_end = min(a.norm.rows, range_begin + a.rows_per_range);
+  const int64_t row_begin = range_begin + part * 128;
+  const int64_t row_step = a.dx_ctas * 128;
+  const int tiles = row_begin < range_end ? (int)((range_end - row_begin + row_step - 1) / row_step) : 0;
+  const int kb = a.w_blocks, cb = a.col_blocks;
+
+  if (warp == 0) {
+    const uint32_t el = elect_one();
+    mbar_expect_tx(el, &sh->w_full, kb * cb * kChunk);
+    for (int k = 0; k < kb; ++k)
+      for (int c = 0; c < cb; ++c)
+        tma_load_3d(el, w_buf + (k * cb + c) * kChunk, &tm_w, &sh->w_full, c * 64, k * 64, 0);
+    int s = 0;
+    uint32_t ph = 1;
+    for (int t = 0; t < tiles; ++t) {
+      const int row = (int)(row_begin + t * row_step);
+      for (int k = 0; k < kb; ++k) {
+        warp_wait(&sh->empty[s], ph, wctx);
+        mbar_expect_tx(el, &sh->full[s], kATile);
+        tma_load_3d(el, ring + s * kATile, &tm_rows, &sh->full[s], k * 64, row, 0);
+        if (++s == kDxStages) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    const uint32_t el = elect_one();
+    const uint32_t idesc = make_idesc_bf16(128, (a.norm.cols + 31) / 32 * 32, false, true);
+    const uint64_t a_desc = make_smem_desc(smem_u32(ring), 16, 1024, swizzle_mode_for_bytes(128));
+    const uint64_t b_desc = make_smem_desc(smem_u32(w_buf), kChunk, 1024, swizzle_mode_for_bytes(128));
+    const uint32_t tmem = sh->tmem;
+    warp_wait(&sh->w_full, 0, wctx);
+    int s = 0;
+    uint32_t ph = 0;
+    for (int t = 0; t < tiles; ++t) {
+      const int acc = t & 1;
+      warp_wait(&sh->second_empty[acc], ((t >> 1) & 1) ^ 1, wctx);
+      tc_fence_after();
+      for (int k = 0; k < kb; ++k) {
+        warp_wait(&sh->full[s], ph, wctx);
+        tc_fence_after();
+        const uint64_t ad = a_desc + ((s * kATile) >> 4), bd = b_desc + ((k * cb * kChunk) >> 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          umma_ss(el, tmem + acc * 128, ad + j * 2, bd + j * (16 * 128 >> 4), idesc, (k | j) != 0 ? 1u : 0u);
+        umma_commit(el, &sh->empty[s]);
+        if (++s == kDxStages) {
+          s = 0;
+          ph ^= 1;
+        }
+      }
+      umma_commit(el, &sh->second_full[acc]);
+    }
+  } else {
+    // Two warps a lane quarter; each has half of the columns of its 32 rows.
+    const int w8 = warp - 2, quarter = warp & 3, half = w8 >> 2;
+    const int width = cb == 2 ? 64 : 32, c0 = half * width;  // columns of a half
+    uint8_t* tile = staging + w8 * 2048;
+    const uint8_t* other = staging + (w8 ^ 4) * 2048;
+    KeptRow<CODES> next;
+    if (tiles > 0) next.load(a.norm, row_begin + quarter * 32 + lane, c0, width);
+    const int blocks = max(0, min(width, a.norm.cols - c0) + 31) / 32;  // of 32 columns that exist: 0, 1 or 2
+    for (int t = 0; t < tiles; ++t) {
+      const int acc = t & 1;
+      const int64_t row0 = row_begin + t * row_step + quarter * 32;
+      const KeptRow<CODES> x = next;
+      if (t + 1 < tiles) next.load(a.norm, row0 + row_step + lane, c0, width);
+      const uint64_t f = f2_dup(CODES ? x.down * x.rstd : x.rstd), m = f2_dup(CODES ? -x.mean * x.rstd : -x.mean);
+      warp_wait(&sh->second_full[acc], (t >> 1) & 1, wctx);
+      tc_fence_after();
+      uint64_t wd[32];
+      {
+        uint32_t v[2][32];
+        const uint32_t at = tmem_addr(sh->tmem, quarter * 32, acc * 128 + c0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (i < blocks) tmem_ld32(at + i * 32, v[i]);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) wd[i * 16 + e] = i < blocks ? f2_pack_bits(v[i][2 * e], v[i][2 * e + 1]) : 0ull;
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->second_empty[acc]);
+      uint64_t s1 = 0, s2 = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i < 2 * blocks) {
+          uint64_t xh[8];
+          x.get(i, f, m, xh);
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            const float4 w = *reinterpret_cast<const float4*>(w_norm + c0 + i * 16 + e * 2);
+            wd[i * 8 + e] = f2_mul(wd[i * 8 + e], f2_pack(w.x, w.y));
+            wd[i * 8 + e + 1] = f2_mul(wd[i * 8 + e + 1], f2_pack(w.z, w.w));
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            s1 = f2_add(s1, wd[i * 8 + e]);
+            s2 = f2_fma(wd[i * 8 + e], xh[e], s2);
+          }
+        }
+      }
+      // the halves' sums meet in the staging tiles, which the last stores have left by now
+      bulk_wait_read<0>();
+      __syncwarp();
+      const float2 own = make_float2(f2_sum(s1), f2_sum(s2));
+      reinterpret_cast<float2*>(tile)[lane] = own;
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+      const float2 far = reinterpret_cast<const float2*>(other)[lane];
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
+      const uint64_t m1 = f2_dup(-(own.x + far.x) * a.norm.inv_cols), mm = f2_dup(-(own.y + far.y) * a.norm.inv_cols);
+      const uint64_t rs = f2_dup(x.rstd);
+      int buf = 0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (i < blocks) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint64_t xh[8];
+            x.get(2 * i + h, f, m, xh);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              float lo, hi;
+              f2_unpack(f2_mul(f2_fma(xh[e], mm, f2_add(wd[i * 16 + h * 8 + e], m1)), rs), lo, hi);
+              pk[h * 8 + e] = pack_bf16x2(lo, hi);
+            }
+          }
+          warp_tile_store_tma<1>(tile, buf, lane, pk, &tm_dx, c0 + i * 32, (int)row0, 0);
+        }
+      }
+    }
+    bulk_wait_all();
+  }
+}
+
+template <int MT, bool CODES>
+__global__ void __launch_bounds__(32 * kWarps, 1)
+    nl_bwd_kernel(const __grid_constant__ CUtensorMap tm_cols, const __grid_constant__ CUtensorMap tm_rows,
+                  const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+                  const __grid_constant__ CUtensorMap tm_dx, const __grid_constant__ BwdArgs a, int* __restrict__ status) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  using Grad = GradConfig<MT, CODES>;
+  const int per = a.g_ctas + a.dx_ctas;
+  const int range = blockIdx.x / per, part = blockIdx.x - range * per;
+  const bool grad = part < a.g_ctas;
+  Shared* sh = reinterpret_cast<Shared*>(smem + (kDxSmem > Grad::SMEM ? kDxSmem : Grad::SMEM) - kSharedBytes);
+  const WaitCtx wctx{&sh->abort_flag, status};
+  const int warp = warp_index();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 8; ++s) {
+      mbar_init(&sh->full[s], 1);
+      mbar_init(&sh->empty[s], grad ? 9 : 1);  // UMMAs; for G the eight warps that read the kept rows too
+    }
+    for (int b = 0; b < 2; ++b) {  // G: the xh~ buffers, dx: the accumulators
+      mbar_init(&sh->second_full[b], grad ? 8 : 1);
+      mbar_init(&sh->second_empty[b], grad ? 1 : 8);
+    }
+    mbar_init(&sh->w_full, 1);
+    mbar_init(&sh->done, 1);
+    sh->abort_flag = 0;
+    mbar_fence_init();
+  }
+  const int tmem_cols = grad ? Grad::TMEM : 256;
+  if (warp == 1) {
+    tmem_alloc(&sh->tmem, tmem_cols);
+    tmem_relinquish();
+  }
+  griddep_wait();
+  if (!grad && threadIdx.x >= 64 && threadIdx.x < 192) {
+    float w;
+    param_load<1, 1>(a.norm.w, threadIdx.x - 64, a.norm.cols, 1.f, &w);
+    reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(sh) + 512)[threadIdx.x - 64] = w;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (grad) grad_role<MT, CODES>(smem, sh, wctx, tm_cols, tm_x, a, part, range);
+  else dx_role<CODES>(smem, sh, wctx, tm_rows, tm_w, tm_dx, a, part - a.g_ctas, range);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tmem_dealloc(sh->tmem, tmem_cols);
+  }
+}
+
+// One CTA an output: G_o and s_o over the ranges (in order), then dW_o = w G_o + b s_o and the output's terms
+// terms[o] = (W_o G_o, W_o s_o) of dw and db.  32 lanes hold four columns each, eight warps a part of the ranges.
+__global__ void __launch_bounds__(256) nl_fold_kernel(const BwdArgs a, int ranges, const bf16* __restrict__ w, ParamOut dw,
+                                                      float* __restrict__ terms) {
+  griddep_wait();
+  __shared__ float4 red[8][32];
+  __shared__ float red_s[8];
+  const int lane = threadIdx.x & 31, g = threadIdx.x >> 5, o = blockIdx.x, cols = a.norm.cols;
+  const int per = (ranges + 7) / 8, k0 = g * per, k1 = min(ranges, k0 + per);
+  const int c = lane * 4;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  float t = 0.f;
+  for (int k = k0; k < k1; k += 8) {
+    float4 v[8];
+    float q[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int64_t at = (int64_t)(k + u) * a.outs + o;
+      v[u] = c < cols && k + u < k1 ? *reinterpret_cast<const float4*>(a.g + at * cols + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+      q[u] = k + u < k1 ? a.s[at] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      s.x += v[u].x;
+      s.y += v[u].y;
+      s.z += v[u].z;
+      s.w += v[u].w;
+      t += q[u];
+    }
+  }
+  red[g][lane] = s;
+  if (lane == 0) red_s[g] = t;
+  __syncthreads();
+  const int e = threadIdx.x;  // one column
+  if (e >= cols) return;
+  const float* r = reinterpret_cast<const float*>(&red[0][0]) + e;
+  float G = r[0], S = red_s[0];
+#pragma unroll
+  for (int k = 1; k < 8; ++k) {
+    G += r[k * 128];
+    S += red_s[k];
+  }
+  float gamma, beta;
+  param_load<1, 1>(a.norm.w, e, cols, 1.f, &gamma);
+  param_load<1, 1>(a.norm.b, e, cols, 0.f, &beta);
+  if (dw.p != nullptr) param_put(dw, (int64_t)o * cols + e, fmaf(gamma, G, beta * S));
+  if (terms != nullptr) {
+    const float wo = __bfloat162float(w[(int64_t)o * cols + e]);
+    terms[(int64_t)o * 2 * cols + e] = wo * G;
+    terms[(int64_t)o * 2 * cols + cols + e] = wo * S;
+  }
+}
+
+struct Plan {
+  int mt, tiles, ranges, g_ctas, dx_ctas;
+  int64_t rows_per_range;
+};
+Plan make_plan(int64_t rows, int64_t outs, bool want_g, bool want_dx) {
+  Plan p;
+  p.mt = outs > 128 ? 2 : 1;
+  p.tiles = (int)((outs + p.mt * 128 - 1) / (p.mt * 128));
+  p.g_ctas = want_g ? p.tiles : 0;
+  p.dx_ctas = want_dx ? p.tiles : 0;
+  int64_t ranges = sm_count() / (p.g_ctas + p.dx_ctas);
+  const int64_t most = (rows + 255) / 256;  // 256 rows at least: G's sums are written and read once more
+  if (ranges > most) ranges = most;
+  if (ranges < 1) ranges = 1;
+  p.rows_per_range = ((rows + ranges - 1) / ranges + 127) / 128 * 128;
+  p.ranges = (int)((rows + p.rows_per_range - 1) / p.rows_per_range);
+  return p;
+}
+// The most ranges that any choice of gradients takes.
+int64_t most_ranges(int64_t rows, int64_t outs) { return make_plan(rows, outs, true, false).ranges; }
+
+int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
+
+template <int MT, bool CODES>
+int launch_bwd(const BwdArgs& a, const Plan& p, const void* d_out, const void* w, void* dx, cudaStream_t stream) {
+  CUtensorMap tm_cols, tm_rows, tm_x, tm_w, tm_dx;
+  const int64_t R = a.norm.rows, C = a.norm.cols, O = a.outs;
+  if (int rc = make_operand_tmap(&tm_cols, d_out, true, O, R, O, 1, 0, 128, 64, kRows)) return rc;
+  if (int rc = make_operand_tmap(&tm_rows, d_out, false, R, O, O, 1, 0, 128, 128, 64)) return rc;
+  if (int rc = make_operand_tmap(&tm_w, w, true, C, O, C, 1, 0, 128, 64, 64)) return rc;
+  if constexpr (CODES) {
+    const uint64_t dims[3] = {(uint64_t)a.norm.code_pitch, (uint64_t)R, 1};
+    const uint64_t strides[2] = {(uint64_t)a.norm.code_pitch, 16};
+    const uint32_t box[3] = {128, (uint32_t)kRows, 1};
+    if (int rc = make_tmap(&tm_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.norm.codes, 3, dims, strides, box, 0)) return rc;
+  } else {
+    const uint64_t dims[3] = {(uint64_t)C, (uint64_t)R, 1};
+    const uint64_t strides[2] = {(uint64_t)a.norm.x_pitch * 2, 16};
+    const uint32_t box[3] = {64, (uint32_t)kRows, 1};
+    if (int rc = make_tmap_bf16(&tm_x, a.norm.x, 3, dims, strides, box, 0)) return rc;
+  }
+  if (dx != nullptr) {
+    if (int rc = make_store_tmap(&tm_dx, dx, C, R, C, 1, 0)) return rc;
+  } else {
+    tm_dx = tm_w;  // not used
+  }
+  int* status = nullptr;
+  static PerDeviceAddress status_at;
+  if (int rc = device_symbol_address(g_nl_bwd_status, status_at, reinterpret_cast<void**>(&status))) return rc;
+  constexpr int smem = kDxSmem > GradConfig<MT, CODES>::SMEM ? kDxSmem : GradConfig<MT, CODES>::SMEM;
+  static_assert(smem <= kSmemMax, "");
+  const auto kern = nl_bwd_kernel<MT, CODES>;
+  static PerDeviceOnce once;
+  if (int rc = ensure_dynamic_smem(kern, smem, once, 1024)) return rc;
+  launch_kernel(kern, dim3(p.ranges * (p.g_ctas + p.dx_ctas)), dim3(32 * kWarps), smem, stream, tm_cols, tm_rows, tm_x, tm_w,
+                tm_dx, a, status);
+  TPF_LAUNCH_OK();
+  return TPF_OK;
+}
+
+}  // namespace
+
+int norm_linear_bwd_status_fetch_and_clear(int* out) {
+  int v = 0, zero = 0;
+  TPF_CUDA_OK(cudaMemcpyFromSymbol(&v, g_nl_bwd_status, sizeof(int)));
+  if (v) TPF_CUDA_OK(cudaMemcpyToSymbol(g_nl_bwd_status, &zero, sizeof(int)));
+  *out = v;
+  return TPF_OK;
+}
+
+bool norm_linear_narrow(int64_t cols, int64_t outs) {
+  return cols <= 128 && (outs + 63) / 64 * ((cols + 63) / 64) * kChunk <= kWBytes;
+}
+
+int64_t norm_linear_narrow_bwd_workspace_bytes(int64_t rows, int64_t cols, int64_t outs) {
+  const int64_t z = rows > 0 ? most_ranges(rows, outs) : 0;
+  return up256(z * outs * cols * 4) + up256(z * outs * 4) + up256(outs * 2 * cols * 4);
+}
+
+int norm_linear_narrow_bwd(const NormArgs& norm, const void* w, int64_t outs, const NormLinearGrads& g, void* workspace,
+                           cudaStream_t stream) {
+  const int64_t R = norm.rows, C = norm.cols;
+  const bool vectors = g.dweight != nullptr || g.dbias != nullptr, want_g = g.dw != nullptr || vectors;
+  if (!want_g && g.dx == nullptr) return TPF_OK;
+  const Plan p = make_plan(R, outs, want_g, g.dx != nullptr);
+  const int64_t z = most_ranges(R, outs);
+  char* base = static_cast<char*>(workspace);
+  float* terms = reinterpret_cast<float*>(base + up256(z * outs * C * 4) + up256(z * outs * 4));
+  const BwdArgs a{norm, p.rows_per_range, (int)outs, p.tiles, p.g_ctas, p.dx_ctas, (int)((outs + 63) / 64),
+                  (int)((C + 63) / 64), reinterpret_cast<float*>(base), reinterpret_cast<float*>(base + up256(z * outs * C * 4))};
+  const bool codes = norm.codes != nullptr;
+  const int rc = p.mt == 2 ? (codes ? launch_bwd<2, true>(a, p, g.d_out, w, g.dx, stream)
+                                    : launch_bwd<2, false>(a, p, g.d_out, w, g.dx, stream))
+                           : (codes ? launch_bwd<1, true>(a, p, g.d_out, w, g.dx, stream)
+                                    : launch_bwd<1, false>(a, p, g.d_out, w, g.dx, stream));
+  if (rc || !want_g) return rc;
+  launch_kernel(nl_fold_kernel, dim3((unsigned)outs), dim3(256), 0, stream, a, p.ranges, static_cast<const bf16*>(w),
+                ParamOut{g.dw, g.dw_type}, vectors ? terms : nullptr);
+  TPF_LAUNCH_OK();
+  if (!vectors) return TPF_OK;
+  return norm_fold(terms, (int)outs, (int)C, g.dweight, g.dweight_type, g.dbias, g.dbias_type, stream);
+}
+
+}  // namespace tpf

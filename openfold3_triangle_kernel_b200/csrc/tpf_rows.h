@@ -31,6 +31,10 @@ struct NormGrads {
 int64_t layer_norm_bwd_workspace_bytes(int64_t rows, int64_t cols);
 int layer_norm_bwd(const NormCall& c, const NormGrads& g, void* workspace, int64_t workspace_bytes, cudaStream_t stream);
 
+// dweight[c], dbias[c] = sums over terms [count][2][cols]; either may be nullptr
+int norm_fold(const float* terms, int count, int cols, void* dweight, int dweight_type, void* dbias, int dbias_type,
+              cudaStream_t stream);
+
 // x [rows, cols] (pitch in elements) <-> codes int8 [rows, cols], scales fp32 [rows, ceil(cols / 128)]
 int int8_pack(const void* x, int64_t x_pitch, int type, void* codes, float* scales, int64_t rows, int64_t cols,
               cudaStream_t stream);

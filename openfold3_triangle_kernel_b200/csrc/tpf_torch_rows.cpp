@@ -49,7 +49,7 @@ Rows as_rows(const Tensor& t) {
 }
 Rows as_vector_rows(const Tensor& t) {  // bf16 rows that start on 16-byte boundaries
   Rows r = as_rows(t);
-  if (r.pitch % 8 == 0 && (reinterpret_cast<uintptr_t>(r.t.data_ptr()) & 15) == 0) return r;
+  if (r.pitch >= r.cols && r.pitch % 8 == 0 && (reinterpret_cast<uintptr_t>(r.t.data_ptr()) & 15) == 0) return r;
   r.t = t.is_contiguous() ? t.clone() : t.contiguous();
   if (reinterpret_cast<uintptr_t>(r.t.data_ptr()) & 15) r.t = r.t.clone();
   r.pitch = r.cols;

@@ -1,7 +1,10 @@
 """turbo_norm_linear on a B200 against the 64-bit oracle.
 
 Bounds: the normalised rows y and the gradient dy are rounded to bf16 (half a step, 2^-8 of the value) on their way into
-products, an fp32 or fp16 weight likewise; the products' sums are fp32, at most K roundings."""
+products, an fp32 or fp16 weight likewise; the products' sums are fp32, at most K roundings.  The gradients of narrow rows
+come from G = d_out^T xh and s = d_out^T 1: there xh is rounded in the place of y, and the norm's gradients are
+sum_o W_oc G_oc and sum_o W_oc s_o: their first error is sum_r dy_rc (what xh_rc is off by), as before, and the sums over r and
+o are fp32 chains of R + O roundings, relative to the magnitudes |d_out|, |W| and |xh| of their terms."""
 import pytest
 import torch
 
@@ -52,18 +55,25 @@ def _check(i, checkpoint=None, eps=1e-5, x_cuda=None, use=(True, True)):
     dy_off = dy_off + H * (dy.abs() + dy_off)
     back = ro.layer_norm_backward(dy, kept, mean, rstd, nw, dy_off)
     ro.check(g["dx"].reshape(R, Cc), back["dx"], back["dx_off"], "dx")
+    xk = (kept.double() - mean) * rstd
+    A = rstd * (kept.double().abs() + mean.abs() + kept.double().abs().mean(-1, keepdim=True))
+    xk_off = 68 * ro.U * A
+    terms = d.abs() @ W.abs()
+    chain = (R + O + 64) * ro.U
     if use[0]:
-        ro.check(g["dnw"], back["dw"], back["dw_off"], "dnw")
+        ro.check(g["dnw"], back["dw"], back["dw_off"] + chain * (terms * xk.abs()).sum(0), "dnw")
     if use[1]:
-        ro.check(g["dnb"], back["db"], back["db_off"], "dnb")
+        ro.check(g["dnb"], back["db"], back["db_off"] + chain * terms.sum(0), "dnb")
     # the kept rows, normalised again: off as y is, with the kept values in the place of x
     one = torch.ones(Cc, dtype=torch.float64)
     nwd, nbd = (one if nw is None else nw.double()), (0 * one if nb is None else nb.double())
-    yk = (kept.double() - mean) * rstd * nwd + nbd
-    A = rstd * (kept.double().abs() + mean.abs() + kept.double().abs().mean(-1, keepdim=True))
-    yk_off = 68 * ro.U * (A * nwd.abs() + nbd.abs())
-    yk_off = yk_off + H * (yk.abs() + yk_off)
-    dw_off = d.abs().t() @ yk_off + (R + 64) * ro.U * (d.abs().t() @ yk.abs())
+    yk = xk * nwd + nbd
+    if Cc <= 128 and -(-O // 64) * -(-Cc // 64) <= 16:   # (the weight stays in shared memory)
+        yk_off = nwd.abs() * (xk_off + H * (xk.abs() + xk_off))
+    else:
+        yk_off = 68 * ro.U * (A * nwd.abs() + nbd.abs())
+        yk_off = yk_off + H * (yk.abs() + yk_off)
+    dw_off = d.abs().t() @ yk_off + (R + 64) * ro.U * (d.abs().t() @ ((xk * nwd).abs() + nbd.abs()))
     assert g["dw"].dtype == i["w"].dtype
     ro.check(g["dw"], d.t() @ yk, dw_off, "dw")
     assert C.device_status() == 0

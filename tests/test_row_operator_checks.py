@@ -208,3 +208,11 @@ def test_norm_linear_entries_want_workspaces():
     lib = C.load()
     assert lib.tpf_norm_linear_fwd_workspace_bytes(0, 16, 8) == 0
     assert lib.tpf_norm_linear_bwd_workspace_bytes(1000, 16, 8) % 256 == 0
+
+
+def test_norm_linear_entries_without_rows():
+    lib = C.load()
+    before = lib.tpf_launch_count()
+    _nl_fwd(rows=0, x=NULL, out=NULL, ws=NULL, wsb=0)
+    _nl_bwd(rows=0, x=NULL, d_out=NULL, mean=NULL, rstd=NULL, ws=NULL, wsb=0)
+    assert lib.tpf_launch_count() == before
