@@ -22,7 +22,8 @@ namespace {
 __device__ int g_nl_bwd_status;
 
 constexpr int kRows = 64;         // of a stage of G
-constexpr int kWarps = 10;        // TMA, UMMA, eight that work on elements
+constexpr int kWorkers = 16;       // warps that work on elements
+constexpr int kWarps = 2 + kWorkers;  // TMA, UMMA
 constexpr int kChunk = kRows * 128;  // 64 rows of 64 bf16 columns
 constexpr int kSmemMax = 227 * 1024;
 
@@ -116,83 +117,61 @@ __device__ __forceinline__ void grad_role(uint8_t* smem, Shared* sh, const WaitC
     }
     umma_commit(el, &sh->done);
   } else {
-    // A lane makes 16 consecutive columns of a row at a time: 8 lanes a row, two rows a stage.
-    const int w8 = warp - 2, piece = lane & 7, sub = lane >> 3;
+    // A lane makes 16 consecutive columns of a row: 8 lanes a row, 4 rows a warp and stage.
+    const int wk = warp - 2, piece = lane & 7, sub = lane >> 3;
     // the block of ones: its first column is 1, the rest 0, in both buffers and for good
-    for (int i = threadIdx.x - 64; i < 2 * kRows * 8; i += 256) {
+    for (int i = threadIdx.x - 64; i < 2 * kRows * 8; i += 32 * kWorkers) {
       const int b = i >= kRows * 8, r = (i >> 3) & (kRows - 1), q = i & 7;
       *reinterpret_cast<uint4*>(b_buf + b * Cfg::B_BYTES + ones * kChunk + r * 128 + ((q ^ (r & 7)) << 4)) =
           make_uint4(q == 0 ? 0x3f80u : 0u, 0u, 0u, 0u);
     }
     const bool mine = piece < 4 * ones;  // (64 columns or fewer: the lanes of the second block have nothing to write)
-    float mean[2], rstd[2], down[2];
-    auto stats = [&](int k) {  // of the rows, one stage ahead
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const int64_t row = min(row_begin + (int64_t)k * kRows + w8 * 8 + p * 4 + sub, a.norm.rows - 1);
-        mean[p] = a.norm.mean[row];
-        rstd[p] = a.norm.rstd[row];
-        down[p] = CODES ? a.norm.scales[row] : 1.f;
-      }
+    const int r = wk * 4 + sub;
+    float mean, rstd, down;
+    auto stats = [&](int k) {  // of the row, one stage ahead
+      const int64_t row = min(row_begin + (int64_t)k * kRows + r, a.norm.rows - 1);
+      mean = a.norm.mean[row];
+      rstd = a.norm.rstd[row];
+      down = CODES ? a.norm.scales[row] : 1.f;
     };
     stats(0);
     int s = 0;
     uint32_t ph = 0;
     for (int k = 0; k < steps; ++k) {
       const int b = k & 1;
-      uint64_t f2[2], m2[2];
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        f2[p] = f2_dup(CODES ? down[p] * rstd[p] : rstd[p]);
-        m2[p] = f2_dup(CODES ? -mean[p] * rstd[p] : -mean[p]);
-      }
+      const uint64_t f2 = f2_dup(CODES ? down * rstd : rstd), m2 = f2_dup(CODES ? -mean * rstd : -mean);
       if (k + 1 < steps) stats(k + 1);
       warp_wait2(&sh->full[s], ph, &sh->second_empty[b], ((k >> 1) & 1) ^ 1, wctx);
       const uint8_t* raw = ring + s * Cfg::STAGE + Cfg::A_BYTES;
-      uint8_t* dst = b_buf + b * Cfg::B_BYTES + (piece >> 2) * kChunk;
-      uint4 u[2][CODES ? 1 : 2];
+      uint64_t x[8];
+      if constexpr (CODES) {
+        const uint4 u = *reinterpret_cast<const uint4*>(raw + r * 128 + piece * 16);
+        unpack_codes(u.x, x);
+        unpack_codes(u.y, x + 2);
+        unpack_codes(u.z, x + 4);
+        unpack_codes(u.w, x + 6);
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const int r = w8 * 8 + p * 4 + sub;
-        if constexpr (CODES) {
-          u[p][0] = *reinterpret_cast<const uint4*>(raw + r * 128 + piece * 16);
-        } else {
-          const uint4* src = reinterpret_cast<const uint4*>(raw + (piece >> 2) * kChunk + r * 128 + (piece & 3) * 32);
-          u[p][0] = src[0];
-          u[p][1] = src[1];
-        }
+        for (int e = 0; e < 8; ++e) x[e] = f2_fma(x[e], f2, m2);
+      } else {
+        const uint4* src = reinterpret_cast<const uint4*>(raw + (piece >> 2) * kChunk + r * 128 + (piece & 3) * 32);
+        const uint4 u = src[0], w = src[1];
+        const uint32_t v[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = f2_mul(f2_add(f2_pack_bits(v[e] << 16, v[e] & 0xffff0000u), m2), f2);
       }
+      uint32_t o[8];
+      const bool live = row_begin + (int64_t)k * kRows + r < row_end;  // (where d_out is zero: a NaN must not meet it)
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const int r = w8 * 8 + p * 4 + sub;
-        uint64_t x[8];
-        if constexpr (CODES) {
-          unpack_codes(u[p][0].x, x);
-          unpack_codes(u[p][0].y, x + 2);
-          unpack_codes(u[p][0].z, x + 4);
-          unpack_codes(u[p][0].w, x + 6);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = f2_fma(x[e], f2[p], m2[p]);
-        } else {
-          const uint32_t v[8] = {u[p][0].x, u[p][0].y, u[p][0].z, u[p][0].w, u[p][1].x, u[p][1].y, u[p][1].z, u[p][1].w};
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            x[e] = f2_mul(f2_add(f2_pack_bits(v[e] << 16, v[e] & 0xffff0000u), m2[p]), f2[p]);
-        }
-        uint32_t o[8];
-        const bool live = row_begin + (int64_t)k * kRows + r < row_end;  // (where d_out is zero: a NaN must not meet it)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float lo, hi;
-          f2_unpack(x[e], lo, hi);
-          o[e] = live ? pack_bf16x2(lo, hi) : 0u;
-        }
-        uint8_t* row = dst + r * 128;
-        const int q = (piece & 3) * 2, sw = r & 7;
-        if (mine) {
-          *reinterpret_cast<uint4*>(row + ((q ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-          *reinterpret_cast<uint4*>(row + (((q + 1) ^ sw) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
-        }
+      for (int e = 0; e < 8; ++e) {
+        float lo, hi;
+        f2_unpack(x[e], lo, hi);
+        o[e] = live ? pack_bf16x2(lo, hi) : 0u;
+      }
+      uint8_t* row = b_buf + b * Cfg::B_BYTES + (piece >> 2) * kChunk + r * 128;
+      const int q = (piece & 3) * 2, sw = r & 7;
+      if (mine) {
+        *reinterpret_cast<uint4*>(row + ((q ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<uint4*>(row + (((q + 1) ^ sw) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
       }
       fence_async_smem();
       __syncwarp();
@@ -205,15 +184,16 @@ __device__ __forceinline__ void grad_role(uint8_t* smem, Shared* sh, const WaitC
         ph ^= 1;
       }
     }
-    // the sums: two warps a lane quarter, a tile each or half the columns
+    // the sums: four warps a lane quarter, which share the tiles and the blocks of 32 columns
     warp_wait(&sh->done, 0, wctx);
     tc_fence_after();
-    const int quarter = warp & 3, half = w8 >> 2;
-    const int o = m0 + (MT == 2 ? half * 128 : 0) + quarter * 32 + lane;
-    const uint32_t t = tmem_addr(sh->tmem, quarter * 32, MT == 2 ? half * 256 : 0);
+    const int quarter = warp & 3, share = wk >> 2;
+    const int i = MT == 2 ? share & 1 : 0;
+    const int o = m0 + i * 128 + quarter * 32 + lane;
+    const uint32_t t = tmem_addr(sh->tmem, quarter * 32, i * 256);
     float* g = a.g + ((int64_t)range * a.outs + o) * a.norm.cols;
 #pragma unroll 1
-    for (int c = MT == 2 ? 0 : half * 32; c < a.norm.cols; c += MT == 2 ? 32 : 64) {
+    for (int c = 32 * (MT == 2 ? share >> 1 : share); c < a.norm.cols; c += MT == 2 ? 64 : 128) {
       uint32_t v[32];
       tmem_ld32(t + c, v);
       tmem_ld_wait();
@@ -223,7 +203,7 @@ __device__ __forceinline__ void grad_role(uint8_t* smem, Shared* sh, const WaitC
           *reinterpret_cast<uint4*>(g + c + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
       __syncwarp();
     }
-    if (MT == 2 || half == 0) {
+    if (share < MT) {
       uint32_t v[8];
       tmem_ld8(t + ones * 64, v);
       tmem_ld_wait();
@@ -235,31 +215,30 @@ __device__ __forceinline__ void grad_role(uint8_t* smem, Shared* sh, const WaitC
 // ---- dx ------------------------------------------------------------------------------------------
 constexpr int kWBytes = 128 * 1024;      // most of the weight
 constexpr int kATile = 128 * 128;        // 128 rows of 64 outputs
-constexpr int kDxStages = 5;
-constexpr int kDxSmem = kSharedBytes + kWBytes + kDxStages * kATile + 8 * 2048;
+constexpr int kDxStages = 4;
+constexpr int kDxSmem = kSharedBytes + kWBytes + kDxStages * kATile + kWorkers * 2048;
 static_assert(kDxSmem <= kSmemMax, "");
 
-// Columns 64 h .. 64 h + 63 of 128 rows (32 h .. where a row has 64 at most): a thread has a row's part of them.
+// 32 columns of a kept row.
 template <bool CODES>
 struct KeptRow {
-  uint4 u[CODES ? 4 : 8];
+  static constexpr int N = CODES ? 2 : 4;
+  uint4 u[N];
   float mean, rstd, down;
-  __device__ __forceinline__ void load(const NormArgs& n, int64_t row, int c0, int width) {
+  __device__ __forceinline__ void load(const NormArgs& n, int64_t row, int c0) {
     const int64_t r = row < n.rows ? row : n.rows - 1;
     mean = n.mean[r];
     rstd = n.rstd[r];
     down = CODES ? n.scales[r] : 1.f;
 #pragma unroll
-    for (int i = 0; i < (CODES ? 4 : 8); ++i) {
-      const int c = c0 + i * (CODES ? 16 : 8);
-      const bool in = i * (CODES ? 16 : 8) < width && c < n.cols;  // (codes: rows have room up to a multiple of 16)
-      if constexpr (CODES) u[i] = in ? *reinterpret_cast<const uint4*>(n.codes + r * n.code_pitch + c) : make_uint4(0u, 0u, 0u, 0u);
-      else
-        u[i] = in ? *reinterpret_cast<const uint4*>(static_cast<const bf16*>(n.x) + r * n.x_pitch + c)
-                  : make_uint4(0u, 0u, 0u, 0u);
+    for (int i = 0; i < N; ++i) {
+      const int c = c0 + i * (32 / N);  // (rows of codes have room up to a multiple of 16)
+      const void* p = CODES ? static_cast<const void*>(n.codes + r * n.code_pitch + c)
+                            : static_cast<const void*>(static_cast<const bf16*>(n.x) + r * n.x_pitch + c);
+      u[i] = c < n.cols ? *static_cast<const uint4*>(p) : make_uint4(0u, 0u, 0u, 0u);
     }
   }
-  // xh of the pairs 8 i .. 8 i + 7 (sixteen columns)
+  // xh of sixteen columns, in pairs
   __device__ __forceinline__ void get(int i, uint64_t f, uint64_t m, uint64_t (&x)[8]) const {
     if constexpr (CODES) {
       unpack_codes(u[i].x, x);
@@ -342,50 +321,37 @@ __device__ __forceinline__ void dx_role(uint8_t* smem, Shared* sh, const WaitCtx
       umma_commit(el, &sh->second_full[acc]);
     }
   } else {
-    // Two warps a lane quarter; each has half of the columns of its 32 rows.
-    const int w8 = warp - 2, quarter = warp & 3, half = w8 >> 2;
-    const int width = cb == 2 ? 64 : 32, c0 = half * width;  // columns of a half
-    uint8_t* tile = staging + w8 * 2048;
-    const uint8_t* other = staging + (w8 ^ 4) * 2048;
+    // Four warps a lane quarter, 32 columns each of its 32 rows; a lane has a row.  With two warps and 64 columns a tile took
+    // 4.2 us, longer than its products and its memory, and with them the kernel 263 us (768 * 768 rows of 128 channels from
+    // codes, 512 outputs).
+    const int wk = warp - 2, quarter = warp & 3, c0 = (wk >> 2) * 32;
+    uint8_t* tile = staging + wk * 2048;
+    const bool exists = c0 < a.norm.cols;
     KeptRow<CODES> next;
-    if (tiles > 0) next.load(a.norm, row_begin + quarter * 32 + lane, c0, width);
-    const int blocks = max(0, min(width, a.norm.cols - c0) + 31) / 32;  // of 32 columns that exist: 0, 1 or 2
+    if (tiles > 0) next.load(a.norm, row_begin + quarter * 32 + lane, c0);
     for (int t = 0; t < tiles; ++t) {
       const int acc = t & 1;
       const int64_t row0 = row_begin + t * row_step + quarter * 32;
       const KeptRow<CODES> x = next;
-      if (t + 1 < tiles) next.load(a.norm, row0 + row_step + lane, c0, width);
+      if (t + 1 < tiles) next.load(a.norm, row0 + row_step + lane, c0);
       const uint64_t f = f2_dup(CODES ? x.down * x.rstd : x.rstd), m = f2_dup(CODES ? -x.mean * x.rstd : -x.mean);
       warp_wait(&sh->second_full[acc], (t >> 1) & 1, wctx);
       tc_fence_after();
-      uint64_t wd[32];
-      {
-        uint32_t v[2][32];
-        const uint32_t at = tmem_addr(sh->tmem, quarter * 32, acc * 128 + c0);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          if (i < blocks) tmem_ld32(at + i * 32, v[i]);
+      uint64_t wd[16], s1 = 0, s2 = 0;
+      if (exists) {
+        uint32_t v[32];
+        tmem_ld32(tmem_addr(sh->tmem, quarter * 32, acc * 128 + c0), v);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int e = 0; e < 16; e += 2) {
+          const float4 w = *reinterpret_cast<const float4*>(w_norm + c0 + e * 2);
+          wd[e] = f2_mul(f2_pack_bits(v[2 * e], v[2 * e + 1]), f2_pack(w.x, w.y));
+          wd[e + 1] = f2_mul(f2_pack_bits(v[2 * e + 2], v[2 * e + 3]), f2_pack(w.z, w.w));
+        }
 #pragma unroll
-          for (int e = 0; e < 16; ++e) wd[i * 16 + e] = i < blocks ? f2_pack_bits(v[i][2 * e], v[i][2 * e + 1]) : 0ull;
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sh->second_empty[acc]);
-      uint64_t s1 = 0, s2 = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (i < 2 * blocks) {
+        for (int i = 0; i < 2; ++i) {
           uint64_t xh[8];
           x.get(i, f, m, xh);
-#pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            const float4 w = *reinterpret_cast<const float4*>(w_norm + c0 + i * 16 + e * 2);
-            wd[i * 8 + e] = f2_mul(wd[i * 8 + e], f2_pack(w.x, w.y));
-            wd[i * 8 + e + 1] = f2_mul(wd[i * 8 + e + 1], f2_pack(w.z, w.w));
-          }
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             s1 = f2_add(s1, wd[i * 8 + e]);
@@ -393,35 +359,37 @@ __device__ __forceinline__ void dx_role(uint8_t* smem, Shared* sh, const WaitCtx
           }
         }
       }
-      // the halves' sums meet in the staging tiles, which the last stores have left by now
+      tc_fence_before();
+      // the four sums of a row meet in the staging tiles, which the last stores have left by now
       bulk_wait_read<0>();
       __syncwarp();
-      const float2 own = make_float2(f2_sum(s1), f2_sum(s2));
-      reinterpret_cast<float2*>(tile)[lane] = own;
-      asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
-      const float2 far = reinterpret_cast<const float2*>(other)[lane];
-      asm volatile("bar.sync %0, 64;" ::"r"(1 + quarter) : "memory");
-      const uint64_t m1 = f2_dup(-(own.x + far.x) * a.norm.inv_cols), mm = f2_dup(-(own.y + far.y) * a.norm.inv_cols);
-      const uint64_t rs = f2_dup(x.rstd);
-      int buf = 0;
+      if (lane == 0) mbar_arrive(&sh->second_empty[acc]);
+      reinterpret_cast<float2*>(tile)[lane] = make_float2(f2_sum(s1), f2_sum(s2));
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory");
+      float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 v = reinterpret_cast<const float2*>(staging + ((wk & 3) + 4 * k) * 2048)[lane];
+        sum.x += v.x;
+        sum.y += v.y;
+      }
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory");
+      if (!exists) continue;
+      const uint64_t m1 = f2_dup(-sum.x * a.norm.inv_cols), mm = f2_dup(-sum.y * a.norm.inv_cols), rs = f2_dup(x.rstd);
+      uint32_t pk[16];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        if (i < blocks) {
-          uint32_t pk[16];
+        uint64_t xh[8];
+        x.get(i, f, m, xh);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint64_t xh[8];
-            x.get(2 * i + h, f, m, xh);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              float lo, hi;
-              f2_unpack(f2_mul(f2_fma(xh[e], mm, f2_add(wd[i * 16 + h * 8 + e], m1)), rs), lo, hi);
-              pk[h * 8 + e] = pack_bf16x2(lo, hi);
-            }
-          }
-          warp_tile_store_tma<1>(tile, buf, lane, pk, &tm_dx, c0 + i * 32, (int)row0, 0);
+        for (int e = 0; e < 8; ++e) {
+          float lo, hi;
+          f2_unpack(f2_mul(f2_fma(xh[e], mm, f2_add(wd[i * 8 + e], m1)), rs), lo, hi);
+          pk[i * 8 + e] = pack_bf16x2(lo, hi);
         }
       }
+      int buf = 0;
+      warp_tile_store_tma<1>(tile, buf, lane, pk, &tm_dx, c0, (int)row0, 0);
     }
     bulk_wait_all();
   }
@@ -443,11 +411,11 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < 8; ++s) {
       mbar_init(&sh->full[s], 1);
-      mbar_init(&sh->empty[s], grad ? 9 : 1);  // UMMAs; for G the eight warps that read the kept rows too
+      mbar_init(&sh->empty[s], grad ? 1 + kWorkers : 1);  // UMMAs; for G the warps that read the kept rows too
     }
     for (int b = 0; b < 2; ++b) {  // G: the xh~ buffers, dx: the accumulators
-      mbar_init(&sh->second_full[b], grad ? 8 : 1);
-      mbar_init(&sh->second_empty[b], grad ? 1 : 8);
+      mbar_init(&sh->second_full[b], grad ? kWorkers : 1);
+      mbar_init(&sh->second_empty[b], grad ? 1 : kWorkers);
     }
     mbar_init(&sh->w_full, 1);
     mbar_init(&sh->done, 1);
