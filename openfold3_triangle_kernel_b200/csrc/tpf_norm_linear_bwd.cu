@@ -23,7 +23,7 @@ __device__ int g_nl_bwd_status;
 
 constexpr int kRows = 64;         // of a stage of G
 constexpr int kWorkers = 16;       // warps that work on elements
-constexpr int kWarps = 2 + kWorkers;  // TMA, UMMA
+constexpr int kWarps = 3 + kWorkers;  // TMA, UMMA; last: TMA of the kept rows (dx)
 constexpr int kChunk = kRows * 128;  // 64 rows of 64 bf16 columns
 constexpr int kSmemMax = 227 * 1024;
 
@@ -33,13 +33,14 @@ struct BwdArgs {
   int outs, tiles, g_ctas, dx_ctas;  // of a range (0: not wanted)
   int w_blocks;    // blocks of 64 outputs
   int col_blocks;  // blocks of 64 columns: 1 or 2
+  int dx_stages, dx_kept;  // dx: blocks of d_out and tiles of kept rows that shared memory holds
   float* g;        // [ranges][outs][cols]
   float* s;        // [ranges][outs]
 };
 
 // Everything in dynamic shared memory, which then starts on a 1024-byte boundary.
 struct Shared {
-  uint64_t full[8], empty[8], second_full[2], second_empty[2], w_full, done;
+  uint64_t full[8], empty[8], second_full[2], second_empty[2], kept_full[2], kept_empty[2], w_full, done;
   uint32_t tmem;
   volatile int abort_flag;
 };
@@ -53,7 +54,7 @@ struct GradConfig {
   static constexpr int B_BYTES = 3 * kChunk;  // up to 128 columns of xh~, a block whose first column is ones
   static constexpr int FIT = (kSmemMax - kSharedBytes - 2 * B_BYTES) / STAGE, STAGES = FIT > 6 ? 6 : FIT;
   static constexpr int SMEM = kSharedBytes + 2 * B_BYTES + STAGES * STAGE;
-  static constexpr int TMEM = MT == 2 ? 512 : 256;  // 256 columns a tile: 128 and 16 are used
+  static constexpr int TMEM = MT == 2 ? 512 : 256;  // 256 columns a tile: up to 144 are used
 };
 
 template <int MT, bool CODES>
@@ -116,71 +117,94 @@ __device__ __forceinline__ void grad_role(uint8_t* smem, Shared* sh, const WaitC
       }
     }
     umma_commit(el, &sh->done);
-  } else {
-    // A lane makes 16 consecutive columns of a row: 8 lanes a row, 4 rows a warp and stage.
-    const int wk = warp - 2, piece = lane & 7, sub = lane >> 3;
+  } else if (warp < 2 + kWorkers) {
+    // Two groups of eight warps make every other stage's xh~, each in a buffer of its own: making one takes longer than its
+    // products.  A lane makes 16 consecutive columns of a row: 8 lanes a row, twice 4 rows a warp.
+    const int wk = warp - 2, group = wk >> 3, piece = lane & 7, sub = lane >> 3;
     // the block of ones: its first column is 1, the rest 0, in both buffers and for good
-    for (int i = threadIdx.x - 64; i < 2 * kRows * 8; i += 32 * kWorkers) {
-      const int b = i >= kRows * 8, r = (i >> 3) & (kRows - 1), q = i & 7;
-      *reinterpret_cast<uint4*>(b_buf + b * Cfg::B_BYTES + ones * kChunk + r * 128 + ((q ^ (r & 7)) << 4)) =
+    for (int i = (wk & 7) * 32 + lane; i < kRows * 8; i += 256) {
+      const int r = i >> 3, q = i & 7;
+      *reinterpret_cast<uint4*>(b_buf + group * Cfg::B_BYTES + ones * kChunk + r * 128 + ((q ^ (r & 7)) << 4)) =
           make_uint4(q == 0 ? 0x3f80u : 0u, 0u, 0u, 0u);
     }
     const bool mine = piece < 4 * ones;  // (64 columns or fewer: the lanes of the second block have nothing to write)
-    const int r = wk * 4 + sub;
-    float mean, rstd, down;
-    auto stats = [&](int k) {  // of the row, one stage ahead
-      const int64_t row = min(row_begin + (int64_t)k * kRows + r, a.norm.rows - 1);
-      mean = a.norm.mean[row];
-      rstd = a.norm.rstd[row];
-      down = CODES ? a.norm.scales[row] : 1.f;
+    const int r0 = (wk & 7) * 8 + sub;
+    float mean[2], rstd[2], down[2];
+    auto stats = [&](int k) {  // of the rows, before their stage is waited for
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const int64_t row = min(row_begin + (int64_t)k * kRows + r0 + p * 4, a.norm.rows - 1);
+        mean[p] = a.norm.mean[row];
+        rstd[p] = a.norm.rstd[row];
+        down[p] = CODES ? a.norm.scales[row] : 1.f;
+      }
     };
-    stats(0);
-    int s = 0;
+    if (group < steps) stats(group);
+    int s = group;
     uint32_t ph = 0;
-    for (int k = 0; k < steps; ++k) {
-      const int b = k & 1;
-      const uint64_t f2 = f2_dup(CODES ? down * rstd : rstd), m2 = f2_dup(CODES ? -mean * rstd : -mean);
-      if (k + 1 < steps) stats(k + 1);
-      warp_wait2(&sh->full[s], ph, &sh->second_empty[b], ((k >> 1) & 1) ^ 1, wctx);
+    for (int k = group; k < steps; k += 2) {
+      uint64_t f2[2], m2[2];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        f2[p] = f2_dup(CODES ? down[p] * rstd[p] : rstd[p]);
+        m2[p] = f2_dup(CODES ? -mean[p] * rstd[p] : -mean[p]);
+      }
+      if (k + 2 < steps) stats(k + 2);
+      warp_wait2(&sh->full[s], ph, &sh->second_empty[group], ((k >> 1) & 1) ^ 1, wctx);
       const uint8_t* raw = ring + s * Cfg::STAGE + Cfg::A_BYTES;
-      uint64_t x[8];
-      if constexpr (CODES) {
-        const uint4 u = *reinterpret_cast<const uint4*>(raw + r * 128 + piece * 16);
-        unpack_codes(u.x, x);
-        unpack_codes(u.y, x + 2);
-        unpack_codes(u.z, x + 4);
-        unpack_codes(u.w, x + 6);
+      uint4 u[2][CODES ? 1 : 2];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = f2_fma(x[e], f2, m2);
-      } else {
-        const uint4* src = reinterpret_cast<const uint4*>(raw + (piece >> 2) * kChunk + r * 128 + (piece & 3) * 32);
-        const uint4 u = src[0], w = src[1];
-        const uint32_t v[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = f2_mul(f2_add(f2_pack_bits(v[e] << 16, v[e] & 0xffff0000u), m2), f2);
+      for (int p = 0; p < 2; ++p) {
+        const int r = r0 + p * 4;
+        if constexpr (CODES) {
+          u[p][0] = *reinterpret_cast<const uint4*>(raw + r * 128 + piece * 16);
+        } else {
+          const uint4* src = reinterpret_cast<const uint4*>(raw + (piece >> 2) * kChunk + r * 128 + (piece & 3) * 32);
+          u[p][0] = src[0];
+          u[p][1] = src[1];
+        }
       }
-      uint32_t o[8];
-      const bool live = row_begin + (int64_t)k * kRows + r < row_end;  // (where d_out is zero: a NaN must not meet it)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float lo, hi;
-        f2_unpack(x[e], lo, hi);
-        o[e] = live ? pack_bf16x2(lo, hi) : 0u;
-      }
-      uint8_t* row = b_buf + b * Cfg::B_BYTES + (piece >> 2) * kChunk + r * 128;
-      const int q = (piece & 3) * 2, sw = r & 7;
-      if (mine) {
-        *reinterpret_cast<uint4*>(row + ((q ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-        *reinterpret_cast<uint4*>(row + (((q + 1) ^ sw) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+      for (int p = 0; p < 2; ++p) {
+        const int r = r0 + p * 4;
+        uint64_t x[8];
+        if constexpr (CODES) {
+          unpack_codes(u[p][0].x, x);
+          unpack_codes(u[p][0].y, x + 2);
+          unpack_codes(u[p][0].z, x + 4);
+          unpack_codes(u[p][0].w, x + 6);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = f2_fma(x[e], f2[p], m2[p]);
+        } else {
+          const uint32_t v[8] = {u[p][0].x, u[p][0].y, u[p][0].z, u[p][0].w, u[p][1].x, u[p][1].y, u[p][1].z, u[p][1].w};
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            x[e] = f2_mul(f2_add(f2_pack_bits(v[e] << 16, v[e] & 0xffff0000u), m2[p]), f2[p]);
+        }
+        uint32_t o[8];
+        const bool live = row_begin + (int64_t)k * kRows + r < row_end;  // (where d_out is zero: a NaN must not meet it)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float lo, hi;
+          f2_unpack(x[e], lo, hi);
+          o[e] = live ? pack_bf16x2(lo, hi) : 0u;
+        }
+        uint8_t* row = b_buf + group * Cfg::B_BYTES + (piece >> 2) * kChunk + r * 128;
+        const int q = (piece & 3) * 2, sw = r & 7;
+        if (mine) {
+          *reinterpret_cast<uint4*>(row + ((q ^ sw) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(row + (((q + 1) ^ sw) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+        }
       }
       fence_async_smem();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&sh->second_full[b]);
+        mbar_arrive(&sh->second_full[group]);
         mbar_arrive(&sh->empty[s]);
       }
-      if (++s == STAGES) {
-        s = 0;
+      s += 2;
+      if (s >= STAGES) {
+        s -= STAGES;
         ph ^= 1;
       }
     }
@@ -213,30 +237,27 @@ __device__ __forceinline__ void grad_role(uint8_t* smem, Shared* sh, const WaitC
 }
 
 // ---- dx ------------------------------------------------------------------------------------------
-constexpr int kWBytes = 128 * 1024;      // most of the weight
-constexpr int kATile = 128 * 128;        // 128 rows of 64 outputs
-constexpr int kDxStages = 4;
-constexpr int kDxSmem = kSharedBytes + kWBytes + kDxStages * kATile + kWorkers * 2048;
-static_assert(kDxSmem <= kSmemMax, "");
-
-// 32 columns of a kept row.
+constexpr int kWBytes = 128 * 1024;  // most of the weight
+constexpr int kATile = 128 * 128;    // 128 rows of 64 outputs
+constexpr int kStaging = kWorkers * 2048;
+constexpr int kSmem = kSmemMax;      // all of it: one CTA an SM
 template <bool CODES>
-struct KeptRow {
+constexpr int kKept = CODES ? 128 * 128 : 2 * 128 * 128;  // 128 rows of 128 codes, or twice 64 bf16
+static_assert(kSharedBytes + kWBytes + kStaging + kKept<false> + 2 * kATile <= kSmem, "");
+
+// 32 columns of a kept row, as they lie in memory.
+template <bool CODES>
+struct KeptBlock {
   static constexpr int N = CODES ? 2 : 4;
   uint4 u[N];
-  float mean, rstd, down;
-  __device__ __forceinline__ void load(const NormArgs& n, int64_t row, int c0) {
-    const int64_t r = row < n.rows ? row : n.rows - 1;
-    mean = n.mean[r];
-    rstd = n.rstd[r];
-    down = CODES ? n.scales[r] : 1.f;
+  // Where 16-byte unit i of columns c0 .. c0 + 31 is in a tile (rows of 128 bytes, 128-byte swizzle).
+  static __device__ __forceinline__ uint8_t* at(uint8_t* tile, int row, int c0, int i) {
+    const int unit = CODES ? c0 / 16 + i : c0 % 64 / 8 + i;
+    return tile + (CODES ? 0 : c0 / 64 * (128 * 128)) + row * 128 + ((unit ^ (row & 7)) << 4);
+  }
+  __device__ __forceinline__ void load(uint8_t* tile, int row, int c0) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = c0 + i * (32 / N);  // (rows of codes have room up to a multiple of 16)
-      const void* p = CODES ? static_cast<const void*>(n.codes + r * n.code_pitch + c)
-                            : static_cast<const void*>(static_cast<const bf16*>(n.x) + r * n.x_pitch + c);
-      u[i] = c < n.cols ? *static_cast<const uint4*>(p) : make_uint4(0u, 0u, 0u, 0u);
-    }
+    for (int i = 0; i < N; ++i) u[i] = *reinterpret_cast<const uint4*>(at(tile, row, c0, i));
   }
   // xh of sixteen columns, in pairs
   __device__ __forceinline__ void get(int i, uint64_t f, uint64_t m, uint64_t (&x)[8]) const {
@@ -258,11 +279,13 @@ struct KeptRow {
 
 template <bool CODES>
 __device__ __forceinline__ void dx_role(uint8_t* smem, Shared* sh, const WaitCtx& wctx, const CUtensorMap& tm_rows,
-                                        const CUtensorMap& tm_w, const CUtensorMap& tm_dx, const BwdArgs& a, int part,
-                                        int range) {
+                                        const CUtensorMap& tm_w, const CUtensorMap& tm_kept, const CUtensorMap& tm_dx,
+                                        const BwdArgs& a, int part, int range) {
+  const int kb = a.w_blocks, cb = a.col_blocks, stages = a.dx_stages;
   uint8_t* w_buf = smem;
-  uint8_t* ring = smem + kWBytes;
-  uint8_t* staging = ring + kDxStages * kATile;
+  uint8_t* ring = smem + kb * cb * kChunk;
+  uint8_t* kept = ring + stages * kATile;
+  uint8_t* staging = kept + a.dx_kept * kKept<CODES>;
   float* w_norm = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(sh) + 512);
   const int warp = warp_index(), lane = threadIdx.x & 31;
   const int64_t range_begin = range * a.rows_per_range;
@@ -270,7 +293,6 @@ __device__ __forceinline__ void dx_role(uint8_t* smem, Shared* sh, const WaitCtx
   const int64_t row_begin = range_begin + part * 128;
   const int64_t row_step = a.dx_ctas * 128;
   const int tiles = row_begin < range_end ? (int)((range_end - row_begin + row_step - 1) / row_step) : 0;
-  const int kb = a.w_blocks, cb = a.col_blocks;
 
   if (warp == 0) {
     const uint32_t el = elect_one();
@@ -286,10 +308,26 @@ __device__ __forceinline__ void dx_role(uint8_t* smem, Shared* sh, const WaitCtx
         warp_wait(&sh->empty[s], ph, wctx);
         mbar_expect_tx(el, &sh->full[s], kATile);
         tma_load_3d(el, ring + s * kATile, &tm_rows, &sh->full[s], k * 64, row, 0);
-        if (++s == kDxStages) {
+        if (++s == stages) {
           s = 0;
           ph ^= 1;
         }
+      }
+    }
+  } else if (warp == 2 + kWorkers) {
+    const uint32_t el = elect_one();
+    int s = 0;
+    uint32_t ph = 1;
+    for (int t = 0; t < tiles; ++t) {
+      warp_wait(&sh->kept_empty[s], ph, wctx);
+      mbar_expect_tx(el, &sh->kept_full[s], kKept<CODES>);
+#pragma unroll
+      for (int c = 0; c < (CODES ? 1 : 2); ++c)
+        tma_load_3d(el, kept + s * kKept<CODES> + c * (128 * 128), &tm_kept, &sh->kept_full[s], c * 64,
+                    (int)(row_begin + t * row_step), 0);
+      if (++s == a.dx_kept) {
+        s = 0;
+        ph ^= 1;
       }
     }
   } else if (warp == 1) {
@@ -313,7 +351,7 @@ __device__ __forceinline__ void dx_role(uint8_t* smem, Shared* sh, const WaitCtx
         for (int j = 0; j < 4; ++j)
           umma_ss(el, tmem + acc * 128, ad + j * 2, bd + j * (16 * 128 >> 4), idesc, (k | j) != 0 ? 1u : 0u);
         umma_commit(el, &sh->empty[s]);
-        if (++s == kDxStages) {
+        if (++s == stages) {
           s = 0;
           ph ^= 1;
         }
@@ -321,26 +359,34 @@ __device__ __forceinline__ void dx_role(uint8_t* smem, Shared* sh, const WaitCtx
       umma_commit(el, &sh->second_full[acc]);
     }
   } else {
-    // Four warps a lane quarter, 32 columns each of its 32 rows; a lane has a row.  With two warps and 64 columns a tile took
-    // 4.2 us, longer than its products and its memory, and with them the kernel 263 us (768 * 768 rows of 128 channels from
-    // codes, 512 outputs).
-    const int wk = warp - 2, quarter = warp & 3, c0 = (wk >> 2) * 32;
+    // Four warps a lane quarter, 32 columns each of its 32 rows; a lane has a row.  The kept rows come by TMA: a lane's loads
+    // of its own row touch 32 lines an instruction (twice as long a tile).  Two warps a quarter took 4.2 us a tile.
+    const int wk = warp - 2, quarter = warp & 3, c0 = (wk >> 2) * 32, r = quarter * 32 + lane;
     uint8_t* tile = staging + wk * 2048;
     const bool exists = c0 < a.norm.cols;
-    KeptRow<CODES> next;
-    if (tiles > 0) next.load(a.norm, row_begin + quarter * 32 + lane, c0);
+    float mean = 0.f, rstd = 0.f, down = 1.f;
+    auto stats = [&](int t) {
+      const int64_t row = min(row_begin + t * row_step + r, a.norm.rows - 1);
+      mean = a.norm.mean[row];
+      rstd = a.norm.rstd[row];
+      if (CODES) down = a.norm.scales[row];
+    };
+    if (tiles > 0) stats(0);
+    int ks = 0;
+    uint32_t kph = 0;
     for (int t = 0; t < tiles; ++t) {
       const int acc = t & 1;
-      const int64_t row0 = row_begin + t * row_step + quarter * 32;
-      const KeptRow<CODES> x = next;
-      if (t + 1 < tiles) next.load(a.norm, row0 + row_step + lane, c0);
-      const uint64_t f = f2_dup(CODES ? x.down * x.rstd : x.rstd), m = f2_dup(CODES ? -x.mean * x.rstd : -x.mean);
-      warp_wait(&sh->second_full[acc], (t >> 1) & 1, wctx);
+      const uint64_t f = f2_dup(CODES ? down * rstd : rstd), m = f2_dup(CODES ? -mean * rstd : -mean), rs = f2_dup(rstd);
+      if (t + 1 < tiles) stats(t + 1);
+      uint8_t* rows = kept + ks * kKept<CODES>;
+      warp_wait2(&sh->second_full[acc], (t >> 1) & 1, &sh->kept_full[ks], kph, wctx);
       tc_fence_after();
+      KeptBlock<CODES> x;
       uint64_t wd[16], s1 = 0, s2 = 0;
       if (exists) {
         uint32_t v[32];
         tmem_ld32(tmem_addr(sh->tmem, quarter * 32, acc * 128 + c0), v);
+        x.load(rows, r, c0);
         tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 16; e += 2) {
@@ -349,47 +395,52 @@ __device__ __forceinline__ void dx_role(uint8_t* smem, Shared* sh, const WaitCtx
           wd[e + 1] = f2_mul(f2_pack_bits(v[2 * e + 2], v[2 * e + 3]), f2_pack(w.z, w.w));
         }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int h = 0; h < 2; ++h) {
           uint64_t xh[8];
-          x.get(i, f, m, xh);
+          x.get(h, f, m, xh);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            s1 = f2_add(s1, wd[i * 8 + e]);
-            s2 = f2_fma(wd[i * 8 + e], xh[e], s2);
+            s1 = f2_add(s1, wd[h * 8 + e]);
+            s2 = f2_fma(wd[h * 8 + e], xh[e], s2);
           }
         }
       }
       tc_fence_before();
-      // the four sums of a row meet in the staging tiles, which the last stores have left by now
-      bulk_wait_read<0>();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh->second_empty[acc]);
-      reinterpret_cast<float2*>(tile)[lane] = make_float2(f2_sum(s1), f2_sum(s2));
+      // The four sums of a row meet where its kept columns were: every lane's own are in registers by now.
+      *reinterpret_cast<float2*>(KeptBlock<CODES>::at(rows, r, c0, 0)) = make_float2(f2_sum(s1), f2_sum(s2));
       asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory");
       float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float2 v = reinterpret_cast<const float2*>(staging + ((wk & 3) + 4 * k) * 2048)[lane];
+        const float2 v = *reinterpret_cast<const float2*>(KeptBlock<CODES>::at(rows, r, k * 32, 0));
         sum.x += v.x;
         sum.y += v.y;
       }
-      asm volatile("bar.sync %0, 128;" ::"r"(1 + quarter) : "memory");
+      fence_async_smem();  // the next tile's rows come through the asynchronous proxy
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->kept_empty[ks]);
+      if (++ks == a.dx_kept) {
+        ks = 0;
+        kph ^= 1;
+      }
       if (!exists) continue;
-      const uint64_t m1 = f2_dup(-sum.x * a.norm.inv_cols), mm = f2_dup(-sum.y * a.norm.inv_cols), rs = f2_dup(x.rstd);
+      const uint64_t m1 = f2_dup(-sum.x * a.norm.inv_cols), m2 = f2_dup(-sum.y * a.norm.inv_cols);
       uint32_t pk[16];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int h = 0; h < 2; ++h) {
         uint64_t xh[8];
-        x.get(i, f, m, xh);
+        x.get(h, f, m, xh);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           float lo, hi;
-          f2_unpack(f2_mul(f2_fma(xh[e], mm, f2_add(wd[i * 8 + e], m1)), rs), lo, hi);
-          pk[i * 8 + e] = pack_bf16x2(lo, hi);
+          f2_unpack(f2_mul(f2_fma(xh[e], m2, f2_add(wd[h * 8 + e], m1)), rs), lo, hi);
+          pk[h * 8 + e] = pack_bf16x2(lo, hi);
         }
       }
       int buf = 0;
-      warp_tile_store_tma<1>(tile, buf, lane, pk, &tm_dx, c0, (int)row0, 0);
+      warp_tile_store_tma<1>(tile, buf, lane, pk, &tm_dx, c0, (int)(row_begin + t * row_step + quarter * 32), 0);
     }
     bulk_wait_all();
   }
@@ -398,24 +449,28 @@ __device__ __forceinline__ void dx_role(uint8_t* smem, Shared* sh, const WaitCtx
 template <int MT, bool CODES>
 __global__ void __launch_bounds__(32 * kWarps, 1)
     nl_bwd_kernel(const __grid_constant__ CUtensorMap tm_cols, const __grid_constant__ CUtensorMap tm_rows,
-                  const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
-                  const __grid_constant__ CUtensorMap tm_dx, const __grid_constant__ BwdArgs a, int* __restrict__ status) {
+                  const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_kept,
+                  const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_dx,
+                  const __grid_constant__ BwdArgs a, int* __restrict__ status) {
   extern __shared__ __align__(1024) uint8_t smem[];
   using Grad = GradConfig<MT, CODES>;
+  static_assert(Grad::SMEM <= kSmem, "");
   const int per = a.g_ctas + a.dx_ctas;
   const int range = blockIdx.x / per, part = blockIdx.x - range * per;
   const bool grad = part < a.g_ctas;
-  Shared* sh = reinterpret_cast<Shared*>(smem + (kDxSmem > Grad::SMEM ? kDxSmem : Grad::SMEM) - kSharedBytes);
+  Shared* sh = reinterpret_cast<Shared*>(smem + kSmem - kSharedBytes);
   const WaitCtx wctx{&sh->abort_flag, status};
   const int warp = warp_index();
   if (threadIdx.x == 0) {
     for (int s = 0; s < 8; ++s) {
       mbar_init(&sh->full[s], 1);
-      mbar_init(&sh->empty[s], grad ? 1 + kWorkers : 1);  // UMMAs; for G the warps that read the kept rows too
+      mbar_init(&sh->empty[s], grad ? 1 + kWorkers / 2 : 1);  // UMMAs; for G the warps that read the kept rows too
     }
     for (int b = 0; b < 2; ++b) {  // G: the xh~ buffers, dx: the accumulators
-      mbar_init(&sh->second_full[b], grad ? kWorkers : 1);
+      mbar_init(&sh->second_full[b], grad ? kWorkers / 2 : 1);
       mbar_init(&sh->second_empty[b], grad ? 1 : kWorkers);
+      mbar_init(&sh->kept_full[b], 1);
+      mbar_init(&sh->kept_empty[b], kWorkers);
     }
     mbar_init(&sh->w_full, 1);
     mbar_init(&sh->done, 1);
@@ -437,7 +492,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
   __syncthreads();
   tc_fence_after();
   if (grad) grad_role<MT, CODES>(smem, sh, wctx, tm_cols, tm_x, a, part, range);
-  else dx_role<CODES>(smem, sh, wctx, tm_rows, tm_w, tm_dx, a, part - a.g_ctas, range);
+  else dx_role<CODES>(smem, sh, wctx, tm_rows, tm_w, tm_kept, tm_dx, a, part - a.g_ctas, range);
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -524,22 +579,18 @@ int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 
 template <int MT, bool CODES>
 int launch_bwd(const BwdArgs& a, const Plan& p, const void* d_out, const void* w, void* dx, cudaStream_t stream) {
-  CUtensorMap tm_cols, tm_rows, tm_x, tm_w, tm_dx;
+  CUtensorMap tm_cols, tm_rows, tm_x, tm_kept, tm_w, tm_dx;
   const int64_t R = a.norm.rows, C = a.norm.cols, O = a.outs;
   if (int rc = make_operand_tmap(&tm_cols, d_out, true, O, R, O, 1, 0, 128, 64, kRows)) return rc;
   if (int rc = make_operand_tmap(&tm_rows, d_out, false, R, O, O, 1, 0, 128, 128, 64)) return rc;
   if (int rc = make_operand_tmap(&tm_w, w, true, C, O, C, 1, 0, 128, 64, 64)) return rc;
-  if constexpr (CODES) {
-    const uint64_t dims[3] = {(uint64_t)a.norm.code_pitch, (uint64_t)R, 1};
-    const uint64_t strides[2] = {(uint64_t)a.norm.code_pitch, 16};
-    const uint32_t box[3] = {128, (uint32_t)kRows, 1};
-    if (int rc = make_tmap(&tm_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.norm.codes, 3, dims, strides, box, 0)) return rc;
-  } else {
-    const uint64_t dims[3] = {(uint64_t)C, (uint64_t)R, 1};
-    const uint64_t strides[2] = {(uint64_t)a.norm.x_pitch * 2, 16};
-    const uint32_t box[3] = {64, (uint32_t)kRows, 1};
-    if (int rc = make_tmap_bf16(&tm_x, a.norm.x, 3, dims, strides, box, 0)) return rc;
-  }
+  const int64_t pitch = CODES ? a.norm.code_pitch : a.norm.x_pitch * 2;  // bytes
+  const uint64_t dims[3] = {(uint64_t)(CODES ? pitch : C), (uint64_t)R, 1}, strides[2] = {(uint64_t)pitch, 16};
+  const uint32_t box[3] = {CODES ? 128u : 64u, (uint32_t)kRows, 1}, kept_box[3] = {CODES ? 128u : 64u, 128, 1};
+  const auto type = CODES ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const void* kept = CODES ? static_cast<const void*>(a.norm.codes) : a.norm.x;
+  if (int rc = make_tmap(&tm_x, type, kept, 3, dims, strides, box, 0)) return rc;
+  if (int rc = make_tmap(&tm_kept, type, kept, 3, dims, strides, kept_box, 128)) return rc;
   if (dx != nullptr) {
     if (int rc = make_store_tmap(&tm_dx, dx, C, R, C, 1, 0)) return rc;
   } else {
@@ -548,13 +599,11 @@ int launch_bwd(const BwdArgs& a, const Plan& p, const void* d_out, const void* w
   int* status = nullptr;
   static PerDeviceAddress status_at;
   if (int rc = device_symbol_address(g_nl_bwd_status, status_at, reinterpret_cast<void**>(&status))) return rc;
-  constexpr int smem = kDxSmem > GradConfig<MT, CODES>::SMEM ? kDxSmem : GradConfig<MT, CODES>::SMEM;
-  static_assert(smem <= kSmemMax, "");
   const auto kern = nl_bwd_kernel<MT, CODES>;
   static PerDeviceOnce once;
-  if (int rc = ensure_dynamic_smem(kern, smem, once, 1024)) return rc;
-  launch_kernel(kern, dim3(p.ranges * (p.g_ctas + p.dx_ctas)), dim3(32 * kWarps), smem, stream, tm_cols, tm_rows, tm_x, tm_w,
-                tm_dx, a, status);
+  if (int rc = ensure_dynamic_smem(kern, kSmem, once, 1024)) return rc;
+  launch_kernel(kern, dim3(p.ranges * (p.g_ctas + p.dx_ctas)), dim3(32 * kWarps), kSmem, stream, tm_cols, tm_rows, tm_x, tm_kept,
+                tm_w, tm_dx, a, status);
   TPF_LAUNCH_OK();
   return TPF_OK;
 }
@@ -587,9 +636,16 @@ int norm_linear_narrow_bwd(const NormArgs& norm, const void* w, int64_t outs, co
   const int64_t z = most_ranges(R, outs);
   char* base = static_cast<char*>(workspace);
   float* terms = reinterpret_cast<float*>(base + up256(z * outs * C * 4) + up256(z * outs * 4));
-  const BwdArgs a{norm, p.rows_per_range, (int)outs, p.tiles, p.g_ctas, p.dx_ctas, (int)((outs + 63) / 64),
-                  (int)((C + 63) / 64), reinterpret_cast<float*>(base), reinterpret_cast<float*>(base + up256(z * outs * C * 4))};
   const bool codes = norm.codes != nullptr;
+  const int w_blocks = (int)((outs + 63) / 64), col_blocks = (int)((C + 63) / 64);
+  // what the weight leaves: a second tile of kept rows where four blocks of d_out still fit beside it
+  const int kept = codes ? kKept<true> : kKept<false>;
+  const int room = kSmem - kSharedBytes - kStaging - w_blocks * col_blocks * kChunk;
+  const int dx_kept = room - 2 * kept >= 4 * kATile ? 2 : 1;
+  int dx_stages = (room - dx_kept * kept) / kATile;
+  if (dx_stages > 8) dx_stages = 8;
+  const BwdArgs a{norm, p.rows_per_range, (int)outs, p.tiles, p.g_ctas, p.dx_ctas, w_blocks, col_blocks, dx_stages, dx_kept,
+                  reinterpret_cast<float*>(base), reinterpret_cast<float*>(base + up256(z * outs * C * 4))};
   const int rc = p.mt == 2 ? (codes ? launch_bwd<2, true>(a, p, g.d_out, w, g.dx, stream)
                                     : launch_bwd<2, false>(a, p, g.d_out, w, g.dx, stream))
                            : (codes ? launch_bwd<1, true>(a, p, g.d_out, w, g.dx, stream)
