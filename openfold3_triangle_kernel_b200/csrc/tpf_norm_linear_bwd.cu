@@ -33,7 +33,8 @@ struct BwdArgs {
   int outs, tiles, g_ctas, dx_ctas;  // of a range (0: not wanted)
   int w_blocks;    // blocks of 64 outputs
   int col_blocks;  // blocks of 64 columns: 1 or 2
-  int dx_stages, dx_kept;  // dx: blocks of d_out and tiles of kept rows that shared memory holds
+  int dx_stages, dx_kept;  // dx: blocks of d_out and tiles of kept rows that shared memory holds,
+  int dx_width;            // columns of dx that a warp stages at a time: 32 or 16
   float* g;        // [ranges][outs][cols]
   float* s;        // [ranges][outs]
 };
@@ -239,11 +240,11 @@ __device__ __forceinline__ void grad_role(uint8_t* smem, Shared* sh, const WaitC
 // ---- dx ------------------------------------------------------------------------------------------
 constexpr int kWBytes = 128 * 1024;  // most of the weight
 constexpr int kATile = 128 * 128;    // 128 rows of 64 outputs
-constexpr int kStaging = kWorkers * 2048;
+constexpr int kHalfTile = 1024;      // 32 rows of 16 columns of dx on their way out; 32 columns: twice as much
 constexpr int kSmem = kSmemMax;      // all of it: one CTA an SM
 template <bool CODES>
 constexpr int kKept = CODES ? 128 * 128 : 2 * 128 * 128;  // 128 rows of 128 codes, or twice 64 bf16
-static_assert(kSharedBytes + kWBytes + kStaging + kKept<false> + 2 * kATile <= kSmem, "");
+static_assert(kSharedBytes + kWBytes + kWorkers * kHalfTile + kKept<false> + 3 * kATile <= kSmem, "");
 
 // 32 columns of a kept row, as they lie in memory.
 template <bool CODES>
@@ -362,7 +363,7 @@ __device__ __forceinline__ void dx_role(uint8_t* smem, Shared* sh, const WaitCtx
     // Four warps a lane quarter, 32 columns each of its 32 rows; a lane has a row.  The kept rows come by TMA: a lane's loads
     // of its own row touch 32 lines an instruction (twice as long a tile).  Two warps a quarter took 4.2 us a tile.
     const int wk = warp - 2, quarter = warp & 3, c0 = (wk >> 2) * 32, r = quarter * 32 + lane;
-    uint8_t* tile = staging + wk * 2048;
+    uint8_t* tile = staging + wk * (a.dx_width / 16) * kHalfTile;
     const bool exists = c0 < a.norm.cols;
     float mean = 0.f, rstd = 0.f, down = 1.f;
     auto stats = [&](int t) {
@@ -439,8 +440,24 @@ __device__ __forceinline__ void dx_role(uint8_t* smem, Shared* sh, const WaitCtx
           pk[h * 8 + e] = pack_bf16x2(lo, hi);
         }
       }
-      int buf = 0;
-      warp_tile_store_tma<1>(tile, buf, lane, pk, &tm_dx, c0, (int)(row_begin + t * row_step + quarter * 32), 0);
+      const int row0 = (int)(row_begin + t * row_step + quarter * 32);
+      if (a.dx_width == 32) {
+        int buf = 0;
+        warp_tile_store_tma<1>(tile, buf, lane, pk, &tm_dx, c0, row0, 0);
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {  // rows of 32 bytes, 32-byte swizzle
+          bulk_wait_read<0>();
+          __syncwarp();
+          const int sw = (lane >> 2) & 1;
+          *reinterpret_cast<uint4*>(tile + lane * 32 + (sw << 4)) = make_uint4(pk[8 * h], pk[8 * h + 1], pk[8 * h + 2], pk[8 * h + 3]);
+          *reinterpret_cast<uint4*>(tile + lane * 32 + ((sw ^ 1) << 4)) =
+              make_uint4(pk[8 * h + 4], pk[8 * h + 5], pk[8 * h + 6], pk[8 * h + 7]);
+          fence_async_smem();
+          __syncwarp();
+          if (c0 + h * 16 < a.norm.cols) tma_store_3d(lane == 0, &tm_dx, tile, c0 + h * 16, row0, 0);
+        }
+      }
     }
     bulk_wait_all();
   }
@@ -563,7 +580,8 @@ Plan make_plan(int64_t rows, int64_t outs, bool want_g, bool want_dx) {
   p.mt = outs > 128 ? 2 : 1;
   p.tiles = (int)((outs + p.mt * 128 - 1) / (p.mt * 128));
   p.g_ctas = want_g ? p.tiles : 0;
-  p.dx_ctas = want_dx ? p.tiles : 0;
+  // with 128 outputs or fewer a CTA for G is done in half the time of one for dx (500000 rows of 128: 97 us, 119 with one each)
+  p.dx_ctas = want_dx ? (p.mt == 1 ? 2 : p.tiles) : 0;
   int64_t ranges = sm_count() / (p.g_ctas + p.dx_ctas);
   const int64_t most = (rows + 255) / 256;  // 256 rows at least: G's sums are written and read once more
   if (ranges > most) ranges = most;
@@ -592,7 +610,9 @@ int launch_bwd(const BwdArgs& a, const Plan& p, const void* d_out, const void* w
   if (int rc = make_tmap(&tm_x, type, kept, 3, dims, strides, box, 0)) return rc;
   if (int rc = make_tmap(&tm_kept, type, kept, 3, dims, strides, kept_box, 128)) return rc;
   if (dx != nullptr) {
-    if (int rc = make_store_tmap(&tm_dx, dx, C, R, C, 1, 0)) return rc;
+    const uint64_t dx_dims[3] = {(uint64_t)C, (uint64_t)R, 1}, dx_strides[2] = {(uint64_t)C * 2, 16};
+    const uint32_t dx_box[3] = {(uint32_t)a.dx_width, 32, 1};
+    if (int rc = make_tmap_bf16(&tm_dx, dx, 3, dx_dims, dx_strides, dx_box, a.dx_width * 2)) return rc;
   } else {
     tm_dx = tm_w;  // not used
   }
@@ -638,14 +658,17 @@ int norm_linear_narrow_bwd(const NormArgs& norm, const void* w, int64_t outs, co
   float* terms = reinterpret_cast<float*>(base + up256(z * outs * C * 4) + up256(z * outs * 4));
   const bool codes = norm.codes != nullptr;
   const int w_blocks = (int)((outs + 63) / 64), col_blocks = (int)((C + 63) / 64);
-  // what the weight leaves: a second tile of kept rows where four blocks of d_out still fit beside it
+  // What the weight leaves: narrow staging where d_out would have two blocks (512 outputs from whole rows: 213 us, 307 with
+  // two blocks; from codes it would be 199 in the place of 190), a second tile of kept rows where four blocks fit beside it.
   const int kept = codes ? kKept<true> : kKept<false>;
-  const int room = kSmem - kSharedBytes - kStaging - w_blocks * col_blocks * kChunk;
+  const int left = kSmem - kSharedBytes - w_blocks * col_blocks * kChunk;
+  const int dx_width = left - kWorkers * 2 * kHalfTile - kept >= 3 * kATile ? 32 : 16;
+  const int room = left - kWorkers * (dx_width / 16) * kHalfTile;
   const int dx_kept = room - 2 * kept >= 4 * kATile ? 2 : 1;
   int dx_stages = (room - dx_kept * kept) / kATile;
   if (dx_stages > 8) dx_stages = 8;
   const BwdArgs a{norm, p.rows_per_range, (int)outs, p.tiles, p.g_ctas, p.dx_ctas, w_blocks, col_blocks, dx_stages, dx_kept,
-                  reinterpret_cast<float*>(base), reinterpret_cast<float*>(base + up256(z * outs * C * 4))};
+                  dx_width, reinterpret_cast<float*>(base), reinterpret_cast<float*>(base + up256(z * outs * C * 4))};
   const int rc = p.mt == 2 ? (codes ? launch_bwd<2, true>(a, p, g.d_out, w, g.dx, stream)
                                     : launch_bwd<2, false>(a, p, g.d_out, w, g.dx, stream))
                            : (codes ? launch_bwd<1, true>(a, p, g.d_out, w, g.dx, stream)
