@@ -45,6 +45,7 @@ int attn_bwd_static_scratch(const void* q, const void* k, const void* v, const v
 int pair_attn_status_fetch_and_clear(int* out);
 int selftest_status_fetch_and_clear(int* out);
 int norm_linear_dw_status_fetch_and_clear(int* out);
+int norm_linear_fwd_status_fetch_and_clear(int* out);
 int norm_linear_bwd_status_fetch_and_clear(int* out);
 int selftest_bounded_wait(unsigned int* report, cudaStream_t stream);
 
@@ -93,6 +94,8 @@ int tpf_device_status(int* status) {
   if ((rc = tpf::pair_attn_status_fetch_and_clear(&v))) return rc;
   total |= v;
   if ((rc = tpf::norm_linear_dw_status_fetch_and_clear(&v))) return rc;
+  total |= v;
+  if ((rc = tpf::norm_linear_fwd_status_fetch_and_clear(&v))) return rc;
   total |= v;
   if ((rc = tpf::norm_linear_bwd_status_fetch_and_clear(&v))) return rc;
   total |= v;

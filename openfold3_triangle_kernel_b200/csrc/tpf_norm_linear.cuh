@@ -10,8 +10,10 @@ int64_t norm_linear_dw_workspace_bytes(int64_t rows, int64_t cols, int64_t outs)
 int norm_linear_dw(const NormArgs& norm, const void* d_out, int64_t outs, void* dw, int dw_type, void* workspace,
                    cudaStream_t stream);
 
-// The backward for narrow rows (tpf_norm_linear_bwd.cu): is it one, scratch, all gradients that g asks for.
+// Narrow rows: up to 128 columns and a weight that stays in shared memory.  Forward (tpf_norm_linear_fwd.cu; no scratch);
+// backward (tpf_norm_linear_bwd.cu): scratch, all gradients that g asks for.
 bool norm_linear_narrow(int64_t cols, int64_t outs);
+int norm_linear_narrow_fwd(const NormArgs& norm, const void* w, int64_t outs, void* out, float eps, cudaStream_t stream);
 int64_t norm_linear_narrow_bwd_workspace_bytes(int64_t rows, int64_t cols, int64_t outs);
 int norm_linear_narrow_bwd(const NormArgs& norm, const void* w, int64_t outs, const NormLinearGrads& g, void* workspace,
                            cudaStream_t stream);

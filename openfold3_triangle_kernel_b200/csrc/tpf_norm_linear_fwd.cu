@@ -1,0 +1,315 @@
+// Forward of the normalised projection for narrow rows (up to 128 columns, a weight that stays in shared memory) and for a
+// few rows.
+//
+// Narrow rows: a tile of 128 rows of x comes by TMA in the layout of a K-major operand, eight warps normalise it where it
+// lies (and write its codes, scales and statistics), the products with the resident weight go to TMEM, 128 outputs at a
+// time, and eight other warps store them.  x is read and out written once; y never leaves the SM.  As two kernels
+// 768 * 768 rows of 128 channels to 512 outputs took 195 us, with y written and read in between; the floor is 833 MB, 127.
+#include "tpf_gemm_host.cuh"
+#include "tpf_norm_linear.cuh"
+
+namespace tpf {
+
+namespace {
+
+__device__ int g_nl_fwd_status;
+
+constexpr int kNormWarps = 8, kStoreWarps = 8, kWarps = 2 + kNormWarps + kStoreWarps;
+constexpr int kBlock = 128 * 128;           // 128 rows of 64 bf16 columns
+constexpr int kWBytes = 128 * 1024;         // most of the weight
+constexpr int kSharedBytes = 1024;
+constexpr int kStaging = kStoreWarps * kTmaTiles;
+constexpr int kSmem = 227 * 1024;
+static_assert(kSharedBytes + kWBytes + kStaging + 2 * 2 * kBlock <= kSmem, "");
+
+struct FwdArgs {
+  NormArgs norm;  // codes, scales, mean and rstd are written where they are not nullptr
+  float eps;
+  int outs, tiles, w_rows;  // w_rows: outs rounded up to 64
+  int col_blocks;           // blocks of 64 columns: 1 or 2
+  int stages;               // tiles of x that shared memory holds
+};
+
+struct Shared {
+  uint64_t full[4], ready[4], empty[4], acc_full[4], acc_empty[4], w_full;
+  uint32_t tmem;
+  volatile int abort_flag;
+};
+static_assert(sizeof(Shared) <= kSharedBytes, "");
+
+template <bool KEEP>
+__global__ void __launch_bounds__(32 * kWarps, 1)
+    nl_fwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+                  const __grid_constant__ CUtensorMap tm_out, const __grid_constant__ FwdArgs a, int* __restrict__ status) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const int cb = a.col_blocks, x_bytes = cb * kBlock;
+  uint8_t* w_buf = smem;
+  uint8_t* ring = smem + a.w_rows * cb * 128;
+  uint8_t* staging = ring + a.stages * x_bytes;
+  Shared* sh = reinterpret_cast<Shared*>(smem + kSmem - kSharedBytes);
+  const WaitCtx wctx{&sh->abort_flag, status};
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(&sh->full[s], 1);
+      mbar_init(&sh->ready[s], kNormWarps);
+      mbar_init(&sh->empty[s], 1);
+      mbar_init(&sh->acc_full[s], 1);
+      mbar_init(&sh->acc_empty[s], kStoreWarps);
+    }
+    mbar_init(&sh->w_full, 1);
+    sh->abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tm_x);
+    tma_prefetch_desc(&tm_w);
+    tma_prefetch_desc(&tm_out);
+  }
+  if (warp == 1) {
+    tmem_alloc(&sh->tmem, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  griddep_wait();
+  const uint32_t tmem = sh->tmem;
+  const int count = (a.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;  // tiles of this CTA
+  const int chunks = (a.outs + 127) / 128;
+
+  if (warp == 0) {
+    const uint32_t el = elect_one();
+    int s = 0;
+    uint32_t ph = 1;
+    for (int t = 0; t < count; ++t) {
+      warp_wait(&sh->empty[s], ph, wctx);
+      mbar_expect_tx(el, &sh->full[s], x_bytes);
+      const int row = ((int)blockIdx.x + t * (int)gridDim.x) * 128;
+      for (int c = 0; c < cb; ++c) tma_load_3d(el, ring + s * x_bytes + c * kBlock, &tm_x, &sh->full[s], c * 64, row, 0);
+      if (t == 0) {  // the first tile is normalised meanwhile
+        mbar_expect_tx(el, &sh->w_full, a.w_rows * cb * 128);
+        for (int c = 0; c < cb; ++c)
+          for (int o = 0; o < a.w_rows; o += 64)
+            tma_load_3d(el, w_buf + (c * a.w_rows + o) * 128, &tm_w, &sh->w_full, c * 64, o, 0);
+      }
+      if (++s == a.stages) {
+        s = 0;
+        ph ^= 1;
+      }
+    }
+  } else if (warp == 1) {
+    const uint32_t el = elect_one();
+    const uint64_t a_desc = make_smem_desc(smem_u32(ring), 16, 1024, swizzle_mode_for_bytes(128));
+    const uint64_t b_desc = make_smem_desc(smem_u32(w_buf), 16, 1024, swizzle_mode_for_bytes(128));
+    const int steps = (a.norm.cols + 15) / 16;  // of 16 columns
+    warp_wait(&sh->w_full, 0, wctx);
+    int s = 0, acc = 0;
+    uint32_t ph = 0, acc_ph = 1;
+    for (int t = 0; t < count; ++t) {
+      warp_wait(&sh->ready[s], ph, wctx);
+      for (int j = 0; j < chunks; ++j) {
+        warp_wait(&sh->acc_empty[acc], acc_ph, wctx);
+        tc_fence_after();
+        const uint32_t idesc = make_idesc_bf16(128, min(128, a.w_rows - j * 128), false, false);
+        for (int k = 0; k < steps; ++k) {
+          const uint64_t ad = a_desc + ((s * x_bytes + (k >> 2) * kBlock + (k & 3) * 32) >> 4);
+          const uint64_t bd = b_desc + ((((k >> 2) * a.w_rows + j * 128) * 128 + (k & 3) * 32) >> 4);
+          umma_ss(el, tmem + acc * 128, ad, bd, idesc, k != 0 ? 1u : 0u);
+        }
+        umma_commit(el, &sh->acc_full[acc]);
+        if (++acc == 4) {
+          acc = 0;
+          acc_ph ^= 1;
+        }
+      }
+      umma_commit(el, &sh->empty[s]);
+      if (++s == a.stages) {
+        s = 0;
+        ph ^= 1;
+      }
+    }
+  } else if (warp < 2 + kNormWarps) {
+    // 16 lanes a row, eight columns each (of one block of 64 the lanes 0 .. 7); a warp has 16 rows, eight at a time.
+    const int wn = warp - 2, t16 = lane & 15, sub = lane >> 4, c = t16 * 8;
+    const bool on = c < a.norm.cols;
+    uint64_t w[4], b[4];
+    {
+      float f[8], h[8];
+      param_load<8, 1>(a.norm.w, c, a.norm.cols, 1.f, f);
+      param_load<8, 1>(a.norm.b, c, a.norm.cols, 0.f, h);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        w[e] = f2_pack(f[2 * e], f[2 * e + 1]);
+        b[e] = f2_pack(h[2 * e], h[2 * e + 1]);
+      }
+    }
+    const bool in_smem = (t16 >> 3) < cb;
+    int s = 0;
+    uint32_t ph = 0;
+    for (int t = 0; t < count; ++t) {
+      const int64_t row0 = (int64_t)((int)blockIdx.x + t * (int)gridDim.x) * 128;
+      uint8_t* tile = ring + s * x_bytes + (in_smem ? t16 >> 3 : 0) * kBlock;
+      warp_wait(&sh->full[s], ph, wctx);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        Piece<bf16, 8> raw[4];
+        uint64_t x[4][4];
+        float sum[4], mean[4], amax[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int r = wn * 16 + half * 8 + u * 2 + sub;
+          raw[u].load(reinterpret_cast<const bf16*>(tile + r * 128 + (((t16 & 7) ^ (r & 7)) << 4)));
+          if (!on) raw[u].zero();
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          float f[8];
+          raw[u].get(f);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[u][e] = f2_pack(f[2 * e], f[2 * e + 1]);
+          sum[u] = f2_sum(f2_add(f2_add(x[u][0], x[u][1]), f2_add(x[u][2], x[u][3])));
+          if constexpr (KEEP) {
+            amax[u] = raw[u].amax();
+#pragma unroll
+            for (int off = 8; off > 0; off >>= 1) amax[u] = max_nan(amax[u], __shfl_xor_sync(0xffffffffu, amax[u], off));
+          }
+        }
+        if (KEEP && a.norm.codes != nullptr) {
+          float up[4];
+          const float down = group_scales<4, 16>(amax, up);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            const int64_t row = row0 + wn * 16 + half * 8 + u * 2 + sub;
+            if (row < a.norm.rows && on) {
+              const uint64_t f = f2_dup(up[u]);
+              const bool good = up[u] == up[u];
+              *reinterpret_cast<uint2*>(a.norm.codes + row * a.norm.code_pitch + c) =
+                  make_uint2(pack_codes(x[u][0], x[u][1], f, good), pack_codes(x[u][2], x[u][3], f, good));
+            }
+          }
+          const int64_t row = row0 + wn * 16 + half * 8 + t16 * 2 + sub;  // lane n of a row's has the scale of its n-th row
+          if (t16 < 4 && row < a.norm.rows) a.norm.scales[row] = down;
+        }
+        warp_sum(sum, 16);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          mean[u] = sum[u] * a.norm.inv_cols;
+          const uint64_t m = f2_dup(-mean[u]);
+          uint64_t q = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[u][e] = on ? f2_add(x[u][e], m) : 0ull;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q = f2_fma(x[u][e], x[u][e], q);
+          sum[u] = f2_sum(q);
+        }
+        warp_sum(sum, 16);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int r = wn * 16 + half * 8 + u * 2 + sub;
+          const float rstd = rsqrtf(fmaf(sum[u], a.norm.inv_cols, a.eps));
+          if (KEEP && t16 == 0 && row0 + r < a.norm.rows) {
+            a.norm.mean[row0 + r] = mean[u];
+            a.norm.rstd[row0 + r] = rstd;
+          }
+          const uint64_t rs = f2_dup(rstd);
+          uint32_t o[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float lo, hi;
+            f2_unpack(f2_fma(f2_mul(x[u][e], rs), w[e], b[e]), lo, hi);
+            o[e] = pack_bf16x2(lo, hi);
+          }
+          // (columns behind the last: zeros, which is what TMA put there and the weight's rows have)
+          if (in_smem && on)
+            *reinterpret_cast<uint4*>(tile + r * 128 + (((t16 & 7) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh->ready[s]);
+      if (++s == a.stages) {
+        s = 0;
+        ph ^= 1;
+      }
+    }
+  } else {
+    // two warps a lane quarter, which take turns with the blocks of 32 outputs
+    const int ws = warp - 2 - kNormWarps, quarter = warp & 3;
+    uint8_t* tiles = staging + ws * kTmaTiles;
+    int buf = 0, acc = 0;
+    uint32_t ph = 0;
+    for (int t = 0; t < count; ++t) {
+      const int row = ((int)blockIdx.x + t * (int)gridDim.x) * 128 + quarter * 32;
+      for (int j = 0; j < chunks; ++j) {
+        warp_wait(&sh->acc_full[acc], ph, wctx);
+        tc_fence_after();
+        const int n = min(128, a.outs - j * 128);
+        uint32_t v[2][32];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int col = ((ws >> 2) + 2 * i) * 32;
+          if (col < n) tmem_ld32(tmem_addr(tmem, quarter * 32, acc * 128 + col), v[i]);
+        }
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh->acc_empty[acc]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int col = ((ws >> 2) + 2 * i) * 32;
+          if (col >= n) continue;
+          uint32_t pk[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) pk[e] = pack_bf16x2(__uint_as_float(v[i][2 * e]), __uint_as_float(v[i][2 * e + 1]));
+          warp_tile_store_tma<2>(tiles, buf, lane, pk, &tm_out, j * 128 + col, row, 0);
+        }
+        if (++acc == 4) {
+          acc = 0;
+          ph ^= 1;
+        }
+      }
+    }
+    bulk_wait_all();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace
+
+int norm_linear_fwd_status_fetch_and_clear(int* out) {
+  int v = 0, zero = 0;
+  TPF_CUDA_OK(cudaMemcpyFromSymbol(&v, g_nl_fwd_status, sizeof(int)));
+  if (v) TPF_CUDA_OK(cudaMemcpyToSymbol(g_nl_fwd_status, &zero, sizeof(int)));
+  *out = v;
+  return TPF_OK;
+}
+
+int norm_linear_narrow_fwd(const NormArgs& norm, const void* w, int64_t outs, void* out, float eps, cudaStream_t stream) {
+  const int64_t R = norm.rows, C = norm.cols;
+  const int cb = (int)((C + 63) / 64), w_rows = (int)((outs + 63) / 64 * 64);
+  int stages = (kSmem - kSharedBytes - kStaging - w_rows * cb * 128) / (cb * kBlock);
+  if (stages > 4) stages = 4;
+  const FwdArgs a{norm, eps, (int)outs, (int)((R + 127) / 128), w_rows, cb, stages};
+  CUtensorMap tm_x, tm_w, tm_out;
+  if (int rc = make_operand_tmap(&tm_x, norm.x, false, R, C, norm.x_pitch, 1, 0, 128, 128, 64)) return rc;
+  if (int rc = make_operand_tmap(&tm_w, w, false, outs, C, C, 1, 0, 128, 64, 64)) return rc;
+  if (int rc = make_store_tmap(&tm_out, out, outs, R, outs, 1, 0)) return rc;
+  int* status = nullptr;
+  static PerDeviceAddress status_at;
+  if (int rc = device_symbol_address(g_nl_fwd_status, status_at, reinterpret_cast<void**>(&status))) return rc;
+  const int grid = a.tiles < sm_count() ? a.tiles : sm_count();
+  const auto go = [&](auto kern, PerDeviceOnce& once) {
+    if (int rc = ensure_dynamic_smem(kern, kSmem, once, 1024)) return rc;
+    launch_kernel(kern, dim3(grid), dim3(32 * kWarps), kSmem, stream, tm_x, tm_w, tm_out, a, status);
+    TPF_LAUNCH_OK();
+    return (int)TPF_OK;
+  };
+  static PerDeviceOnce once_keep, once_plain;
+  return norm.mean != nullptr ? go(nl_fwd_kernel<true>, once_keep) : go(nl_fwd_kernel<false>, once_plain);
+}
+
+}  // namespace tpf

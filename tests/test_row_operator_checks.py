@@ -202,11 +202,13 @@ def test_norm_linear_backward_entry_refuses(kw, text):
 
 def test_norm_linear_entries_want_workspaces():
     with pytest.raises(C.TpfError, match="workspace of"):
-        _nl_fwd(rows=1000, wsb=0, ws=NULL)
+        _nl_fwd(rows=1000, cols=256, pitch=256, wsb=0, ws=NULL)
     with pytest.raises(C.TpfError, match="workspace of"):
         _nl_bwd(wsb=8)
     lib = C.load()
-    assert lib.tpf_norm_linear_fwd_workspace_bytes(0, 16, 8) == 0
+    assert lib.tpf_norm_linear_fwd_workspace_bytes(0, 256, 8) == 0
+    assert lib.tpf_norm_linear_fwd_workspace_bytes(1000, 256, 8) == 1000 * 256 * 2
+    assert lib.tpf_norm_linear_fwd_workspace_bytes(1000, 128, 512) == 0     # y stays on the SM
     assert lib.tpf_norm_linear_bwd_workspace_bytes(1000, 16, 8) % 256 == 0
 
 
