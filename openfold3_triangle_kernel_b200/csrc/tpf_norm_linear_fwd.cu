@@ -4,7 +4,9 @@
 // Narrow rows: a tile of 128 rows of x comes by TMA in the layout of a K-major operand, eight warps normalise it where it
 // lies (and write its codes, scales and statistics), the products with the resident weight go to TMEM, 128 outputs at a
 // time, and eight other warps store them.  x is read and out written once; y never leaves the SM.  As two kernels
-// 768 * 768 rows of 128 channels to 512 outputs took 195 us, with y written and read in between; the floor is 833 MB, 127.
+// 768 * 768 rows of 128 channels to 512 outputs, with codes, took 195 us, with y written and read in between; this takes
+// 145, the floor is 833 MB, 127.  With 128 outputs (97 us at 500000 rows, floor 49) the normalising warps are what it waits
+// for; sixteen of them took 90 there and 167 at 512 outputs, where the storing warps then lack issue slots.
 #include "tpf_gemm_host.cuh"
 #include "tpf_norm_linear.cuh"
 
@@ -17,7 +19,7 @@ __device__ int g_nl_fwd_status;
 constexpr int kNormWarps = 8, kStoreWarps = 8, kWarps = 2 + kNormWarps + kStoreWarps;
 constexpr int kBlock = 128 * 128;           // 128 rows of 64 bf16 columns
 constexpr int kWBytes = 128 * 1024;         // most of the weight
-constexpr int kSharedBytes = 1024;
+constexpr int kSharedBytes = 2048;           // barriers; from 1024 on the norm's weight and bias
 constexpr int kStaging = kStoreWarps * kTmaTiles;
 constexpr int kSmem = 227 * 1024;
 static_assert(kSharedBytes + kWBytes + kStaging + 2 * 2 * kBlock <= kSmem, "");
@@ -26,7 +28,6 @@ struct FwdArgs {
   NormArgs norm;  // codes, scales, mean and rstd are written where they are not nullptr
   float eps;
   int outs, tiles, w_rows;  // w_rows: outs rounded up to 64
-  int col_blocks;           // blocks of 64 columns: 1 or 2
   int stages;               // tiles of x that shared memory holds
 };
 
@@ -35,14 +36,14 @@ struct Shared {
   uint32_t tmem;
   volatile int abort_flag;
 };
-static_assert(sizeof(Shared) <= kSharedBytes, "");
+static_assert(sizeof(Shared) <= 1024, "");
 
-template <bool KEEP>
+template <bool KEEP, int CB>
 __global__ void __launch_bounds__(32 * kWarps, 1)
     nl_fwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                   const __grid_constant__ CUtensorMap tm_out, const __grid_constant__ FwdArgs a, int* __restrict__ status) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  const int cb = a.col_blocks, x_bytes = cb * kBlock;
+  constexpr int cb = CB, x_bytes = CB * kBlock;
   uint8_t* w_buf = smem;
   uint8_t* ring = smem + a.w_rows * cb * 128;
   uint8_t* staging = ring + a.stages * x_bytes;
@@ -68,10 +69,15 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
     tmem_alloc(&sh->tmem, 512);
     tmem_relinquish();
   }
+  griddep_wait();
+  float* params = reinterpret_cast<float*>(smem + kSmem - kSharedBytes + 1024);  // weight, bias
+  if (threadIdx.x < 256) {
+    const int i = threadIdx.x & 127;
+    param_load<1, 1>(threadIdx.x < 128 ? a.norm.w : a.norm.b, i, a.norm.cols, threadIdx.x < 128 ? 1.f : 0.f, params + threadIdx.x);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  griddep_wait();
   const uint32_t tmem = sh->tmem;
   const int count = (a.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;  // tiles of this CTA
   const int chunks = (a.outs + 127) / 128;
@@ -128,99 +134,125 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
       }
     }
   } else if (warp < 2 + kNormWarps) {
-    // 16 lanes a row, eight columns each (of one block of 64 the lanes 0 .. 7); a warp has 16 rows, eight at a time.
-    const int wn = warp - 2, t16 = lane & 15, sub = lane >> 4, c = t16 * 8;
-    const bool on = c < a.norm.cols;
-    uint64_t w[4], b[4];
-    {
-      float f[8], h[8];
-      param_load<8, 1>(a.norm.w, c, a.norm.cols, 1.f, f);
-      param_load<8, 1>(a.norm.b, c, a.norm.cols, 0.f, h);
+    // Eight lanes a row, eight columns of each block of 64, four rows side by side.  (With 16 lanes a row the sums took a
+    // step more, and what is done once a row weighed twice as much: 64 columns 54.7 us at 262144 rows and 256 outputs.)
+    constexpr int P = 4 * CB, ROWS = 128 / kNormWarps, U = 2;
+    const int wn = warp - 2, piece = lane & 7, sub = lane >> 3;
+    bool on[CB];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        w[e] = f2_pack(f[2 * e], f[2 * e + 1]);
-        b[e] = f2_pack(h[2 * e], h[2 * e + 1]);
-      }
-    }
-    const bool in_smem = (t16 >> 3) < cb;
+    for (int i = 0; i < CB; ++i) on[i] = i * 64 + piece * 8 < a.norm.cols;
     int s = 0;
     uint32_t ph = 0;
     for (int t = 0; t < count; ++t) {
-      const int64_t row0 = (int64_t)((int)blockIdx.x + t * (int)gridDim.x) * 128;
-      uint8_t* tile = ring + s * x_bytes + (in_smem ? t16 >> 3 : 0) * kBlock;
+      const int64_t row0 = (int64_t)((int)blockIdx.x + t * (int)gridDim.x) * 128 + wn * ROWS;
+      uint8_t* tile = ring + s * x_bytes + wn * ROWS * 128;
+      const int left = (int)(a.norm.rows - row0 < ROWS ? a.norm.rows - row0 : ROWS);  // rows that exist
       warp_wait(&sh->full[s], ph, wctx);
+#pragma unroll 1
+      for (int r0 = 0; r0 < ROWS; r0 += 4 * U) {
+        uint64_t x[U][P];
+        float sum[U], mean[U], amax[U];
+        uint8_t* at[U];  // of the lane's piece in the first block
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        Piece<bf16, 8> raw[4];
-        uint64_t x[4][4];
-        float sum[4], mean[4], amax[4];
+        for (int u = 0; u < U; ++u) {
+          const int r = r0 + u * 4 + sub;
+          at[u] = tile + r * 128 + ((piece ^ (r & 7)) << 4);
+          Piece<bf16, 8> raw[CB];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int r = wn * 16 + half * 8 + u * 2 + sub;
-          raw[u].load(reinterpret_cast<const bf16*>(tile + r * 128 + (((t16 & 7) ^ (r & 7)) << 4)));
-          if (!on) raw[u].zero();
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          float f[8];
-          raw[u].get(f);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[u][e] = f2_pack(f[2 * e], f[2 * e + 1]);
-          sum[u] = f2_sum(f2_add(f2_add(x[u][0], x[u][1]), f2_add(x[u][2], x[u][3])));
-          if constexpr (KEEP) {
-            amax[u] = raw[u].amax();
-#pragma unroll
-            for (int off = 8; off > 0; off >>= 1) amax[u] = max_nan(amax[u], __shfl_xor_sync(0xffffffffu, amax[u], off));
+          for (int i = 0; i < CB; ++i) {
+            raw[i].load(reinterpret_cast<const bf16*>(at[u] + i * kBlock));
+            if (!on[i]) raw[i].zero();
           }
-        }
-        if (KEEP && a.norm.codes != nullptr) {
-          float up[4];
-          const float down = group_scales<4, 16>(amax, up);
+          uint64_t q = 0;
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const int64_t row = row0 + wn * 16 + half * 8 + u * 2 + sub;
-            if (row < a.norm.rows && on) {
-              const uint64_t f = f2_dup(up[u]);
-              const bool good = up[u] == up[u];
-              *reinterpret_cast<uint2*>(a.norm.codes + row * a.norm.code_pitch + c) =
-                  make_uint2(pack_codes(x[u][0], x[u][1], f, good), pack_codes(x[u][2], x[u][3], f, good));
+          for (int i = 0; i < CB; ++i) {
+            float f[8];
+            raw[i].get(f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              x[u][i * 4 + e] = f2_pack(f[2 * e], f[2 * e + 1]);
+              q = f2_add(q, x[u][i * 4 + e]);
             }
           }
-          const int64_t row = row0 + wn * 16 + half * 8 + t16 * 2 + sub;  // lane n of a row's has the scale of its n-th row
-          if (t16 < 4 && row < a.norm.rows) a.norm.scales[row] = down;
+          sum[u] = f2_sum(q);
+          if constexpr (KEEP) amax[u] = CB == 2 ? max_nan(raw[0].amax(), raw[CB - 1].amax()) : raw[0].amax();
         }
-        warp_sum(sum, 16);
+        if (KEEP && a.norm.codes != nullptr) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+          for (int off = 4; off > 0; off >>= 1)
+#pragma unroll
+            for (int u = 0; u < U; ++u) amax[u] = max_nan(amax[u], __shfl_xor_sync(0xffffffffu, amax[u], off));
+          float up[U];
+          const float down = group_scales<U, 8>(amax, up);
+          int8_t* codes = a.norm.codes + (row0 + r0) * a.norm.code_pitch + piece * 8;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int r = u * 4 + sub;
+            const uint64_t f = f2_dup(up[u]);
+            const bool good = up[u] == up[u];
+#pragma unroll
+            for (int i = 0; i < CB; ++i)
+              if (r0 + r < left && on[i])
+                *reinterpret_cast<uint2*>(codes + r * a.norm.code_pitch + i * 64) =
+                    make_uint2(pack_codes(x[u][4 * i], x[u][4 * i + 1], f, good),
+                               pack_codes(x[u][4 * i + 2], x[u][4 * i + 3], f, good));
+          }
+          const int r = r0 + piece * 4 + sub;  // lane n of a row's has the scale of its n-th row
+          if (piece < U && r < left) a.norm.scales[row0 + r] = down;
+        }
+        warp_sum(sum, 8);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
           mean[u] = sum[u] * a.norm.inv_cols;
           const uint64_t m = f2_dup(-mean[u]);
           uint64_t q = 0;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) x[u][e] = on ? f2_add(x[u][e], m) : 0ull;
+          for (int i = 0; i < CB; ++i) {
+            if (!on[i]) continue;  // (its values stay zeros)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) q = f2_fma(x[u][e], x[u][e], q);
+            for (int e = 0; e < 4; ++e) {
+              x[u][i * 4 + e] = f2_add(x[u][i * 4 + e], m);
+              q = f2_fma(x[u][i * 4 + e], x[u][i * 4 + e], q);
+            }
+          }
           sum[u] = f2_sum(q);
         }
-        warp_sum(sum, 16);
+        warp_sum(sum, 8);
+        float rstd[U];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int r = wn * 16 + half * 8 + u * 2 + sub;
-          const float rstd = rsqrtf(fmaf(sum[u], a.norm.inv_cols, a.eps));
-          if (KEEP && t16 == 0 && row0 + r < a.norm.rows) {
+        for (int u = 0; u < U; ++u) {
+          const int r = r0 + u * 4 + sub;
+          rstd[u] = rsqrtf(fmaf(sum[u], a.norm.inv_cols, a.eps));
+          if (KEEP && piece == 0 && r < left) {
             a.norm.mean[row0 + r] = mean[u];
-            a.norm.rstd[row0 + r] = rstd;
+            a.norm.rstd[row0 + r] = rstd[u];
           }
-          const uint64_t rs = f2_dup(rstd);
-          uint32_t o[4];
+        }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float lo, hi;
-            f2_unpack(f2_fma(f2_mul(x[u][e], rs), w[e], b[e]), lo, hi);
-            o[e] = pack_bf16x2(lo, hi);
+        for (int i = 0; i < CB; ++i) {
+          if (!on[i]) continue;  // (columns behind the last: zeros, which is what TMA put there and the weight's rows have)
+          uint64_t w[4], b[4];
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            const float* q = params + i * 64 + piece * 8 + 2 * e;
+            const float4 f = *reinterpret_cast<const float4*>(q), h = *reinterpret_cast<const float4*>(q + 128);
+            w[e] = f2_pack(f.x, f.y);
+            w[e + 1] = f2_pack(f.z, f.w);
+            b[e] = f2_pack(h.x, h.y);
+            b[e + 1] = f2_pack(h.z, h.w);
           }
-          // (columns behind the last: zeros, which is what TMA put there and the weight's rows have)
-          if (in_smem && on)
-            *reinterpret_cast<uint4*>(tile + r * 128 + (((t16 & 7) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const uint64_t rs = f2_dup(rstd[u]);
+            uint32_t o[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float lo, hi;
+              f2_unpack(f2_fma(f2_mul(x[u][i * 4 + e], rs), w[e], b[e]), lo, hi);
+              o[e] = pack_bf16x2(lo, hi);
+            }
+            *reinterpret_cast<uint4*>(at[u] + i * kBlock) = make_uint4(o[0], o[1], o[2], o[3]);
+          }
         }
       }
       fence_async_smem();
@@ -293,7 +325,7 @@ int norm_linear_narrow_fwd(const NormArgs& norm, const void* w, int64_t outs, vo
   const int cb = (int)((C + 63) / 64), w_rows = (int)((outs + 63) / 64 * 64);
   int stages = (kSmem - kSharedBytes - kStaging - w_rows * cb * 128) / (cb * kBlock);
   if (stages > 4) stages = 4;
-  const FwdArgs a{norm, eps, (int)outs, (int)((R + 127) / 128), w_rows, cb, stages};
+  const FwdArgs a{norm, eps, (int)outs, (int)((R + 127) / 128), w_rows, stages};
   CUtensorMap tm_x, tm_w, tm_out;
   if (int rc = make_operand_tmap(&tm_x, norm.x, false, R, C, norm.x_pitch, 1, 0, 128, 128, 64)) return rc;
   if (int rc = make_operand_tmap(&tm_w, w, false, outs, C, C, 1, 0, 128, 64, 64)) return rc;
@@ -308,8 +340,9 @@ int norm_linear_narrow_fwd(const NormArgs& norm, const void* w, int64_t outs, vo
     TPF_LAUNCH_OK();
     return (int)TPF_OK;
   };
-  static PerDeviceOnce once_keep, once_plain;
-  return norm.mean != nullptr ? go(nl_fwd_kernel<true>, once_keep) : go(nl_fwd_kernel<false>, once_plain);
+  static PerDeviceOnce once[4];
+  if (norm.mean != nullptr) return cb == 2 ? go(nl_fwd_kernel<true, 2>, once[0]) : go(nl_fwd_kernel<true, 1>, once[1]);
+  return cb == 2 ? go(nl_fwd_kernel<false, 2>, once[2]) : go(nl_fwd_kernel<false, 1>, once[3]);
 }
 
 }  // namespace tpf
