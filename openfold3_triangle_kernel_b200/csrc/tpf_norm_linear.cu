@@ -32,7 +32,7 @@ int check_linear(const NormCall& c, const void* w, int64_t outs, const char* who
 }  // namespace
 
 int64_t norm_linear_fwd_workspace_bytes(int64_t rows, int64_t cols, int64_t outs) {
-  return norm_linear_narrow(cols, outs) ? 0 : up256(rows * cols * 2);
+  return norm_linear_few(rows) || norm_linear_narrow(cols, outs) ? 0 : up256(rows * cols * 2);
 }
 
 int norm_linear_fwd(const NormCall& norm, const void* w, int64_t outs, void* out, float eps, void* workspace,
@@ -42,12 +42,11 @@ int norm_linear_fwd(const NormCall& norm, const void* w, int64_t outs, void* out
   if (norm.rows == 0) return TPF_OK;
   TPF_REQUIRE(out != nullptr && norm.x != nullptr, TPF_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
   TPF_REQUIRE_ALIGNED16(out, who, "out");
-  if (norm_linear_narrow(norm.cols, outs)) {
-    NormArgs a;
-    if (int rc = make_norm_args(&a, norm, who)) return rc;
-    TPF_REQUIRE(norm.codes == nullptr || norm.mean != nullptr, TPF_ERR_INVALID_ARGUMENT, "%s: codes without mean and rstd", who);
-    return norm_linear_narrow_fwd(a, w, outs, out, eps, stream);
-  }
+  NormArgs a;
+  if (int rc = make_norm_args(&a, norm, who)) return rc;
+  TPF_REQUIRE(norm.codes == nullptr || norm.mean != nullptr, TPF_ERR_INVALID_ARGUMENT, "%s: codes without mean and rstd", who);
+  if (norm_linear_few(norm.rows)) return norm_linear_few_fwd(a, w, outs, out, eps, stream);
+  if (norm_linear_narrow(norm.cols, outs)) return norm_linear_narrow_fwd(a, w, outs, out, eps, stream);
   const int64_t need = norm_linear_fwd_workspace_bytes(norm.rows, norm.cols, outs);
   TPF_REQUIRE(workspace != nullptr && workspace_bytes >= need, TPF_ERR_WORKSPACE,
               "%s: workspace of %lld bytes required, %lld given", who, (long long)need, (long long)workspace_bytes);

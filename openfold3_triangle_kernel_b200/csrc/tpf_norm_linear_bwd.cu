@@ -151,7 +151,10 @@ __device__ __forceinline__ void grad_role(uint8_t* smem, Shared* sh, const WaitC
         m2[p] = f2_dup(CODES ? -mean[p] * rstd[p] : -mean[p]);
       }
       if (k + 2 < steps) stats(k + 2);
-      warp_wait2(&sh->full[s], ph, &sh->second_empty[group], ((k >> 1) & 1) ^ 1, wctx);
+      // In this order: with an odd number of stages a stage goes from group to group, and its barrier may be a phase further
+      // back than `ph` tells from the one before.  The products of step k - 2 are done, so that step k - STAGES has landed.
+      warp_wait(&sh->second_empty[group], ((k >> 1) & 1) ^ 1, wctx);
+      warp_wait(&sh->full[s], ph, wctx);
       const uint8_t* raw = ring + s * Cfg::STAGE + Cfg::A_BYTES;
       uint4 u[2][CODES ? 1 : 2];
 #pragma unroll

@@ -76,6 +76,13 @@ def _check(i, checkpoint=None, eps=1e-5, x_cuda=None, use=(True, True)):
     dw_off = d.abs().t() @ yk_off + (R + 64) * ro.U * (d.abs().t() @ ((xk * nwd).abs() + nbd.abs()))
     assert g["dw"].dtype == i["w"].dtype
     ro.check(g["dw"], d.t() @ yk, dw_off, "dw")
+    # The bounds above are for the worst signs, and wide where many rows are added.  Roundings are as often up as down: with
+    # at most three on a way, each H / sqrt(3) of its value in the root mean square, a whole result is off by about H.
+    for name, got, ref in (("out", out, y @ W.t()), ("dx", g["dx"], back["dx"]), ("dnw", g.get("dnw"), back["dw"]),
+                           ("dnb", g.get("dnb"), back["db"]), ("dw", g["dw"], d.t() @ yk)):
+        if got is not None:
+            off = (got.detach().cpu().double().view(ref.shape) - ref).norm() / ref.norm()
+            assert off < 2 * H, (name, float(off))
     assert C.device_status() == 0
     return out, g
 
@@ -97,6 +104,25 @@ def test_outputs(outs, cols):
 @pytest.mark.parametrize("checkpoint", [None, "int8"])
 def test_row_counts(rows, cols, outs, checkpoint):
     _check(_inputs(rows, cols, outs, seed=rows), checkpoint)
+
+
+@pytest.mark.parametrize("rows, cols, outs", [(66049, 96, 384), (66049, 64, 1024), (50000, 128, 512), (70001, 128, 104),
+                                              (9001, 200, 512)])
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_many_rows(rows, cols, outs, checkpoint):
+    """Every stage of the rings is used many times over; several runs, since what goes wrong there goes wrong now and then."""
+    i = _inputs(rows, cols, outs, seed=rows)
+    out, g = _check(i, checkpoint)
+    for _ in range(5):
+        again, h = _run(i, checkpoint)
+        assert torch.equal(out, again) and all(torch.equal(g[n], h[n]) for n in g)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("cols, outs", [(8, 8), (40, 2504), (136, 24), (1000, 4096), (1024, 520), (8192, 40)])
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_few_rows(rows, cols, outs, checkpoint):
+    _check(_inputs(rows, cols, outs, seed=rows + cols), checkpoint)
 
 
 @pytest.mark.parametrize("wdtype", [torch.float32, torch.float16])
