@@ -56,10 +56,6 @@ Rows as_vector_rows(const Tensor& t) {  // bf16 rows that start on 16-byte bound
   return r;
 }
 
-Tensor contiguous_as(const Tensor& g, at::ScalarType type) {
-  return (g.scalar_type() == type ? g : g.to(type)).contiguous();
-}
-
 using MaybeTensor = std::optional<Tensor>;
 Tensor value_or_none(const MaybeTensor& t) { return t ? t->detach().contiguous() : Tensor(); }
 void* ptr_of(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -160,8 +156,6 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
       // x itself where its rows were read in place, so that a change to it before the backward is noticed
       const Tensor kept_x = int8 ? Tensor() : x.t.data_ptr() == x_in.data_ptr() ? x_in : x.t;
       ctx->save_for_backward({kept_x, k.stats, k.codes, k.scales, w_in ? *w_in : Tensor(), b_in ? *b_in : Tensor()});
-      ctx->saved_data["sizes"] = x_in.sizes().vec();
-      ctx->saved_data["type"] = (int64_t)x_in.scalar_type();
     }
     return y;
   }
@@ -174,11 +168,10 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
     variable_list r(6);
     if (!grads[0].defined()) return r;
     const auto saved = ctx->get_saved_variables();
-    const auto sizes = ctx->saved_data["sizes"].toIntVector();
-    const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
     c10::cuda::CUDAGuard guard(grads[0].device());
     at::NoGradGuard no_grad;
-    const Tensor dy = contiguous_as(grads[0], type);
+    const Tensor dy = grads[0].contiguous();  // (the engine has seen to y's type and shape, which are x's)
+    const auto sizes = dy.sizes();
     const Tensor w = saved[4].defined() ? saved[4].contiguous() : Tensor(), &b = saved[5];
     const Rows x = saved[0].defined() ? as_rows(saved[0]) : Rows{};
     const tpf::NormCall c = kept_call(x, {saved[1], saved[2], saved[3]}, w, Tensor(), row_type(dy), sizes.back());
@@ -250,7 +243,6 @@ struct NormLinearFn : public torch::autograd::Function<NormLinearFn> {
       const Tensor kept_x = int8 ? Tensor() : x.t.data_ptr() == x_in.data_ptr() ? x_in : x.t;
       ctx->save_for_backward(
           {kept_x, k.stats, k.codes, k.scales, nw_in ? *nw_in : Tensor(), nb_in ? *nb_in : Tensor(), w_in});
-      ctx->saved_data["sizes"] = x_in.sizes().vec();
     }
     return out;
   }
@@ -263,10 +255,10 @@ struct NormLinearFn : public torch::autograd::Function<NormLinearFn> {
     variable_list r(7);
     if (!grads[0].defined()) return r;
     const auto saved = ctx->get_saved_variables();
-    const auto sizes = ctx->saved_data["sizes"].toIntVector();
     c10::cuda::CUDAGuard guard(grads[0].device());
     at::NoGradGuard no_grad;
     const Tensor d_out = aligned_bf16(grads[0]);
+    const std::vector<int64_t> sizes = with_last(d_out.sizes(), saved[6].size(1));
     const Tensor nw = saved[4].defined() ? saved[4].contiguous() : Tensor();
     const Tensor nb = saved[5].defined() ? saved[5].contiguous() : Tensor();
     const Rows x = saved[0].defined() ? as_vector_rows(saved[0]) : Rows{};
