@@ -30,6 +30,11 @@ def _groups(cols):
     return -(-cols // GROUP)
 
 
+def _countable(x):
+    cols = x.shape[-1]
+    return cols == 0 or (cols < 2 ** 31 - GROUP and x.numel() // cols * _groups(cols) < _MAX_GROUPS)
+
+
 def check_pack_support(x, *, check_device=True) -> SupportResult:
     """Metadata-only contract check of :func:`pack_activation`."""
     if not isinstance(x, torch.Tensor):
@@ -38,9 +43,7 @@ def check_pack_support(x, *, check_device=True) -> SupportResult:
         return SupportResult(False, "x_shape", "x must have shape [*,C]")
     if x.dtype not in ROW_DTYPES:
         return SupportResult(False, "x_dtype", "x must be BF16, FP16 or FP32")
-    cols = x.shape[-1]
-    rows = x.numel() // cols if cols else 0
-    if cols >= 2 ** 31 - GROUP or rows * _groups(cols) >= _MAX_GROUPS:
+    if not _countable(x):
         return SupportResult(False, "extent", "x must have fewer than 2^31 groups of 128 elements")
     if check_device:
         if not x.is_cuda:
@@ -56,6 +59,8 @@ def check_unpack_support(codes, scales, dtype, *, check_device=True) -> SupportR
         return SupportResult(False, "x_type", "codes and scales must be torch.Tensor instances")
     if codes.dtype != torch.int8 or scales.dtype != torch.float32:
         return SupportResult(False, "x_dtype", "codes must be int8 and scales FP32")
+    if codes.ndim >= 1 and not _countable(codes):
+        return SupportResult(False, "extent", "codes must have fewer than 2^31 groups of 128 elements")
     if codes.ndim < 1 or tuple(scales.shape) != tuple(codes.shape[:-1]) + (_groups(codes.shape[-1]),):
         return SupportResult(False, "x_shape", "scales must have one entry per 128 elements of a row of codes")
     if dtype not in ROW_DTYPES:
@@ -94,12 +99,12 @@ def _(codes, scales, dtype):
 def pack_activation(x):
     """``x [*, C]`` -> ``(codes int8 [*, C], scales fp32 [*, ceil(C / 128)])``."""
     if not torch.compiler.is_compiling():
-        res = check_pack_support(x)
-        if not res.supported:
-            raise ValueError(f"pack_activation unsupported [{res.code}]: {res.reason}")
         packed = C.native().int8_pack(x)
         if packed is not None:
             return packed
+        res = check_pack_support(x)
+        if not res.supported:
+            raise ValueError(f"pack_activation unsupported [{res.code}]: {res.reason}")
     codes, scales = torch.ops.tpf_b200.int8_pack(x.detach())
     return codes, scales
 
@@ -107,12 +112,12 @@ def pack_activation(x):
 def unpack_activation(codes, scales, dtype=torch.bfloat16):
     """The values that ``(codes, scales)`` of :func:`pack_activation` stand for, in ``dtype``."""
     if not torch.compiler.is_compiling():
-        res = check_unpack_support(codes, scales, dtype)
-        if not res.supported:
-            raise ValueError(f"unpack_activation unsupported [{res.code}]: {res.reason}")
         x = C.native().int8_unpack(codes, scales, dtype)
         if x is not None:
             return x
+        res = check_unpack_support(codes, scales, dtype)
+        if not res.supported:
+            raise ValueError(f"unpack_activation unsupported [{res.code}]: {res.reason}")
     return torch.ops.tpf_b200.int8_unpack(codes, scales.detach(), dtype)
 
 

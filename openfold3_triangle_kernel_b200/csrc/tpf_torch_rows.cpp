@@ -407,11 +407,17 @@ Tensor int8_unpack(const Tensor& codes_in, const Tensor& scales_in, int64_t type
   return x;
 }
 
+// Fewer groups and columns than the kernels can count?
+bool few_groups(const Tensor& x) {
+  const int64_t cols = x.size(-1);
+  return cols == 0 || (cols < (1ll << 31) - 128 && x.numel() / cols * ((cols + 127) / 128) < (1ll << 31) - 1024);
+}
+
 // The eager calls of the 8-bit checkpoint: None as above.
 py::object py_int8_pack(py::handle hx) {
   if (!plain_type(hx) || !plain_context()) return py::none();
   const Tensor& x = THPVariable_Unpack(hx.ptr());
-  if (!plain_cuda(x) || !device_supported(x) || row_type(x) < 0 || x.dim() < 1) return py::none();
+  if (!plain_cuda(x) || !device_supported(x) || row_type(x) < 0 || x.dim() < 1 || !few_groups(x)) return py::none();
   std::vector<Tensor> r;
   {
     py::gil_scoped_release release;
@@ -427,7 +433,7 @@ py::object py_int8_unpack(py::handle hc, py::handle hs, py::object dtype) {
   const auto type = reinterpret_cast<THPDtype*>(dtype.ptr())->scalar_type;
   if (!plain_cuda(codes) || !plain_cuda(scales) || !device_supported(codes) || scales.device() != codes.device() ||
       codes.scalar_type() != at::kChar || scales.scalar_type() != at::kFloat || codes.dim() < 1 ||
-      (type != at::kFloat && type != at::kBFloat16 && type != at::kHalf) ||
+      (type != at::kFloat && type != at::kBFloat16 && type != at::kHalf) || !few_groups(codes) ||
       scales.sizes().vec() != with_last(codes.sizes(), (codes.size(-1) + 127) / 128))
     return py::none();
   Tensor x;

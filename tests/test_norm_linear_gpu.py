@@ -140,6 +140,53 @@ def test_wide_rows():
     _check(_inputs(70, 8192, 64), "int8")
 
 
+def test_more_than_2_31_elements():
+    rows = 2 ** 24 + 5
+    x = torch.zeros(rows, 128, device="cuda", dtype=torch.bfloat16)
+    i = _inputs(9, 128, 8)
+    x[-9:] = i["x"].cuda()
+    d = torch.zeros(rows, 8, device="cuda", dtype=torch.bfloat16)
+    d[-9:] = i["d_out"].cuda()
+    nw, w = (i[n].cuda().requires_grad_(True) for n in ("nw", "w"))
+    x.requires_grad_(True)
+    for keep in (None, "int8"):
+        # the nine rows by themselves give the same products in another order of sums
+        small, g = _run(i, keep, use=(True, False))
+        out = tk.turbo_norm_linear(x, nw, None, w, checkpoint=keep)
+        gx, gn, gw = torch.autograd.grad(out, (x, nw, w), d)
+        assert torch.equal(out[-9:], small) and not out[:-9].any()
+        assert torch.equal(gx[-9:], g["dx"]) and not gx[:-9].any()
+        for a, b in ((gn, g["dnw"]), (gw, g["dw"])):
+            assert ((a.float() - b.float()).abs() <= 2 * H * b.float().abs() + 2 * 64 * ro.U * 9 * 16).all()
+        del out, gx
+
+
+def test_host_threads():
+    """Four threads with a stream each, different sizes at once."""
+    import threading
+
+    cases = [_inputs(r, c, o, seed=r) for r, c, o in ((700, 128, 512), (333, 64, 128), (90, 256, 136), (3, 128, 64))]
+    ref = [_run(c, "int8") for c in cases]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(k):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(10):
+                out, g = _run(cases[k], "int8")
+                stream.synchronize()
+                if not (torch.equal(out, ref[k][0]) and all(torch.equal(g[n], ref[k][1][n]) for n in g)):
+                    bad.append(k)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
 def test_layouts():
     i = _inputs(60, 128, 64)
     for first, pitch in ((0, 256), (8, 264), (3, 256), (0, 301)):
