@@ -47,7 +47,20 @@ __global__ void __launch_bounds__(Tm::MAXB, min_ctas<Tm, true>())
       rstd[r] = a.rstd[row];
     }
   };
+  // Three rounds ahead into L2: what a request waits for is then L2's latency (8192 rows of 4096 channels 51.3 -> 48.0 us,
+  // 5000 of 8192 61.4 -> 57.6; two rounds and five the same or less).
+  constexpr int AHEAD = 3;
+  auto prefetch = [&](int64_t first) {
+    if constexpr (Tm::VEC == 8) {
+      constexpr int NR = Tm::TEAMS * ROWS;
+      if (threadIdx.x != 0 || first + NR > a.rows) return;
+      bulk_prefetch(dy + first * a.cols, NR * a.cols * (int)sizeof(T));
+      if constexpr (CODES) bulk_prefetch(a.codes + first * a.code_pitch, NR * a.code_pitch);
+      else if (a.x_pitch == a.cols) bulk_prefetch(static_cast<const T*>(a.x) + first * a.x_pitch, NR * a.cols * (int)sizeof(T));
+    }
+  };
   request(base + tm.index * ROWS);
+  for (int k = 1; k < AHEAD; ++k) prefetch(base + k * step);
   uint64_t w[P], aw[P], ab[P];
   {
     float f[E];
@@ -62,6 +75,7 @@ __global__ void __launch_bounds__(Tm::MAXB, min_ctas<Tm, true>())
   // every team of a block makes the same number of rounds: the sums over a team are converged
   for (; base < a.rows; base += step) {
     const RowSet<ROWS> rows(base + tm.index * ROWS, a.rows);
+    prefetch(base + AHEAD * step);
     uint64_t d[ROWS][P], xh[ROWS][P];
     float rs[ROWS];
 #pragma unroll

@@ -212,13 +212,9 @@ __device__ __forceinline__ void tma_load_5d(uint32_t elected, void* dst, const C
       : "memory");
 }
 
-// A stretch of memory (both addresses and the size multiples of 16 bytes).
-__device__ __forceinline__ void bulk_load(uint32_t elected, void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile(
-      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %4, 0;\n\t"
-      "@q cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n\t}"
-      ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)), "r"(elected)
-      : "memory");
+// Brings a stretch of memory (address and size multiples of 16 bytes) into L2 only.
+__device__ __forceinline__ void bulk_prefetch(const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
 }
 
 // TMA tile stores (shared memory -> global).  Every lane that wrote the tile calls fence_async_smem() first; one lane
