@@ -10,7 +10,8 @@ Operator contract:
 * ``checkpoint``: as in :func:`turbo_layer_norm`.  Only x is kept, whole or in 8 bits: the normalised rows are made again
   in the backward pass, for the weight's gradient too.
 * returns bf16 ``[*, O]``; autograd for x, norm_weight, norm_bias and weight (first order only).  The normalised rows and
-  the gradient that reaches them are rounded to bf16 on their way to the tensor cores, sums are fp32.
+  the gradient that reaches them are rounded to bf16 on their way to the tensor cores, sums are fp32 (four rows and fewer
+  are not rounded on the way out).
 
 Unsupported inputs raise ``ValueError("turbo_norm_linear unsupported [code]: reason")``.  There is no counterpart among the
 reference's kernels (it calls torch's LayerNorm and Linear).
