@@ -30,7 +30,7 @@ constexpr int kSmemMax = 227 * 1024;
 struct BwdArgs {
   NormArgs norm;
   int64_t rows_per_range;
-  int outs, tiles, g_ctas, dx_ctas;  // of a range (0: not wanted)
+  int outs, g_ctas, dx_ctas;  // CTAs of a range (0: not wanted)
   int w_blocks;    // blocks of 64 outputs
   int col_blocks;  // blocks of 64 columns: 1 or 2
   int dx_stages, dx_kept;  // dx: blocks of d_out and tiles of kept rows that shared memory holds,
@@ -670,7 +670,7 @@ int norm_linear_narrow_bwd(const NormArgs& norm, const void* w, int64_t outs, co
   const int dx_kept = room - 2 * kept >= 4 * kATile ? 2 : 1;
   int dx_stages = (room - dx_kept * kept) / kATile;
   if (dx_stages > 8) dx_stages = 8;
-  const BwdArgs a{norm, p.rows_per_range, (int)outs, p.tiles, p.g_ctas, p.dx_ctas, w_blocks, col_blocks, dx_stages, dx_kept,
+  const BwdArgs a{norm, p.rows_per_range, (int)outs, p.g_ctas, p.dx_ctas, w_blocks, col_blocks, dx_stages, dx_kept,
                   dx_width, reinterpret_cast<float*>(base), reinterpret_cast<float*>(base + up256(z * outs * C * 4))};
   const int rc = p.mt == 2 ? (codes ? launch_bwd<2, true>(a, p, g.d_out, w, g.dx, stream)
                                     : launch_bwd<2, false>(a, p, g.d_out, w, g.dx, stream))

@@ -26,7 +26,7 @@ struct DwConfig {
   static constexpr bool CODES = CODES_;
   static constexpr int A_BYTES = MT * 128 * kRows * 2, RAW_BYTES = BN * kRows * (CODES ? 1 : 2), B_BYTES = BN * kRows * 2;
   static constexpr int STAGE = A_BYTES + RAW_BYTES;
-  static constexpr int STAGES = (227 * 1024 - 3072 - 2 * B_BYTES) / STAGE > 5 ? 5 : (227 * 1024 - 3072 - 2 * B_BYTES) / STAGE;
+  static constexpr int STAGES = (224 * 1024 - 2 * B_BYTES) / STAGE > 5 ? 5 : (224 * 1024 - 2 * B_BYTES) / STAGE;
   static constexpr int SMEM = STAGES * STAGE + 2 * B_BYTES + 2048;
   static constexpr int TMEM_COLS = MT * BN;
   static constexpr int WARPS = 10;  // TMA, UMMA, eight that make y~ and write the sums
@@ -371,8 +371,9 @@ int norm_linear_dw(const NormArgs& norm, const void* d_out, int64_t outs, void* 
   const bool codes = norm.codes != nullptr;
   if (p.mt == 2 && p.bn == 256) return codes ? dw_launch<2, 256, true>(a, p, d_out, stream) : dw_launch<2, 256, false>(a, p, d_out, stream);
   if (p.mt == 2) return codes ? dw_launch<2, 128, true>(a, p, d_out, stream) : dw_launch<2, 128, false>(a, p, d_out, stream);
-  if (p.bn == 256) return codes ? dw_launch<1, 256, true>(a, p, d_out, stream) : dw_launch<1, 256, false>(a, p, d_out, stream);
-  return codes ? dw_launch<1, 128, true>(a, p, d_out, stream) : dw_launch<1, 128, false>(a, p, d_out, stream);
+  // (128 outputs or fewer and 128 columns or fewer are a narrow projection)
+  TPF_REQUIRE(p.bn == 256, TPF_ERR_UNSUPPORTED, "norm_linear: a narrow projection");
+  return codes ? dw_launch<1, 256, true>(a, p, d_out, stream) : dw_launch<1, 256, false>(a, p, d_out, stream);
 }
 
 }  // namespace tpf
