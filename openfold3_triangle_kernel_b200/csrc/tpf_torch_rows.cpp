@@ -1,6 +1,9 @@
 // Row-wise operators for eager CUDA tensors: layer norm, 8-bit checkpoints, normalised projection.
 #include <torch/csrc/Dtype.h>
 
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
+
 #include "tpf_rows.h"
 #include "tpf_torch.h"
 #include "tpf_torch_trimul.h"
@@ -10,6 +13,19 @@ namespace tpf_torch {
 namespace {
 
 constexpr int64_t kMaxCols = 8192;  // of a layer norm (tpf_layer_norm_fwd)
+
+// Straight from the allocator of the current device: a tensor through the dispatcher costs 1.2 us, and a small training
+// pass makes six.
+Tensor make(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+struct Scratch {  // device memory of a call
+  c10::DataPtr p;
+  explicit Scratch(int64_t bytes) {
+    if (bytes > 0) p = c10::cuda::CUDACachingAllocator::get()->allocate(bytes);
+  }
+  void* get() const { return p.get(); }
+};
 
 cudaStream_t cu_stream() { return static_cast<cudaStream_t>(stream()); }
 
@@ -83,12 +99,12 @@ struct Kept {
 Kept make_kept(tpf::NormCall& c, const Tensor& like, bool save, bool int8) {
   Kept k;
   if (!save) return k;
-  k.stats = empty_f32({2, c.rows}, like);
+  k.stats = make({2, c.rows}, at::kFloat, like);
   c.mean = fptr(k.stats);
   c.rstd = c.mean + c.rows;
   if (int8) {
-    k.codes = at::empty({c.rows, tpf::code_pitch(c.cols)}, like.options().dtype(at::kChar));
-    k.scales = empty_f32({c.rows, (c.cols + 127) / 128}, like);
+    k.codes = make({c.rows, tpf::code_pitch(c.cols)}, at::kChar, like);
+    k.scales = make({c.rows, (c.cols + 127) / 128}, at::kFloat, like);
     c.codes = k.codes.data_ptr();
     c.scales = fptr(k.scales);
   }
@@ -117,13 +133,13 @@ tpf::NormCall kept_call(const Rows& x, const Kept& k, const Tensor& w, const Ten
   return c;
 }
 
-Tensor param_grad(const Tensor& p) { return at::empty(p.sizes(), p.options()); }
+Tensor param_grad(const Tensor& p) { return make(p.sizes(), p.scalar_type(), p); }
 
 Tensor layer_norm_out(const Rows& x, at::IntArrayRef sizes, const Tensor& w, const Tensor& b, double eps, Kept* kept,
                       bool int8) {
   tpf::NormCall c = norm_call(x, w, b);
   Kept k = make_kept(c, x.t, kept != nullptr, int8);
-  Tensor y = at::empty(sizes, x.t.options());
+  Tensor y = make(sizes, x.t.scalar_type(), x.t);
   check(tpf::layer_norm_fwd(c, y.data_ptr(), (float)eps, cu_stream()), "tpf_layer_norm_fwd");
   if (kept != nullptr) *kept = k;
   return y;
@@ -135,13 +151,13 @@ struct NormGradTensors {
 NormGradTensors layer_norm_grads(const tpf::NormCall& c, const Tensor& dy, at::IntArrayRef sizes, const Tensor& w,
                                  const Tensor& b, bool need_x, bool need_w, bool need_b) {
   NormGradTensors r;
-  if (need_x) r.dx = at::empty(sizes, dy.options());
+  if (need_x) r.dx = make(sizes, dy.scalar_type(), dy);
   if (need_w) r.dw = param_grad(w);
   if (need_b) r.db = param_grad(b);
   const int64_t n = need_w || need_b ? tpf_layer_norm_bwd_workspace_bytes(c.rows, c.cols) : 0;
-  Tensor ws = n > 0 ? empty_bytes(n, dy) : Tensor();
+  const Scratch ws(n);
   const tpf::NormGrads g{dy.data_ptr(), ptr_of(r.dx), ptr_of(r.dw), ptr_of(r.db), type_of(w), type_of(b)};
-  check(tpf::layer_norm_bwd(c, g, ptr_of(ws), n, cu_stream()), "tpf_layer_norm_bwd");
+  check(tpf::layer_norm_bwd(c, g, ws.get(), n, cu_stream()), "tpf_layer_norm_bwd");
   return r;
 }
 
@@ -201,10 +217,10 @@ Tensor norm_linear_out(const Rows& x, at::IntArrayRef sizes, const Tensor& nw, c
   tpf::NormCall c = norm_call(x, nw, nb);
   Kept k = make_kept(c, x.t, kept != nullptr, int8);
   const int64_t outs = w.size(0);
-  Tensor out = empty_bf16(with_last(sizes, outs), x.t);
+  Tensor out = make(with_last(sizes, outs), at::kBFloat16, x.t);
   const int64_t n = tpf_norm_linear_fwd_workspace_bytes(c.rows, c.cols, outs);
-  Tensor ws = n > 0 ? empty_bytes(n, x.t) : Tensor();
-  check(tpf::norm_linear_fwd(c, w.data_ptr(), outs, out.data_ptr(), (float)eps, ptr_of(ws), n, cu_stream()),
+  const Scratch ws(n);
+  check(tpf::norm_linear_fwd(c, w.data_ptr(), outs, out.data_ptr(), (float)eps, ws.get(), n, cu_stream()),
         "tpf_norm_linear_fwd");
   if (kept != nullptr) *kept = k;
   return out;
@@ -220,15 +236,15 @@ LinearGradTensors norm_linear_grads(const tpf::NormCall& c, const Tensor& d_out,
   LinearGradTensors r;
   const int64_t outs = w.size(0);
   const Tensor wb = as_bf16_matrix(w);
-  if (need_x) r.dx = at::empty(sizes, d_out.options());
+  if (need_x) r.dx = make(sizes, at::kBFloat16, d_out);
   if (need_nw) r.dnw = param_grad(nw);
   if (need_nb) r.dnb = param_grad(nb);
-  if (need_w) r.dw = at::empty({outs, c.cols}, w.options());
+  if (need_w) r.dw = make({outs, c.cols}, w.scalar_type(), w);
   const int64_t n = tpf_norm_linear_bwd_workspace_bytes(c.rows, c.cols, outs);
-  Tensor ws = n > 0 ? empty_bytes(n, d_out) : Tensor();
+  const Scratch ws(n);
   const tpf::NormLinearGrads g{d_out.data_ptr(), ptr_of(r.dx), ptr_of(r.dnw), ptr_of(r.dnb), type_of(nw), type_of(nb),
                                ptr_of(r.dw), row_type(w)};
-  check(tpf::norm_linear_bwd(c, wb.data_ptr(), outs, g, ptr_of(ws), n, cu_stream()), "tpf_norm_linear_bwd");
+  check(tpf::norm_linear_bwd(c, wb.data_ptr(), outs, g, ws.get(), n, cu_stream()), "tpf_norm_linear_bwd");
   return r;
 }
 
@@ -389,7 +405,7 @@ std::vector<Tensor> int8_pack(const Tensor& t) {
   c10::cuda::CUDAGuard guard(t.device());
   const Rows x = as_rows(t);
   std::vector<int64_t> groups = with_last(t.sizes(), (x.cols + 127) / 128);
-  Tensor codes = at::empty(t.sizes(), t.options().dtype(at::kChar)), scales = empty_f32(groups, t);
+  Tensor codes = make(t.sizes(), at::kChar, t), scales = make(groups, at::kFloat, t);
   check(tpf::int8_pack(x.t.data_ptr(), x.pitch, row_type(t), codes.data_ptr(), fptr(scales), x.rows, x.cols, cu_stream()),
         "tpf_int8_pack");
   return {codes, scales};
@@ -401,7 +417,7 @@ Tensor int8_unpack(const Tensor& codes_in, const Tensor& scales_in, int64_t type
   const int64_t cols = codes.size(-1);
   int64_t rows = 1;
   for (int64_t i = 0; i < codes.dim() - 1; ++i) rows *= codes.size(i);
-  Tensor x = at::empty(codes.sizes(), codes.options().dtype((at::ScalarType)type));
+  Tensor x = make(codes.sizes(), (at::ScalarType)type, codes);
   check(tpf::int8_unpack(codes.data_ptr(), fptr(scales), row_type(x), x.data_ptr(), rows, cols, cu_stream()),
         "tpf_int8_unpack");
   return x;
