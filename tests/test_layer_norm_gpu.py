@@ -58,7 +58,7 @@ def test_int8_checkpoint(cols, dtype):
     _check(_inputs(41, cols, DT[dtype], seed=cols + 1), checkpoint="int8")
 
 
-@pytest.mark.parametrize("rows", [1, 2, 3, 31, 64, 257, 4099])
+@pytest.mark.parametrize("rows", [1, 2, 3, 31, 33, 64, 65, 97, 257, 4099])
 @pytest.mark.parametrize("cols", [96, 128, 384, 1001])
 @pytest.mark.parametrize("checkpoint", [None, "int8"])
 def test_row_counts(rows, cols, checkpoint):
