@@ -1,12 +1,11 @@
 // Forward of the normalised projection for narrow rows (up to 128 columns, a weight that stays in shared memory) and for a
 // few rows.
 //
-// Narrow rows: a tile of 128 rows of x comes by TMA in the layout of a K-major operand, eight warps normalise it where it
+// Narrow rows: a tile of 128 rows of x comes by TMA in the layout of a K-major operand, some warps normalise it where it
 // lies (and write its codes, scales and statistics), the products with the resident weight go to TMEM, 128 outputs at a
 // time, and eight other warps store them.  x is read and out written once; y never leaves the SM.  As two kernels
 // 768 * 768 rows of 128 channels to 512 outputs, with codes, took 195 us, with y written and read in between; this takes
-// 145, the floor is 833 MB, 127.  With 128 outputs (97 us at 500000 rows, floor 49) the normalising warps are what it waits
-// for; sixteen of them took 90 there and 167 at 512 outputs, where the storing warps then lack issue slots.
+// 143, the floor is 833 MB, 127.
 #include "tpf_gemm_host.cuh"
 #include "tpf_norm_linear.cuh"
 
@@ -16,13 +15,19 @@ namespace {
 
 __device__ int g_nl_fwd_status;
 
-constexpr int kNormWarps = 8, kStoreWarps = 8, kWarps = 2 + kNormWarps + kStoreWarps;
+// Warps that normalise and warps that store.  With few outputs a tile waits for the former, with many for the latter, which
+// sixteen normalising warps keep from issuing (16 and 4 / 8 and 8, us: 500000 rows of 128 to 128 outputs 72 / 90, 262144 to
+// 256 50 / 57, 589824 to 512 166 / 143).
+template <int NORM_, int STORE_>
+struct Split {
+  static constexpr int NORM = NORM_, STORE = STORE_, WARPS = 2 + NORM + STORE;
+  static constexpr int STAGING = STORE * kTmaTiles;
+};
 constexpr int kBlock = 128 * 128;           // 128 rows of 64 bf16 columns
 constexpr int kWBytes = 128 * 1024;         // most of the weight
 constexpr int kSharedBytes = 2048;           // barriers; from 1024 on the norm's weight and bias
-constexpr int kStaging = kStoreWarps * kTmaTiles;
 constexpr int kSmem = 227 * 1024;
-static_assert(kSharedBytes + kWBytes + kStaging + 2 * 2 * kBlock <= kSmem, "");
+static_assert(kSharedBytes + kWBytes + Split<8, 8>::STAGING + 2 * 2 * kBlock <= kSmem, "");
 
 struct FwdArgs {
   NormArgs norm;  // codes, scales, mean and rstd are written where they are not nullptr
@@ -38,12 +43,12 @@ struct Shared {
 };
 static_assert(sizeof(Shared) <= 1024, "");
 
-template <bool KEEP, int CB>
-__global__ void __launch_bounds__(32 * kWarps, 1)
+template <bool KEEP, int CB, class Warps>
+__global__ void __launch_bounds__(32 * Warps::WARPS, 1)
     nl_fwd_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
                   const __grid_constant__ CUtensorMap tm_out, const __grid_constant__ FwdArgs a, int* __restrict__ status) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  constexpr int cb = CB, x_bytes = CB * kBlock;
+  constexpr int cb = CB, x_bytes = CB * kBlock, kNormWarps = Warps::NORM, kStoreWarps = Warps::STORE;
   uint8_t* w_buf = smem;
   uint8_t* ring = smem + a.w_rows * cb * 128;
   uint8_t* staging = ring + a.stages * x_bytes;
@@ -275,24 +280,31 @@ __global__ void __launch_bounds__(32 * kWarps, 1)
         warp_wait(&sh->acc_full[acc], ph, wctx);
         tc_fence_after();
         const int n = min(128, a.outs - j * 128);
-        uint32_t v[2][32];
+        // two blocks of 32 outputs at a time
+        constexpr int GROUPS = kStoreWarps / 4, ROUNDS = 2 / GROUPS;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int col = ((ws >> 2) + 2 * i) * 32;
-          if (col < n) tmem_ld32(tmem_addr(tmem, quarter * 32, acc * 128 + col), v[i]);
-        }
-        tmem_ld_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sh->acc_empty[acc]);
+        for (int q = 0; q < ROUNDS; ++q) {
+          uint32_t v[2][32];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int col = ((ws >> 2) + 2 * i) * 32;
-          if (col >= n) continue;
-          uint32_t pk[16];
+          for (int i = 0; i < 2; ++i) {
+            const int col = ((ws >> 2) + GROUPS * (2 * q + i)) * 32;
+            if (col < n) tmem_ld32(tmem_addr(tmem, quarter * 32, acc * 128 + col), v[i]);
+          }
+          tmem_ld_wait();
+          if (q == ROUNDS - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh->acc_empty[acc]);
+          }
 #pragma unroll
-          for (int e = 0; e < 16; ++e) pk[e] = pack_bf16x2(__uint_as_float(v[i][2 * e]), __uint_as_float(v[i][2 * e + 1]));
-          warp_tile_store_tma<2>(tiles, buf, lane, pk, &tm_out, j * 128 + col, row, 0);
+          for (int i = 0; i < 2; ++i) {
+            const int col = ((ws >> 2) + GROUPS * (2 * q + i)) * 32;
+            if (col >= n) continue;
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) pk[e] = pack_bf16x2(__uint_as_float(v[i][2 * e]), __uint_as_float(v[i][2 * e + 1]));
+            warp_tile_store_tma<2>(tiles, buf, lane, pk, &tm_out, j * 128 + col, row, 0);
+          }
         }
         if (++acc == 4) {
           acc = 0;
@@ -443,7 +455,9 @@ int norm_linear_fwd_status_fetch_and_clear(int* out) {
 int norm_linear_narrow_fwd(const NormArgs& norm, const void* w, int64_t outs, void* out, float eps, cudaStream_t stream) {
   const int64_t R = norm.rows, C = norm.cols;
   const int cb = (int)((C + 63) / 64), w_rows = (int)((outs + 63) / 64 * 64);
-  int stages = (kSmem - kSharedBytes - kStaging - w_rows * cb * 128) / (cb * kBlock);
+  const bool few_outs = outs <= 256;
+  const int staging = few_outs ? Split<16, 4>::STAGING : Split<8, 8>::STAGING;
+  int stages = (kSmem - kSharedBytes - staging - w_rows * cb * 128) / (cb * kBlock);
   if (stages > 4) stages = 4;
   const FwdArgs a{norm, eps, (int)outs, (int)((R + 127) / 128), w_rows, stages};
   CUtensorMap tm_x, tm_w, tm_out;
@@ -454,15 +468,20 @@ int norm_linear_narrow_fwd(const NormArgs& norm, const void* w, int64_t outs, vo
   static PerDeviceAddress status_at;
   if (int rc = device_symbol_address(g_nl_fwd_status, status_at, reinterpret_cast<void**>(&status))) return rc;
   const int grid = a.tiles < sm_count() ? a.tiles : sm_count();
-  const auto go = [&](auto kern, PerDeviceOnce& once) {
+  const auto go = [&](auto kern, int warps, PerDeviceOnce& once) {
     if (int rc = ensure_dynamic_smem(kern, kSmem, once, 1024)) return rc;
-    launch_kernel(kern, dim3(grid), dim3(32 * kWarps), kSmem, stream, tm_x, tm_w, tm_out, a, status);
+    launch_kernel(kern, dim3(grid), dim3(32 * warps), kSmem, stream, tm_x, tm_w, tm_out, a, status);
     TPF_LAUNCH_OK();
     return (int)TPF_OK;
   };
-  static PerDeviceOnce once[4];
-  if (norm.mean != nullptr) return cb == 2 ? go(nl_fwd_kernel<true, 2>, once[0]) : go(nl_fwd_kernel<true, 1>, once[1]);
-  return cb == 2 ? go(nl_fwd_kernel<false, 2>, once[2]) : go(nl_fwd_kernel<false, 1>, once[3]);
+  const auto by_split = [&](auto split, PerDeviceOnce* once) {
+    using S = decltype(split);
+    if (norm.mean != nullptr)
+      return cb == 2 ? go(nl_fwd_kernel<true, 2, S>, S::WARPS, once[0]) : go(nl_fwd_kernel<true, 1, S>, S::WARPS, once[1]);
+    return cb == 2 ? go(nl_fwd_kernel<false, 2, S>, S::WARPS, once[2]) : go(nl_fwd_kernel<false, 1, S>, S::WARPS, once[3]);
+  };
+  static PerDeviceOnce once[2][4];
+  return few_outs ? by_split(Split<16, 4>{}, once[0]) : by_split(Split<8, 8>{}, once[1]);
 }
 
 }  // namespace tpf
