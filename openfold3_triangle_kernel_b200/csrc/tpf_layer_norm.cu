@@ -85,7 +85,8 @@ __global__ void __launch_bounds__(Tm::MAXB, min_ctas<Tm, false>()) norm_fwd_kern
       // of the lanes that hold a group, number n (mod N) has the scale of group n
       const int mine = threadIdx.x & (N - 1), first = threadIdx.x & (Groups<Tm>::LANES - 1);
       const int r = mine / NG, g = mine % NG;
-      const int c0 = tm.column(0) + (Tm::VEC == 8 ? g * 32 * 8 - first * 8 : g * 128 - first);  // first column of the group
+      // first column of the group
+      const int c0 = tm.column(0) + (Tm::VEC == 8 ? (g * (Tm::BLOCK ? 32 : Tm::TS) - first) * 8 : g * 128 - first);
       if (first == mine && r < rows.count && c0 < a.cols) a.scales[(rows.first + r) * a.groups + c0 / kGroup] = down;
     }
     float sum[ROWS], mean[ROWS];
@@ -177,6 +178,14 @@ struct FwdLaunch {
   int by_width(int cols, bool vec) const {
     if (vec) {
       if (cols <= 32) return run<T, Team<8, 4, 1>>();
+      // 16-bit types: half the lanes with two pieces each, which saves a step of every sum over the team and shares the
+      // bookkeeping of a row (768 * 768 rows of 128 bf16 channels: 49.8 us against 50.5, with codes 60.0 against 63.4;
+      // 147456 rows 11.4 against 12.5).  32-bit ones have no registers for it (300000 rows with codes: 59 against 57).
+      if constexpr (sizeof(T) == 2) {
+        if (cols <= 64) return run<T, Team<8, 4, 2>>();
+        if (cols <= 128) return run<T, Team<8, 8, 2>>();
+        if (cols <= 256) return run<T, Team<8, 16, 2>>();
+      }
       if (cols <= 64) return run<T, Team<8, 8, 1>>();
       if (cols <= 128) return run<T, Team<8, 16, 1>>();
       if (cols <= 256) return run<T, Team<8, 32, 1>>();

@@ -298,7 +298,7 @@ __device__ __forceinline__ void team_sum(float (&v)[N], float* red, int& turn) {
   }
 }
 
-// Groups of 128 a thread takes part in: VEC = 8: one a piece (fewer where a team is narrower than a group), VEC = 1: one per
+// Groups of 128 a thread takes part in: VEC = 8: one a piece (a team narrower than 16 lanes: one of all pieces), VEC = 1: one per
 // four items; LANES lanes share one.
 template <class Tm>
 struct Groups {
@@ -401,8 +401,9 @@ __device__ __forceinline__ void store_codes(int8_t* row, const uint64_t (&x)[Tm:
   } else {
 #pragma unroll
     for (int i = 0; i < Tm::ITEMS; ++i) {
-      const uint64_t u = f2_dup(up[i]);
-      const bool good = up[i] == up[i];
+      const float f = up[i * Groups<Tm>::N / Tm::ITEMS];
+      const uint64_t u = f2_dup(f);
+      const bool good = f == f;
       if (on[i])
         *reinterpret_cast<uint2*>(row + at[i]) =
             make_uint2(pack_codes(x[4 * i], x[4 * i + 1], u, good), pack_codes(x[4 * i + 2], x[4 * i + 3], u, good));
