@@ -19,7 +19,7 @@ int check_linear(const NormCall& c, const void* w, int64_t outs, const char* who
   TPF_REQUIRE(c.type == kRowBF16, TPF_ERR_UNSUPPORTED, "%s: bf16 only", who);
   TPF_REQUIRE(c.cols >= 8 && c.cols <= kMaxNormCols && c.cols % 8 == 0 && outs >= 8 && outs % 8 == 0, TPF_ERR_UNSUPPORTED,
               "%s: columns and outputs must be multiples of 8, columns at most %lld", who, (long long)kMaxNormCols);
-  TPF_REQUIRE(c.rows >= 0 && c.rows < (1ll << 31) - 256 && outs < (1ll << 31) - 256, TPF_ERR_UNSUPPORTED,
+  TPF_REQUIRE(c.rows >= 0 && c.rows < (1ll << 31) - 256 && outs <= (1ll << 30), TPF_ERR_UNSUPPORTED,
               "%s: extent too large", who);
   TPF_REQUIRE(w != nullptr, TPF_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
   TPF_REQUIRE_ALIGNED16(w, who, "weight");

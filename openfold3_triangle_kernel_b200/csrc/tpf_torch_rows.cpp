@@ -13,6 +13,7 @@ namespace tpf_torch {
 namespace {
 
 constexpr int64_t kMaxCols = 8192;  // of a layer norm (tpf_layer_norm_fwd)
+constexpr int64_t kMaxLinearRows = (1ll << 31) - 256, kMaxOuts = 1ll << 30;  // of a projection (tpf_norm_linear_fwd)
 
 // Straight from the allocator of the current device: a tensor through the dispatcher costs 1.2 us, and a small training
 // pass makes six.
@@ -334,7 +335,9 @@ py::object py_norm_linear(py::handle hx, py::handle hnw, py::handle hnb, py::han
       w.device() != x.device() || w.dim() != 2 || row_type(w) < 0 || !(eps >= 0))
     return py::none();
   const int64_t cols = x.size(-1), outs = w.size(0);
-  if (cols < 8 || cols % 8 || cols > kMaxCols || w.size(1) != cols || outs < 8 || outs % 8) return py::none();
+  if (cols < 8 || cols % 8 || cols > kMaxCols || w.size(1) != cols || outs < 8 || outs % 8 || outs > kMaxOuts ||
+      x.numel() / cols >= kMaxLinearRows)
+    return py::none();
   MaybeTensor nw, nb;
   if (!unpack_param(hnw, x, cols, nw) || !unpack_param(hnb, x, cols, nb)) return py::none();
   const bool save =

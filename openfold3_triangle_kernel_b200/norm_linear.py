@@ -6,7 +6,8 @@ Operator contract:
 
 * ``x``: bf16 ``[*, C]``, C a multiple of 8 up to 8192; ``weight``: ``[O, C]``, O a multiple of 8, bf16, fp16 or fp32
   (rounded to bf16 inside, like the projections of :func:`turbo_trimul`); ``norm_weight``, ``norm_bias``: as in
-  :func:`turbo_layer_norm`.  Projections that share an input (q, k, v, gate) go into one weight.
+  :func:`turbo_layer_norm`.  Projections that share an input (q, k, v, gate) go into one weight.  Fewer than 2^31 - 256
+  rows, at most 2^30 outputs.
 * ``checkpoint``: as in :func:`turbo_layer_norm`.  Only x is kept, whole or in 8 bits: the normalised rows are made again
   in the backward pass, for the weight's gradient too.
 * returns bf16 ``[*, O]``; autograd for x, norm_weight, norm_bias and weight (first order only).  The normalised rows and
@@ -27,6 +28,9 @@ from . import _cabi as C
 from .layer_norm import CHECKPOINTS, ROW_DTYPES, check_parameter, check_rows, kept_like
 from .trimul import SupportResult
 
+MAX_ROWS = 2 ** 31 - 256
+MAX_OUTPUTS = 2 ** 30
+
 
 def check_norm_linear_support(x, norm_weight, norm_bias, weight, eps=1e-5, checkpoint=None, *,
                               check_device=True) -> SupportResult:
@@ -41,6 +45,8 @@ def check_norm_linear_support(x, norm_weight, norm_bias, weight, eps=1e-5, check
         return SupportResult(False, "columns", f"C={cols} is not a multiple of 8")
     if not isinstance(weight, torch.Tensor) or weight.ndim != 2 or weight.shape[1] != cols:
         return SupportResult(False, "weight_shape", f"weight must have shape (O, {cols})")
+    if math.prod(x.shape[:-1]) >= MAX_ROWS or weight.shape[0] > MAX_OUTPUTS:
+        return SupportResult(False, "extent", f"at most {MAX_ROWS - 1} rows and {MAX_OUTPUTS} outputs")
     if weight.shape[0] < 8 or weight.shape[0] % 8:
         return SupportResult(False, "outputs", f"O={weight.shape[0]} is not a positive multiple of 8")
     if weight.dtype not in ROW_DTYPES:

@@ -47,6 +47,8 @@ def test_layer_norm_support_accepts():
     (dict(weight=torch.zeros(16)), "weight_shape"),
     (dict(weight=torch.zeros(12, 16)), "outputs"),
     (dict(weight=torch.zeros(0, 16)), "outputs"),
+    (dict(weight=torch.zeros(1).expand(2 ** 30 + 8, 16)), "extent"),
+    (dict(x=torch.zeros(1).bfloat16().expand(2 ** 31 - 256, 16)), "extent"),
     (dict(weight=torch.zeros(8, 16, dtype=torch.int8)), "weight_dtype"),
     (dict(norm_weight=torch.zeros(8)), "weight_shape"),
     (dict(norm_bias=torch.zeros(16, dtype=torch.float64)), "weight_dtype"),
@@ -175,6 +177,7 @@ def _nl_fwd(**kw):
     (dict(w=NULL), "null pointer"), (dict(x=NULL), "null pointer"), (dict(out=NULL), "null pointer"),
     (dict(w=ctypes.c_void_p(264)), "weight must be 16-byte aligned"), (dict(out=ctypes.c_void_p(264)), "out must be 16-byte"),
     (dict(x=ctypes.c_void_p(258)), "x must"), (dict(pitch=20), "x must"), (dict(rows=1 << 31), "too large"),
+    (dict(outs=(1 << 30) + 8), "too large"),  # (a few rows: outputs are counted in 32 bits, up to a grid's more than there are)
 ])
 def test_norm_linear_forward_entry_refuses(kw, text):
     with pytest.raises(ValueError, match=text):
