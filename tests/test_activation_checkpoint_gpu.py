@@ -184,3 +184,29 @@ def test_context_around_the_framework_operators():
     assert m1 < m0
     # each kept value is off by a / 254 of its group, about 1 % of a typical one; three of them enter each gradient
     assert (g1 - g0).norm() / g0.norm() < 0.04
+
+
+def test_context_inside_a_capture():
+    """What is packed while a graph is captured is packed again by every replay."""
+    w = torch.randn(64, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    x = torch.randn(100, 64, device="cuda", dtype=torch.bfloat16)
+    d = torch.randn(100, 64, device="cuda", dtype=torch.bfloat16)
+
+    def step():
+        with tk.int8_activations(min_elements=1000):
+            y = torch.tanh(x * 2) @ w
+        return torch.autograd.grad(y, w, d)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for seed in (1, 2):
+        x.copy_(torch.randn(100, 64, generator=torch.Generator().manual_seed(seed)))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, step())

@@ -326,6 +326,39 @@ def test_two_captured_training_passes(checkpoint):
     assert torch.equal(got[0], ref[2][0]) and torch.equal(got[4], ref[2][1]["dw"])
 
 
+@pytest.mark.parametrize("rows, cols, outs", [(3, 200, 72), (1500, 264, 136), (900, 64, 1024)])
+def test_captured_replays_follow_the_inputs(rows, cols, outs):
+    """The route of a few rows, of wide ones, and of a weight that fills shared memory; other work runs between the replays."""
+    cases = [_inputs(rows, cols, outs, seed=s) for s in (1, 2)]
+    ref = [_run(c, "int8") for c in cases]
+    leaves = [cases[0][n].cuda().requires_grad_(True) for n in ("x", "nw", "nb", "w")]
+    d = cases[0]["d_out"].cuda()
+
+    def step():
+        out = tk.turbo_norm_linear(*leaves, checkpoint="int8")
+        return (out.detach(), *torch.autograd.grad(out, leaves, d))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for k in (0, 1, 0):
+        with torch.no_grad():
+            for v, n in zip(leaves, ("x", "nw", "nb", "w")):
+                v.copy_(cases[k][n].cuda())
+            d.copy_(cases[k]["d_out"].cuda())
+        graph.replay()
+        other = _run(cases[1 - k], "int8")
+        torch.cuda.synchronize()
+        for have, (out, g) in ((got, ref[k]), ((other[0], *(other[1][n] for n in ("dx", "dnw", "dnb", "dw"))), ref[1 - k])):
+            assert torch.equal(have[0], out)
+            assert all(torch.equal(a, g[n]) for a, n in zip(have[1:], ("dx", "dnw", "dnb", "dw")))
+
+
 @pytest.mark.parametrize("checkpoint", [None, "int8"])
 def test_traced_route_matches_eager(checkpoint):
     i = _inputs(60, 96, 64)
