@@ -258,7 +258,7 @@ int tpf_layer_norm_fwd(const void* x, int64_t x_pitch, int type, const void* wei
 
 /* Its backward pass: dx (of `type`, contiguous, may be NULL), dweight and dbias [cols] (of their types, may be NULL; zeros
  * for no rows).  dy is contiguous.  x is taken from codes and scales when they are given (x may be NULL then).
- * Deterministic: fixed summation orders.  workspace: 4-byte aligned, needed for dweight and dbias only. */
+ * Deterministic: fixed summation orders.  workspace: 16-byte aligned, needed for dweight and dbias only. */
 int64_t tpf_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t cols);
 int tpf_layer_norm_bwd(const void* dy, const void* x, int64_t x_pitch, const void* codes, const float* scales, int type,
                        const float* mean, const float* rstd, const void* weight, int weight_type, void* dx, void* dweight,

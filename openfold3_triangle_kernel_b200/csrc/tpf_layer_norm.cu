@@ -179,7 +179,7 @@ struct FwdLaunch {
     if (vec) {
       if (cols <= 32) return run<T, Team<8, 4, 1>>();
       // 16-bit types: half the lanes with two pieces each, which saves a step of every sum over the team and shares the
-      // bookkeeping of a row (768 * 768 rows of 128 bf16 channels: 49.8 us against 50.5, with codes 60.0 against 63.4;
+      // bookkeeping of a row (768 * 768 rows of 128 bf16 channels: 49.7 us against 50.6, with codes 62.8 against 63.5;
       // 147456 rows 11.4 against 12.5).  32-bit ones have no registers for it (300000 rows with codes: 59 against 57).
       if constexpr (sizeof(T) == 2) {
         if (cols <= 64) return run<T, Team<8, 4, 2>>();

@@ -159,9 +159,19 @@ __global__ void __launch_bounds__(Tm::MAXB, min_ctas<Tm, true>())
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
       const int c = tm.column(i);
-      if (c < a.cols)
+      if (c >= a.cols) continue;
+      if (Tm::VEC == 8 && out.terms != nullptr) {  // (element by element: 10 us at 296 CTAs of 4096 columns)
+        float* t = out.terms + (int64_t)blockIdx.x * 2 * a.cols + c;
 #pragma unroll
-        for (int e = 0; e < Tm::VEC; ++e) out.put(a.cols, c + e, fw[i * Tm::VEC + e], fb[i * Tm::VEC + e]);
+        for (int e = 0; e < Tm::VEC; e += 4) {
+          const int k = i * Tm::VEC + e;
+          *reinterpret_cast<float4*>(t + e) = make_float4(fw[k], fw[k + 1], fw[k + 2], fw[k + 3]);
+          *reinterpret_cast<float4*>(t + a.cols + e) = make_float4(fb[k], fb[k + 1], fb[k + 2], fb[k + 3]);
+        }
+        continue;
+      }
+#pragma unroll
+      for (int e = 0; e < Tm::VEC; ++e) out.put(a.cols, c + e, fw[i * Tm::VEC + e], fb[i * Tm::VEC + e]);
     }
   } else {
     // the teams of a warp, then the warps one after the other
@@ -313,8 +323,7 @@ int layer_norm_bwd(const NormCall& c, const NormGrads& g, void* workspace, int64
   const int64_t need = layer_norm_bwd_workspace_bytes(c.rows, c.cols);
   TPF_REQUIRE(!params || (workspace != nullptr && workspace_bytes >= need), TPF_ERR_WORKSPACE,
               "layer_norm_bwd: workspace of %lld bytes required, %lld given", (long long)need, (long long)workspace_bytes);
-  TPF_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 3) == 0, TPF_ERR_INVALID_ARGUMENT,
-              "layer_norm_bwd: misaligned workspace");
+  TPF_REQUIRE_ALIGNED16(workspace, "layer_norm_bwd", "workspace");
   const bool from_codes = c.codes != nullptr;
   const bool vec = c.cols % 8 == 0 && (from_codes ? (reinterpret_cast<uintptr_t>(c.codes) & 15) == 0
                                                   : rows_vec_ok(c.x, c.x_pitch, c.type)) &&
