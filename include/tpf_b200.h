@@ -276,8 +276,8 @@ int tpf_int8_unpack(const void* codes, const float* scales, int type, void* x, i
 
 /* Normalised projection out = layer_norm(x) weight^T: x bf16 [rows, cols] (16-byte aligned rows), weight bf16 [outs, cols],
  * out bf16 [rows, outs], cols and outs multiples of 8, cols <= 8192, rows < 2^31 - 256, outs <= 2^30.  The norm's arguments
- * are those of tpf_layer_norm_fwd and _bwd.  d_weight is [outs, cols] of its own type; gradients whose pointer is NULL are
- * not computed.  Workspaces are 16-byte aligned and sized for the current device; where the size is 0 it may be NULL. */
+ * are those of tpf_layer_norm_fwd and _bwd.  d_weight is [outs, cols] of its own type, 16-byte aligned; gradients whose
+ * pointer is NULL are not computed.  Workspaces are sized for the current device; where the size is 0 they may be NULL. */
 int64_t tpf_norm_linear_fwd_workspace_bytes(int64_t rows, int64_t cols, int64_t outs);
 int64_t tpf_norm_linear_bwd_workspace_bytes(int64_t rows, int64_t cols, int64_t outs);
 int tpf_norm_linear_fwd(const void* x, int64_t x_pitch, const void* norm_weight, int norm_weight_type,

@@ -71,6 +71,7 @@ int norm_linear_bwd(const NormCall& norm, const void* w, int64_t outs, const Nor
               TPF_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
   TPF_REQUIRE_ALIGNED16(g.d_out, who, "d_out");
   TPF_REQUIRE_ALIGNED16(g.dx, who, "dx");
+  TPF_REQUIRE_ALIGNED16(g.dw, who, "d_weight");
   TPF_REQUIRE(g.dw == nullptr || row_type_ok(g.dw_type), TPF_ERR_INVALID_ARGUMENT, "%s: unknown parameter type", who);
   const int64_t need = norm_linear_bwd_workspace_bytes(norm.rows, norm.cols, outs);
   TPF_REQUIRE(norm.rows == 0 || (workspace != nullptr && workspace_bytes >= need), TPF_ERR_WORKSPACE,

@@ -55,6 +55,7 @@ struct GradConfig {
   static constexpr int B_BYTES = 3 * kChunk;  // up to 128 columns of xh~, a block whose first column is ones
   static constexpr int FIT = (kSmemMax - kSharedBytes - 2 * B_BYTES) / STAGE, STAGES = FIT > 6 ? 6 : FIT;
   static constexpr int SMEM = kSharedBytes + 2 * B_BYTES + STAGES * STAGE;
+  static_assert(kWorkers * kBlockStaging <= SMEM - kSharedBytes, "");
   static constexpr int TMEM = MT == 2 ? 512 : 256;  // 256 columns a tile: up to 144 are used
 };
 
@@ -219,17 +220,17 @@ __device__ __forceinline__ void grad_role(uint8_t* smem, Shared* sh, const WaitC
     const int i = MT == 2 ? share & 1 : 0;
     const int o = m0 + i * 128 + quarter * 32 + lane;
     const uint32_t t = tmem_addr(sh->tmem, quarter * 32, i * 256);
-    float* g = a.g + ((int64_t)range * a.outs + o) * a.norm.cols;
+    float* g = a.g + ((int64_t)range * a.outs + o - lane) * a.norm.cols;
 #pragma unroll 1
     for (int c = 32 * (MT == 2 ? share >> 1 : share); c < a.norm.cols; c += MT == 2 ? 64 : 128) {
       uint32_t v[32];
       tmem_ld32(t + c, v);
       tmem_ld_wait();
-#pragma unroll
-      for (int e = 0; e < 32; e += 4)
-        if (o < a.outs && c + e < a.norm.cols)
-          *reinterpret_cast<uint4*>(g + c + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-      __syncwarp();
+      // (the stages and the buffers of xh~ are all used up)
+      put_block(smem + wk * kBlockStaging, v, lane, [&](int r, int e, const float4& x) {
+        if (o - lane + r < a.outs && c + e < a.norm.cols)
+          *reinterpret_cast<float4*>(g + (int64_t)r * a.norm.cols + c + e) = x;
+      });
     }
     if (share < MT) {
       uint32_t v[8];

@@ -30,6 +30,7 @@ struct DwConfig {
   static constexpr int SMEM = STAGES * STAGE + 2 * B_BYTES + 2048;
   static constexpr int TMEM_COLS = MT * BN;
   static constexpr int WARPS = 10;  // TMA, UMMA, eight that make y~ and write the sums
+  static_assert(8 * kBlockStaging <= STAGES * STAGE, "");
   static_assert(STAGES >= 2 && TMEM_COLS >= 128 && TMEM_COLS <= 512, "");
 };
 
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(32 * Cfg::WARPS, 1)
     tc_fence_after();
     const int quarter = warp & 3, half = w8 >> 2;
     constexpr int COLS = MT == 2 ? BN : BN / 2;  // of a warp
-    const int o = m0 + (MT == 2 ? half * 128 : 0) + quarter * 32 + lane;
+    const int o = m0 + (MT == 2 ? half * 128 : 0) + quarter * 32;  // first output of the warp
     const int first = MT == 2 ? 0 : half * COLS;
     const uint32_t t = tmem_addr(tmem, quarter * 32, (MT == 2 ? half * BN : 0) + first);
 #pragma unroll 1
@@ -247,17 +248,13 @@ __global__ void __launch_bounds__(32 * Cfg::WARPS, 1)
       tmem_ld_wait();
       const int64_t at = (int64_t)o * a.norm.cols + n0 + first + c;
       const int left = a.norm.cols - (n0 + first + c);
-      if (a.part != nullptr) {
-        float* p = a.part + (int64_t)blockIdx.z * a.outs * a.norm.cols + at;
-#pragma unroll
-        for (int e = 0; e < 32; e += 4)
-          if (o < a.outs && e < left) *reinterpret_cast<uint4*>(p + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 32; ++e)
-          if (o < a.outs && e < left) param_put(a.out, at + e, __uint_as_float(v[e]));
-      }
-      __syncwarp();
+      float* p = a.part + (int64_t)blockIdx.z * a.outs * a.norm.cols + at;
+      // (the stages are all used up)
+      put_block(smem + w8 * kBlockStaging, v, lane, [&](int r, int e, const float4& x) {
+        if (o + r >= a.outs || e >= left) return;
+        if (a.part != nullptr) *reinterpret_cast<float4*>(p + (int64_t)r * a.norm.cols + e) = x;
+        else param_put4(a.out, at + (int64_t)r * a.norm.cols + e, x);
+      });
     }
   }
   tc_fence_before();
@@ -288,10 +285,7 @@ __global__ void __launch_bounds__(256) dw_fold_kernel(const float* __restrict__ 
       s.w += v[u].w;
     }
   }
-  param_put(out, i, s.x);
-  param_put(out, i + 1, s.y);
-  param_put(out, i + 2, s.z);
-  param_put(out, i + 3, s.w);
+  param_put4(out, i, s);
 }
 
 struct DwPlan {

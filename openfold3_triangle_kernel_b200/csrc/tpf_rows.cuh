@@ -171,6 +171,27 @@ __device__ __forceinline__ void param_put(const ParamOut& v, int64_t i, float x)
   else static_cast<__half*>(v.p)[i] = __float2half_rn(x);
 }
 
+// Four in a row, i a multiple of 4, p on a 16-byte boundary.
+__device__ __forceinline__ void param_put4(const ParamOut& v, int64_t i, const float4& x) {
+  if (v.type == kRowF32) {
+    *reinterpret_cast<float4*>(static_cast<float*>(v.p) + i) = x;
+  } else {
+    union {
+      bf16 b[4];
+      __half h[4];
+      uint2 u;
+    } o;
+    if (v.type == kRowBF16) {
+      o.b[0] = __float2bfloat16_rn(x.x), o.b[1] = __float2bfloat16_rn(x.y);
+      o.b[2] = __float2bfloat16_rn(x.z), o.b[3] = __float2bfloat16_rn(x.w);
+    } else {
+      o.h[0] = __float2half_rn(x.x), o.h[1] = __float2half_rn(x.y);
+      o.h[2] = __float2half_rn(x.z), o.h[3] = __float2half_rn(x.w);
+    }
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(v.p) + i) = o.u;
+  }
+}
+
 // ---- 8-bit format --------------------------------------------------------------------------------
 struct GroupScale {
   float up, down;  // code = rint(x up), value = code down; up is NaN where down is
