@@ -22,14 +22,15 @@ struct SumsOut {
   }
 };
 
-// A CTA walks the row groups blockIdx.x, + gridDim.x, ... as in the forward.  From codes xh = code (s rstd) - mean rstd, one FMA, off by three roundings of what it subtracts; from x
-// itself the mean is taken off first, where it may be large.
+// A CTA walks the row groups blockIdx.x, + gridDim.x, ... as in the forward.  From codes xh = code (s rstd) - mean rstd, one
+// FMA, off by three roundings of what it subtracts; from x itself the mean is taken off first, where it may be large.
 template <typename T, class Tm, int ROWS, bool CODES>
 __global__ void __launch_bounds__(Tm::MAXB, min_ctas<Tm, true>())
     norm_bwd_kernel(const NormArgs a, const T* __restrict__ dy, T* __restrict__ dx, const SumsOut out) {
   griddep_wait();
   constexpr int E = Tm::E, P = E / 2, ITEMS = Tm::ITEMS, NG = Groups<Tm>::N;
-  __shared__ float red[Tm::BLOCK ? 2 * 32 : 2 * Tm::COLS];
+  constexpr int WARPS = Tm::MAXB / 32;
+  __shared__ __align__(16) float red[Tm::BLOCK ? 2 * 32 : WARPS * 2 * Tm::COLS];
   const Tm tm;
   int turn = 0;
   int at[ITEMS];
@@ -174,7 +175,8 @@ __global__ void __launch_bounds__(Tm::MAXB, min_ctas<Tm, true>())
       for (int e = 0; e < Tm::VEC; ++e) out.put(a.cols, c + e, fw[i * Tm::VEC + e], fb[i * Tm::VEC + e]);
     }
   } else {
-    // the teams of a warp, then the warps one after the other
+    // the teams of a warp, then the warps in order (one warp after the other into the same place: 30000 rows of 512, 24.5 us
+    // in the place of 19.7)
 #pragma unroll
     for (int k = 0; k < E; ++k)
 #pragma unroll
@@ -182,21 +184,34 @@ __global__ void __launch_bounds__(Tm::MAXB, min_ctas<Tm, true>())
         fw[k] += __shfl_xor_sync(0xffffffffu, fw[k], off);
         fb[k] += __shfl_xor_sync(0xffffffffu, fb[k], off);
       }
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int now = 0; now < Tm::MAXB / 32; ++now) {
-      if (warp == now && lane < Tm::TS) {
+    const int warp = threadIdx.x >> 5;
+    float* own = red + warp * 2 * Tm::COLS;
+    if ((threadIdx.x & 31) < Tm::TS) {
 #pragma unroll
-        for (int i = 0; i < ITEMS; ++i)
+      for (int i = 0; i < ITEMS; ++i) {
+        const int c = tm.column(i), k = i * Tm::VEC;
+        if constexpr (Tm::VEC == 8) {
 #pragma unroll
-          for (int e = 0; e < Tm::VEC; ++e) {
-            const int c = tm.column(i) + e, k = i * Tm::VEC + e;
-            red[c] = now == 0 ? fw[k] : red[c] + fw[k];
-            red[Tm::COLS + c] = now == 0 ? fb[k] : red[Tm::COLS + c] + fb[k];
+          for (int e = 0; e < 8; e += 4) {
+            *reinterpret_cast<float4*>(own + c + e) = make_float4(fw[k + e], fw[k + e + 1], fw[k + e + 2], fw[k + e + 3]);
+            *reinterpret_cast<float4*>(own + Tm::COLS + c + e) = make_float4(fb[k + e], fb[k + e + 1], fb[k + e + 2], fb[k + e + 3]);
           }
+        } else {
+          own[c] = fw[k];
+          own[Tm::COLS + c] = fb[k];
+        }
       }
-      __syncthreads();
     }
-    for (int c = threadIdx.x; c < a.cols; c += Tm::MAXB) out.put(a.cols, c, red[c], red[Tm::COLS + c]);
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.cols; c += Tm::MAXB) {
+      float w0 = red[c], b0 = red[Tm::COLS + c];
+#pragma unroll
+      for (int n = 1; n < WARPS; ++n) {
+        w0 += red[n * 2 * Tm::COLS + c];
+        b0 += red[(n * 2 + 1) * Tm::COLS + c];
+      }
+      out.put(a.cols, c, w0, b0);
+    }
   }
 }
 
