@@ -255,7 +255,7 @@ __device__ __forceinline__ float f2_sum(uint64_t v) {
 // ---- a team of threads on a row ------------------------------------------------------------------
 // A thread owns ITEMS pieces of VEC consecutive elements.  The pieces of one item lie side by side over the lanes of a
 // warp (coalesced accesses), the items of a warp follow one another, the warps of a team as well.  So a group of 128
-// elements is always inside one warp: 16 lanes of an item (VEC = 8), or 4 items (VEC = 1).
+// elements is always inside one warp: 16 lanes of an item (VEC = 8), or 128 / TS items of all lanes (VEC = 1).
 // TS = 4 .. 32: teams of TS lanes, 256 threads a block.  TS = 0: the block is the team, up to MAXB threads.
 template <int VEC_, int TS_, int ITEMS_, int MAXB_ = 256>
 struct Team {
@@ -263,7 +263,7 @@ struct Team {
   static constexpr bool BLOCK = TS == 0;
   static constexpr int TEAMS = BLOCK ? 1 : MAXB / TS;
   static constexpr int COLS = BLOCK ? MAXB * E : TS * E;  // widest row
-  static_assert(VEC == 8 || (VEC == 1 && (BLOCK || TS == 32) && ITEMS % 4 == 0), "groups stay inside a warp");
+  static_assert(VEC == 8 || (VEC == 1 && ITEMS % 4 == 0 && (BLOCK || COLS <= 128 || COLS % 128 == 0)), "groups stay inside a warp");
   static int threads(int cols) {  // of a block
     return BLOCK ? ((cols + E - 1) / E + 31) / 32 * 32 : MAXB;
   }
@@ -320,11 +320,11 @@ __device__ __forceinline__ void team_sum(float (&v)[N], float* red, int& turn) {
 }
 
 // Groups of 128 a thread takes part in: VEC = 8: one a piece (a team narrower than 16 lanes: one of all pieces), VEC = 1: one per
-// four items; LANES lanes share one.
+// 128 columns; LANES lanes share one.
 template <class Tm>
 struct Groups {
-  static constexpr int LANES = Tm::VEC == 1 ? 32 : Tm::BLOCK || Tm::TS >= 16 ? 16 : Tm::TS;
-  static constexpr int N = Tm::VEC == 1 ? Tm::ITEMS / 4 : (Tm::ITEMS * LANES + 15) / 16;
+  static constexpr int LANES = Tm::VEC == 1 ? (Tm::BLOCK ? 32 : Tm::TS) : Tm::BLOCK || Tm::TS >= 16 ? 16 : Tm::TS;
+  static constexpr int N = Tm::VEC == 1 ? (Tm::BLOCK ? Tm::ITEMS / 4 : (Tm::COLS + 127) / 128) : (Tm::ITEMS * LANES + 15) / 16;
 };
 
 // A thread's part of a row, as it lies in memory and as pairs of floats (sm_100 works on two at once).  `at`: the columns
@@ -417,7 +417,7 @@ __device__ __forceinline__ void store_codes(int8_t* row, const uint64_t (&x)[Tm:
     for (int i = 0; i < Tm::ITEMS; ++i) {
       float lo, hi;
       f2_unpack(x[i / 2], lo, hi);
-      if (on[i]) row[at[i]] = code_of(i % 2 ? hi : lo, up[i / 4]);
+      if (on[i]) row[at[i]] = code_of(i % 2 ? hi : lo, up[i * Groups<Tm>::N / Tm::ITEMS]);
     }
   } else {
 #pragma unroll

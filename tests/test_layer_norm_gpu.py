@@ -58,6 +58,13 @@ def test_int8_checkpoint(cols, dtype):
     _check(_inputs(41, cols, DT[dtype], seed=cols + 1), checkpoint="int8")
 
 
+@pytest.mark.parametrize("cols", [17, 31, 63, 127, 130, 250, 255, 301, 511])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_odd_widths_of_many_rows(cols, dtype, checkpoint):
+    _check(_inputs(3001, cols, DT[dtype], seed=cols + 2), checkpoint=checkpoint)
+
+
 @pytest.mark.parametrize("rows", [1, 2, 3, 31, 33, 64, 65, 97, 257, 4099])
 @pytest.mark.parametrize("cols", [96, 128, 384, 1001])
 @pytest.mark.parametrize("checkpoint", [None, "int8"])
