@@ -65,15 +65,16 @@ __global__ void __launch_bounds__(Tm::MAXB, min_ctas<Tm, true>())
     }
   };
   // Three rounds ahead into L2: what a request waits for is then L2's latency (8192 rows of 4096 channels 51.3 -> 48.0 us,
-  // 5000 of 8192 61.4 -> 57.6; two rounds and five the same or less).
+  // 5000 of 8192 61.4 -> 57.6; two rounds and five the same or less).  Single elements: 8000 rows of 4099 257 -> 197, narrower ones
+  // gain nothing.
   constexpr int AHEAD = 3;
   auto prefetch = [&](int64_t first) {
-    if constexpr (Tm::VEC == 8) {
+    if constexpr (Tm::VEC == 8 || Tm::E >= 16) {
       constexpr int NR = Tm::TEAMS * ROWS;
       if (threadIdx.x != 0 || first + NR > a.rows) return;
-      bulk_prefetch(dy + first * a.cols, NR * a.cols * (int)sizeof(T));
-      if constexpr (CODES) bulk_prefetch(a.codes + first * a.code_pitch, NR * a.code_pitch);
-      else if (a.x_pitch == a.cols) bulk_prefetch(static_cast<const T*>(a.x) + first * a.x_pitch, NR * a.cols * (int)sizeof(T));
+      row_prefetch(dy + first * a.cols, NR * a.cols * (int)sizeof(T));
+      if constexpr (CODES) row_prefetch(a.codes + first * a.code_pitch, NR * a.code_pitch);
+      else if (a.x_pitch == a.cols) row_prefetch(static_cast<const T*>(a.x) + first * a.x_pitch, NR * a.cols * (int)sizeof(T));
     }
   };
   request(base + tm.index * ROWS);

@@ -408,6 +408,12 @@ struct CodeFrag {
     }
   }
 };
+// Brings what lies in whole 16-byte units of `bytes` bytes at p into L2.
+__device__ __forceinline__ void row_prefetch(const void* p, int bytes) {
+  const uint64_t first = (reinterpret_cast<uint64_t>(p) + 15) & ~15ull, last = (reinterpret_cast<uint64_t>(p) + bytes) & ~15ull;
+  if (last > first) bulk_prefetch(reinterpret_cast<const void*>(first), (uint32_t)(last - first));
+}
+
 // Codes of a row; up: the factor of each group.
 template <class Tm>
 __device__ __forceinline__ void store_codes(int8_t* row, const uint64_t (&x)[Tm::E / 2], const float* up,

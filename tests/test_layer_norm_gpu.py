@@ -58,11 +58,43 @@ def test_int8_checkpoint(cols, dtype):
     _check(_inputs(41, cols, DT[dtype], seed=cols + 1), checkpoint="int8")
 
 
-@pytest.mark.parametrize("cols", [17, 31, 63, 127, 130, 250, 255, 301, 511])
+@pytest.mark.parametrize("cols", [9, 17, 31, 57, 58, 63, 121, 122, 127, 130, 249, 250, 255, 301, 505, 511, 513, 1018, 1022, 2049, 4090,
+                                  8185, 8191])
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 @pytest.mark.parametrize("checkpoint", [None, "int8"])
 def test_odd_widths_of_many_rows(cols, dtype, checkpoint):
-    _check(_inputs(3001, cols, DT[dtype], seed=cols + 2), checkpoint=checkpoint)
+    _check(_inputs(3001 if cols < 600 else 301, cols, DT[dtype], seed=cols + 2), checkpoint=checkpoint)
+
+
+@pytest.mark.parametrize("rows", [63, 64, 65, 66, 71, 72, 120, 1001])
+@pytest.mark.parametrize("cols", [9, 93, 517])
+def test_odd_widths_of_some_rows(rows, cols):
+    _check(_inputs(rows, cols, torch.bfloat16, seed=rows))
+
+
+@pytest.mark.parametrize("cols", [9, 45, 333, 1001])
+def test_odd_widths_keep_rows_apart(cols):
+    """Infinities and NaN of a row stay in it where rows begin at any address, and nothing behind the last row is read or written."""
+    rows = 200
+    i = _inputs(rows, cols, torch.bfloat16)
+    bad = list(range(0, rows, 3)) + [rows - 1]
+    good = [r for r in range(rows) if r not in bad]
+
+    def run(x, dy):
+        buf = torch.full((rows * cols + 64,), float("nan"), device="cuda", dtype=torch.bfloat16)
+        xc = buf[:rows * cols].view(rows, cols).copy_(x.cuda()).requires_grad_(True)
+        y = tk.turbo_layer_norm(xc, i["w"].cuda(), i["b"].cuda())
+        (g,) = torch.autograd.grad(y, xc, dy.cuda())
+        assert torch.isnan(buf[rows * cols:].float()).all()
+        return y, g
+
+    y0, g0 = run(i["x"], i["dy"])
+    x, dy = i["x"].clone(), i["dy"].clone()
+    x[bad, 0], x[bad, cols - 1] = float("inf"), float("nan")
+    dy[bad, 0], dy[bad, cols - 1] = float("nan"), float("inf")
+    y1, g1 = run(x, dy)
+    assert torch.equal(y0[good], y1[good]) and torch.equal(g0[good], g1[good])
+    assert torch.isnan(y1[bad].float()).all() and torch.isnan(g1[bad].float()).all()
 
 
 @pytest.mark.parametrize("rows", [1, 2, 3, 31, 33, 64, 65, 97, 257, 4099])
