@@ -131,6 +131,7 @@ def test_layer_norm_forward_entry_refuses(kw, text):
 @pytest.mark.parametrize("kw, text", [
     (dict(x=NULL), "null pointer"), (dict(mean=NULL, rstd=NULL), "null pointer"), (dict(dy=NULL), "null pointer"),
     (dict(dw=ONE, dwt=9), "unknown parameter type"), (dict(cols=9000, pitch=9000), "1 to 8192 columns"),
+    (dict(dw=ONE, ws=ctypes.c_void_p(260), wsb=1 << 20), "workspace must be 16-byte aligned"),
 ])
 def test_layer_norm_backward_entry_refuses(kw, text):
     with pytest.raises(ValueError, match=text):
@@ -197,6 +198,8 @@ def _nl_bwd(**kw):
     (dict(dx=ctypes.c_void_p(264)), "16-byte aligned"), (dict(dw=ONE, dwt=4), "unknown parameter type"),
     (dict(outs=4), "multiples of 8"), (dict(x=ctypes.c_void_p(258)), "x must"),
     (dict(codes=ctypes.c_void_p(260), scales=ONE), "codes must"),
+    (dict(dw=ctypes.c_void_p(264)), "d_weight must be 16-byte aligned"),
+    (dict(ws=ctypes.c_void_p(264)), "workspace must be 16-byte aligned"),
 ])
 def test_norm_linear_backward_entry_refuses(kw, text):
     with pytest.raises(ValueError, match=text):
