@@ -41,6 +41,20 @@ def test_pack_and_unpack(rows, cols, dtype):
     _check(_x(rows, cols, DT[dtype], seed=rows + cols))
 
 
+@pytest.mark.parametrize("cols", [1, 3, 5, 7, 9, 17, 30, 60, 63, 97, 121, 127, 130, 131, 135, 250, 259, 381, 1029, 4099])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_odd_widths_of_many_rows(cols, dtype):
+    _check(_x(max(3, 20011 // cols), cols, DT[dtype], seed=cols))
+
+
+@pytest.mark.parametrize("cols", [5, 30, 97, 131])
+def test_unpacking_from_and_to_odd_addresses(cols):
+    codes, scales = _check(_x(50, cols, torch.bfloat16, seed=cols))
+    buf = torch.empty(50 * cols + 1, device="cuda", dtype=torch.int8)
+    buf[1:] = codes.view(-1)
+    assert torch.equal(tk.unpack_activation(buf[1:].view(50, cols), scales), tk.unpack_activation(codes, scales))
+
+
 def test_ties_go_to_the_even_code():
     # amax 127 makes the factor exactly 1, so that halves are ties
     x = torch.zeros(1, 128)
