@@ -123,8 +123,9 @@ __device__ __forceinline__ void grad_role(uint8_t* smem, Shared* sh, const WaitC
     // Two groups of eight warps make every other stage's xh~, each in a buffer of its own: making one takes longer than its
     // products.  A lane makes 16 consecutive columns of a row: 8 lanes a row, twice 4 rows a warp.
     const int wk = warp - 2, group = wk >> 3, piece = lane & 7, sub = lane >> 3;
-    // the block of ones: its first column is 1, the rest 0, in both buffers and for good
-    for (int i = (wk & 7) * 32 + lane; i < kRows * 8; i += 256) {
+    // The block of ones: its first column is 1, the rest 0, in both buffers and for good.  In a range of one step the second
+    // group must not write it: nothing that `done` stands for would come after its stores, and the sums are staged over them.
+    for (int i = (wk & 7) * 32 + lane; group < steps && i < kRows * 8; i += 256) {
       const int r = i >> 3, q = i & 7;
       *reinterpret_cast<uint4*>(b_buf + group * Cfg::B_BYTES + ones * kChunk + r * 128 + ((q ^ (r & 7)) << 4)) =
           make_uint4(q == 0 ? 0x3f80u : 0u, 0u, 0u, 0u);

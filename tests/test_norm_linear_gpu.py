@@ -118,6 +118,19 @@ def test_many_rows(rows, cols, outs, checkpoint):
         assert torch.equal(out, again) and all(torch.equal(g[n], h[n]) for n in g)
 
 
+@pytest.mark.parametrize("rows", [1, 33, 64, 257, 320, 1281])
+@pytest.mark.parametrize("cols, outs", [(64, 64), (128, 128), (40, 1024), (128, 512)])
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_ranges_of_one_step(rows, cols, outs, checkpoint):
+    """Up to 64 rows in a range, or in its last: of the two groups of warps that make xh, the second has no step.  The sums
+    are staged over its buffer, so nothing may be on its way there; what could go wrong would do so now and then."""
+    i = _inputs(rows, cols, outs, seed=rows)
+    out, g = _check(i, checkpoint)
+    for _ in range(20):
+        again, h = _run(i, checkpoint)
+        assert torch.equal(out, again) and all(torch.equal(g[n], h[n]) for n in g)
+
+
 @pytest.mark.parametrize("rows", [1, 2, 3, 4, 5])
 @pytest.mark.parametrize("cols, outs", [(8, 8), (40, 2504), (136, 24), (1000, 4096), (1024, 520), (8192, 40)])
 @pytest.mark.parametrize("checkpoint", [None, "int8"])
