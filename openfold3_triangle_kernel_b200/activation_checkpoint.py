@@ -10,7 +10,8 @@ that holds an infinity or a NaN comes back as NaN.
 * ``checkpoint="int8"`` of :func:`turbo_layer_norm` and :func:`turbo_norm_linear`, whose kernels write the codes in the
   forward pass and read them in the backward pass, without a pass of their own.
 
-None of them is differentiated.  Unsupported inputs raise ``ValueError("... unsupported [code]: reason")``.  The reference
+None of them is differentiated.  Unsupported inputs raise ``ValueError("... unsupported [code]: reason")``, traced ones as in
+:func:`turbo_layer_norm`.  The reference
 has no counterpart: it keeps activations whole or computes them again (openfold3/core/utils/checkpointing.py).
 """
 from __future__ import annotations
@@ -18,6 +19,7 @@ from __future__ import annotations
 import torch
 
 from . import _cabi as C
+from ._checks import certain, differs, refuse
 from .layer_norm import ROW_DTYPES
 from .trimul import SupportResult
 
@@ -32,7 +34,9 @@ def _groups(cols):
 
 def _countable(x):
     cols = x.shape[-1]
-    return cols == 0 or (cols < 2 ** 31 - GROUP and x.numel() // cols * _groups(cols) < _MAX_GROUPS)
+    if isinstance(cols, torch.SymInt):
+        return True     # (a free size: the launch sees to it)
+    return cols == 0 or (cols < 2 ** 31 - GROUP and not certain(x.numel() // cols * _groups(cols) >= _MAX_GROUPS))
 
 
 def check_pack_support(x, *, check_device=True) -> SupportResult:
@@ -61,7 +65,7 @@ def check_unpack_support(codes, scales, dtype, *, check_device=True) -> SupportR
         return SupportResult(False, "x_dtype", "codes must be int8 and scales FP32")
     if codes.ndim >= 1 and not _countable(codes):
         return SupportResult(False, "extent", "codes must have fewer than 2^31 groups of 128 elements")
-    if codes.ndim < 1 or tuple(scales.shape) != tuple(codes.shape[:-1]) + (_groups(codes.shape[-1]),):
+    if codes.ndim < 1 or differs(scales.shape, tuple(codes.shape[:-1]) + (_groups(codes.shape[-1]),)):
         return SupportResult(False, "x_shape", "scales must have one entry per 128 elements of a row of codes")
     if dtype not in ROW_DTYPES:
         return SupportResult(False, "dtype", "dtype must be torch.bfloat16, float16 or float32")
@@ -77,22 +81,26 @@ def check_unpack_support(codes, scales, dtype, *, check_device=True) -> SupportR
 
 @torch.library.custom_op("tpf_b200::int8_pack", mutates_args=())
 def _int8_pack(x: torch.Tensor) -> list[torch.Tensor]:
+    refuse("pack_activation", check_pack_support(x))
     return C.native().int8_pack_op(x)
 
 
 @_int8_pack.register_fake
 def _(x):
+    refuse("pack_activation", check_pack_support(x, check_device=False))
     return [x.new_empty(x.shape, dtype=torch.int8),
             x.new_empty(x.shape[:-1] + (_groups(x.shape[-1]),), dtype=torch.float32)]
 
 
 @torch.library.custom_op("tpf_b200::int8_unpack", mutates_args=())
 def _int8_unpack(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    refuse("unpack_activation", check_unpack_support(codes, scales, dtype))
     return C.native().int8_unpack_op(codes, scales, _SCALAR_TYPES[dtype])
 
 
 @_int8_unpack.register_fake
 def _(codes, scales, dtype):
+    refuse("unpack_activation", check_unpack_support(codes, scales, dtype, check_device=False))
     return codes.new_empty(codes.shape, dtype=dtype)
 
 
@@ -102,9 +110,7 @@ def pack_activation(x):
         packed = C.native().int8_pack(x)
         if packed is not None:
             return packed
-        res = check_pack_support(x)
-        if not res.supported:
-            raise ValueError(f"pack_activation unsupported [{res.code}]: {res.reason}")
+        refuse("pack_activation", check_pack_support(x))
     codes, scales = torch.ops.tpf_b200.int8_pack(x.detach())
     return codes, scales
 
@@ -115,9 +121,7 @@ def unpack_activation(codes, scales, dtype=torch.bfloat16):
         x = C.native().int8_unpack(codes, scales, dtype)
         if x is not None:
             return x
-        res = check_unpack_support(codes, scales, dtype)
-        if not res.supported:
-            raise ValueError(f"unpack_activation unsupported [{res.code}]: {res.reason}")
+        refuse("unpack_activation", check_unpack_support(codes, scales, dtype))
     return torch.ops.tpf_b200.int8_unpack(codes, scales.detach(), dtype)
 
 

@@ -356,7 +356,10 @@ py::object py_norm_linear(py::handle hx, py::handle hnw, py::handle hnb, py::han
   return py::cast(out);
 }
 
-// Launches behind the torch.library operators.  Absent tensors of an output list are empty.
+// Launches behind the torch.library operators, which have checked the arguments.  Absent tensors of an output list are empty.
+Kept kept_args(const MaybeTensor& x, const Tensor& stats, const Tensor& codes, const Tensor& scales) {
+  return {stats.contiguous(), x ? Tensor() : codes.contiguous(), scales.contiguous()};
+}
 std::vector<Tensor> layer_norm_fwd(const Tensor& x, const MaybeTensor& w, const MaybeTensor& b, double eps, bool int8) {
   c10::cuda::CUDAGuard guard(x.device());
   Kept k;
@@ -373,7 +376,8 @@ std::vector<Tensor> layer_norm_bwd(const Tensor& dy, const MaybeTensor& x, const
   c10::cuda::CUDAGuard guard(dy.device());
   const Rows rows = x ? as_rows(*x) : Rows{};
   const Tensor wc = value_or_none(w), bc = value_or_none(b), d = dy.contiguous();
-  const tpf::NormCall c = kept_call(rows, {stats, x ? Tensor() : codes, scales}, wc, Tensor(), row_type(dy), dy.size(-1));
+  const Kept k = kept_args(x, stats, codes, scales);
+  const tpf::NormCall c = kept_call(rows, k, wc, Tensor(), row_type(dy), dy.size(-1));
   NormGradTensors g = layer_norm_grads(c, d, dy.sizes(), wc, bc, true, wc.defined(), bc.defined());
   const Tensor none = empty_f32({0}, dy);
   return {g.dx, g.dw.defined() ? g.dw : none, g.db.defined() ? g.db : none.clone()};
@@ -397,7 +401,8 @@ std::vector<Tensor> norm_linear_bwd(const Tensor& d_out, const MaybeTensor& x, c
   c10::cuda::CUDAGuard guard(d_out.device());
   const Rows rows = x ? as_vector_rows(*x) : Rows{};
   const Tensor nwc = value_or_none(nw), nbc = value_or_none(nb), d = aligned_bf16(d_out);
-  const tpf::NormCall c = kept_call(rows, {stats, x ? Tensor() : codes, scales}, nwc, nbc, TPF_BF16, w.size(1));
+  const Kept k = kept_args(x, stats, codes, scales);
+  const tpf::NormCall c = kept_call(rows, k, nwc, nbc, TPF_BF16, w.size(1));
   LinearGradTensors g = norm_linear_grads(c, d, with_last(d_out.sizes(), w.size(1)), nwc, nbc, w, true, nwc.defined(),
                                           nbc.defined(), true);
   const Tensor none = empty_f32({0}, d_out);

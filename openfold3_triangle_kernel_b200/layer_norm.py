@@ -13,7 +13,8 @@ Operator contract:
   order only.  Statistics and sums are fp32 in a fixed order: the same inputs give the same bits.
 
 A row that holds an infinity or a NaN is NaN; the others are not touched by it.  Unsupported inputs raise
-``ValueError("turbo_layer_norm unsupported [code]: reason")``.  There is no counterpart among the reference's kernels (it
+``ValueError("turbo_layer_norm unsupported [code]: reason")``, in a traced call when it is traced (inside the compiler's own
+exception) or, for sizes that are free there, when it runs.  There is no counterpart among the reference's kernels (it
 calls torch's LayerNorm, openfold3/core/model/primitives/normalization.py).
 """
 from __future__ import annotations
@@ -24,6 +25,7 @@ from typing import Optional
 import torch
 
 from . import _cabi as C
+from ._checks import certain, differs, refuse
 from .trimul import SupportResult
 
 ROW_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
@@ -35,7 +37,7 @@ def check_parameter(name, p, cols, x):
     """The first failure of an optional ``[C]`` parameter, or ``None``."""
     if p is None:
         return None
-    if not isinstance(p, torch.Tensor) or tuple(p.shape) != (cols,):
+    if not isinstance(p, torch.Tensor) or differs(p.shape, (cols,)):
         return SupportResult(False, "weight_shape", f"{name} must have shape ({cols},)")
     if p.dtype not in ROW_DTYPES:
         return SupportResult(False, "weight_dtype", f"{name} must be BF16, FP16 or FP32")
@@ -48,9 +50,9 @@ def check_rows(x, eps, checkpoint, check_device):
     """Checks that the row-wise operators share; the first failure, or ``None``."""
     if not isinstance(x, torch.Tensor):
         return SupportResult(False, "x_type", "x must be a torch.Tensor")
-    if x.ndim < 1 or x.shape[-1] < 1:
+    if x.ndim < 1 or certain(x.shape[-1] < 1):
         return SupportResult(False, "x_shape", "x must have shape [*,C], C >= 1")
-    if x.shape[-1] > MAX_COLUMNS:
+    if certain(x.shape[-1] > MAX_COLUMNS):
         return SupportResult(False, "columns", f"C={x.shape[-1]} exceeds {MAX_COLUMNS}")
     if checkpoint not in CHECKPOINTS:
         return SupportResult(False, "checkpoint", "checkpoint must be None or 'int8'")
@@ -78,6 +80,33 @@ def check_layer_norm_support(x, weight=None, bias=None, eps=1e-5, checkpoint=Non
     return SupportResult(True, "ok", "supported")
 
 
+def check_kept(d_out, rows_shape, cols, x, stats, codes, scales):
+    """What a backward pass is given of its forward: ``x`` or its codes, and the statistics; the first failure, or ``None``."""
+    rows = math.prod(rows_shape)
+    if any(t is not None and t.device != d_out.device for t in (x, stats, codes, scales)):
+        return SupportResult(False, "device", "all tensors must share one device")
+    if stats.dtype != torch.float32 or differs(stats.shape, (2, rows)):
+        return SupportResult(False, "stats", "stats must be FP32 [2, rows]")
+    if x is not None:
+        if differs(x.shape, tuple(rows_shape) + (cols,)):
+            return SupportResult(False, "x_shape", "x does not belong to this gradient")
+        return None
+    if codes.dtype != torch.int8 or differs(codes.shape, (rows, -(-cols // 16) * 16)):
+        return SupportResult(False, "codes", "codes must be INT8, rows at a pitch of C rounded up to 16")
+    if scales.dtype != torch.float32 or differs(scales.shape, (rows, -(-cols // 128))):
+        return SupportResult(False, "scales", "scales must be FP32 [rows, ceil(C / 128)]")
+    return None
+
+
+def _check_backward(dy, x, stats, codes, scales, weight, bias, check_device):
+    res = check_layer_norm_support(dy, weight, bias, check_device=check_device)
+    if not res.supported:
+        return res
+    if x is not None and x.dtype != dy.dtype:
+        return SupportResult(False, "x_dtype", "x and its gradient must have one type")
+    return check_kept(dy, dy.shape[:-1], dy.shape[-1], x, stats, codes, scales) or res
+
+
 # --------------------------------------------------------------------------------------
 # custom ops: what a traced graph holds.  An eager call on plain CUDA tensors goes to `_native.layer_norm`.
 # --------------------------------------------------------------------------------------
@@ -93,11 +122,13 @@ def kept_like(x, int8):
 @torch.library.custom_op("tpf_b200::layer_norm_fwd", mutates_args=())
 def _layer_norm_fwd(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float,
                     int8: bool) -> list[torch.Tensor]:
+    refuse("turbo_layer_norm", check_layer_norm_support(x, weight, bias, eps, "int8" if int8 else None))
     return C.native().layer_norm_fwd(x, weight, bias, eps, int8)
 
 
 @_layer_norm_fwd.register_fake
 def _(x, weight, bias, eps, int8):
+    refuse("turbo_layer_norm", check_layer_norm_support(x, weight, bias, eps, check_device=False))
     return [torch.empty_like(x, memory_format=torch.contiguous_format), *kept_like(x, int8)]
 
 
@@ -105,11 +136,13 @@ def _(x, weight, bias, eps, int8):
 def _layer_norm_bwd(dy: torch.Tensor, x: Optional[torch.Tensor], stats: torch.Tensor, codes: torch.Tensor,
                     scales: torch.Tensor, weight: Optional[torch.Tensor],
                     bias: Optional[torch.Tensor]) -> list[torch.Tensor]:
+    refuse("layer norm backward", _check_backward(dy, x, stats, codes, scales, weight, bias, True))
     return C.native().layer_norm_bwd(dy, x, stats, codes, scales, weight, bias)
 
 
 @_layer_norm_bwd.register_fake
 def _(dy, x, stats, codes, scales, weight, bias):
+    refuse("layer norm backward", _check_backward(dy, x, stats, codes, scales, weight, bias, False))
     none = lambda: dy.new_empty((0,), dtype=torch.float32)  # noqa: E731
     return [torch.empty_like(dy, memory_format=torch.contiguous_format),
             none() if weight is None else weight.new_empty(weight.shape),
@@ -143,7 +176,5 @@ def turbo_layer_norm(x, weight=None, bias=None, *, eps=1e-5, checkpoint=None):
             y = C.native().layer_norm(x, weight, bias, eps, checkpoint == "int8")
             if y is not None:
                 return y
-        res = check_layer_norm_support(x, weight, bias, eps, checkpoint)
-        if not res.supported:
-            raise ValueError(f"turbo_layer_norm unsupported [{res.code}]: {res.reason}")
+        refuse("turbo_layer_norm", check_layer_norm_support(x, weight, bias, eps, checkpoint))
     return torch.ops.tpf_b200.layer_norm_fwd(x, weight, bias, eps, checkpoint == "int8")[0]

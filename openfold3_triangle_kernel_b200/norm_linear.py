@@ -14,7 +14,8 @@ Operator contract:
   the gradient that reaches them are rounded to bf16 on their way to the tensor cores, sums are fp32 (four rows and fewer
   are not rounded on the way out).
 
-Unsupported inputs raise ``ValueError("turbo_norm_linear unsupported [code]: reason")``.  There is no counterpart among the
+Unsupported inputs raise ``ValueError("turbo_norm_linear unsupported [code]: reason")``, traced ones as in
+:func:`turbo_layer_norm`.  There is no counterpart among the
 reference's kernels (it calls torch's LayerNorm and Linear).
 """
 from __future__ import annotations
@@ -25,7 +26,8 @@ from typing import Optional
 import torch
 
 from . import _cabi as C
-from .layer_norm import CHECKPOINTS, ROW_DTYPES, check_parameter, check_rows, kept_like
+from ._checks import certain, differs, refuse
+from .layer_norm import CHECKPOINTS, ROW_DTYPES, check_kept, check_parameter, check_rows, kept_like
 from .trimul import SupportResult
 
 MAX_ROWS = 2 ** 31 - 256
@@ -41,13 +43,13 @@ def check_norm_linear_support(x, norm_weight, norm_bias, weight, eps=1e-5, check
     if x.dtype != torch.bfloat16:
         return SupportResult(False, "x_dtype", "x must be BF16")
     cols = x.shape[-1]
-    if cols % 8:
+    if certain(cols % 8 != 0):
         return SupportResult(False, "columns", f"C={cols} is not a multiple of 8")
-    if not isinstance(weight, torch.Tensor) or weight.ndim != 2 or weight.shape[1] != cols:
+    if not isinstance(weight, torch.Tensor) or weight.ndim != 2 or certain(weight.shape[1] != cols):
         return SupportResult(False, "weight_shape", f"weight must have shape (O, {cols})")
-    if math.prod(x.shape[:-1]) >= MAX_ROWS or weight.shape[0] > MAX_OUTPUTS:
+    if certain(math.prod(x.shape[:-1]) >= MAX_ROWS) or certain(weight.shape[0] > MAX_OUTPUTS):
         return SupportResult(False, "extent", f"at most {MAX_ROWS - 1} rows and {MAX_OUTPUTS} outputs")
-    if weight.shape[0] < 8 or weight.shape[0] % 8:
+    if certain(weight.shape[0] < 8) or certain(weight.shape[0] % 8 != 0):
         return SupportResult(False, "outputs", f"O={weight.shape[0]} is not a positive multiple of 8")
     if weight.dtype not in ROW_DTYPES:
         return SupportResult(False, "weight_dtype", "weight must be BF16, FP16 or FP32")
@@ -60,17 +62,31 @@ def check_norm_linear_support(x, norm_weight, norm_bias, weight, eps=1e-5, check
     return SupportResult(True, "ok", "supported")
 
 
+def _check_backward(d_out, x, stats, codes, scales, norm_weight, norm_bias, weight, check_device):
+    # x's part of the contract, on a stand-in of x's type and shape where only its codes are left
+    like = d_out.new_empty((1,), dtype=torch.bfloat16).expand(d_out.shape[:-1] + weight.shape[1:]) if x is None else x
+    res = check_norm_linear_support(like, norm_weight, norm_bias, weight, check_device=check_device)
+    if not res.supported:
+        return res
+    if differs(d_out.shape, tuple(like.shape[:-1]) + (weight.shape[0],)):
+        return SupportResult(False, "d_out_shape", "d_out does not belong to these rows and this weight")
+    return check_kept(d_out, d_out.shape[:-1], weight.shape[1], x, stats, codes, scales) or res
+
+
 # --------------------------------------------------------------------------------------
 # custom ops: what a traced graph holds.  An eager call on plain CUDA tensors goes to `_native.norm_linear`.
 # --------------------------------------------------------------------------------------
 @torch.library.custom_op("tpf_b200::norm_linear_fwd", mutates_args=())
 def _norm_linear_fwd(x: torch.Tensor, norm_weight: Optional[torch.Tensor], norm_bias: Optional[torch.Tensor],
                      weight: torch.Tensor, eps: float, int8: bool) -> list[torch.Tensor]:
+    refuse("turbo_norm_linear",
+           check_norm_linear_support(x, norm_weight, norm_bias, weight, eps, "int8" if int8 else None))
     return C.native().norm_linear_fwd(x, norm_weight, norm_bias, weight, eps, int8)
 
 
 @_norm_linear_fwd.register_fake
 def _(x, norm_weight, norm_bias, weight, eps, int8):
+    refuse("turbo_norm_linear", check_norm_linear_support(x, norm_weight, norm_bias, weight, eps, check_device=False))
     return [x.new_empty(x.shape[:-1] + (weight.shape[0],)), *kept_like(x, int8)]
 
 
@@ -78,11 +94,15 @@ def _(x, norm_weight, norm_bias, weight, eps, int8):
 def _norm_linear_bwd(d_out: torch.Tensor, x: Optional[torch.Tensor], stats: torch.Tensor, codes: torch.Tensor,
                      scales: torch.Tensor, norm_weight: Optional[torch.Tensor], norm_bias: Optional[torch.Tensor],
                      weight: torch.Tensor) -> list[torch.Tensor]:
+    refuse("normalised projection backward",
+           _check_backward(d_out, x, stats, codes, scales, norm_weight, norm_bias, weight, True))
     return C.native().norm_linear_bwd(d_out, x, stats, codes, scales, norm_weight, norm_bias, weight)
 
 
 @_norm_linear_bwd.register_fake
 def _(d_out, x, stats, codes, scales, norm_weight, norm_bias, weight):
+    refuse("normalised projection backward",
+           _check_backward(d_out, x, stats, codes, scales, norm_weight, norm_bias, weight, False))
     none = lambda: d_out.new_empty((0,), dtype=torch.float32)  # noqa: E731
     return [d_out.new_empty(d_out.shape[:-1] + (weight.shape[1],)), weight.new_empty(weight.shape),
             none() if norm_weight is None else norm_weight.new_empty(norm_weight.shape),
@@ -116,7 +136,5 @@ def turbo_norm_linear(x, norm_weight, norm_bias, weight, *, eps=1e-5, checkpoint
             out = C.native().norm_linear(x, norm_weight, norm_bias, weight, eps, checkpoint == "int8")
             if out is not None:
                 return out
-        res = check_norm_linear_support(x, norm_weight, norm_bias, weight, eps, checkpoint)
-        if not res.supported:
-            raise ValueError(f"turbo_norm_linear unsupported [{res.code}]: {res.reason}")
+        refuse("turbo_norm_linear", check_norm_linear_support(x, norm_weight, norm_bias, weight, eps, checkpoint))
     return torch.ops.tpf_b200.norm_linear_fwd(x, norm_weight, norm_bias, weight, eps, checkpoint == "int8")[0]

@@ -337,6 +337,47 @@ def test_traced_route_matches_eager(checkpoint):
                           test_utils=("test_schema", "test_autograd_registration", "test_faketensor"))
 
 
+def test_a_traced_graph_meets_the_contract_when_it_runs():
+    """Sizes and devices that differ from the traced ones are refused before a launch."""
+    x, w = torch.randn(6, 64, device="cuda"), torch.ones(64, device="cuda")
+    wide, mat = torch.randn(6, 128, device="cuda"), torch.zeros(16, 64, device="cuda")
+    norm = torch.jit.trace(lambda t: tk.turbo_layer_norm(t, w), (x,), check_trace=False)
+    proj = torch.jit.trace(lambda t: tk.turbo_norm_linear(t.bfloat16(), None, None, mat), (x,), check_trace=False)
+    unpack = torch.jit.trace(lambda c, s: tk.unpack_activation(c, s), tuple(tk.pack_activation(x)), check_trace=False)
+    codes, scales = tk.pack_activation(wide)
+    more = torch.randn(9, 64, device="cuda")
+    assert torch.equal(norm(more), tk.turbo_layer_norm(more, w))
+    ops = torch.ops.tpf_b200
+    dy, stats = torch.zeros(6, 64, device="cuda"), torch.zeros(2, 6, device="cuda")
+    none = torch.empty(0, device="cuda", dtype=torch.int8)
+    before = C.load().tpf_launch_count()
+    for call in (lambda: norm(wide), lambda: proj(wide), lambda: unpack(codes, scales[:1]),
+                 lambda: ops.layer_norm_fwd(x, w.cpu(), None, 1e-5, False),
+                 lambda: ops.norm_linear_fwd(x.bfloat16(), None, None, mat.cpu(), 1e-5, False),
+                 lambda: ops.layer_norm_bwd(dy, None, stats, none, scales, w, None),
+                 lambda: ops.layer_norm_bwd(dy, x, stats[:, :3], none, scales, w, None),
+                 lambda: ops.norm_linear_bwd(dy, x.bfloat16(), stats, none, scales, None, None, mat)):
+        with pytest.raises(Exception, match=r"unsupported \["):
+            call()
+    with pytest.raises(Exception):
+        norm(x.cpu())
+    kernels = C.load().tpf_launch_count() - before
+    assert kernels == 0
+
+
+def test_backward_operators_take_strided_statistics():
+    i = _inputs(40, 96, torch.bfloat16)
+    x, w, b, dy = (i[n].cuda() for n in ("x", "w", "b", "dy"))
+    ops = torch.ops.tpf_b200
+    for int8 in (False, True):
+        y, stats, codes, scales = ops.layer_norm_fwd(x, w, b, 1e-5, int8)
+        both = torch.stack([stats, stats], 2)[..., 0]
+        wide = torch.cat([codes, codes], -1)[..., :codes.shape[-1]]
+        ref = ops.layer_norm_bwd(dy, None if int8 else x, stats, codes, scales, w, b)
+        got = ops.layer_norm_bwd(dy, None if int8 else x, both, wide, scales, w, b)
+        assert not both.is_contiguous() and all(torch.equal(s, t) for s, t in zip(ref, got))
+
+
 def test_refusals_leave_no_launch():
     before = C.load().tpf_launch_count()
     x = torch.zeros(4, 128, device="cuda")

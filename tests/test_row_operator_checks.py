@@ -92,6 +92,94 @@ def test_operators_refuse_cpu_tensors():
         tk.unpack_activation(x.to(torch.int8), torch.zeros(4, 1))
 
 
+# ---- traced calls ---------------------------------------------------------------------------------
+BF, I8 = torch.bfloat16, torch.int8
+OPS = torch.ops.tpf_b200
+E = lambda *s, dt=torch.float32: torch.empty(*s, dtype=dt)  # noqa: E731
+# a call of an operator and the reason for its refusal; sizes are those of x [64, 128] unless they say otherwise
+WRONG = [
+    (lambda: OPS.layer_norm_fwd(E(64, 128), E(16), None, 1e-5, False), "weight_shape"),
+    (lambda: OPS.layer_norm_fwd(E(64, 128), None, E(128, dt=torch.float64), 1e-5, True), "weight_dtype"),
+    (lambda: OPS.layer_norm_fwd(E(64, 128, dt=I8), None, None, 1e-5, False), "x_dtype"),
+    (lambda: OPS.layer_norm_fwd(E(4, 9000), None, None, 1e-5, False), "columns"),
+    (lambda: OPS.layer_norm_fwd(E(64, 128), None, None, -1.0, False), "eps"),
+    (lambda: OPS.layer_norm_bwd(E(64, 128), E(64, 64), E(2, 64), E(0, dt=I8), E(0), None, None), "x_shape"),
+    (lambda: OPS.layer_norm_bwd(E(64, 128), E(64, 128, dt=BF), E(2, 64), E(0, dt=I8), E(0), None, None), "x_dtype"),
+    (lambda: OPS.layer_norm_bwd(E(64, 128), E(64, 128), E(2, 32), E(0, dt=I8), E(0), None, None), "stats"),
+    (lambda: OPS.layer_norm_bwd(E(64, 128), None, E(2, 64), E(0, dt=I8), E(64, 1), None, None), "codes"),
+    (lambda: OPS.layer_norm_bwd(E(64, 120), None, E(2, 64), E(64, 120, dt=I8), E(64, 1), None, None), "codes"),
+    (lambda: OPS.layer_norm_bwd(E(64, 128), None, E(2, 64), E(64, 128, dt=I8), E(1, 1), None, None), "scales"),
+    (lambda: OPS.layer_norm_bwd(E(64, 128), E(64, 128), E(2, 64), E(0, dt=I8), E(0), E(8), None), "weight_shape"),
+    (lambda: OPS.norm_linear_fwd(E(64, 128, dt=BF), None, None, E(64, 16), 1e-5, False), "weight_shape"),
+    (lambda: OPS.norm_linear_fwd(E(64, 128, dt=BF), E(8), None, E(64, 128), 1e-5, False), "weight_shape"),
+    (lambda: OPS.norm_linear_fwd(E(64, 128, dt=BF), None, None, E(12, 128), 1e-5, False), "outputs"),
+    (lambda: OPS.norm_linear_fwd(E(64, 128), None, None, E(64, 128), 1e-5, False), "x_dtype"),
+    (lambda: OPS.norm_linear_bwd(E(64, 8), E(64, 128, dt=BF), E(2, 64), E(0, dt=I8), E(0), None, None, E(16, 128)),
+     "d_out_shape"),
+    (lambda: OPS.norm_linear_bwd(E(64, 16), E(32, 128, dt=BF), E(2, 64), E(0, dt=I8), E(0), None, None, E(16, 128)),
+     "d_out_shape"),
+    (lambda: OPS.norm_linear_bwd(E(64, 16), E(64, 128, dt=BF), E(2, 63), E(0, dt=I8), E(0), None, None, E(16, 128)), "stats"),
+    (lambda: OPS.norm_linear_bwd(E(64, 16), None, E(2, 64), E(64, 112, dt=I8), E(64, 1), None, None, E(16, 128)), "codes"),
+    (lambda: OPS.norm_linear_bwd(E(64, 16), None, E(2, 64), E(64, 128, dt=I8), E(64, 2), None, None, E(16, 128)), "scales"),
+    (lambda: OPS.int8_pack(E(64, 128, dt=torch.float64)), "x_dtype"),
+    (lambda: OPS.int8_unpack(E(64, 128, dt=I8), E(1, 1), BF), "x_shape"),
+    (lambda: OPS.int8_unpack(E(64, 128, dt=I8), E(64, 1, dt=torch.float16), BF), "x_dtype"),
+    (lambda: OPS.int8_unpack(E(64, 128, dt=I8), E(64, 1), torch.float64), "dtype"),
+]
+
+
+@pytest.mark.parametrize("call, code", WRONG, ids=[f"{c}{n}" for n, (_, c) in enumerate(WRONG)])
+def test_operators_of_a_traced_graph_refuse(call, code):
+    """Where the fake kernels run and where the operator would launch."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode(), pytest.raises(ValueError, match=rf"unsupported \[{code}\]"):
+        call()
+    with pytest.raises(ValueError, match=r"unsupported \["):   # (on the CPU the device may be what it names)
+        call()
+
+
+def test_fake_tensors_of_two_devices_are_refused():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x, w = torch.empty(64, 128, dtype=BF, device="cuda"), E(64, 128)
+        codes = torch.empty(64, 128, dtype=I8, device="cuda")
+        for call in (lambda: OPS.norm_linear_fwd(x, None, None, w, 1e-5, False),
+                     lambda: OPS.layer_norm_fwd(x, E(128), None, 1e-5, False),
+                     lambda: OPS.layer_norm_bwd(x, x, E(2, 64), codes, E(0), None, None),
+                     lambda: OPS.int8_unpack(codes, E(64, 1), BF)):
+            with pytest.raises(ValueError, match=r"unsupported \[(weight_)?device\]"):
+                call()
+
+
+@pytest.mark.parametrize("f, args, code", [
+    (lambda x, w: tk.turbo_layer_norm(x, w), (E(64, 128), E(16)), "weight_shape"),
+    (lambda x, w: tk.turbo_norm_linear(x, None, None, w), (E(64, 128, dt=BF), E(64, 16)), "weight_shape"),
+    (lambda c, s: tk.unpack_activation(c, s), (E(64, 128, dt=I8), E(1, 1)), "x_shape"),
+    (lambda x, w: tk.pack_activation(x), (E(64, 128, dt=I8), E(1)), "x_dtype"),
+])
+def test_tracing_refuses_wrong_shapes(f, args, code):
+    torch.compiler.reset()
+    with pytest.raises(Exception, match=rf"unsupported \[{code}\]"):
+        torch.compile(f, backend="eager", fullgraph=True)(*args)
+
+
+def test_free_sizes_stay_free():
+    """The checks of a fake kernel pin no size of an exported graph."""
+    from torch.export import Dim, export
+
+    class M(torch.nn.Module):
+        def forward(self, x, nw, w, keep):
+            y = tk.turbo_layer_norm(x, nw, checkpoint="int8")
+            codes, scales = tk.pack_activation(y)
+            z = tk.unpack_activation(codes, scales)
+            return tk.turbo_norm_linear(z, nw, None, w), tk.turbo_norm_linear(z[keep], None, None, w)
+
+    rows, outs = Dim("rows"), Dim("outs")
+    args = (E(10, 64), E(64), E(24, 64), torch.ones(10, dtype=torch.bool))
+    exported = export(M(), args, dynamic_shapes=({0: rows}, None, {0: outs}, {0: rows}))
+    assert sum("tpf_b200" in str(n.target) for n in exported.graph.nodes) == 5
+
+
 def test_int8_activations_leaves_cpu_tensors_alone():
     x = torch.randn(300, 300, requires_grad=True)
     with tk.int8_activations(min_elements=1):
