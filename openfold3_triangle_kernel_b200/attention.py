@@ -29,6 +29,7 @@ import math
 import torch
 
 from . import _cabi as C
+from ._checks import certain, differs
 
 _HEAD_LANES = (16, 32, 64)
 _MAX_BROADCAST_PREFIX_RANK = 16
@@ -105,14 +106,47 @@ def is_turbo_attention_supported(q, k, v, res_mask, pair_bias, *, check_device=T
 # custom ops (flattened batch, padded head dim): what a traced graph (torch.compile, torch.export, fake tensors) holds.
 # An eager call on plain CUDA tensors goes to `_native.attention`, which does the same in one C++ call.
 # --------------------------------------------------------------------------------------
+def _refuse_operands(q, k, v, mask, bias, check_device, d_out=None, out=None, lse=None):
+    def refuse(reason):
+        raise ValueError("unsupported TurboPairFormer case: " + reason)
+
+    if q.ndim != 5 or all(certain(q.shape[-1] != lane) for lane in _HEAD_LANES):
+        refuse("q must have shape [B,O,H,N,D], D padded to a lane")
+    B, O, H, N, D = q.shape
+    if any(certain(n < 1) for n in (B, O, H, N)):
+        refuse("requires positive dimensions")
+    if differs(k.shape, q.shape) or differs(v.shape, q.shape):
+        refuse("k and v must have q's shape")
+    if any(t.dtype != torch.bfloat16 for t in (q, k, v)):
+        refuse("q/k/v must be BF16")
+    if mask.dtype not in (torch.float32, torch.bfloat16, torch.float16) or differs(mask.shape, (B, O, N)):
+        refuse("the mask must be floating [B,O,N]")
+    if bias.dtype not in (torch.bfloat16, torch.float32) or (differs(bias.shape, (1, H, N, N))
+                                                              and differs(bias.shape, (B, H, N, N))):
+        refuse("the bias must be BF16 or FP32 [1 or B,H,N,N]")
+    if d_out is not None and (d_out.dtype != torch.bfloat16 or out.dtype != torch.bfloat16
+                              or differs(d_out.shape, (B, O, N, H, D)) or differs(out.shape, (B, O, N, H, D))):
+        refuse("the output and its gradient must be BF16 [B,O,N,H,D]")
+    if lse is not None and (lse.dtype != torch.float32 or differs(lse.shape, (B, O, H, N))):
+        refuse("the log-sum-exp must be FP32 [B,O,H,N]")
+    if any(t is not None and t.device != q.device for t in (k, v, mask, bias, d_out, out, lse)):
+        refuse("all operands must share one device")
+    if check_device and not q.is_cuda:
+        refuse("operands must be CUDA tensors")
+    if check_device and torch.cuda.get_device_capability(q.device)[0] != 10:
+        refuse("these kernels require a Blackwell sm_100a device")
+
+
 @torch.library.custom_op("tpf_b200::attn_fwd", mutates_args=())
 def _attn_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: torch.Tensor, bias: torch.Tensor,
               scale: float) -> tuple[torch.Tensor, torch.Tensor]:
+    _refuse_operands(q, k, v, mask, bias, True)
     return C.native().attn_fwd(q, k, v, mask, bias, scale)
 
 
 @_attn_fwd.register_fake
 def _(q, k, v, mask, bias, scale):
+    _refuse_operands(q, k, v, mask, bias, False)
     B, O, H, N, D = q.shape
     return (q.new_empty((B, O, N, H, D), dtype=torch.bfloat16), q.new_empty((B, O, H, N), dtype=torch.float32))
 
@@ -121,11 +155,13 @@ def _(q, k, v, mask, bias, scale):
 def _attn_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, d_out: torch.Tensor, out: torch.Tensor,
               lse: torch.Tensor, mask: torch.Tensor, bias: torch.Tensor,
               scale: float) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    _refuse_operands(q, k, v, mask, bias, True, d_out, out, lse)
     return C.native().attn_bwd(q, k, v, d_out, out, lse, mask, bias, scale)
 
 
 @_attn_bwd.register_fake
 def _(q, k, v, d_out, out, lse, mask, bias, scale):
+    _refuse_operands(q, k, v, mask, bias, False, d_out, out, lse)
     B, O, H, N, D = q.shape
     e = lambda: q.new_empty((B, O, H, N, D), dtype=torch.bfloat16)  # noqa: E731
     return e(), e(), e(), q.new_empty((bias.shape[0], H, N, N), dtype=torch.float32)
@@ -170,12 +206,13 @@ def turbo_attention(q, k, v, pair_bias=None, res_mask=None, *, return_lse=False)
         if not isinstance(q, torch.Tensor) or q.ndim < 5:
             raise ValueError("unsupported TurboPairFormer case: q must have shape [*B,O,H,N,D]")
         res_mask = q.new_zeros(q.shape[:-4] + (q.shape[-4], 1, 1, q.shape[-2]), dtype=torch.float32)
-    # Under torch.compile / torch.export the function is traced once on fake tensors: the metadata
-    # contract is checked when it runs eagerly, and by the fake kernel and the C ABI in either case.
-    if not torch.compiler.is_compiling():
-        ok, reason = is_turbo_attention_supported(q, k, v, res_mask, pair_bias)
-        if not ok:
-            raise ValueError(f"unsupported TurboPairFormer case: {reason}")
+    # Under torch.compile / torch.export the function is traced on fake tensors, which have no device to ask; the operators
+    # of the graph see to that, and to their own operands, whenever they run.
+    tracing = torch.compiler.is_compiling()
+    ok, reason = is_turbo_attention_supported(q, k, v, res_mask, pair_bias, check_device=not tracing)
+    if not ok:
+        raise ValueError("unsupported TurboPairFormer case: " + reason)
+    if not tracing:
         C.load()  # fail loudly when the native library is missing
         _INVOCATIONS += 1
 

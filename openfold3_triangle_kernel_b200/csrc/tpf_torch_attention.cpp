@@ -280,7 +280,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attn_bwd(const Tensor& q_, const Tens
   c10::cuda::CUDAGuard guard(q_.device());
   const Shape s{q_.size(0), q_.size(1), q_.size(2), q_.size(3), q_.size(4), bias.size(0)};
   const Tensor q = kernel_layout(q_), k = kernel_layout(k_), v = kernel_layout(v_);
-  const Grads g = launch_bwd(q, k, v, d_out.contiguous(), out.contiguous(), lse, prepare(mask, bias, s), s, scale,
+  const Grads g = launch_bwd(q, k, v, d_out.contiguous(), out.contiguous(), lse.contiguous(), prepare(mask, bias, s), s, scale,
                              TPF_ATTN_BWD_STAGE_ALL);
   return {g.dq, g.dk, g.dv, g.dbias};
 }

@@ -258,6 +258,7 @@ std::vector<Tensor> trimul_bwd(const Tensor& d_out_, const Tensor& z_, const Ten
   c10::cuda::CUDAGuard guard(z_.device());
   const Tensor z = aligned_bf16(z_), mask = mask_.to(at::kFloat).contiguous(), d_out = aligned_bf16(d_out_);
   const int64_t B = z.size(0), N = z.size(1), C = z.size(3);
+  for (Tensor& t : s) t = t.contiguous();
   std::vector<Tensor> w;
   for (const Tensor& t : w_) w.push_back(f32c(t));
   std::vector<Tensor> gw;

@@ -34,6 +34,7 @@ import operator
 import torch
 
 from . import _cabi as C
+from ._checks import certain, differs, refuse
 
 SUPPORTED_CHANNELS = (32, 64, 96, 128)
 _LN_EPS = 1e-5
@@ -109,21 +110,56 @@ def check_trimul_support(z, direction, mask, weights, *, check_device=True) -> S
 # custom ops: what a traced graph (torch.compile, torch.export, fake tensors) holds.  An eager call on plain CUDA
 # tensors goes to `_native.trimul`, which does the same in one C++ call.
 # --------------------------------------------------------------------------------------
+def _saved_like(z):
+    """Type and shape of what the forward operator returns."""
+    B, N, _, c = z.shape
+    R = B * N * N
+    bf, f32 = torch.bfloat16, torch.float32
+    return [(bf, (B, N, N, c)), (bf, (R, c)), (f32, (R,)), (f32, (R,)), (bf, (B * c, N * N)), (bf, (B * c, N * N)),
+            (bf, (R, c)), (bf, (B * c, N * N)), (bf, (R, c)), (f32, (R,)), (f32, (R,))]
+
+
+def _check_operands(z, mask, matrices, vectors, check_device, d_out=None, saved=()):
+    if z.ndim != 4 or certain(z.shape[1] != z.shape[2]) or certain(z.shape[1] < 1) or certain(z.shape[1] % 8 != 0):
+        return SupportResult(False, "z_shape", "z must have shape [B,N,N,C], N a multiple of 8")
+    if z.dtype != torch.bfloat16:
+        return SupportResult(False, "z_dtype", "z must be BF16")
+    c = z.shape[-1]
+    if all(certain(c != n) for n in SUPPORTED_CHANNELS):
+        return SupportResult(False, "channels", f"C={c} not in {SUPPORTED_CHANNELS}")
+    if differs(mask.shape, z.shape[:-1]):
+        return SupportResult(False, "mask_shape", "the mask must have shape [B,N,N]")
+    for w, shape in [*zip(matrices, ((2 * c, c), (2 * c, c), (c, c), (c, c))), *((v, (c,)) for v in vectors)]:
+        if differs(w.shape, shape):
+            return SupportResult(False, "weight_shape", f"a weight must have shape {shape}")
+        if not w.dtype.is_floating_point:
+            return SupportResult(False, "weight_dtype", "weights must be floating point")
+    if d_out is not None and differs(d_out.shape, z.shape):
+        return SupportResult(False, "d_out_shape", "d_out must have z's shape")
+    if any(t.dtype != dtype or differs(t.shape, shape) for t, (dtype, shape) in zip(saved, _saved_like(z))):
+        return SupportResult(False, "saved", "what the forward kept does not belong to this z")
+    if any(t.device != z.device for t in (mask, *matrices, *vectors, *saved, z if d_out is None else d_out)):
+        return SupportResult(False, "device", "all operands must share one device")
+    if check_device:
+        if not z.is_cuda:
+            return SupportResult(False, "device", "z must be a CUDA tensor")
+        if torch.cuda.get_device_capability(z.device)[0] != 10:
+            return SupportResult(False, "device_arch", "these kernels require a Blackwell sm_100a device")
+    return SupportResult(True, "ok", "supported")
+
+
 @torch.library.custom_op("tpf_b200::trimul_fwd", mutates_args=())
 def _trimul_fwd(z: torch.Tensor, mask: torch.Tensor, p_in: torch.Tensor, g_in: torch.Tensor, p_out: torch.Tensor,
                 g_out: torch.Tensor, nin_w: torch.Tensor, nin_b: torch.Tensor, nout_w: torch.Tensor,
                 nout_b: torch.Tensor, incoming: bool) -> list[torch.Tensor]:
+    refuse("turbo_trimul", _check_operands(z, mask, (p_in, g_in, p_out, g_out), (nin_w, nin_b, nout_w, nout_b), True))
     return C.native().trimul_fwd(z, mask, [p_in, g_in, p_out, g_out, nin_w, nin_b, nout_w, nout_b], incoming)
 
 
 @_trimul_fwd.register_fake
 def _(z, mask, p_in, g_in, p_out, g_out, nin_w, nin_b, nout_w, nout_b, incoming):
-    B, N, _, Cc = z.shape
-    R = B * N * N
-    bf = lambda *s: z.new_empty(s, dtype=torch.bfloat16)  # noqa: E731
-    f32 = lambda *s: z.new_empty(s, dtype=torch.float32)  # noqa: E731
-    return [bf(B, N, N, Cc), bf(R, Cc), f32(R), f32(R), bf(B * Cc, N * N), bf(B * Cc, N * N), bf(R, Cc),
-            bf(B * Cc, N * N), bf(R, Cc), f32(R), f32(R)]
+    refuse("turbo_trimul", _check_operands(z, mask, (p_in, g_in, p_out, g_out), (nin_w, nin_b, nout_w, nout_b), False))
+    return [z.new_empty(shape, dtype=dtype) for dtype, shape in _saved_like(z)]
 
 
 @torch.library.custom_op("tpf_b200::trimul_bwd", mutates_args=())
@@ -132,6 +168,9 @@ def _trimul_bwd(d_out: torch.Tensor, z: torch.Tensor, mask: torch.Tensor, p_in: 
                 out: torch.Tensor, zln: torch.Tensor, mean_in: torch.Tensor, rstd_in: torch.Tensor,
                 a_cm: torch.Tensor, b_cm: torch.Tensor, gate: torch.Tensor, x_cm: torch.Tensor, xln: torch.Tensor,
                 mean_out: torch.Tensor, rstd_out: torch.Tensor) -> list[torch.Tensor]:
+    refuse("turbo_trimul backward",
+           _check_operands(z, mask, (p_in, g_in, p_out, g_out), (nin_w, nout_w), True, d_out,
+                           (out, zln, mean_in, rstd_in, a_cm, b_cm, gate, x_cm, xln, mean_out, rstd_out)))
     return C.native().trimul_bwd(d_out, z, mask, [p_in, g_in, p_out, g_out, nin_w, nout_w], incoming,
                                  [out, zln, mean_in, rstd_in, a_cm, b_cm, gate, x_cm, xln, mean_out, rstd_out])
 
@@ -139,6 +178,9 @@ def _trimul_bwd(d_out: torch.Tensor, z: torch.Tensor, mask: torch.Tensor, p_in: 
 @_trimul_bwd.register_fake
 def _(d_out, z, mask, p_in, g_in, p_out, g_out, nin_w, nout_w, incoming, out, zln, mean_in, rstd_in, a_cm, b_cm,
       gate, x_cm, xln, mean_out, rstd_out):
+    refuse("turbo_trimul backward",
+           _check_operands(z, mask, (p_in, g_in, p_out, g_out), (nin_w, nout_w), False, d_out,
+                           (out, zln, mean_in, rstd_in, a_cm, b_cm, gate, x_cm, xln, mean_out, rstd_out)))
     Cc = z.shape[-1]
     f32 = lambda *s: z.new_empty(s, dtype=torch.float32)  # noqa: E731
     return [torch.empty_like(z), f32(2 * Cc, Cc), f32(2 * Cc, Cc), f32(Cc, Cc), f32(Cc, Cc), f32(Cc), f32(Cc),
@@ -221,12 +263,11 @@ def turbo_trimul(z, direction="outgoing", mask=None, *, generator=None, **weight
     unknown = set(weights) - set(_WEIGHT_NAMES)
     if unknown:
         raise TypeError(f"turbo_trimul got unexpected keyword arguments {sorted(unknown)}")
-    # Under torch.compile / torch.export the function is traced once on fake tensors: the metadata
-    # contract is checked when it runs eagerly, and by the fake kernel and the C ABI in either case.
-    if not torch.compiler.is_compiling():
-        res = check_trimul_support(z, direction, mask, weights)
-        if not res.supported:
-            raise ValueError(f"turbo_trimul unsupported [{res.code}]: {res.reason}")
+    # Under torch.compile / torch.export the function is traced on fake tensors, which have no device to ask; the operators
+    # of the graph see to that, and to their own operands, whenever they run.
+    tracing = torch.compiler.is_compiling()
+    refuse("turbo_trimul", check_trimul_support(z, direction, mask, weights, check_device=not tracing))
+    if not tracing:
         C.load()
 
     c = int(z.shape[-1])

@@ -231,6 +231,20 @@ def test_custom_ops_pass_opcheck():
     assert all(v == "SUCCESS" for v in res.values()), res
 
 
+def test_backward_operators_take_strided_statistics():
+    """What the forward kept may come back in another layout."""
+    att, d_a, tri, d_t = _op_inputs(torch.device("cuda", 0))
+    ops = torch.ops.tpf_b200
+    other = lambda t: torch.stack([t, t], -1)[..., 0]  # noqa: E731
+    with torch.no_grad():
+        out, lse = ops.attn_fwd(*att)
+        saved = ops.trimul_fwd(*tri)
+        ref = ops.attn_bwd(*att[:3], d_a, out, lse, *att[3:])
+        assert _same(ref, ops.attn_bwd(*att[:3], d_a, other(out), other(lse), *att[3:]))
+        args = (d_t, *tri[:7], tri[8], tri[10])
+        assert _same(ops.trimul_bwd(*args, *saved), ops.trimul_bwd(*args, *(other(t) for t in saved)))
+
+
 class _TrimulModule(torch.nn.Module):
     def __init__(self, w, direction):
         super().__init__()
