@@ -8,6 +8,8 @@ from __future__ import annotations
 
 import torch
 
+from . import _cabi
+
 
 def certain(comparison) -> bool:
     """Is a comparison of sizes true?  One of free sizes that can go either way counts as false."""
@@ -20,6 +22,27 @@ def certain(comparison) -> bool:
 def differs(shape, expected) -> bool:
     """Are two shapes certainly different?"""
     return len(shape) != len(expected) or any(certain(a != b) for a, b in zip(shape, expected))
+
+
+def has_tangent(*tensors) -> bool:
+    """Does any of them carry a forward-mode tangent?  No operator propagates one: a dual tensor is refused."""
+    from torch.autograd import forward_ad
+    if forward_ad._current_level < 0:
+        return False
+    functorch, native = torch._C._functorch, _cabi.native()
+    for t in tensors:
+        if not isinstance(t, torch.Tensor):
+            continue
+        while not native.has_tangent(t):    # (torch.func: of any level, which a dispatched call would not see)
+            if not functorch.is_functorch_wrapped_tensor(t):
+                break
+            t = functorch.get_unwrapped(t)
+        else:
+            return True
+    return False
+
+
+NO_TANGENT = "there is no forward-mode derivative"
 
 
 def refuse(operator, res):

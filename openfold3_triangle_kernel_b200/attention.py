@@ -16,7 +16,7 @@ and README.md:84-115):
   large finite mask such as -1e9, below -2**24.  Its output is zero in the first case
   and a mean of v in the second.
 * returns bf16 ``[*B, O, N, H, D]``; autograd for q, k, v and pair_bias
-  (the bias gradient has pair_bias's shape and dtype).
+  (the bias gradient has pair_bias's shape and dtype), first order, reverse mode only.
 
 Unsupported inputs raise ``ValueError("unsupported TurboPairFormer case: ...")``
 before anything is launched.  There is no fallback path: the device is reached
@@ -29,7 +29,7 @@ import math
 import torch
 
 from . import _cabi as C
-from ._checks import certain, differs
+from ._checks import NO_TANGENT, certain, differs, has_tangent
 
 _HEAD_LANES = (16, 32, 64)
 _MAX_BROADCAST_PREFIX_RANK = 16
@@ -99,6 +99,8 @@ def is_turbo_attention_supported(q, k, v, res_mask, pair_bias, *, check_device=T
         return False, "pair_bias broadcast supports at most 16 target-prefix dimensions"
     if res_mask.requires_grad:
         return False, "res_mask must not require gradients"
+    if has_tangent(*named.values()):
+        return False, NO_TANGENT
     return True, "supported"
 
 
@@ -131,6 +133,8 @@ def _refuse_operands(q, k, v, mask, bias, check_device, d_out=None, out=None, ls
         refuse("the log-sum-exp must be FP32 [B,O,H,N]")
     if any(t is not None and t.device != q.device for t in (k, v, mask, bias, d_out, out, lse)):
         refuse("all operands must share one device")
+    if has_tangent(q, k, v, mask, bias, d_out):
+        refuse(NO_TANGENT)
     if check_device and not q.is_cuda:
         refuse("operands must be CUDA tensors")
     if check_device and torch.cuda.get_device_capability(q.device)[0] != 10:

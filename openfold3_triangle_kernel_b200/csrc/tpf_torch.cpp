@@ -15,7 +15,7 @@ bool plain_cuda(const Tensor& t) {
                                             DispatchKey::FuncTorchBatched, DispatchKey::FuncTorchGradWrapper,
                                             DispatchKey::Functionalize, DispatchKey::Conjugate, DispatchKey::Negative,
                                             DispatchKey::ZeroTensor});
-  return t.is_cuda() && t.layout() == at::kStrided && !t.key_set().has_any(special);
+  return t.is_cuda() && t.layout() == at::kStrided && !t.key_set().has_any(special) && !t._fw_grad(/*level=*/0).defined();
 }
 
 // Parameter carries torch's marker for "no __torch_function__", and a subclass inherits it unless it defines one.
@@ -51,6 +51,9 @@ bool device_supported(const Tensor& t) {
 // (autograd.grad) would prune it and leave the term out.
 variable_list first_order(const variable_list& incoming, variable_list grads) {
   namespace ag = torch::autograd;
+  for (const Tensor& t : incoming)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(),
+                                "the gradients of these operators have no forward-mode derivative");
   if (!at::GradMode::is_enabled()) return grads;
   ag::edge_list edges = ag::get_current_node()->next_edges();
   for (const Tensor& t : incoming)
@@ -76,6 +79,7 @@ PYBIND11_MODULE(_native, m) {
   m.def("trimul_fwd", &tpf_torch::trimul_fwd);
   m.def("pair_block", &tpf_torch::py_pair_block);
   m.def("trimul_bwd", &tpf_torch::trimul_bwd);
+  m.def("has_tangent", [](const tpf_torch::Tensor& t) { return t._fw_grad(/*level=*/0).defined(); });
   m.def("layer_norm", &tpf_torch::py_layer_norm);
   m.def("layer_norm_fwd", &tpf_torch::layer_norm_fwd);
   m.def("layer_norm_bwd", &tpf_torch::layer_norm_bwd);

@@ -36,8 +36,9 @@ inline Tensor f32c(const Tensor& t) {
   return t.detach().to(at::kFloat).contiguous();
 }
 
-// A plain eager CUDA tensor: no functorch wrapper, no lazy conjugation or negation, no subclass that dispatches.  Anything
-// else (and any active dispatch mode) takes the torch.library route, which every such mechanism sees.
+// A plain eager CUDA tensor: no functorch wrapper, no lazy conjugation or negation, no forward-mode tangent (no operator
+// propagates one, and the Python route refuses it), no subclass that dispatches.  Anything else (and any active dispatch
+// mode) takes the torch.library route, which every such mechanism sees.
 bool plain_cuda(const Tensor& t);
 // ... and no subclass whose __torch_function__ wants to see the call, which the Python object tells: tensors, parameters and
 // subclasses of Parameter without one of their own pass.

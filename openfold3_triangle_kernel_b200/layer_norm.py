@@ -10,7 +10,7 @@ Operator contract:
   those of the true ``x``, the gradients are computed from the kept values.  The format is relative to the largest
   magnitude of a group, so rows whose mean is large against their spread lose more.
 * returns ``x``'s type and shape, contiguous; autograd for x, weight and bias (a gradient has its parameter's type), first
-  order only.  Statistics and sums are fp32 in a fixed order: the same inputs give the same bits.
+  order, reverse mode only.  Statistics and sums are fp32 in a fixed order: the same inputs give the same bits.
 
 A row that holds an infinity or a NaN is NaN; the others are not touched by it.  Unsupported inputs raise
 ``ValueError("turbo_layer_norm unsupported [code]: reason")``, in a traced call when it is traced (inside the compiler's own
@@ -25,7 +25,7 @@ from typing import Optional
 import torch
 
 from . import _cabi as C
-from ._checks import certain, differs, refuse
+from ._checks import NO_TANGENT, certain, differs, has_tangent, refuse
 from .trimul import SupportResult
 
 ROW_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
@@ -77,6 +77,8 @@ def check_layer_norm_support(x, weight=None, bias=None, eps=1e-5, checkpoint=Non
         bad = check_parameter(name, p, x.shape[-1], x)
         if bad is not None:
             return bad
+    if has_tangent(x, weight, bias):
+        return SupportResult(False, "tangent", NO_TANGENT)
     return SupportResult(True, "ok", "supported")
 
 

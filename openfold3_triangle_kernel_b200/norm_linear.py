@@ -10,7 +10,7 @@ Operator contract:
   rows, at most 2^30 outputs.
 * ``checkpoint``: as in :func:`turbo_layer_norm`.  Only x is kept, whole or in 8 bits: the normalised rows are made again
   in the backward pass, for the weight's gradient too.
-* returns bf16 ``[*, O]``; autograd for x, norm_weight, norm_bias and weight (first order only).  The normalised rows and
+* returns bf16 ``[*, O]``; autograd for x, norm_weight, norm_bias and weight (first order, reverse mode only).  The normalised rows and
   the gradient that reaches them are rounded to bf16 on their way to the tensor cores, sums are fp32 (four rows and fewer
   are not rounded on the way out).
 
@@ -26,7 +26,7 @@ from typing import Optional
 import torch
 
 from . import _cabi as C
-from ._checks import certain, differs, refuse
+from ._checks import NO_TANGENT, certain, differs, has_tangent, refuse
 from .layer_norm import CHECKPOINTS, ROW_DTYPES, check_kept, check_parameter, check_rows, kept_like
 from .trimul import SupportResult
 
@@ -59,6 +59,8 @@ def check_norm_linear_support(x, norm_weight, norm_bias, weight, eps=1e-5, check
         bad = check_parameter(name, p, cols, x)
         if bad is not None:
             return bad
+    if has_tangent(x, norm_weight, norm_bias, weight):
+        return SupportResult(False, "tangent", NO_TANGENT)
     return SupportResult(True, "ok", "supported")
 
 
@@ -68,6 +70,8 @@ def _check_backward(d_out, x, stats, codes, scales, norm_weight, norm_bias, weig
     res = check_norm_linear_support(like, norm_weight, norm_bias, weight, check_device=check_device)
     if not res.supported:
         return res
+    if has_tangent(d_out):
+        return SupportResult(False, "tangent", NO_TANGENT)
     if differs(d_out.shape, tuple(like.shape[:-1]) + (weight.shape[0],)):
         return SupportResult(False, "d_out_shape", "d_out does not belong to these rows and this weight")
     return check_kept(d_out, d_out.shape[:-1], weight.shape[1], x, stats, codes, scales) or res

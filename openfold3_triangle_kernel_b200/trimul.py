@@ -20,7 +20,7 @@ contract turbopairformer_trimul_support.py:153-400):
   ``TriangleMultiplicativeUpdate``-like module (``linear_{a_p,a_g,b_p,b_g,g,z}``,
   ``layer_norm_{in,out}``, ``_outgoing``).
 * returns bf16 ``[*B, N, N, C]``; autograd for z, the six matrices and the four norm
-  vectors (first order only).
+  vectors (first order, reverse mode only).
 
 Unlike the reference (N > 100 only) any ``N >= 1`` is accepted; N that is not a multiple
 of 8 is zero-padded with masked-out rows/columns and cropped again.
@@ -34,7 +34,7 @@ import operator
 import torch
 
 from . import _cabi as C
-from ._checks import certain, differs, refuse
+from ._checks import NO_TANGENT, certain, differs, has_tangent, refuse
 
 SUPPORTED_CHANNELS = (32, 64, 96, 128)
 _LN_EPS = 1e-5
@@ -103,6 +103,8 @@ def check_trimul_support(z, direction, mask, weights, *, check_device=True) -> S
             return SupportResult(False, "weight_dtype", f"{name} must be floating point")
         if w.device != z.device:
             return SupportResult(False, "weight_device", f"{name} must live on z's device")
+    if has_tangent(z, mask, *weights.values()):
+        return SupportResult(False, "tangent", NO_TANGENT)
     return SupportResult(True, "ok", "supported")
 
 
@@ -140,6 +142,8 @@ def _check_operands(z, mask, matrices, vectors, check_device, d_out=None, saved=
         return SupportResult(False, "saved", "what the forward kept does not belong to this z")
     if any(t.device != z.device for t in (mask, *matrices, *vectors, *saved, z if d_out is None else d_out)):
         return SupportResult(False, "device", "all operands must share one device")
+    if has_tangent(z, mask, *matrices, *vectors, d_out):
+        return SupportResult(False, "tangent", NO_TANGENT)
     if check_device:
         if not z.is_cuda:
             return SupportResult(False, "device", "z must be a CUDA tensor")
