@@ -149,9 +149,24 @@ def _is_dense(t):
     return True
 
 
+# what makes a copy of a tensor in another type or arrangement
+_COPIES = frozenset(n + "Backward0" for n in ("ToCopy", "Clone", "T", "Transpose", "Permute", "View", "UnsafeView", "ReshapeAlias",
+                                              "Expand", "Squeeze", "Unsqueeze", "Slice", "Select", "Split", "AsStrided", "Cat",
+                                              "Stack"))
+
+
 def _is_parameter(t):
+    """A parameter, trained or frozen; a view of one; a copy of trained ones (autocast and stacked projections make some)."""
     base = t if t._base is None else t._base
-    return base.is_leaf and base.requires_grad
+    if isinstance(base, torch.nn.Parameter) or (base.is_leaf and base.requires_grad):
+        return True
+    nodes = [t.grad_fn]
+    while nodes:
+        node = nodes.pop()
+        if node is None or node.name() not in _COPIES:
+            return False
+        nodes.extend(n for n, _ in node.next_functions if n is not None and n.name() != "torch::autograd::AccumulateGrad")
+    return True
 
 
 def _packable(t, min_elements):
@@ -167,9 +182,11 @@ def int8_activations(min_elements=65536, keep_whole=None):
     these stand for.
 
     That holds for bf16 and fp16 CUDA tensors of at least ``min_elements`` elements (the groups follow their memory order).
-    fp32 tensors (statistics, log-sum-exps), leaves that require gradients and views of them (parameters), tensors whose
-    elements overlap or leave gaps, and tensors for which ``keep_whole(t)`` is true are kept as they are.  An activation
-    that holds an infinity (logits behind a mask) would come back as NaN in its groups: keep such tensors whole.
+    fp32 tensors (statistics, log-sum-exps), parameters (``nn.Parameter``, frozen ones too, leaves that require gradients, views
+    of either, and casts, transposes or concatenations of trained ones), tensors whose elements overlap or leave gaps, and
+    tensors for which ``keep_whole(t)`` is true are kept as they are.  What else takes no gradient cannot be told from an
+    activation: name a large constant table and a 16-bit copy of a frozen fp32 weight, as autocast makes it, in ``keep_whole``
+    (or freeze the weight in 16 bits).  An activation that holds an infinity (logits behind a mask) would come back as NaN in its groups: keep such tensors whole.
     """
     def pack(t):
         if not _packable(t, min_elements) or (keep_whole is not None and keep_whole(t)):

@@ -174,6 +174,35 @@ def test_context_keeps_parameters_statistics_and_small_tensors_whole():
     assert torch.equal(torch.autograd.grad(y.sum(), w)[0], g2)
 
 
+@pytest.mark.parametrize("frozen", [True, False])
+def test_context_leaves_weights_alone(frozen):
+    """A frozen weight, or autocast's copy of a trained one: the input's gradient is that without the context, bit by bit,
+    and nothing more is kept."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    w = torch.randn(256, 256, device="cuda", generator=g)
+    w = torch.nn.Parameter(w.bfloat16() if frozen else w, requires_grad=not frozen)
+    x = torch.randn(512, 256, device="cuda", generator=g).bfloat16().requires_grad_(True)
+    d = torch.randn(512, 256, device="cuda", generator=g).bfloat16()
+
+    def run(context):
+        h = x * 1.0
+        before = torch.cuda.memory_allocated()
+        with torch.autocast("cuda", torch.bfloat16, enabled=not frozen), context:
+            y = torch.nn.functional.linear(h, w)
+        kept = torch.cuda.memory_allocated() - before
+        return torch.autograd.grad(y, x, d)[0], kept
+
+    import contextlib
+    run(contextlib.nullcontext())
+    g0, m0 = run(contextlib.nullcontext())
+    g1, m1 = run(tk.int8_activations(min_elements=1))
+    assert torch.equal(g0, g1)
+    if frozen:
+        assert m1 == m0
+    w8 = _value_of(w.detach().bfloat16().t())
+    assert not torch.equal(g0, (d.float() @ w8.t().float()).bfloat16())   # (the codes would have been seen)
+
+
 def test_context_around_the_framework_operators():
     """TriMul, layer norm and projection inside the context: gradients near those without it, less memory kept."""
     from openfold3_triangle_kernel_b200.synthetic import trimul_inputs

@@ -190,6 +190,38 @@ def test_int8_activations_leaves_cpu_tensors_alone():
     assert torch.equal(x.grad, x2.grad)
 
 
+def test_what_int8_activations_takes_for_a_parameter():
+    from openfold3_triangle_kernel_b200.activation_checkpoint import _is_parameter
+    lin = torch.nn.functional.linear
+    h = torch.randn(3, 8, dtype=BF, requires_grad=True) * 2
+
+    def kept(f, autocast=False):
+        """(is a parameter, shape) of what f keeps."""
+        seen = []
+        hooks = torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append((_is_parameter(t), tuple(t.shape))) or t,
+                                                         lambda t: t)
+        with torch.autocast("cpu", BF, enabled=autocast), hooks:
+            f()
+        assert seen
+        return {s for p, s in seen if p}, {s for p, s in seen if not p}
+
+    for grad in (True, False):
+        w = torch.nn.Parameter(torch.randn(4, 8, dtype=BF), requires_grad=grad)
+        acts = {(3, 8)} if grad else set()
+        assert kept(lambda: lin(h, w)) == ({(8, 4)}, acts)
+        assert kept(lambda: h @ w[:2].t()) == ({(8, 2)}, acts)
+        assert kept(lambda: h * w[0]) == ({(8,)}, acts)
+    m = torch.nn.Parameter(torch.randn(4, 8))
+    assert kept(lambda: lin(h, m), autocast=True) == ({(8, 4)}, {(3, 8)})
+    assert kept(lambda: lin(h, torch.cat([m, m * 1]).to(BF))) == (set(), {(8, 8), (3, 8)})
+    assert kept(lambda: lin(h, torch.cat([m, m]).to(BF))) == ({(8, 8)}, {(3, 8)})
+    assert kept(lambda: h * h) == (set(), {(3, 8)})
+    assert kept(lambda: torch.softmax(h, -1)) == (set(), {(3, 8)})
+    x = torch.randn(3, 8, dtype=BF)     # data: an activation
+    w = torch.nn.Parameter(torch.randn(4, 8, dtype=BF))
+    assert kept(lambda: lin(x, w)) == (set(), {(3, 8)})
+
+
 # ---- the C entries -------------------------------------------------------------------------------
 def _ln_fwd(**kw):
     a = dict(x=ONE, pitch=8, type=1, w=NULL, wt=0, b=NULL, bt=0, y=ONE, codes=NULL, scales=NULL, mean=NULL, rstd=NULL, rows=4,
