@@ -266,8 +266,9 @@ int tpf_layer_norm_bwd(const void* dy, const void* x, int64_t x_pitch, const voi
                        int64_t rows, int64_t cols, void* stream);
 
 /* Activations in 8 bits.  Groups of 128 consecutive elements of a row (the last one ragged) share a scale: with a = max |x|,
- * code = rint(x * fl32(127 / a)), scale = fl32(a / 127), value = code * scale.  Groups with a < 2^-119 are kept as zeros;
- * the scale of a group that holds an infinity or a NaN is NaN and its codes are 0.
+ * code = rint(x * fl32(127 / a)), scale = fl32(a / 127) (at most 0x1.020406p121, so that no value overflows), value =
+ * code * scale.  Groups with a < 2^-119 are kept as zeros; the scale of a group that holds an infinity or a NaN is NaN and
+ * its codes are 0.
  *   codes int8 [rows, cols] contiguous, scales fp32 [rows, ceil(cols / 128)]; fewer than 2^31 groups.
  * tpf_int8_unpack writes x contiguous. */
 int tpf_int8_pack(const void* x, int64_t x_pitch, int type, void* codes, float* scales, int64_t rows, int64_t cols,

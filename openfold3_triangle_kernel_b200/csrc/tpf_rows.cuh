@@ -4,7 +4,8 @@
 // 8-bit format.  Groups of 128 consecutive elements of a row (the last one ragged) share a scale.  With a = max |x| of
 // the group, f = fl32(127 / a) and s = fl32(a / 127): code = rint(x f), value = code s.  The product x f is exact in the
 // FMA that rounds it (ties to even), so the codes do not depend on the order of any operation.  |x f| <= 127 (1 + 2^-24)
-// rounds to at most 127.  a < 2^-119 (where f would overflow): the group is kept as zeros.  A group that holds an
+// rounds to at most 127.  s is the largest value with a finite 127 s at most (FLT_MAX / 127 rounds up, so that FLT_MAX, a common
+// fill of masks, would come back as infinity; no other a is touched).  a < 2^-119 (where f would overflow): the group is kept as zeros.  A group that holds an
 // infinity or a NaN has the scale NaN and codes 0, and comes back as NaN.
 #pragma once
 
@@ -21,6 +22,7 @@ typedef __nv_bfloat16 bf16;
 
 constexpr int kGroup = 128;             // elements of a row that share one scale
 constexpr float kTiny = 0x1p-119f;      // smallest amax that is kept
+constexpr float kMaxScale = 0x1.020406p121f;  // 127 times this is finite, of the next float it is not
 constexpr int64_t kMaxNormCols = 8192;  // widest row of the layer norm: 256 threads with 32 elements each
 
 enum RowType : int { kRowF32 = 0, kRowBF16 = 1, kRowF16 = 2 };
@@ -200,7 +202,7 @@ __device__ __forceinline__ GroupScale group_scale(float amax) {
   const float nan = __int_as_float(0x7fc00000);
   if (!(amax <= 3.402823466e38f)) return {nan, nan};  // (NaN compares false)
   if (amax < kTiny) return {0.f, 0.f};
-  return {__fdiv_rn(127.f, amax), __fdiv_rn(amax, 127.f)};
+  return {__fdiv_rn(127.f, amax), fminf(__fdiv_rn(amax, 127.f), kMaxScale)};
 }
 // The factors of N groups (1, 2 or 4) that LANES lanes hold together, each lane with every amax: the quotients cost more than
 // all else, so each lane computes those of one group, and they are handed round.  Returns the `down` of group

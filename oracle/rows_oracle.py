@@ -13,6 +13,7 @@ import torch
 U = 2.0 ** -24
 GROUP = 128
 TINY = 2.0 ** -119
+MAX_SCALE = float.fromhex("0x1.020406p121")     # the largest fp32 value with a finite product with 127
 
 
 def half_step(dtype):
@@ -31,7 +32,7 @@ def pack(x):
     empty = a < TINY
     safe = torch.where(bad | empty, 1.0, a)
     up = torch.where(empty, 0.0, 127.0 / safe).float().double()
-    down = torch.where(empty, 0.0, safe / 127.0).float().double()
+    down = torch.where(empty, 0.0, safe / 127.0).float().double().clamp(max=MAX_SCALE)
     codes = torch.round(torch.where(bad, 0.0, p) * up)
     down = torch.where(bad, float("nan"), down)
     return (codes.view(rows, -1)[:, :cols], down.view(rows, groups), (codes * down).view(rows, -1)[:, :cols])

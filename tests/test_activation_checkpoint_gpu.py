@@ -78,6 +78,19 @@ def test_extremes():
 
 
 @pytest.mark.parametrize("cols", [128, 200, 97])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_the_largest_values_stay_finite(cols, dtype):
+    """finfo.max and finfo.min fill masks.  127 scales of FLT_MAX / 127, rounded up, would be infinity."""
+    info = torch.finfo(DT[dtype])
+    x = _x(5, cols, DT[dtype])
+    x[1], x[2, 3], x[3, 7], x[3, 8] = info.min, info.max, info.min, info.max
+    codes, scales = _check(x)
+    back = tk.unpack_activation(codes, scales, DT[dtype])
+    assert torch.isfinite(back).all() and codes[1].eq(-127).all()
+    assert ((back[1].cpu().double() / x[1].double() - 1).abs() <= 2.0 ** -23 + ro.half_step(DT[dtype])).all()
+
+
+@pytest.mark.parametrize("cols", [128, 200, 97])
 @pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
 def test_infinities_mark_their_group(cols, value):
     x = _x(6, cols, torch.bfloat16)
