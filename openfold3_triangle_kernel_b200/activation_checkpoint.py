@@ -2,8 +2,9 @@
 
 Format: groups of 128 consecutive elements of a row (the last one ragged) share an fp32 scale.  With ``a`` the largest
 magnitude of a group, ``code = rint(x * fl32(127 / a))`` (ties to even, the product exact), ``scale = fl32(a / 127)`` and
-``value = code * scale``: off by half a step, ``a / 254``, at most.  (The scale of ``a = FLT_MAX`` is one step less, so that no
-value overflows.)  Groups with ``a < 2**-119`` are kept as zeros; a group
+``value = code * scale``.  (The scale of ``a = FLT_MAX`` is one step less, so that no value overflows.)  A value is off by half a
+step of the codes, ``a / 254``, and by the roundings of the two factors and the product, ``a 2^-21``, at most; one that is
+given back in 16 bits is rounded to them, half a step of that type on top.  Groups with ``a < 2**-119`` are kept as zeros; a group
 that holds an infinity or a NaN comes back as NaN.
 
 * :func:`pack_activation` / :func:`unpack_activation`: the two directions, for any ``[*, C]`` in bf16, fp16 or fp32.

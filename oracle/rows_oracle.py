@@ -38,6 +38,22 @@ def pack(x):
     return (codes.view(rows, -1)[:, :cols], down.view(rows, groups), (codes * down).view(rows, -1)[:, :cols])
 
 
+def pack_off(x, dtype):
+    """What the values given back in ``dtype`` may be off by from x itself.  With f = (127 / a)(1 + e1), s = (a / 127)(1 + e2), code =
+    x f + d, |d| <= 1/2, the value is (x (1 + e1)(1 + e2) + d (a / 127)(1 + e2))(1 + e3); |e1|, |e3| <= U, |e2| <= 2 U (U, but for the
+    largest scale), |x| <= a: off by a (1 / 254 + 5 U) in fp32, below a (1 / 254 + 2^-21).  Then half a step of the type, of a
+    subnormal the smallest normal's.  Groups below the smallest amax are off by all they have."""
+    rows, cols = x.shape
+    groups = -(-cols // GROUP)
+    p = torch.zeros(rows, groups * GROUP, dtype=torch.float64)
+    p[:, :cols] = x.double().abs()
+    a = p.view(rows, groups, GROUP).amax(-1, keepdim=True).expand(-1, -1, GROUP).reshape(rows, -1)[:, :cols]
+    off = torch.where(a < TINY, a, a * (1 / 254 + 2.0 ** -21))
+    if dtype == torch.float32:
+        return off
+    return off + half_step(dtype) * torch.clamp(x.double().abs() + off, min=torch.finfo(dtype).tiny)
+
+
 def layer_norm(x, w, b, eps):
     """``y``, ``mean``, ``rstd`` and the bound on y before it is rounded."""
     x = x.double()

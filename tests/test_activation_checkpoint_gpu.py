@@ -41,6 +41,17 @@ def test_pack_and_unpack(rows, cols, dtype):
     _check(_x(rows, cols, DT[dtype], seed=rows + cols))
 
 
+@pytest.mark.parametrize("cols", [5, 97, 128, 200, 1000])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_values_are_near_what_was_put_away(cols, dtype):
+    """The bound that the documents give, against x itself."""
+    for scale in (1.0, 1.0625, 2.0 ** -10, 300.0):
+        x = _x(200, cols, DT[dtype], seed=cols) * scale
+        x[::7, cols // 2] = scale * 1.0625
+        back = tk.unpack_activation(*tk.pack_activation(x.cuda()), DT[dtype])
+        assert ((back.cpu().double() - x.double()).abs() <= ro.pack_off(x, DT[dtype])).all()
+
+
 @pytest.mark.parametrize("cols", [1, 3, 5, 7, 9, 17, 30, 60, 63, 97, 121, 127, 130, 131, 135, 250, 259, 381, 1029, 4099])
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_odd_widths_of_many_rows(cols, dtype):

@@ -222,6 +222,20 @@ def test_what_int8_activations_takes_for_a_parameter():
     assert kept(lambda: lin(x, w)) == (set(), {(3, 8)})
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_the_8_bit_format_is_as_near_as_the_documents_say(dtype):
+    """Half a step of the codes alone (a / 254) is not the bound: values are rounded once more."""
+    from oracle import rows_oracle as ro
+    g = torch.Generator().manual_seed(1)
+    x = (torch.randn(4000, 128, generator=g) * torch.exp(3 * torch.randn(4000, 1, generator=g))).to(dtype)
+    x[::3, 0] = 1.0625
+    x[1::3] = (torch.randint(-254, 255, (len(x[1::3]), 128), generator=g) / 254).to(dtype)      # (ties and near ties)
+    x[7], x[8], x[9] = torch.finfo(dtype).max, torch.finfo(dtype).tiny, torch.finfo(dtype).tiny / 4
+    off = (ro.pack(x)[2].float().to(dtype).double() - x.double()).abs()
+    assert (off <= ro.pack_off(x, dtype)).all()
+    assert (off > x.double().abs().amax(-1, keepdim=True) / 254).any()
+
+
 # ---- the C entries -------------------------------------------------------------------------------
 def _ln_fwd(**kw):
     a = dict(x=ONE, pitch=8, type=1, w=NULL, wt=0, b=NULL, bt=0, y=ONE, codes=NULL, scales=NULL, mean=NULL, rstd=NULL, rows=4,
