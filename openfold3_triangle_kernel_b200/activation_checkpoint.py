@@ -183,12 +183,20 @@ def int8_activations(min_elements=65536, keep_whole=None):
     """Context manager: what autograd keeps inside it for the backward pass, it keeps in 8 bits and gives back as the values
     these stand for.
 
-    That holds for bf16 and fp16 CUDA tensors of at least ``min_elements`` elements (the groups follow their memory order).
+    A 16-bit tensor then takes 1 + 4 / 128 bytes an element in the place of 2, once for each node that keeps it: nothing is
+    looked up by a tensor's address, which kernels and replayed graphs write to without autograd's knowledge.  What one node
+    keeps (layer norm, activation function, one stacked projection) takes half; what two keep takes what it took, and an input
+    of separate q, k, v and gate projections, which autograd holds once for all, twice that: stack them, or name it in
+    ``keep_whole``.  The TriMul and the pair-stack block hold their intermediates in byte buffers of their own; of theirs,
+    inputs and outputs are reached.
+
+    This is done to bf16 and fp16 CUDA tensors of at least ``min_elements`` elements (the groups follow their memory order).
     fp32 tensors (statistics, log-sum-exps), parameters (``nn.Parameter``, frozen ones too, leaves that require gradients, views
     of either, and casts, transposes or concatenations of trained ones), tensors whose elements overlap or leave gaps, and
     tensors for which ``keep_whole(t)`` is true are kept as they are.  What else takes no gradient cannot be told from an
     activation: name a large constant table and a 16-bit copy of a frozen fp32 weight, as autocast makes it, in ``keep_whole``
-    (or freeze the weight in 16 bits).  An activation that holds an infinity (logits behind a mask) would come back as NaN in its groups: keep such tensors whole.
+    (or freeze the weight in 16 bits).  An activation that holds an infinity (logits behind a mask) would come back as NaN in
+    its groups: keep such tensors whole.
     """
     def pack(t):
         if not _packable(t, min_elements) or (keep_whole is not None and keep_whole(t)):

@@ -227,6 +227,48 @@ def test_context_leaves_weights_alone(frozen):
     assert not torch.equal(g0, (d.float() @ w8.t().float()).bfloat16())   # (the codes would have been seen)
 
 
+def test_what_the_context_keeps():
+    """Bytes of one tensor of 2^20 elements with one, two and four nodes that keep it, each with codes of its own; without the
+    context autograd holds it once."""
+    import contextlib
+    n = 2 ** 20
+    packed = n + 4 * n // 128
+    x = torch.randn(4096, 256, device="cuda").bfloat16()
+    ws = [torch.nn.Parameter(torch.randn(8, 256, device="cuda").bfloat16()) for _ in range(4)]
+    linears = lambda k: (lambda h: [torch.nn.functional.linear(h, w) for w in ws[:k]])  # noqa: E731
+
+    def kept(f, context):
+        with context:
+            h = x * 1.0
+            before = torch.cuda.memory_allocated()
+            out = f(h)
+        size = sum(t.numel() * t.element_size() for t in out)
+        del h
+        return torch.cuda.memory_allocated() - before - size    # of h and of what is kept, but for h's 2 n
+
+    slack = 4096
+    for f, codes in ((linears(1), 1), (linears(2), 2), (linears(4), 4)):
+        assert abs(kept(f, contextlib.nullcontext())) <= slack
+        assert abs(kept(f, tk.int8_activations(min_elements=n)) - (codes * packed - 2 * n)) <= slack * codes
+
+
+def test_context_keeps_what_a_tensor_held_when_it_was_kept():
+    """A buffer that is written behind autograd's back (a replayed graph, a kernel) between two nodes that keep it."""
+    x = torch.nn.Parameter(torch.zeros(256, device="cuda", dtype=torch.bfloat16))
+    buf = torch.empty(64, 256, device="cuda", dtype=torch.bfloat16)
+    parts = [_x(64, 256, torch.bfloat16, seed=s).cuda() for s in (1, 2)]
+    with tk.int8_activations(min_elements=1):
+        out = []
+        for p in parts:
+            buf.data.copy_(p)
+            out.append((buf * x).float().sum())
+    (g,) = torch.autograd.grad(out[0] + out[1], x)
+    ref = sum(_value_of(p).double().sum(0) for p in parts)
+    # two bf16 gradients (sums of 64 terms in fp32), and their bf16 sum
+    mags = sum(_value_of(p).double().abs().sum(0) for p in parts)
+    assert ((g.double() - ref).abs() <= 2.0 ** -8 * 3 * mags + 64 * 2.0 ** -24 * mags).all()
+
+
 def test_context_around_the_framework_operators():
     """TriMul, layer norm and projection inside the context: gradients near those without it, less memory kept."""
     from openfold3_triangle_kernel_b200.synthetic import trimul_inputs
