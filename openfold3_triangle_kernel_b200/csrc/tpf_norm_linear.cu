@@ -2,6 +2,12 @@
 //
 //   forward    y = w xh + b (bf16), out = y W^T
 //   backward   dy = d_out W (bf16), the layer norm's backward on it, dW = d_out^T y~ with y~ from what was kept of x
+//
+// dy of wide rows goes through memory in bf16, as it does behind any bf16 Linear (narrow rows never leave the SM and stay in
+// fp32).  In fp32 d_x and the norm's gradients would be off by their own rounding only, 0.0017 of their norm in the place of
+// 0.0024, for twice the traffic between the two kernels: the whole backward of 4099 rows, 1024 -> 4096, takes 100 us in the
+// place of 94, 16384 of 1024 -> 1024 131 / 115, 100000 of 256 -> 1024 174 / 156, 60000 of 512 -> 512 152 / 121, 300000 of 136 ->
+// 512 389 / 295 (cold L2).
 #include "tpf_norm_linear.cuh"
 
 namespace tpf {
