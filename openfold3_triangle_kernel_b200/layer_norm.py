@@ -30,6 +30,7 @@ from .trimul import SupportResult
 
 ROW_DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 MAX_COLUMNS = 8192
+MAX_EPS = torch.finfo(torch.float32).max
 CHECKPOINTS = (None, "int8")
 
 
@@ -56,8 +57,8 @@ def check_rows(x, eps, checkpoint, check_device):
         return SupportResult(False, "columns", f"C={x.shape[-1]} exceeds {MAX_COLUMNS}")
     if checkpoint not in CHECKPOINTS:
         return SupportResult(False, "checkpoint", "checkpoint must be None or 'int8'")
-    if not (isinstance(eps, (int, float)) and eps >= 0 and math.isfinite(eps)):
-        return SupportResult(False, "eps", "eps must be a finite number, not negative")
+    if not (isinstance(eps, (int, float)) and 0 <= eps <= MAX_EPS):
+        return SupportResult(False, "eps", "eps must be a finite FP32 number, not negative")
     if check_device:
         if not x.is_cuda:
             return SupportResult(False, "device", "x must be a CUDA tensor")
@@ -174,7 +175,7 @@ _layer_norm_fwd.register_autograd(_backward, setup_context=_setup_context)
 def turbo_layer_norm(x, weight=None, bias=None, *, eps=1e-5, checkpoint=None):
     """Layer norm over the last dimension; see the module docstring for the contract."""
     if not torch.compiler.is_compiling():
-        if checkpoint in CHECKPOINTS and isinstance(eps, (int, float)) and math.isfinite(eps):
+        if checkpoint in CHECKPOINTS and isinstance(eps, (int, float)) and eps <= MAX_EPS:
             y = C.native().layer_norm(x, weight, bias, eps, checkpoint == "int8")
             if y is not None:
                 return y

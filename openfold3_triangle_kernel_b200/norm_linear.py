@@ -28,7 +28,7 @@ import torch
 
 from . import _cabi as C
 from ._checks import NO_TANGENT, certain, differs, has_tangent, refuse
-from .layer_norm import CHECKPOINTS, ROW_DTYPES, check_kept, check_parameter, check_rows, kept_like
+from .layer_norm import CHECKPOINTS, MAX_EPS, ROW_DTYPES, check_kept, check_parameter, check_rows, kept_like
 from .trimul import SupportResult
 
 MAX_ROWS = 2 ** 31 - 256
@@ -137,7 +137,7 @@ _norm_linear_fwd.register_autograd(_backward, setup_context=_setup_context)
 def turbo_norm_linear(x, norm_weight, norm_bias, weight, *, eps=1e-5, checkpoint=None):
     """Layer norm and Linear in one operator; see the module docstring for the contract."""
     if not torch.compiler.is_compiling():
-        if checkpoint in CHECKPOINTS and isinstance(eps, (int, float)) and math.isfinite(eps):
+        if checkpoint in CHECKPOINTS and isinstance(eps, (int, float)) and eps <= MAX_EPS:
             out = C.native().norm_linear(x, norm_weight, norm_bias, weight, eps, checkpoint == "int8")
             if out is not None:
                 return out

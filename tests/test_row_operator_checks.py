@@ -80,6 +80,19 @@ def test_unpack_support(codes, scales, dtype, code):
     assert _codes(check_unpack_support(codes, scales, dtype, check_device=False)) == (False, code)
 
 
+@pytest.mark.parametrize("eps", [float("inf"), 1e39, 10 ** 400, -1e-300], ids=["inf", "1e39", "1e400", "-1e-300"])
+def test_eps_is_a_number_of_32_bits(eps):
+    """A larger one became an infinity, and every row its bias."""
+    x = torch.zeros(4, 16)
+    assert tk.check_layer_norm_support(x, eps=torch.finfo(torch.float32).max, check_device=False).supported
+    assert _codes(tk.check_layer_norm_support(x, eps=eps, check_device=False)) == (False, "eps")
+    assert _codes(tk.check_norm_linear_support(x.bfloat16(), None, None, torch.zeros(8, 16), eps, check_device=False)) == (
+        False, "eps")
+    for f in (lambda: tk.turbo_layer_norm(x, eps=eps), lambda: tk.turbo_norm_linear(x.bfloat16(), None, None, x[:, :], eps=eps)):
+        with pytest.raises(ValueError, match=r"unsupported \[eps\]"):
+            f()
+
+
 def test_operators_refuse_cpu_tensors():
     x = torch.zeros(4, 16)
     with pytest.raises(ValueError, match=r"turbo_layer_norm unsupported \[device\]"):
