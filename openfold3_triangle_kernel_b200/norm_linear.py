@@ -10,14 +10,14 @@ Operator contract:
   rows, at most 2^30 outputs.
 * ``checkpoint``: as in :func:`turbo_layer_norm`.  Only x is kept, whole or in 8 bits: the normalised rows are made again
   in the backward pass, for the weight's gradient too.
-* returns bf16 ``[*, O]``; autograd for x, norm_weight, norm_bias and weight (first order, reverse mode only).  The normalised rows are
-  rounded to bf16 on their way to the tensor cores (but in the forward of four rows and fewer), sums are fp32.  The gradient
+* returns bf16 ``[*, O]``; autograd for x, norm_weight, norm_bias and weight (first order, reverse mode only).  The
+  normalised rows are rounded to bf16 on their way to the tensor cores (but in the forward of four rows and fewer), sums are
+  fp32.  The gradients of weight and, where rows are narrow, of norm_weight are made of rows rounded that way.  The gradient
   that reaches the normalised rows is rounded to bf16 on its way to the layer norm's backward, as a bf16 Linear would leave
   it, but where rows are narrow (up to 128 columns, a weight of up to 128 KB).
 
 Unsupported inputs raise ``ValueError("turbo_norm_linear unsupported [code]: reason")``, traced ones as in
-:func:`turbo_layer_norm`.  There is no counterpart among the
-reference's kernels (it calls torch's LayerNorm and Linear).
+:func:`turbo_layer_norm`.  There is no counterpart among the reference's kernels (it calls torch's LayerNorm and Linear).
 """
 from __future__ import annotations
 
