@@ -151,10 +151,11 @@ def _is_dense(t):
     return True
 
 
-# what makes a copy of a tensor in another type or arrangement
-_COPIES = frozenset(n + "Backward0" for n in ("ToCopy", "Clone", "T", "Transpose", "Permute", "View", "UnsafeView", "ReshapeAlias",
-                                              "Expand", "Squeeze", "Unsqueeze", "Slice", "Select", "Split", "AsStrided", "Cat",
-                                              "Stack"))
+# what makes a copy of a tensor in another type or arrangement (autograd numbers the overloads)
+_COPIES = frozenset(n + "Backward" for n in ("ToCopy", "Clone", "T", "Transpose", "Permute", "View", "UnsafeView", "ReshapeAlias",
+                                             "Expand", "Squeeze", "Unsqueeze", "Slice", "Select", "Split", "SplitWithSizes",
+                                             "Unbind", "AsStrided", "Cat", "Stack"))
+_MOST_COPIES = 256
 
 
 def _is_parameter(t):
@@ -162,10 +163,10 @@ def _is_parameter(t):
     base = t if t._base is None else t._base
     if isinstance(base, torch.nn.Parameter) or (base.is_leaf and base.requires_grad):
         return True
-    nodes = [t.grad_fn]
+    nodes, count = [t.grad_fn], 0
     while nodes:
-        node = nodes.pop()
-        if node is None or node.name() not in _COPIES:
+        node, count = nodes.pop(), count + 1
+        if node is None or node.name().rstrip("0123456789") not in _COPIES or count > _MOST_COPIES:
             return False
         nodes.extend(n for n, _ in node.next_functions if n is not None and n.name() != "torch::autograd::AccumulateGrad")
     return True

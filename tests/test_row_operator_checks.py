@@ -228,6 +228,12 @@ def test_what_int8_activations_takes_for_a_parameter():
     assert kept(lambda: lin(h, m), autocast=True) == ({(8, 4)}, {(3, 8)})
     assert kept(lambda: lin(h, torch.cat([m, m * 1]).to(BF))) == (set(), {(8, 8), (3, 8)})
     assert kept(lambda: lin(h, torch.cat([m, m]).to(BF))) == ({(8, 8)}, {(3, 8)})
+    assert kept(lambda: lin(h, m.to(BF).split([1, 3])[1])) == ({(8, 3)}, {(3, 8)})
+    assert kept(lambda: lin(h, m.to(BF).unsqueeze(0).squeeze(0))) == ({(8, 4)}, {(3, 8)})
+    doubled = m.to(BF)[:, :1]
+    for _ in range(40):     # (a walk over every path would take 2^40 steps)
+        doubled = torch.cat([doubled, doubled])[:4]
+    assert kept(lambda: h[:, :1] @ doubled.t())[1] >= {(1, 4)}
     assert kept(lambda: h * h) == (set(), {(3, 8)})
     assert kept(lambda: torch.softmax(h, -1)) == (set(), {(3, 8)})
     x = torch.randn(3, 8, dtype=BF)     # data: an activation
