@@ -143,3 +143,46 @@ def test_right_calls_are_traced_whole():
         torch.compile(CALLS[0][0], backend="eager", fullgraph=True)(*_att_call())
     with pytest.raises(ValueError, match=r"\[device\]"):
         torch.compile(CALLS[3][0], backend="eager", fullgraph=True)(*_tri_call())
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA device")
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+def test_dynamic_sizes_train_as_eager_ones(checkpoint):
+    """The checks of the fake kernels meet free sizes, forward and backward."""
+    g = torch.Generator(device="cuda").manual_seed(0)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    nw, nb = r(64).requires_grad_(True), r(64).requires_grad_(True)
+    w = r(24, 64).requires_grad_(True)
+
+    def f(x):
+        y = tk.turbo_layer_norm(x, nw, nb, checkpoint=checkpoint)
+        codes, scales = tk.pack_activation(x)
+        return tk.turbo_norm_linear(y.bfloat16(), None, nb, w, checkpoint=checkpoint), tk.unpack_activation(codes, scales)
+
+    torch.compiler.reset()
+    compiled = torch.compile(f, fullgraph=True, dynamic=True, backend="aot_eager")
+    for rows in (10, 33, 200):
+        x, d = r(rows, 64).requires_grad_(True), r(rows, 24).bfloat16()
+        res = []
+        for call in (f, compiled):
+            o, v = call(x)
+            res.append([o, v, *torch.autograd.grad(o, (x, nw, nb, w), d)])
+        assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA device")
+def test_triangle_operators_follow_dynamic_sizes():
+    g = torch.Generator(device="cuda").manual_seed(0)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+    from openfold3_triangle_kernel_b200.synthetic import trimul_weights
+    tw = {n: t.cuda() for n, t in trimul_weights(32, 0).items()}
+    torch.compiler.reset()
+    att = lambda q, b: tk.turbo_attention(q, q, q, pair_bias=b)  # noqa: E731
+    tri = lambda z, m: tk.turbo_trimul(z, "incoming", m, **tw)  # noqa: E731
+    for n in (16, 24):
+        q, b = r(1, n, 2, n, 32).bfloat16(), r(1, 1, 2, n, n)
+        assert torch.equal(torch.compile(att, fullgraph=True, dynamic=True, backend="aot_eager")(q, b), att(q, b))
+        z, m = r(1, n, n, 32).bfloat16(), (r(1, n, n) > 0).float()
+        assert torch.equal(torch.compile(tri, fullgraph=True, dynamic=True, backend="aot_eager")(z, m), tri(z, m))
