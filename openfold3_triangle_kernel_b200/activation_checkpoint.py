@@ -197,7 +197,9 @@ def int8_activations(min_elements=65536, keep_whole=None):
     tensors for which ``keep_whole(t)`` is true are kept as they are.  What else takes no gradient cannot be told from an
     activation: name a large constant table and a 16-bit copy of a frozen fp32 weight, as autocast makes it, in ``keep_whole``
     (or freeze the weight in 16 bits).  An activation that holds an infinity (logits behind a mask) would come back as NaN in
-    its groups: keep such tensors whole.
+    its groups: keep such tensors whole.  An attention makes its probabilities again from the kept q and k, so what these are
+    off by grows with the logits: gradients of :func:`turbo_attention` are off by 1.5 % of their norm at logits of a standard
+    deviation of 1, 5 % at 4, 9 % at 8.
     """
     def pack(t):
         if not _packable(t, min_elements) or (keep_whole is not None and keep_whole(t)):

@@ -295,6 +295,28 @@ def test_context_around_the_framework_operators():
     assert (g1 - g0).norm() / g0.norm() < 0.04
 
 
+def test_context_around_a_masked_attention():
+    """The additive mask is fp32 and stays whole, its infinities with it.  At logits of a standard deviation of 1 each kept value
+    is off by 0.6 % (root mean square), a logit by 0.006 sqrt(2), and P, v and the output by as much again: below 4 % in all."""
+    import contextlib
+    g = torch.Generator(device="cuda").manual_seed(2)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g).bfloat16().requires_grad_(True)  # noqa: E731
+    q, k, v, bias = r(1, 16, 4, 96, 32), r(1, 16, 4, 96, 32), r(1, 16, 4, 96, 32), r(1, 1, 4, 96, 96)
+    mask = torch.zeros(1, 16, 1, 1, 96, device="cuda")
+    mask[:, :, ..., 80:] = -float("inf")
+    mask[:, 3] = -float("inf")      # a row without a key
+    d = r(1, 16, 96, 4, 32).detach()
+
+    def run(context):
+        with context:
+            o = tk.turbo_attention(q * 1, k * 1, v * 1, pair_bias=bias * 1, res_mask=mask)
+        return torch.autograd.grad(o, (q, k, v, bias), d)
+
+    for a, b in zip(run(contextlib.nullcontext()), run(tk.int8_activations(min_elements=1))):
+        assert torch.isfinite(b).all()
+        assert 0 < (a.float() - b.float()).norm() / a.float().norm() < 0.04
+
+
 def test_context_inside_a_capture():
     """What is packed while a graph is captured is packed again by every replay."""
     w = torch.randn(64, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True)
