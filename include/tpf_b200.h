@@ -292,6 +292,58 @@ int tpf_norm_linear_bwd(const void* d_out, const void* x, int64_t x_pitch, const
                         int d_weight_type, void* workspace, int64_t workspace_bytes, int64_t rows, int64_t cols,
                         int64_t outs, void* stream);
 
+/* ---- dropout, and the operators around a sequence attention (no counterparts in the reference) ---------------------------
+ * Dropout: out = residual + (kept ? x * 65536 / (65536 - threshold) : 0).  Element m of the mask is kept where its 16 random bits
+ * are not below `threshold` (0 .. 65536): half word m & 7 (the low half of a word first) of Philox 4x32-10 with key = seed and
+ * counter = (m >> 3, offset).  The backward pass is the same call with x = the output's gradient and no residual.
+ *   sizes    elements (p, q, s, e); e is contiguous in all tensors, the strides (in elements) are those of p, q and s
+ *   shared   1: the mask is shared along s, m = (p Q + q) E + e; 0: m = ((p Q + q) S + s) E + e
+ *   residual NULL: none
+ *   seed_offset  (seed, offset) in device memory, or NULL: the two numbers that follow */
+int tpf_dropout(const void* x, const int64_t* x_strides, const void* residual, const int64_t* residual_strides, void* out,
+                const int64_t* out_strides, const int64_t* sizes, int type, int shared, int threshold, const int64_t* seed_offset,
+                int64_t seed, int64_t offset, void* stream);
+
+/* Position rotation of heads, with an RMS norm of each head before it where `norm` is set: y = x / sqrt(mean(x^2) + eps) * weight;
+ * pair i of the first `rot` elements (half: i with i + rot / 2; else 2 i with 2 i + 1): (a, b) -> magnitude (a cos t - b sin t,
+ * a sin t + b cos t), t = 2 pi position turns[i] / 2^64.
+ *   q, k     [batch, tokens, heads, dim] of `type`, strides of batch, token and head in elements; k_heads = 0: no k
+ *   weights  [dim] of their own types, or NULL (ones); dim 2 .. 256, rot even, 2 .. dim
+ *   positions  int64 [batch, tokens], or NULL: first, first + 1, ...
+ * Outputs are contiguous.  The backward pass takes the outputs' gradients (contiguous); x may be NULL without a norm, and weights'
+ * gradients that are not wanted are NULL.  workspace: 16-byte aligned, needed for the weights' gradients only. */
+int tpf_rotary_fwd(const void* q, const int64_t* q_strides, int64_t q_heads, const void* q_weight, int q_weight_type, void* q_out,
+                   const void* k, const int64_t* k_strides, int64_t k_heads, const void* k_weight, int k_weight_type, void* k_out,
+                   int type, int64_t batch, int64_t tokens, int64_t dim, int64_t rot, const int64_t* turns, float magnitude,
+                   const int64_t* positions, int64_t first, int half, int norm, float eps, void* stream);
+int64_t tpf_rotary_bwd_workspace_bytes(int64_t dim);
+int tpf_rotary_bwd(const void* dq_out, const void* q, const int64_t* q_strides, int64_t q_heads, const void* q_weight,
+                   int q_weight_type, void* dq, void* d_q_weight, const void* dk_out, const void* k, const int64_t* k_strides,
+                   int64_t k_heads, const void* k_weight, int k_weight_type, void* dk, void* d_k_weight, int type, int64_t batch,
+                   int64_t tokens, int64_t dim, int64_t rot, const int64_t* turns, float magnitude, const int64_t* positions,
+                   int64_t first, int half, int norm, float eps, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Window attention: out = softmax(scale q k^T) v over the keys that a query sees.  Query i of batch b stands at position
+ * p = offset_b + i and sees key j where j < length_b, j <= p + right, and j >= p - left or j < sinks; a query that sees nothing gives
+ * zeros and lse = -inf.
+ *   q [B, N, H, D], k and v [B, M, HK, D], BF16 or FP16, strides of batch, token and head (positive multiples of 8 elements), 16-byte
+ *            aligned; H a multiple of HK, D a multiple of 8 up to 128; out [B, N, H, D] contiguous; lse fp32 [B, H, N] or NULL
+ *   left, right  reach of the window, below 2^28; negative: unlimited.  sinks: 0 .. 64
+ *   offsets  int32 [B] (clamped to +-2^29), or NULL: `offset` (within 2^28); lengths  int32 [B] (clamped to 0 .. M), or NULL: M
+ * The backward pass writes dq [B, N, H, D], dk and dv [B, M, HK, D] (contiguous; dq, or dk and dv, may be NULL).  It is
+ * deterministic.  workspace: 256-byte aligned. */
+int tpf_window_attn_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                        const int64_t* v_strides, void* out, float* lse, int type, int64_t B, int64_t N, int64_t M, int64_t H,
+                        int64_t HK, int64_t D, float scale, int64_t left, int64_t right, int64_t sinks, const int* offsets,
+                        int64_t offset, const int* lengths, void* stream);
+int64_t tpf_window_attn_bwd_workspace_bytes(int64_t B, int64_t N, int64_t M, int64_t H, int64_t HK, int64_t D, int64_t left,
+                                            int64_t right, int64_t sinks);
+int tpf_window_attn_bwd(const void* d_out, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                        const void* v, const int64_t* v_strides, const void* out, const float* lse, void* dq, void* dk, void* dv,
+                        int type, int64_t B, int64_t N, int64_t M, int64_t H, int64_t HK, int64_t D, float scale, int64_t left,
+                        int64_t right, int64_t sinks, const int* offsets, int64_t offset, const int* lengths, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

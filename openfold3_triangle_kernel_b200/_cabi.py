@@ -52,6 +52,13 @@ SIGNATURES = {
     "tpf_norm_linear_fwd": [_P, _I, _P, _i, _P, _i] + [_P] * 7 + [_I, _I, _I, _I, _f, _P],
     "tpf_norm_linear_bwd": [_P, _P, _I] + [_P] * 4 + [_P, _i, _P, _i, _P, _P, _P, _i, _P, _i, _P, _i, _P, _I, _I, _I, _I,
                                                    _P],
+    "tpf_dropout": [_P, _PI, _P, _PI, _P, _PI, _PI, _i, _i, _i, _P, _I, _I, _P],
+    "tpf_rotary_fwd": [_P, _PI, _I, _P, _i, _P] * 2 + [_i, _I, _I, _I, _I, _P, _f, _P, _I, _i, _i, _f, _P],
+    "tpf_rotary_bwd_workspace_bytes": [_I],
+    "tpf_rotary_bwd": [_P, _P, _PI, _I, _P, _i, _P, _P] * 2 + [_i, _I, _I, _I, _I, _P, _f, _P, _I, _i, _i, _f, _P, _I, _P],
+    "tpf_window_attn_fwd": [_P, _PI, _P, _PI, _P, _PI, _P, _P, _i] + [_I] * 6 + [_f, _I, _I, _I, _P, _I, _P, _P],
+    "tpf_window_attn_bwd_workspace_bytes": [_I] * 9,
+    "tpf_window_attn_bwd": [_P, _P, _PI, _P, _PI, _P, _PI] + [_P] * 5 + [_i] + [_I] * 6 + [_f, _I, _I, _I, _P, _I, _P, _P, _I, _P],
 }
 _RESTYPES = {"tpf_trimul_fwd_workspace_bytes": ctypes.c_int64, "tpf_trimul_bwd_workspace_bytes": ctypes.c_int64,
              "tpf_trimul_bwd_stages_workspace_bytes": ctypes.c_int64,
@@ -59,6 +66,7 @@ _RESTYPES = {"tpf_trimul_fwd_workspace_bytes": ctypes.c_int64, "tpf_trimul_bwd_w
              "tpf_layer_norm_bwd_workspace_bytes": ctypes.c_int64,
              "tpf_norm_linear_fwd_workspace_bytes": ctypes.c_int64,
              "tpf_norm_linear_bwd_workspace_bytes": ctypes.c_int64,
+             "tpf_rotary_bwd_workspace_bytes": ctypes.c_int64, "tpf_window_attn_bwd_workspace_bytes": ctypes.c_int64,
              "tpf_attn_bwd_static_scratch_capacity": ctypes.c_int64, "tpf_launch_count": ctypes.c_int64,
              "tpf_version": ctypes.c_char_p, "tpf_last_error_string": ctypes.c_char_p}
 

@@ -1,8 +1,11 @@
 // extern "C" surface of libtpf_b200.so (declarations: include/tpf_b200.h).
 #include "../../include/tpf_b200.h"
 #include "tpf_host.cuh"
+#include "tpf_dropout.h"
 #include "tpf_internal.h"
+#include "tpf_rotary.h"
 #include "tpf_rows.h"
+#include "tpf_window.h"
 
 namespace tpf {
 
@@ -47,6 +50,8 @@ int selftest_status_fetch_and_clear(int* out);
 int norm_linear_dw_status_fetch_and_clear(int* out);
 int norm_linear_fwd_status_fetch_and_clear(int* out);
 int norm_linear_bwd_status_fetch_and_clear(int* out);
+int window_fwd_status_fetch_and_clear(int* out);
+int window_bwd_status_fetch_and_clear(int* out);
 int selftest_bounded_wait(unsigned int* report, cudaStream_t stream);
 
 int trimul_status_fetch_and_clear(int* out);
@@ -98,6 +103,10 @@ int tpf_device_status(int* status) {
   if ((rc = tpf::norm_linear_fwd_status_fetch_and_clear(&v))) return rc;
   total |= v;
   if ((rc = tpf::norm_linear_bwd_status_fetch_and_clear(&v))) return rc;
+  total |= v;
+  if ((rc = tpf::window_fwd_status_fetch_and_clear(&v))) return rc;
+  total |= v;
+  if ((rc = tpf::window_bwd_status_fetch_and_clear(&v))) return rc;
   total |= v;
   if ((rc = tpf::selftest_status_fetch_and_clear(&v))) return rc;
   total |= v;
@@ -322,6 +331,107 @@ int tpf_norm_linear_bwd(const void* d_out, const void* x, int64_t x_pitch, const
   const tpf::NormLinearGrads g{d_out, dx, d_norm_weight, d_norm_bias, d_norm_weight_type, d_norm_bias_type, d_weight,
                                d_weight_type};
   return tpf::norm_linear_bwd(c, weight, outs, g, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int tpf_dropout(const void* x, const int64_t* x_strides, const void* residual, const int64_t* residual_strides, void* out,
+                const int64_t* out_strides, const int64_t* sizes, int type, int shared, int threshold, const int64_t* seed_offset,
+                int64_t seed, int64_t offset, void* stream) {
+  TPF_REQUIRE(x_strides && out_strides && sizes && (residual == nullptr || residual_strides), TPF_ERR_INVALID_ARGUMENT,
+              "dropout: null pointer");
+  tpf::DropoutCall c = {};
+  c.x = x, c.residual = residual, c.out = out;
+  for (int i = 0; i < 3; ++i) {
+    c.x_strides[i] = x_strides[i];
+    c.residual_strides[i] = residual != nullptr ? residual_strides[i] : 0;
+    c.out_strides[i] = out_strides[i];
+  }
+  for (int i = 0; i < 4; ++i) c.sizes[i] = sizes[i];
+  c.type = type, c.shared = shared, c.threshold = threshold;
+  c.seed_ptr = seed_offset, c.seed = seed, c.offset = offset;
+  return tpf::dropout(c, static_cast<cudaStream_t>(stream));
+}
+
+static int rotary_tensor(tpf::RotaryTensor* t, const void* x, const int64_t* strides, int64_t heads, const void* weight,
+                         int weight_type, const void* dy, void* out, void* dweight) {
+  TPF_REQUIRE(heads <= 0 || x == nullptr || strides != nullptr, TPF_ERR_INVALID_ARGUMENT, "rotary: null pointer");
+  *t = {x, {0, 0, 0}, heads, weight, weight_type, dy, out, dweight};
+  for (int i = 0; i < 3 && strides != nullptr; ++i) t->strides[i] = strides[i];
+  return TPF_OK;
+}
+
+int tpf_rotary_fwd(const void* q, const int64_t* q_strides, int64_t q_heads, const void* q_weight, int q_weight_type, void* q_out,
+                   const void* k, const int64_t* k_strides, int64_t k_heads, const void* k_weight, int k_weight_type, void* k_out,
+                   int type, int64_t batch, int64_t tokens, int64_t dim, int64_t rot, const int64_t* turns, float magnitude,
+                   const int64_t* positions, int64_t first, int half, int norm, float eps, void* stream) {
+  tpf::RotaryCall c = {};
+  if (int rc = rotary_tensor(&c.t[0], q, q_strides, q_heads, q_weight, q_weight_type, nullptr, q_out, nullptr)) return rc;
+  if (int rc = rotary_tensor(&c.t[1], k, k_strides, k_heads, k_weight, k_weight_type, nullptr, k_out, nullptr)) return rc;
+  c.type = type, c.batch = batch, c.tokens = tokens, c.dim = dim, c.rot = rot, c.turns = turns, c.magnitude = magnitude;
+  c.positions = positions, c.first = first, c.half = half, c.norm = norm, c.eps = eps;
+  return tpf::rotary_fwd(c, static_cast<cudaStream_t>(stream));
+}
+
+int64_t tpf_rotary_bwd_workspace_bytes(int64_t dim) { return tpf::rotary_bwd_workspace_bytes(dim); }
+
+int tpf_rotary_bwd(const void* dq_out, const void* q, const int64_t* q_strides, int64_t q_heads, const void* q_weight,
+                   int q_weight_type, void* dq, void* d_q_weight, const void* dk_out, const void* k, const int64_t* k_strides,
+                   int64_t k_heads, const void* k_weight, int k_weight_type, void* dk, void* d_k_weight, int type, int64_t batch,
+                   int64_t tokens, int64_t dim, int64_t rot, const int64_t* turns, float magnitude, const int64_t* positions,
+                   int64_t first, int half, int norm, float eps, void* workspace, int64_t workspace_bytes, void* stream) {
+  tpf::RotaryCall c = {};
+  if (int rc = rotary_tensor(&c.t[0], q, q_strides, q_heads, q_weight, q_weight_type, dq_out, dq, d_q_weight)) return rc;
+  if (int rc = rotary_tensor(&c.t[1], k, k_strides, k_heads, k_weight, k_weight_type, dk_out, dk, d_k_weight)) return rc;
+  c.type = type, c.batch = batch, c.tokens = tokens, c.dim = dim, c.rot = rot, c.turns = turns, c.magnitude = magnitude;
+  c.positions = positions, c.first = first, c.half = half, c.norm = norm, c.eps = eps;
+  return tpf::rotary_bwd(c, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+static tpf::WindowCall window_call(int type, int64_t B, int64_t N, int64_t M, int64_t H, int64_t HK, int64_t D, float scale,
+                                   int64_t left, int64_t right, int64_t sinks, const int* offsets, int64_t offset,
+                                   const int* lengths) {
+  auto reach = [](int64_t n) { return n < 0 ? tpf::kWindowUnlimited : n < tpf::kWindowMost ? (int)n : -1; };  // -1 is refused
+  tpf::WindowCall c = {};
+  c.B = B, c.N = N, c.M = M, c.H = H, c.HK = HK, c.D = D, c.type = type, c.scale = scale;
+  c.left = reach(left), c.right = reach(right);
+  c.sinks = sinks < 0 || sinks > tpf::kMostSinks ? -1 : (int)sinks;
+  c.offsets = offsets, c.offset = offset, c.lengths = lengths;
+  return c;
+}
+
+static int window_operands(tpf::WindowCall* c, const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* v,
+                           const int64_t* vs) {
+  TPF_REQUIRE(qs && ks && vs, TPF_ERR_INVALID_ARGUMENT, "window_attn: null pointer");
+  c->q = q, c->k = k, c->v = v;
+  for (int i = 0; i < 3; ++i) c->qs[i] = qs[i], c->ks[i] = ks[i], c->vs[i] = vs[i];
+  return TPF_OK;
+}
+
+int tpf_window_attn_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                        const int64_t* v_strides, void* out, float* lse, int type, int64_t B, int64_t N, int64_t M, int64_t H,
+                        int64_t HK, int64_t D, float scale, int64_t left, int64_t right, int64_t sinks, const int* offsets,
+                        int64_t offset, const int* lengths, void* stream) {
+  tpf::WindowCall c = window_call(type, B, N, M, H, HK, D, scale, left, right, sinks, offsets, offset, lengths);
+  if (int rc = window_operands(&c, q, q_strides, k, k_strides, v, v_strides)) return rc;
+  c.out = out, c.lse = lse;
+  return tpf::window_attn_fwd(c, static_cast<cudaStream_t>(stream));
+}
+
+int64_t tpf_window_attn_bwd_workspace_bytes(int64_t B, int64_t N, int64_t M, int64_t H, int64_t HK, int64_t D, int64_t left,
+                                            int64_t right, int64_t sinks) {
+  const tpf::WindowCall c = window_call(TPF_BF16, B, N, M, H, HK, D, 1.f, left, right, sinks, nullptr, 0, nullptr);
+  return c.left >= 0 && c.right >= 0 && c.sinks >= 0 ? tpf::window_attn_bwd_workspace_bytes(c) : 0;
+}
+
+int tpf_window_attn_bwd(const void* d_out, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                        const void* v, const int64_t* v_strides, const void* out, const float* lse, void* dq, void* dk, void* dv,
+                        int type, int64_t B, int64_t N, int64_t M, int64_t H, int64_t HK, int64_t D, float scale, int64_t left,
+                        int64_t right, int64_t sinks, const int* offsets, int64_t offset, const int* lengths, void* workspace,
+                        int64_t workspace_bytes, void* stream) {
+  tpf::WindowCall c = window_call(type, B, N, M, H, HK, D, scale, left, right, sinks, offsets, offset, lengths);
+  if (int rc = window_operands(&c, q, q_strides, k, k_strides, v, v_strides)) return rc;
+  c.out = const_cast<void*>(out), c.lse = const_cast<float*>(lse);
+  c.d_out = d_out, c.dq = dq, c.dk = dk, c.dv = dv;
+  return tpf::window_attn_bwd(c, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

@@ -90,4 +90,12 @@ PYBIND11_MODULE(_native, m) {
   m.def("int8_unpack", &tpf_torch::py_int8_unpack);
   m.def("int8_pack_op", &tpf_torch::int8_pack);
   m.def("int8_unpack_op", &tpf_torch::int8_unpack);
+  m.def("dropout", &tpf_torch::py_dropout);
+  m.def("dropout_op", &tpf_torch::dropout_op);
+  m.def("rotary", &tpf_torch::py_rotary);
+  m.def("rotary_fwd", &tpf_torch::rotary_fwd_op);
+  m.def("rotary_bwd", &tpf_torch::rotary_bwd_op);
+  m.def("window_attention", &tpf_torch::py_window_attention);
+  m.def("window_attn_fwd", &tpf_torch::window_fwd_op);
+  m.def("window_attn_bwd", &tpf_torch::window_bwd_op);
 }

@@ -99,4 +99,28 @@ py::object py_int8_unpack(py::handle codes, py::handle scales, py::object dtype)
 std::vector<Tensor> int8_pack(const Tensor& x);
 Tensor int8_unpack(const Tensor& codes, const Tensor& scales, int64_t type);
 
+// ---- dropout, rotation, window attention (tpf_torch_sequence.cpp) -----------------------------
+py::object py_dropout(py::handle x, py::handle residual, py::handle seed_tensor, int64_t seed, int64_t offset, int64_t threshold,
+                      int64_t shared);
+Tensor dropout_op(const Tensor& x, const std::optional<Tensor>& residual, const std::optional<Tensor>& seed_tensor, int64_t seed,
+                  int64_t offset, int64_t threshold, int64_t shared);
+py::object py_rotary(py::handle q, py::handle k, py::handle qw, py::handle kw, py::handle turns, py::handle positions, int64_t first,
+                     double magnitude, bool half, bool norm, double eps);
+std::vector<Tensor> rotary_fwd_op(const Tensor& q, const std::optional<Tensor>& k, const std::optional<Tensor>& qw,
+                                  const std::optional<Tensor>& kw, const Tensor& turns, const std::optional<Tensor>& positions,
+                                  int64_t first, double magnitude, bool half, bool norm, double eps);
+std::vector<Tensor> rotary_bwd_op(const std::optional<Tensor>& dq, const std::optional<Tensor>& dk, const std::optional<Tensor>& q,
+                                  const std::optional<Tensor>& k, const std::optional<Tensor>& qw, const std::optional<Tensor>& kw,
+                                  const Tensor& turns, const std::optional<Tensor>& positions, int64_t first, double magnitude,
+                                  bool half, bool norm, double eps);
+py::object py_window_attention(py::handle q, py::handle k, py::handle v, py::handle offsets, py::handle lengths, int64_t offset,
+                               int64_t left, int64_t right, int64_t sinks, double scale, bool return_lse);
+std::tuple<Tensor, Tensor> window_fwd_op(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& offsets,
+                                         const std::optional<Tensor>& lengths, int64_t offset, int64_t left, int64_t right,
+                                         int64_t sinks, double scale);
+std::tuple<Tensor, Tensor, Tensor> window_bwd_op(const Tensor& d_out, const Tensor& q, const Tensor& k, const Tensor& v,
+                                                 const Tensor& out, const Tensor& lse, const std::optional<Tensor>& offsets,
+                                                 const std::optional<Tensor>& lengths, int64_t offset, int64_t left, int64_t right,
+                                                 int64_t sinks, double scale);
+
 }  // namespace tpf_torch

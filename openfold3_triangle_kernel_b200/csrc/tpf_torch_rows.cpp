@@ -1,11 +1,8 @@
 // Row-wise operators for eager CUDA tensors: layer norm, 8-bit checkpoints, normalised projection.
 #include <torch/csrc/Dtype.h>
 
-#include <ATen/cuda/EmptyTensor.h>
-#include <c10/cuda/CUDACachingAllocator.h>
-
 #include "tpf_rows.h"
-#include "tpf_torch.h"
+#include "tpf_torch_memory.h"
 #include "tpf_torch_trimul.h"
 
 namespace tpf_torch {
@@ -14,30 +11,6 @@ namespace {
 
 constexpr int64_t kMaxCols = 8192;  // of a layer norm (tpf_layer_norm_fwd)
 constexpr int64_t kMaxLinearRows = (1ll << 31) - 256, kMaxOuts = 1ll << 30;  // of a projection (tpf_norm_linear_fwd)
-
-// Straight from the allocator of the current device: a tensor through the dispatcher costs 1.2 us, and a small training
-// pass makes six.
-Tensor make(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
-  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
-}
-struct Scratch {  // device memory of a call
-  c10::DataPtr p;
-  explicit Scratch(int64_t bytes) {
-    if (bytes > 0) p = c10::cuda::CUDACachingAllocator::get()->allocate(bytes);
-  }
-  void* get() const { return p.get(); }
-};
-
-cudaStream_t cu_stream() { return static_cast<cudaStream_t>(stream()); }
-
-int row_type(const Tensor& t) {  // -1: not a type of these operators
-  switch (t.scalar_type()) {
-    case at::kFloat: return TPF_F32;
-    case at::kBFloat16: return TPF_BF16;
-    case at::kHalf: return TPF_F16;
-    default: return -1;
-  }
-}
 
 // A tensor [*, C] as rows of one pitch: read in place where its strides allow it, else a contiguous copy.
 struct Rows {
@@ -73,10 +46,7 @@ Rows as_vector_rows(const Tensor& t) {  // bf16 rows that start on 16-byte bound
   return r;
 }
 
-using MaybeTensor = std::optional<Tensor>;
 Tensor value_or_none(const MaybeTensor& t) { return t ? t->detach().contiguous() : Tensor(); }
-void* ptr_of(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-int type_of(const Tensor& t) { return t.defined() ? row_type(t) : 0; }
 
 tpf::NormCall norm_call(const Rows& x, const Tensor& w, const Tensor& b) {
   tpf::NormCall c = {};

@@ -1,0 +1,535 @@
+// Window attention, backward, for sm_100a.
+//
+//   P = exp(S - lse) where a key is seen (0 elsewhere, and in rows that see nothing),  dP = dO V^T,  dS = P (dP - delta)
+//   dV = P^T dO,  dK = scale dS^T Q,  dQ = scale dS K,       delta = rowsum(dO out)
+//
+// Three kernels: `stats` makes -lse log2(e) and -delta of every query, padded to whole tiles; `window_bwd_kernel` then runs
+// twice, once with the keys as rows (dK and dV) and once with the queries (dQ).  It makes S and dP again for each: seven
+// products a tile instead of five, but every gradient is summed by one CTA in a fixed order, without atomics and without partial
+// sums of dQ in memory (at a window of 1024 keys those would be 9 times dQ in fp32, written and read).
+//
+// A CTA keeps 128 rows (keys: K and V; queries: Q and dO) in shared memory and walks over tiles of 64 columns.  S and dP are made
+// with the rows as TMEM lanes, so that P and dS, written over them as 16-bit numbers, are the A operands of the second products
+// straight from TMEM; a thread has a row.  Two groups of four warps take turns with the tiles: while one computes, the products of
+// the other run.  With the keys as rows the CTA goes through all query heads that share them.
+//
+// The sinks are seen by every later query, which would make the first keys' CTA walk over the whole sequence.  It does its window;
+// the queries beyond are split over CTAs of their own, whose sums of the sinks' rows a last kernel adds up in a fixed order.
+#include "tpf_window_kernels.h"
+
+namespace tpf {
+
+static __device__ int g_window_bwd_status;
+
+int window_bwd_status_fetch_and_clear(int* out) {
+  int v = 0, zero = 0;
+  TPF_CUDA_OK(cudaMemcpyFromSymbol(&v, g_window_bwd_status, sizeof(int)));
+  if (v) TPF_CUDA_OK(cudaMemcpyToSymbol(g_window_bwd_status, &zero, sizeof(int)));
+  *out = v;
+  return TPF_OK;
+}
+
+namespace {
+
+constexpr int kTile = 64;  // columns of a tile
+
+// ---- stats ------------------------------------------------------------------------------------------------
+// [B, H, NP] of -lse log2(e) (-inf: the row sees nothing, or lies behind the last one) and of -delta.
+template <typename T>
+__global__ void __launch_bounds__(256) window_stats_kernel(const T* __restrict__ out, const T* __restrict__ d_out,
+                                                           const float* __restrict__ lse, float* __restrict__ nlse,
+                                                           float* __restrict__ ndelta, int N, int NP, int H, int D, int64_t rows) {
+  griddep_wait();
+  const int lane = threadIdx.x & 15;
+  const int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);  // (b, i of NP, h)
+  const int64_t bi = r / H;
+  const int h = (int)(r - bi * H);
+  const int64_t b = bi / NP;
+  const int i = (int)(bi - b * NP);
+  float s[1] = {0.f};
+  const bool on = r < rows && i < N;
+  if (on && lane * 8 < D) {
+    const int64_t at = ((b * N + i) * H + h) * D + lane * 8;
+    Piece<T, 8> x, y;
+    x.load(out + at);
+    y.load(d_out + at);
+    float u[8], v[8];
+    x.get(u);
+    y.get(v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[0] = fmaf(u[e], v[e], s[0]);
+  }
+  warp_sum(s, 16);
+  if (lane == 0 && r < rows) {
+    const int64_t at = (b * H + h) * NP + i;
+    const float l = on ? lse[(b * H + h) * N + i] : -INFINITY;
+    nlse[at] = l == -INFINITY ? -INFINITY : -l * kWindowLog2e;
+    ndelta[at] = -s[0];
+  }
+}
+
+// ---- gradients --------------------------------------------------------------------------------------------
+struct BwdArgs {
+  const float *nlse, *ndelta;  // [B, H, NP]
+  int NP;
+  void *g1, *g2;               // KEYS: dV and dK; else dQ and nothing
+  float* parts;                // KEYS: [B, HK, 1 + far][2][sinks][D] of the sinks' rows, or nullptr
+  int key_tiles, far, far_tiles;  // KEYS: CTAs of far queries, and query tiles of each
+};
+
+template <typename T_, int DP_, bool KEYS_>
+struct BwdCfg {
+  using T = T_;
+  static constexpr bool KEYS = KEYS_;
+  static constexpr int DP = DP_, CHUNKS = DP / 64, NS = DP == 128 ? 4 : 6;
+  static constexpr int R_CHUNK = 128 * 128, C_CHUNK = kTile * 128;
+  static constexpr int R_TILE = CHUNKS * R_CHUNK, C_TILE = CHUNKS * C_CHUNK;
+  static constexpr int OFF_R = 0;                              // two tiles of rows
+  static constexpr int OFF_C = OFF_R + 2 * R_TILE;             // [NS] two tiles of columns
+  static constexpr int OFF_VEC = OFF_C + NS * 2 * C_TILE;      // [NS] nlse and ndelta of the columns (KEYS)
+  static constexpr int OFF_BAR = OFF_VEC + (KEYS ? NS * 2 * kTile * 4 : 0);
+  static constexpr int N_BAR = 2 + 2 * NS + 4;
+  static constexpr int SMEM = OFF_BAR + N_BAR * 8 + 16;
+  static constexpr int THREADS = 320, WARP_TMA = 8, WARP_MMA = 9;
+  static constexpr int TM_ACC1 = 256, TM_ACC2 = 256 + DP, TMEM_COLS = 512;
+  static_assert(SMEM + 1024 <= 233472 && TM_ACC2 + DP <= TMEM_COLS, "");
+};
+
+__device__ __forceinline__ void bulk_load(uint32_t elected, void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %4, 0;\n\t"
+      "@q cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n\t}" ::"r"(smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar)), "r"(elected)
+      : "memory");
+}
+
+// The column tiles of a CTA: for each of `heads` heads [extra tile 0,] lo .. hi - 1.
+struct Columns {
+  int extra, lo, hi, heads;
+  __device__ __forceinline__ int per_head() const { return extra + max(0, hi - lo); }
+};
+
+template <class Cfg>
+__global__ void __launch_bounds__(Cfg::THREADS, 1)
+window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constant__ CUtensorMap tmR2,
+                  const __grid_constant__ CUtensorMap tmC1, const __grid_constant__ CUtensorMap tmC2, const WindowParams p,
+                  const BwdArgs a, int* __restrict__ status) {
+  griddep_wait();
+  using T = typename Cfg::T;
+  constexpr bool KEYS = Cfg::KEYS;
+  constexpr int DP = Cfg::DP, NS = Cfg::NS, CHUNKS = Cfg::CHUNKS;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
+  uint64_t* r_full = bars;
+  uint64_t* acc_full = bars + 1;
+  uint64_t* c_full = bars + 2;           // [NS]
+  uint64_t* c_empty = c_full + NS;
+  uint64_t* sdp_full = c_empty + NS;     // [2]
+  uint64_t* pds_ready = sdp_full + 2;    // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::N_BAR);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const WaitCtx wctx{abort_flag, status};
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    mbar_init(r_full, 1);
+    mbar_init(acc_full, 1);
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&c_full[s], 1);
+      mbar_init(&c_empty[s], 1);
+    }
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(&sdp_full[g], 1);
+      mbar_init(&pds_ready[g], 4);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tmR1);
+    tma_prefetch_desc(&tmR2);
+    tma_prefetch_desc(&tmC1);
+    tma_prefetch_desc(&tmC2);
+  }
+  if (warp == Cfg::WARP_MMA) {
+    tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  const int b = blockIdx.z, head = blockIdx.y;  // KEYS: a key head, else a query head
+  const int len = p.length(b), off = p.first_position(b);
+  const bool far = KEYS && (int)blockIdx.x >= a.key_tiles;  // queries beyond the first key tile's window
+  const int r0 = far ? 0 : (int)blockIdx.x * 128;
+  Columns cols;
+  cols.extra = 0;
+  if constexpr (KEYS) {
+    cols.heads = p.G;
+    const int last = min(r0 + 127, len - 1);
+    const int lo = min(max(0, r0 - p.right - off), p.N), hi = max(0, min(p.N, last + p.left - off + 1));
+    cols.lo = lo / kTile;
+    cols.hi = r0 < len ? max(cols.lo, (hi + kTile - 1) / kTile) : cols.lo;
+    if (far) {
+      const int c = (int)blockIdx.x - a.key_tiles, all = (p.N + kTile - 1) / kTile;
+      cols.lo = max(cols.hi, c * a.far_tiles);
+      cols.hi = len > 0 ? min(all, (c + 1) * a.far_tiles) : cols.lo;
+    }
+  } else {
+    cols.heads = 1;
+    const KeyRange kr = key_range(p, len, off + r0, off + min(r0 + 127, p.N - 1));
+    cols.extra = kr.lo >= kTile && kr.sink > 0 ? 1 : 0;
+    cols.lo = kr.sink > 0 && !cols.extra ? 0 : kr.lo / kTile;
+    cols.hi = (kr.hi + kTile - 1) / kTile;
+  }
+  const int per_head = cols.per_head(), tiles = per_head * cols.heads;
+  // tile u of a head starts at column
+  auto first = [&](int u) { return u < cols.extra ? 0 : (cols.lo + u - cols.extra) * kTile; };
+
+  if (warp == Cfg::WARP_TMA) {
+    const uint32_t el = elect_one();
+    if (tiles > 0) {
+      mbar_expect_tx(el, r_full, 2 * Cfg::R_TILE);
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) {
+        tma_load_4d(el, smem + Cfg::OFF_R + c * Cfg::R_CHUNK, &tmR1, r_full, 64 * c, r0, head, b);
+        tma_load_4d(el, smem + Cfg::OFF_R + Cfg::R_TILE + c * Cfg::R_CHUNK, &tmR2, r_full, 64 * c, r0, head, b);
+      }
+    }
+    int s = 0;
+    uint32_t ph = 1;
+    for (int hh = 0; hh < cols.heads && per_head > 0; ++hh) {
+      const int ch = KEYS ? head * p.G + hh : head / p.G;
+      const int64_t vec = ((int64_t)b * p.H + ch) * a.NP;
+      for (int u = 0; u < per_head; ++u) {
+        const int c0 = first(u);
+        warp_wait(&c_empty[s], ph, wctx);
+        mbar_expect_tx(el, &c_full[s], 2 * Cfg::C_TILE + (KEYS ? 2 * kTile * 4 : 0));
+        uint8_t* dst = smem + Cfg::OFF_C + s * 2 * Cfg::C_TILE;
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+          tma_load_4d(el, dst + c * Cfg::C_CHUNK, &tmC1, &c_full[s], 64 * c, c0, ch, b);
+          tma_load_4d(el, dst + Cfg::C_TILE + c * Cfg::C_CHUNK, &tmC2, &c_full[s], 64 * c, c0, ch, b);
+        }
+        if constexpr (KEYS) {
+          uint8_t* v = smem + Cfg::OFF_VEC + s * 2 * kTile * 4;
+          bulk_load(el, v, a.nlse + vec + c0, kTile * 4, &c_full[s]);
+          bulk_load(el, v + kTile * 4, a.ndelta + vec + c0, kTile * 4, &c_full[s]);
+        }
+        if (++s == NS) s = 0, ph ^= 1;
+      }
+    }
+  } else if (warp == Cfg::WARP_MMA) {
+    const uint32_t el = elect_one();
+    constexpr uint32_t idesc_s = window_idesc<T>(128, kTile, false), idesc_acc = window_idesc<T>(128, DP, true);
+    constexpr uint32_t hi = smem_desc_hi(1024, swizzle_mode_for_bytes(128));
+    const uint32_t d_r1 = smem_desc_lo(smem_u32(smem + Cfg::OFF_R), 16);
+    const uint32_t d_r2 = smem_desc_lo(smem_u32(smem + Cfg::OFF_R + Cfg::R_TILE), 16);
+    const uint32_t d_c = smem_desc_lo(smem_u32(smem + Cfg::OFF_C), 16);
+    const uint32_t d_cmn = smem_desc_lo(smem_u32(smem + Cfg::OFF_C), Cfg::C_CHUNK);
+    constexpr uint32_t kStage = 2 * Cfg::C_TILE >> 4, kSecond = Cfg::C_TILE >> 4;
+    int s = 0;
+    uint32_t ph = 0;
+    auto issue_sdp = [&](int t) {
+      warp_wait(&c_full[s], ph, wctx);
+      tc_fence_after();
+      const uint32_t d1 = d_c + s * kStage, d2 = d1 + kSecond, to = tmem + 128 * (t & 1);
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d)
+        umma_ss_w<hi, hi, idesc_s>(el, to, d_r1 + ((d / 4 * Cfg::R_CHUNK + d % 4 * 32) >> 4),
+                                   d1 + ((d / 4 * Cfg::C_CHUNK + d % 4 * 32) >> 4), d != 0);
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d)
+        umma_ss_w<hi, hi, idesc_s>(el, to + 64, d_r2 + ((d / 4 * Cfg::R_CHUNK + d % 4 * 32) >> 4),
+                                   d2 + ((d / 4 * Cfg::C_CHUNK + d % 4 * 32) >> 4), d != 0);
+      umma_commit(el, &sdp_full[t & 1]);
+      if (++s == NS) s = 0, ph ^= 1;
+    };
+    if (tiles > 0) {
+      warp_wait(r_full, 0, wctx);
+      issue_sdp(0);
+      if (tiles > 1) issue_sdp(1);
+    }
+    int bs = 0;
+    for (int t = 0; t < tiles; ++t) {
+      const int g = t & 1;
+      warp_wait(&pds_ready[g], (t >> 1) & 1, wctx);
+      tc_fence_after();
+      const uint32_t d1 = d_cmn + bs * kStage, d2 = d1 + kSecond, from = tmem + 128 * g;
+      if constexpr (KEYS) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          umma_ts_w<hi, idesc_acc>(el, tmem + Cfg::TM_ACC1, from + 8 * k, d2 + k * 128, (k | t) != 0);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        umma_ts_w<hi, idesc_acc>(el, tmem + (KEYS ? Cfg::TM_ACC2 : Cfg::TM_ACC1), from + 64 + 8 * k, d1 + k * 128, (k | t) != 0);
+      umma_commit(el, &c_empty[bs]);
+      if (++bs == NS) bs = 0;
+      if (t + 1 == tiles) umma_commit(el, acc_full);
+      // over P and dS, which the products just issued have to read: the UMMAs of a thread go through the tensor pipe in order (as in
+      // the triangle attention's backward pass)
+      if (t + 2 < tiles) issue_sdp(t + 2);
+    }
+  } else {
+    // ------------------------------------------------------------------ compute warps: one thread per row
+    const int g = warp >> 2, lane_base = 32 * (warp & 3), row = lane_base + lane;
+    const uint32_t t_s = tmem_addr(tmem, lane_base, 128 * g), t_dp = t_s + 64;
+    const float c2 = p.scale * kWindowLog2e;
+    const uint64_t c22 = f2_pack(c2, c2);
+    const int mine = r0 + row;
+    float nl = 0.f, nd = 0.f;
+    if (!KEYS && mine < p.N) {
+      const int64_t at = ((int64_t)b * p.H + head) * a.NP + mine;
+      nl = __ldg(a.nlse + at);
+      nd = __ldg(a.ndelta + at);
+    }
+    const uint64_t nl2 = f2_pack(nl, nl), nd2 = f2_pack(nd, nd);
+    const int w0 = r0 + lane_base, w1 = w0 + 31;  // the warp's rows
+    int u = 0;
+    auto advance = [&](int n) {
+      u += n;
+      while (u >= per_head) u -= per_head;
+    };
+    if (tiles > 0) advance(g);
+    for (int t = g; t < tiles; t += 2) {
+      const int c0 = first(u);
+      const int s = t % NS;
+      warp_wait(&sdp_full[g], (t >> 1) & 1, wctx);
+      tc_fence_after();
+      uint64_t seen;
+      bool whole;
+      if constexpr (KEYS) {
+        seen = seeing_queries(p, len, mine, off + c0);
+        whole = w1 < len && off + c0 >= w1 - p.right && off + c0 + kTile - 1 <= w0 + p.left;
+      } else {
+        seen = seen_keys(p, len, off + mine, c0);
+        whole = c0 + kTile <= min(len, off + w0 + p.right + 1) && c0 >= off + w1 - p.left;
+      }
+      const float* vec = reinterpret_cast<const float*>(smem + Cfg::OFF_VEC + s * 2 * kTile * 4);
+      auto tile = [&](auto masked) {
+        constexpr bool MASKED = decltype(masked)::value;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t rs[32], rd[32];
+          tmem_ld32(t_s + 32 * half, rs);
+          tmem_ld32(t_dp + 32 * half, rd);
+          tmem_ld_wait();
+          const uint32_t bits = (uint32_t)(seen >> (32 * half));
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            uint32_t pk[8], dk[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int c = 16 * q + 2 * e;
+              uint64_t l2 = nl2, de2 = nd2;
+              if constexpr (KEYS) {
+                const float2 x = *reinterpret_cast<const float2*>(vec + 32 * half + c);
+                const float2 y = *reinterpret_cast<const float2*>(vec + kTile + 32 * half + c);
+                l2 = f2_pack(x.x, x.y);
+                de2 = f2_pack(y.x, y.y);
+              }
+              float a0, a1;
+              f2_unpack(f2_fma(f2_pack_bits(rs[c], rs[c + 1]), c22, l2), a0, a1);
+              float p0 = ex2_approx(a0), p1 = ex2_approx(a1), d0, d1;
+              f2_unpack(f2_mul(f2_pack(p0, p1), f2_add(f2_pack_bits(rd[c], rd[c + 1]), de2)), d0, d1);
+              if (MASKED) {  // (what is masked may be a NaN)
+                if (!(bits >> c & 1u)) p0 = d0 = 0.f;
+                if (!(bits >> (c + 1) & 1u)) p1 = d1 = 0.f;
+              }
+              // 16 bits, as operands of the products
+              pk[e] = pack2<T>(p0, p1);
+              dk[e] = pack2<T>(d0, d1);
+            }
+            if (KEYS) tmem_st8(t_s + 16 * half + 8 * q, pk);
+            tmem_st8(t_dp + 16 * half + 8 * q, dk);
+          }
+        }
+      };
+      if (whole) tile(std::false_type{});
+      else tile(std::true_type{});
+      if constexpr (!KEYS) {
+        // Keys behind the last one are anything, and a dS of zero times a NaN is one (S has been made from them, and masked).
+        if (c0 + kTile > len) {
+          uint8_t* kt = smem + Cfg::OFF_C + s * 2 * Cfg::C_TILE;
+          for (int e = threadIdx.x & 127; e < CHUNKS * kTile * 8; e += 128) {
+            const int r = e / 8 % kTile;
+            if (c0 + r >= len)
+              *reinterpret_cast<uint4*>(kt + e / (8 * kTile) * Cfg::C_CHUNK + r * 128 + e % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fence_async_smem();
+        }
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&pds_ready[g]);
+      advance(2);
+    }
+    if (tiles > 0) {
+      warp_wait(acc_full, 0, wctx);
+      tc_fence_after();
+    }
+    // KEYS: group 0 stores dV and group 1 dK; else each a half of dQ's columns
+    const int cb = KEYS ? 0 : g * (DP / 2), ce = KEYS ? DP : cb + DP / 2;
+    const uint32_t src = tmem_addr(tmem, lane_base, KEYS && g == 1 ? Cfg::TM_ACC2 : Cfg::TM_ACC1);
+    const float mul = KEYS && g == 0 ? 1.f : p.scale;
+    const int rows = KEYS ? p.M : p.N, heads = KEYS ? p.HK : p.H;
+    void* grad = KEYS && g == 1 ? a.g2 : a.g1;
+    // rows whose sum is finished by the last kernel
+    const bool part = KEYS && a.parts != nullptr && r0 == 0 && row < min(p.sinks, p.M);
+    T* out = static_cast<T*>(grad) + (((int64_t)b * rows + mine) * heads + head) * p.D;
+    float* sums = nullptr;
+    if (part)
+      sums = a.parts + (((((int64_t)b * p.HK + head) * (1 + a.far) + (far ? (int)blockIdx.x - a.key_tiles + 1 : 0)) * 2 + g) * p.sinks +
+                        row) * p.D;
+#pragma unroll 1
+    for (int c = cb; c < ce; c += 16) {
+      uint32_t r[16];
+      if (tiles > 0) {
+        tmem_ld16(src + c, r);
+        tmem_ld_wait();
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) r[e] = 0u;
+      }
+      float v[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(r[e]) * mul;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (c + 8 * k >= p.D) continue;
+        if (part) {
+          *reinterpret_cast<float4*>(sums + c + 8 * k) = make_float4(v[8 * k], v[8 * k + 1], v[8 * k + 2], v[8 * k + 3]);
+          *reinterpret_cast<float4*>(sums + c + 8 * k + 4) = make_float4(v[8 * k + 4], v[8 * k + 5], v[8 * k + 6], v[8 * k + 7]);
+        } else if (!far && mine < rows) {
+          store_vec<T, 8>(out + c + 8 * k, v + 8 * k);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == Cfg::WARP_MMA) {
+    __syncwarp();
+    tmem_dealloc(tmem, Cfg::TMEM_COLS);
+  }
+}
+
+// ---- the sinks' rows ----------------------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(128) window_sinks_kernel(const float* __restrict__ parts, int count, int sinks, int rows, int D, int M,
+                                                           int HK, T* __restrict__ dv, T* __restrict__ dk) {
+  griddep_wait();
+  const int head = blockIdx.x, b = blockIdx.y;
+  const float* from = parts + ((int64_t)b * HK + head) * count * 2 * sinks * D;
+  for (int e = threadIdx.x; e < 2 * rows * D; e += 128) {
+    const int which = e / (rows * D), rest = e - which * rows * D;
+    float s = 0.f;
+    for (int k = 0; k < count; ++k) s += from[((int64_t)k * 2 + which) * sinks * D + rest];
+    const int row = rest / D, d = rest - row * D;
+    (which == 0 ? dv : dk)[(((int64_t)b * M + row) * HK + head) * D + d] = from_f32<T>(s);
+  }
+}
+
+// Query tiles of a CTA of far queries: as many as a key tile's window has.
+void far_plan(const WindowCall& c, int* far, int* far_tiles) {
+  *far = 0;
+  *far_tiles = 1;
+  if (c.sinks == 0 || c.left == kWindowUnlimited) return;
+  if (c.offsets == nullptr && c.offset + c.N - 1 <= c.left) return;  // every query's window reaches key 0
+  const int64_t all = (c.N + kTile - 1) / kTile;
+  int64_t window = ((int64_t)c.left + (c.right == kWindowUnlimited ? 0 : c.right) + 128) / kTile + 1;
+  if (window < 8) window = 8;
+  if (window > all) window = all;
+  *far_tiles = (int)window;
+  *far = (int)((all + window - 1) / window);
+}
+int64_t padded(int64_t n) { return (n + kTile - 1) / kTile * kTile; }
+int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
+
+template <class Cfg>
+int launch(const CUtensorMap& r1, const CUtensorMap& r2, const CUtensorMap& c1, const CUtensorMap& c2, const WindowParams& p,
+           const BwdArgs& a, dim3 grid, cudaStream_t stream) {
+  auto kern = window_bwd_kernel<Cfg>;
+  static PerDeviceOnce once;
+  if (int rc = ensure_dynamic_smem(kern, Cfg::SMEM, once, 1024)) return rc;
+  int* status = nullptr;
+  static PerDeviceAddress cache;
+  if (int rc = device_symbol_address(g_window_bwd_status, cache, reinterpret_cast<void**>(&status))) return rc;
+  launch_kernel(kern, grid, dim3(Cfg::THREADS), Cfg::SMEM, stream, r1, r2, c1, c2, p, a, status);
+  TPF_LAUNCH_OK();
+  return TPF_OK;
+}
+
+template <typename T, int DP>
+int run(const WindowCall& c, const WindowParams& p, uint8_t* ws, cudaStream_t stream) {
+  const int64_t NP = padded(c.N), stat = round256(c.B * c.H * NP * 4);
+  BwdArgs a = {};
+  float* nlse = reinterpret_cast<float*>(ws);
+  float* ndelta = reinterpret_cast<float*>(ws + stat);
+  a.nlse = nlse, a.ndelta = ndelta;
+  a.NP = (int)NP;
+  const int64_t rows = c.B * NP * c.H;
+  launch_kernel(window_stats_kernel<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, stream, static_cast<const T*>(c.out),
+                static_cast<const T*>(c.d_out), c.lse, nlse, ndelta, (int)c.N, (int)NP, (int)c.H, (int)c.D, rows);
+  TPF_LAUNCH_OK();
+  const int64_t os[3] = {c.N * c.H * c.D, c.H * c.D, c.D};
+  int rc;
+  if (c.dk != nullptr) {
+    CUtensorMap tk, tv, tq, tg;
+    if ((rc = make_window_tmap(&tk, c.k, c.type, c.B, c.M, c.HK, c.D, c.ks, 128))) return rc;
+    if ((rc = make_window_tmap(&tv, c.v, c.type, c.B, c.M, c.HK, c.D, c.vs, 128))) return rc;
+    if ((rc = make_window_tmap(&tq, c.q, c.type, c.B, c.N, c.H, c.D, c.qs, kTile))) return rc;
+    if ((rc = make_window_tmap(&tg, c.d_out, c.type, c.B, c.N, c.H, c.D, os, kTile))) return rc;
+    a.g1 = c.dv, a.g2 = c.dk;
+    a.key_tiles = (int)((c.M + 127) / 128);
+    far_plan(c, &a.far, &a.far_tiles);
+    if (a.far > 0) a.parts = reinterpret_cast<float*>(ws + 2 * stat);
+    if ((rc = launch<BwdCfg<T, DP, true>>(tk, tv, tq, tg, p, a, dim3(a.key_tiles + a.far, (unsigned)c.HK, (unsigned)c.B), stream)))
+      return rc;
+    if (a.far > 0) {
+      launch_kernel(window_sinks_kernel<T>, dim3((unsigned)c.HK, (unsigned)c.B), dim3(128), 0, stream,
+                    static_cast<const float*>(a.parts), 1 + a.far, c.sinks, (int)(c.sinks < c.M ? c.sinks : c.M), (int)c.D, (int)c.M,
+                    (int)c.HK, static_cast<T*>(c.dv), static_cast<T*>(c.dk));
+      TPF_LAUNCH_OK();
+    }
+  }
+  if (c.dq != nullptr) {
+    CUtensorMap tk, tv, tq, tg;
+    if ((rc = make_window_tmap(&tq, c.q, c.type, c.B, c.N, c.H, c.D, c.qs, 128))) return rc;
+    if ((rc = make_window_tmap(&tg, c.d_out, c.type, c.B, c.N, c.H, c.D, os, 128))) return rc;
+    if ((rc = make_window_tmap(&tk, c.k, c.type, c.B, c.M, c.HK, c.D, c.ks, kTile))) return rc;
+    if ((rc = make_window_tmap(&tv, c.v, c.type, c.B, c.M, c.HK, c.D, c.vs, kTile))) return rc;
+    a.g1 = c.dq, a.g2 = nullptr;
+    a.parts = nullptr;
+    if ((rc = launch<BwdCfg<T, DP, false>>(tq, tg, tk, tv, p, a, dim3((unsigned)((c.N + 127) / 128), (unsigned)c.H, (unsigned)c.B),
+                                           stream)))
+      return rc;
+  }
+  return TPF_OK;
+}
+
+}  // namespace
+
+int64_t window_bwd_workspace_bytes(const WindowCall& c) {
+  WindowCall any = c;
+  static const int some = 0;
+  any.offsets = &some;  // (the plan for positions that only the device knows is the larger one)
+  int far, far_tiles;
+  far_plan(any, &far, &far_tiles);
+  return 2 * round256(c.B * c.H * padded(c.N) * 4) + (far > 0 ? c.B * c.HK * (1 + far) * 2 * c.sinks * c.D * 4 : 0);
+}
+
+int window_bwd(const WindowCall& c, const WindowParams& p, void* workspace, int64_t workspace_bytes, cudaStream_t stream) {
+  TPF_REQUIRE(workspace != nullptr && workspace_bytes >= window_bwd_workspace_bytes(c), TPF_ERR_WORKSPACE,
+              "window_attn_bwd: the workspace is too small");
+  TPF_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, TPF_ERR_INVALID_ARGUMENT,
+              "window_attn_bwd: the workspace must be 256-byte aligned");
+  TPF_REQUIRE(c.H <= 65535 && c.B * c.H * padded(c.N) < (1ll << 34), TPF_ERR_UNSUPPORTED, "window_attn_bwd: extent too large");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (c.type == kRowBF16) return c.D <= 64 ? run<bf16, 64>(c, p, ws, stream) : run<bf16, 128>(c, p, ws, stream);
+  return c.D <= 64 ? run<__half, 64>(c, p, ws, stream) : run<__half, 128>(c, p, ws, stream);
+}
+
+}  // namespace tpf

@@ -1,8 +1,7 @@
 """The pair-stack part of an OpenFold3 PairBlock on the B200 operators, optionally sharded
 axially over the GPUs of one node.
 
-Mirrors ``PairBlock.forward`` (openfold3/core/model/latent/base_blocks.py:433-534, dropout inactive,
-pair transition excluded) and ``TriangleAttention.forward``
+Mirrors ``PairBlock.forward`` (openfold3/core/model/latent/base_blocks.py:433-534, pair transition excluded) and ``TriangleAttention.forward``
 (openfold3/core/model/layers/triangular_attention.py:245-409).  On one GPU the block is one C++ call
 (csrc/tpf_torch_block.cpp) whose kernels contain the LayerNorms, the bias-free q/k/v/g/o/bias Linears, the
 gates and the residual adds (csrc/tpf_pair_attn.cu, csrc/tpf_trimul.cu).  The sharded block, and shapes that
@@ -25,6 +24,7 @@ import torch.nn.functional as F
 from . import _cabi as C
 from . import dap
 from .attention import count_invocations, turbo_attention
+from .dropout import turbo_dropout
 from .trimul import native_weight_order, turbo_trimul
 
 _attention_order = operator.itemgetter("ln_w", "ln_b", "w_z", "w_q", "w_k", "w_v", "w_g", "w_o")
@@ -91,14 +91,29 @@ def triangle_attention_update(z, mask, p, heads, transpose_bias=False, inf=1e9, 
     return F.linear((o * gate).reshape(o.shape[:-2] + (heads * d,)), p["w_o"].to(z.dtype))
 
 
-def pair_stack_block(z, mask, params, heads, group=None, trimul_backend=None, attention_fn=None):
+def _site_seeds(seed):
+    """Seeds of the block's four dropouts from the caller's one: the offsets 4 n .. 4 n + 3 of its offset n."""
+    if seed is None:
+        return [None] * 4
+    if isinstance(seed, torch.Tensor):
+        return list(torch.stack([seed[:1].expand(4), 4 * seed[1:] + torch.arange(4, device=seed.device)], 1))
+    number, offset = seed if isinstance(seed, (tuple, list)) else (seed, 0)
+    return [(number, 4 * offset + i) for i in range(4)]
+
+
+def pair_stack_block(z, mask, params, heads, group=None, trimul_backend=None, attention_fn=None, dropout=0.0, seed=None,
+                     dropout_fn=None):
     """TriMul outgoing -> TriMul incoming -> attention starting node -> attention ending node, each
-    with its residual add.  ``z`` bf16 ``[B, N, N, C]`` (or the local rows ``[B, N/P, N, C]`` with
+    with its residual add.  With ``dropout`` (a probability; training) every update passes a row-wise dropout on its way to the
+    residual (one mask for all rows of the pair tensor, of the transposed one at the ending node); ``seed`` as in
+    :func:`turbo_dropout`, and the same on all ranks of a ``group``, whose masks are then those of the unsharded block.  ``z`` bf16 ``[B, N, N, C]`` (or the local rows ``[B, N/P, N, C]`` with
     ``group``); ``mask`` ``[B, N, N]`` (local rows likewise).  ``params`` as produced by
     ``synthetic.block_params`` (fp32 masters).  ``trimul_backend`` / ``attention_fn`` replace the
     CUDA stage back end of :func:`dap.axial_trimul` and :func:`turbo_attention` in the sharded
-    path (used to test the collectives on CPU ranks); the defaults are the B200 operators."""
-    if group is None and not torch.compiler.is_compiling():
+    path (used to test the collectives on CPU ranks), ``dropout_fn`` :func:`turbo_dropout`; the defaults are the B200 operators."""
+    if dropout and group is not None and seed is None:
+        raise ValueError("pair_stack_block: a sharded block with dropout needs a seed that all ranks share")
+    if group is None and not dropout and not torch.compiler.is_compiling():
         # one C++ call with fused kernels (residual adds, gates and projections inside); None: a shape, type or
         # context it does not cover (head dims other than 16 and 32, tensor subclasses, ...), composed below
         out = C.native().pair_block(z, mask, native_weight_order(params["tri_mul_out"]),
@@ -108,19 +123,26 @@ def pair_stack_block(z, mask, params, heads, group=None, trimul_backend=None, at
         if out is not None:
             count_invocations(2)
             return out
+    seeds = _site_seeds(seed) if dropout else None
+
+    def add(z, site, update):
+        if not dropout:
+            return z + update
+        return (dropout_fn or turbo_dropout)(update, dropout, seeds[site], shared_dim=-3, residual=z)
+
     if group is None:
-        z = z + turbo_trimul(z, "outgoing", mask, **params["tri_mul_out"])
-        z = z + turbo_trimul(z, "incoming", mask, **params["tri_mul_in"])
-        z = z + triangle_attention_update(z, mask, params["tri_att_start"], heads)
+        z = add(z, 0, turbo_trimul(z, "outgoing", mask, **params["tri_mul_out"]))
+        z = add(z, 1, turbo_trimul(z, "incoming", mask, **params["tri_mul_in"]))
+        z = add(z, 2, triangle_attention_update(z, mask, params["tri_att_start"], heads))
         zt = z.transpose(-2, -3)
-        zt = zt + triangle_attention_update(zt, mask.transpose(-1, -2), params["tri_att_end"], heads,
-                                            transpose_bias=True)
+        zt = add(zt, 3, triangle_attention_update(zt, mask.transpose(-1, -2), params["tri_att_end"], heads,
+                                                  transpose_bias=True))
         return zt.transpose(-2, -3)
-    z = z + dap.axial_trimul(z, "outgoing", mask, group=group, backend=trimul_backend, **params["tri_mul_out"])
-    z = z + dap.axial_trimul(z, "incoming", mask, group=group, backend=trimul_backend, **params["tri_mul_in"])
-    z = z + triangle_attention_update(z, mask, params["tri_att_start"], heads, group=group, attention_fn=attention_fn)
+    z = add(z, 0, dap.axial_trimul(z, "outgoing", mask, group=group, backend=trimul_backend, **params["tri_mul_out"]))
+    z = add(z, 1, dap.axial_trimul(z, "incoming", mask, group=group, backend=trimul_backend, **params["tri_mul_in"]))
+    z = add(z, 2, triangle_attention_update(z, mask, params["tri_att_start"], heads, group=group, attention_fn=attention_fn))
     zt = _ShardedTranspose.apply(z, group)
     mt = _sharded_transpose(mask.unsqueeze(-1).float().contiguous(), group).squeeze(-1)
-    zt = zt + triangle_attention_update(zt, mt, params["tri_att_end"], heads, transpose_bias=True, group=group,
-                                        attention_fn=attention_fn)
+    zt = add(zt, 3, triangle_attention_update(zt, mt, params["tri_att_end"], heads, transpose_bias=True, group=group,
+                                              attention_fn=attention_fn))
     return _ShardedTranspose.apply(zt.contiguous(), group)

@@ -1,0 +1,243 @@
+"""turbo_dropout on a B200 against the 64-bit oracle (bounds derived in oracle/sequence_oracle.py), and the block that calls it."""
+import math
+
+import pytest
+import torch
+
+import openfold3_triangle_kernel_b200 as tk
+from oracle import sequence_oracle as so
+
+pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA device")]
+
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def _rn(*s, seed=0, dtype=torch.float32):
+    return torch.randn(*s, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def _check(x, p=0.25, seed=7, offset=0, shared=None, residual=None, x_cuda=None, r_cuda=None, as_tensor=False):
+    kept = so.dropout_mask(x.shape, p, seed, offset, shared)
+    xc = (x.cuda() if x_cuda is None else x_cuda).detach().requires_grad_(True)
+    rc = None if residual is None else (residual.cuda() if r_cuda is None else r_cuda).detach().requires_grad_(True)
+    s = torch.tensor([seed, offset], device="cuda") if as_tensor else (seed, offset)
+    out = tk.turbo_dropout(xc, p, s, shared_dim=shared, residual=rc)
+    assert out.dtype == x.dtype and out.shape == x.shape and out.is_contiguous()
+    ref, off = so.dropout(x, kept, p, residual)
+    so.check(out.cpu(), ref, off, "out")
+    d = _rn(*x.shape, seed=99, dtype=x.dtype)
+    leaves = [xc] if rc is None else [xc, rc]
+    grads = torch.autograd.grad(out, leaves, d.cuda())
+    ref, off = so.dropout(d, kept, p)
+    so.check(grads[0].cpu(), ref, off, "d_x")
+    assert not (grads[0].cpu()[~kept] != 0).any()
+    if rc is not None:
+        assert torch.equal(grads[1].cpu(), d)
+    with torch.no_grad():
+        assert torch.equal(tk.turbo_dropout(xc, p, s, shared_dim=shared, residual=rc), out)
+    return out
+
+
+@pytest.mark.parametrize("n", [1, 2, 7, 8, 9, 255, 256, 257, 2048, 100003])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("residual", [False, True])
+def test_lengths(n, dtype, residual):
+    _check(_rn(n, seed=n, dtype=DT[dtype]), residual=_rn(n, seed=n + 1, dtype=DT[dtype]) if residual else None)
+
+
+@pytest.mark.parametrize("shape", [(1, 5, 7, 8), (2, 3, 9, 24), (1, 20, 20, 64), (2, 17, 17, 9), (1, 9, 13, 1), (3, 8, 1, 16), (1, 1, 6, 33),
+                                   (2, 11, 5, 257), (1, 40, 33, 31)])
+@pytest.mark.parametrize("shared", [None, -2, -3, 0])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_shared_masks(shape, shared, dtype):
+    x = _rn(*shape, seed=3, dtype=DT[dtype])
+    _check(x, shared=shared, residual=_rn(*shape, seed=4, dtype=DT[dtype]))
+    _check(x, shared=shared, p=0.5)
+
+
+@pytest.mark.parametrize("shared", [None, -2, -3])
+@pytest.mark.parametrize("cols", [16, 15])
+def test_strides(shared, cols):
+    """Transposed pair tensors, slices, expanded and misaligned ones: what counts is the logical index."""
+    x, r = _rn(2, 10, 12, cols, seed=1).bfloat16(), _rn(2, 10, 12, cols, seed=2).bfloat16()
+    big = torch.zeros(2, 12, 10, 2 * cols + 3, dtype=torch.bfloat16, device="cuda")
+    big[..., 1:cols + 1] = x.transpose(1, 2).cuda()
+    views = [x.cuda().transpose(1, 2).contiguous().transpose(1, 2), big[..., 1:cols + 1].transpose(1, 2),
+             x.cuda().permute(3, 0, 1, 2).contiguous().permute(1, 2, 3, 0),
+             x.cuda().permute(1, 2, 0, 3).contiguous().permute(2, 0, 1, 3)]
+    plain = _check(x, shared=shared, residual=r)
+    for v in views:
+        assert torch.equal(_check(x, shared=shared, residual=r, x_cuda=v), plain)
+        rv = r.cuda().transpose(1, 2).contiguous().transpose(1, 2)
+        assert torch.equal(_check(x, shared=shared, residual=r, x_cuda=v, r_cuda=rv), plain)
+    one = x[:, :1].expand(2, 10, 12, cols)
+    _check(one.contiguous(), shared=shared, x_cuda=x[:, :1].cuda().expand(2, 10, 12, cols))
+
+
+@pytest.mark.parametrize("p", [0.0, 1e-6, 0.1, 1 / 3, 0.9999, 1.0])
+def test_probabilities(p):
+    _check(_rn(3, 1000, seed=5).bfloat16(), p=p, residual=_rn(3, 1000, seed=6).bfloat16())
+
+
+def test_share_of_dropped_elements():
+    """1e6 elements at p: a standard deviation of sqrt(p (1 - p) / 1e6) = 4.3e-4 at 0.25; six of them."""
+    out = tk.turbo_dropout(torch.ones(1000, 1000, device="cuda"), 0.25, 12345)
+    assert abs((out == 0).float().mean().item() - 0.25) < 6 * math.sqrt(0.25 * 0.75 / 1e6)
+    assert set(out.unique().tolist()) == {0.0, torch.tensor(4 / 3).item()}
+
+
+@pytest.mark.parametrize("seed, offset", [(0, 0), (-1, 5), (2 ** 63 - 1, 2 ** 40), (2 ** 64 - 1, 0), (1, -1), (3, 2 ** 64 - 2)])
+@pytest.mark.parametrize("as_tensor", [False, True])
+def test_seeds(seed, offset, as_tensor):
+    wrap = lambda n: n - 2 ** 64 if n >= 2 ** 63 else n  # noqa: E731
+    _check(_rn(777, seed=8), seed=wrap(seed) if as_tensor else seed, offset=wrap(offset) if as_tensor else offset, as_tensor=as_tensor)
+
+
+def test_seeds_differ_and_an_int_is_offset_zero():
+    x = torch.ones(4096, device="cuda")
+    a = tk.turbo_dropout(x, 0.5, 1)
+    assert torch.equal(a, tk.turbo_dropout(x, 0.5, (1, 0)))
+    for other in (2, (1, 1), (2 ** 32 + 1, 0), (1, 2 ** 32)):
+        assert 1500 < (a != tk.turbo_dropout(x, 0.5, other)).sum() < 2600
+
+
+def test_drawn_seeds_follow_torchs_generator():
+    x = torch.ones(4096, device="cuda", requires_grad=True)
+    torch.manual_seed(3)
+    a, b = tk.turbo_dropout(x, 0.5), tk.turbo_dropout(x, 0.5)
+    torch.manual_seed(3)
+    assert torch.equal(a, tk.turbo_dropout(x, 0.5)) and not torch.equal(a, b)
+    a.sum().backward()
+    assert torch.equal(x.grad, a.detach())
+
+
+def test_infinities_and_nan():
+    """A dropped one is a zero, forward and backward; a kept one stays."""
+    kept = so.dropout_mask((4, 1001), 0.5, 11)
+    for value in (math.inf, -math.inf, math.nan):
+        x = torch.full((4, 1001), value)
+        out = tk.turbo_dropout(x.cuda(), 0.5, 11, residual=torch.ones(4, 1001, device="cuda")).cpu()
+        assert (out[~kept] == 1).all() and not torch.isfinite(out[kept]).any()
+        leaf = torch.zeros(4, 1001, device="cuda", requires_grad=True)
+        tk.turbo_dropout(leaf, 0.5, 11).backward(x.cuda())
+        assert (leaf.grad.cpu()[~kept] == 0).all() and not torch.isfinite(leaf.grad.cpu()[kept]).any()
+
+
+def test_nothing_in_nothing_out():
+    for shape in ((0,), (3, 0), (0, 5)):
+        x = torch.zeros(shape, device="cuda", requires_grad=True)
+        out = tk.turbo_dropout(x, 0.5, 1)
+        assert out.shape == shape
+        out.sum().backward()
+        assert x.grad.shape == shape
+    assert tk.turbo_dropout(torch.zeros((), device="cuda").view(1), 0.5, 1).shape == (1,)
+
+
+def test_evaluation_changes_nothing():
+    x, r = torch.randn(5, 6, device="cuda"), torch.randn(5, 6, device="cuda")
+    assert tk.turbo_dropout(x, 0.5, training=False) is x
+    assert torch.equal(tk.turbo_dropout(x, 0.5, residual=r, training=False), r + x)
+
+
+def test_mask_beyond_32_bits_of_elements():
+    """The last elements of a tensor whose index needs more than 32 bits."""
+    n = 2 ** 32 + 4096 + 3
+    x = torch.ones(n, device="cuda", dtype=torch.bfloat16)
+    out = tk.turbo_dropout(x, 0.5, 21)
+    first = n // 8 * 8 - 4096
+    bits = [h >= 32768 for g in range(first // 8, -(-n // 8)) for w in so.philox(21, 0, g) for h in (w & 0xFFFF, w >> 16)]
+    assert torch.equal(out[first:].cpu() != 0, torch.tensor(bits[:n - first]))
+
+
+def test_captured_replays_read_the_seed():
+    x, r = torch.randn(1, 9, 9, 64, device="cuda").bfloat16().requires_grad_(True), torch.randn(1, 9, 9, 64, device="cuda").bfloat16()
+    seed = torch.tensor([5, 0], device="cuda")
+    d = torch.randn(1, 9, 9, 64, device="cuda").bfloat16()
+
+    def step():
+        out = tk.turbo_dropout(x, 0.25, seed, shared_dim=-3, residual=r)
+        return out.detach(), torch.autograd.grad(out, x, d)[0]
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, grad = step()
+    for s in (5, 6, 2 ** 40):
+        seed.copy_(torch.tensor([s, s + 1]))
+        graph.replay()
+        expected = step()
+        assert torch.equal(out, expected[0]) and torch.equal(grad, expected[1])
+        assert not torch.equal(out, r)
+
+
+def test_a_changed_seed_is_noticed():
+    x, seed = torch.ones(64, device="cuda", requires_grad=True), torch.tensor([5, 0], device="cuda")
+    out = tk.turbo_dropout(x, 0.5, seed)
+    seed.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
+def test_other_streams():
+    x = torch.randn(300, 512, device="cuda")
+    expected = tk.turbo_dropout(x, 0.3, 4)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        out = tk.turbo_dropout(x, 0.3, 4)
+    s.synchronize()
+    assert torch.equal(out, expected)
+
+
+@pytest.mark.parametrize("shared", [None, -3])
+def test_traced_calls(shared):
+    x, r = torch.randn(2, 6, 7, 16, device="cuda").bfloat16().requires_grad_(True), torch.randn(2, 6, 7, 16, device="cuda").bfloat16()
+    seed = torch.tensor([5, 9], device="cuda")
+    f = lambda x, r, s: tk.turbo_dropout(x, 0.25, s, shared_dim=shared, residual=r)  # noqa: E731
+    torch.compiler.reset()
+    g = torch.compile(f, fullgraph=True, backend="aot_eager")
+    d = torch.randn(2, 6, 7, 16, device="cuda").bfloat16()
+    a, b = f(x, r, seed), g(x, r, seed)
+    assert torch.equal(a, b)
+    assert torch.equal(torch.autograd.grad(a, x, d)[0], torch.autograd.grad(b, x, d)[0])
+    torch.library.opcheck(torch.ops.tpf_b200.dropout, (x.detach().requires_grad_(True), r, seed, 0, 0, 16384,
+                                                       -1 if shared is None else 1))
+
+
+def test_gradients_are_first_order():
+    x = torch.randn(64, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad(tk.turbo_dropout(x, 0.5, 1).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        g.sum().backward()
+
+
+@pytest.mark.parametrize("seed", [17, (17, 2), "tensor"])
+def test_pair_block_trains_with_dropout(seed):
+    """The block with dropout is its four updates, each dropped with the mask of its site and added."""
+    from openfold3_triangle_kernel_b200 import pair_block as pb
+    from openfold3_triangle_kernel_b200.synthetic import block_params
+    B, N, C, H = 1, 24, 32, 2
+    params = block_params(C, H, 16, seed=0)
+    params = {k: {n: t.cuda() for n, t in v.items()} for k, v in params.items()}
+    z = _rn(B, N, N, C, seed=1).bfloat16().cuda().requires_grad_(True)
+    mask = torch.ones(B, N, N, device="cuda")
+    number, offset = (17, 0) if seed == 17 else (17, 2)
+    given = torch.tensor([17, 2], device="cuda") if seed == "tensor" else seed
+    out = pb.pair_stack_block(z, mask, params, H, dropout=0.25, seed=given)
+
+    def drop(update, z, site):
+        kept = so.dropout_mask(update.shape, 0.25, number, 4 * offset + site, -3).cuda()
+        return (z.float() + torch.where(kept, update.float() * (65536 / (65536 - 16384)), 0.0)).bfloat16()
+
+    x = z
+    x = drop(tk.turbo_trimul(x, "outgoing", mask, **params["tri_mul_out"]), x, 0)
+    x = drop(tk.turbo_trimul(x, "incoming", mask, **params["tri_mul_in"]), x, 1)
+    x = drop(pb.triangle_attention_update(x, mask, params["tri_att_start"], H), x, 2)
+    xt = x.transpose(-2, -3)
+    xt = drop(pb.triangle_attention_update(xt, mask.transpose(-1, -2), params["tri_att_end"], H, transpose_bias=True), xt, 3)
+    expected = xt.transpose(-2, -3)
+    assert torch.equal(out, expected)
+    d = _rn(B, N, N, C, seed=2).bfloat16().cuda()
+    got, want = torch.autograd.grad(out, z, d)[0].float(), torch.autograd.grad(expected, z, d)[0].float()
+    # the same kernels, and sums of bf16 gradients: a handful of roundings of each
+    assert (got - want).norm() <= 2.0 ** -7 * want.norm()
