@@ -11,7 +11,7 @@
 //
 // What bounds it: memory.  Ten rounds are twenty 32 x 32 -> 64 bit products, about 90 instructions for eight elements; a
 // shared mask is made once by a thread that then walks along the shared dimension.
-// Measured (B200, bf16, mask shared along dimension -3 of 1 x 384 x 384 x 128, forward with a residual and backward): see kRun.
+// Measured (B200, bf16, 1 x 384 x 384 x 128, with a residual and without): FIGURES
 #include "tpf_dropout.h"
 
 #include "tpf_rows.cuh"
@@ -27,12 +27,13 @@ struct DropoutParams {
   int64_t inner;
   uint32_t P, Q, S;
   int s_in_mask;                // 0: the mask is shared along S
-  uint32_t threshold;
+  uint32_t border;              // the threshold times 2^16
+  int none;                     // the threshold is 2^16: nothing is kept
   float scale;
   const int64_t* seed_ptr;      // (seed, offset) on the device, or nullptr
   uint64_t seed, offset;
-  uint32_t cells;               // vectors (or chunks of 32 groups) of a row
-  FastDiv div_cells, div_q;
+  uint32_t cells;               // vectors of a row
+  FastDiv div_cells, div_q, div_inner;
 };
 
 struct Philox {
@@ -46,8 +47,7 @@ struct Philox {
     k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
     o0 = (uint32_t)offset, o1 = (uint32_t)(offset >> 32);
   }
-  // Bit h: element h of a group of eight is kept.
-  __device__ __forceinline__ uint32_t kept(uint64_t group, uint32_t threshold) const {
+  __device__ __forceinline__ void words(uint64_t group, uint32_t (&w)[4]) const {
     uint32_t c0 = (uint32_t)group, c1 = (uint32_t)(group >> 32), c2 = o0, c3 = o1, a = k0, b = k1;
 #pragma unroll
     for (int i = 0; i < 10; ++i) {
@@ -59,35 +59,37 @@ struct Philox {
       a += 0x9E3779B9u;
       b += 0xBB67AE85u;
     }
-    const uint32_t w[4] = {c0, c1, c2, c3};
-    uint32_t bits = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      bits |= ((w[i] & 0xffffu) >= threshold ? 1u : 0u) << (2 * i);
-      bits |= ((w[i] >> 16) >= threshold ? 1u : 0u) << (2 * i + 1);
-    }
-    return bits;
+    w[0] = c0, w[1] = c1, w[2] = c2, w[3] = c3;
   }
 };
+// Is element h of a group kept?  `border`: the threshold in the upper half word; 2^16 does not fit there, and `none` says it.
+__device__ __forceinline__ bool is_kept(const uint32_t (&w)[4], int h, uint32_t border, bool none) {
+  return (h & 1 ? w[h >> 1] : w[h >> 1] << 16) >= border && !none;
+}
+__device__ __forceinline__ uint32_t kept_bits(const uint32_t (&w)[4], uint32_t border, bool none) {
+  uint32_t bits = 0;
+#pragma unroll
+  for (int h = 0; h < 8; ++h) bits |= is_kept(w, h, border, none) ? 1u << h : 0u;
+  return bits;
+}
 
 constexpr int kThreads = 256;
-// Elements of the shared dimension that a thread walks with one mask.
-constexpr int kRun = 8;
-
 template <typename T, bool RES>
-__device__ __forceinline__ void drop_vec(const Piece<T, 8>& x, const Piece<T, 8>& r, uint32_t bits, float scale, T* out) {
+__device__ __forceinline__ void drop_vec(const Piece<T, 8>& x, const Piece<T, 8>& r, const bool (&kept)[8], float scale, T* out) {
   float v[8], w[8];
   x.get(v);
   if (RES) r.get(w);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float y = bits >> i & 1u ? v[i] * scale : 0.f;  // (a dropped infinity is a zero)
+    const float y = kept[i] ? v[i] * scale : 0.f;  // (a dropped infinity is a zero)
     v[i] = RES ? y + w[i] : y;
   }
   store_vec<T, 8>(out, v);
 }
 
 // Rows that start on vector boundaries and on groups of the mask: a thread per vector of the mask and run of the shared dimension.
+// (Without a shared dimension the products and the selections bound it, 21 us for 11.5 at the copy rate; four vectors a thread, with
+// their keys made once, took as long, and with a residual 28 for 23.)
 template <typename T, bool RES, int RUN>
 __global__ void __launch_bounds__(kThreads) dropout_vec_kernel(const DropoutParams p) {
   griddep_wait();
@@ -100,10 +102,12 @@ __global__ void __launch_bounds__(kThreads) dropout_vec_kernel(const DropoutPara
   const T* x = static_cast<const T*>(p.x) + pi * p.xp + qi * p.xq + s0 * p.xs + e;
   const T* r = RES ? static_cast<const T*>(p.r) + pi * p.rp + qi * p.rq + s0 * p.rs + e : nullptr;
   T* out = static_cast<T*>(p.out) + pi * p.op + qi * p.oq + s0 * p.os + e;
-  const Philox gen(p);
   const uint64_t m = ((uint64_t)row * (p.s_in_mask ? p.S : 1u) + (p.s_in_mask ? s0 : 0u)) * (uint64_t)p.inner + (uint64_t)e;
+  const Philox gen(p);
+  uint32_t words[4];
   if (p.inner - e < 8) {  // the tail of a single row
-    const uint32_t bits = gen.kept(m >> 3, p.threshold);
+    gen.words(m >> 3, words);
+    const uint32_t bits = kept_bits(words, p.border, p.none);
     for (int i = 0; i < (int)(p.inner - e); ++i) {
       const float y = bits >> i & 1u ? to_f32(x[i]) * p.scale : 0.f;
       out[i] = from_f32<T>(RES ? y + to_f32(r[i]) : y);
@@ -118,58 +122,94 @@ __global__ void __launch_bounds__(kThreads) dropout_vec_kernel(const DropoutPara
     px[i].load(x + k * p.xs);
     if (RES) pr[i].load(r + k * p.rs);
   }
-  const uint32_t bits = gen.kept(m >> 3, p.threshold);  // while the loads are on their way
+  gen.words(m >> 3, words);  // while the loads are on their way
+  bool kept[8];
+#pragma unroll
+  for (int h = 0; h < 8; ++h) kept[h] = is_kept(words, h, p.border, p.none);
 #pragma unroll
   for (int i = 0; i < RUN; ++i)
-    if (i < n) drop_vec<T, RES>(px[i], pr[i], bits, p.scale, out + i * p.os);
+    if (i < n) drop_vec<T, RES>(px[i], pr[i], kept, p.scale, out + i * p.os);
 }
 
-// Rows at any address: a warp takes 32 groups of the mask, each lane makes the bits of one, and the elements, which lie side by side
-// over the lanes, take theirs by a shuffle.
+// Rows at any address: a warp takes 32 groups of the mask, whatever rows they belong to; each lane makes the bits of one, and the
+// elements, which lie side by side over the lanes, take theirs by a shuffle.
 template <typename T, bool RES, int RUN>
 __global__ void __launch_bounds__(kThreads) dropout_any_kernel(const DropoutParams p) {
   griddep_wait();
   const int lane = threadIdx.x & 31;
-  const uint32_t cell = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-  const uint32_t row = p.div_cells.div(cell), chunk = cell - row * p.cells;
-  const uint32_t pi = p.div_q.div(row), qi = row - pi * p.Q;
-  if (pi >= p.P) return;
-  const uint32_t s0 = blockIdx.y * RUN;
-  const T* x = static_cast<const T*>(p.x) + pi * p.xp + qi * p.xq + s0 * p.xs;
-  const T* r = RES ? static_cast<const T*>(p.r) + pi * p.rp + qi * p.rq + s0 * p.rs : nullptr;
-  T* out = static_cast<T*>(p.out) + pi * p.op + qi * p.oq + s0 * p.os;
-  const Philox gen(p);
-  const uint64_t m = ((uint64_t)row * (p.s_in_mask ? p.S : 1u) + (p.s_in_mask ? s0 : 0u)) * (uint64_t)p.inner;
-  const uint64_t first = (m >> 3) + 32ull * chunk;  // group of lane 0
-  const int64_t at = (int64_t)(first * 8 - m);      // element of that group's first bit; negative at the start of a row
-  const uint32_t bits = gen.kept(first + lane, p.threshold);
+  const uint64_t m0 = ((uint64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * 256;
+  const uint64_t row0 = m0 / (uint64_t)p.inner, e0 = m0 - row0 * p.inner;
+  const uint32_t s0 = blockIdx.y * RUN;  // (of a shared dimension; else 0)
   const int n = RUN == 1 ? 1 : min(RUN, (int)(p.S - s0));
-  for (int k = 0; k < n; ++k, x += p.xs, r += RES ? p.rs : 0, out += p.os) {
+  T v[RUN][8], w[RUN][8];
+  T* out[8];
+  uint64_t row_i = row0;
+  int64_t e = (int64_t)e0 + lane;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int64_t e = at + 32 * i + lane;
-      const bool on = e >= 0 && e < p.inner;
-      const float v = on ? to_f32(x[e]) : 0.f, w = RES && on ? to_f32(r[e]) : 0.f;
-      const uint32_t b = __shfl_sync(0xffffffffu, bits, 4 * i + (lane >> 3)) >> (lane & 7);
-      const float y = b & 1u ? v * p.scale : 0.f;
-      if (on) out[e] = from_f32<T>(RES ? y + w : y);
+  for (int i = 0; i < 8; ++i, e += 32) {
+    if (e >= p.inner) {  // (rows of 32 elements and more end once at most)
+      const uint32_t rows = p.inner >= 32 ? 1u : p.div_inner.div((uint32_t)e);
+      row_i += rows;
+      e -= rows * p.inner;
+    }
+    uint64_t row = row_i;
+    int64_t xs = s0 * p.xs, rs = s0 * p.rs, os = s0 * p.os;
+    if (p.s_in_mask && p.S > 1) {
+      const uint32_t pq = (uint32_t)(row / p.S), s = (uint32_t)(row - (uint64_t)pq * p.S);
+      xs = s * p.xs, rs = s * p.rs, os = s * p.os;
+      row = pq;
+    }
+    const bool on = row < (uint64_t)p.P * p.Q;
+    const uint32_t pi = on ? p.div_q.div((uint32_t)row) : 0u, qi = on ? (uint32_t)row - pi * p.Q : 0u;
+    const T* x = static_cast<const T*>(p.x) + pi * p.xp + qi * p.xq + xs + e;
+    const T* r = RES ? static_cast<const T*>(p.r) + pi * p.rp + qi * p.rq + rs + e : nullptr;
+    out[i] = on ? static_cast<T*>(p.out) + pi * p.op + qi * p.oq + os + e : nullptr;
+#pragma unroll
+    for (int k = 0; k < RUN; ++k) {
+      v[k][i] = on && k < n ? x[k * p.xs] : T(0.f);
+      if (RES) w[k][i] = on && k < n ? r[k * p.rs] : T(0.f);
+    }
+  }
+  const Philox gen(p);
+  uint32_t words[4];
+  gen.words((m0 >> 3) + lane, words);
+  const uint32_t bits = kept_bits(words, p.border, p.none);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const bool kept = __shfl_sync(0xffffffffu, bits, 4 * i + (lane >> 3)) >> (lane & 7) & 1u;
+#pragma unroll
+    for (int k = 0; k < RUN; ++k) {
+      const float y = kept ? to_f32(v[k][i]) * p.scale : 0.f;
+      if (out[i] != nullptr && k < n) out[i][k * p.os] = from_f32<T>(RES ? y + to_f32(w[k][i]) : y);
     }
   }
 }
 
+// `cells`: vectors or, where there are none, groups of 256 elements of the mask.
 template <typename T, bool RES, int RUN>
-int launch(const DropoutParams& p, bool vec, uint32_t blocks, cudaStream_t stream) {
-  const dim3 grid(blocks, (p.S + RUN - 1) / RUN);
+int launch(const DropoutParams& p, bool vec, int64_t cells, cudaStream_t stream) {
+  const int64_t per_block = vec ? kThreads : kThreads / 32;
+  const dim3 grid((unsigned)((cells + per_block - 1) / per_block), p.s_in_mask && !vec ? 1 : (p.S + RUN - 1) / RUN);
   TPF_REQUIRE(grid.y <= 65535, TPF_ERR_UNSUPPORTED, "dropout: the shared dimension is too long");
   if (vec) launch_kernel(dropout_vec_kernel<T, RES, RUN>, grid, dim3(kThreads), 0, stream, p);
-  else launch_kernel(dropout_any_kernel<T, RES, RUN>, grid, dim3(kThreads), 0, stream, p);
+  else if constexpr (RUN <= 4) launch_kernel(dropout_any_kernel<T, RES, RUN>, grid, dim3(kThreads), 0, stream, p);
   TPF_LAUNCH_OK();
   return TPF_OK;
 }
+template <typename T, bool RES>
+int launch(const DropoutParams& p, bool vec, int64_t cells, cudaStream_t stream) {
+  // Long runs make few masks, and few threads: a run is shortened while there would be fewer blocks than eight an SM (two, where
+  // a thread has eight elements of every row).
+  const int64_t enough = (vec ? 8ll : 2ll) * sm_count(), blocks = cells / (vec ? kThreads : kThreads / 32);
+  const int64_t s = p.s_in_mask ? 1 : p.S;
+  if (s >= 8 && vec && blocks * (s / 8) >= enough) return launch<T, RES, 8>(p, vec, cells, stream);
+  if (s >= 4 && blocks * (s / 4) >= enough) return launch<T, RES, 4>(p, vec, cells, stream);
+  if (s >= 2) return launch<T, RES, 2>(p, vec, cells, stream);
+  return launch<T, RES, 1>(p, vec, cells, stream);
+}
 template <typename T>
-int launch(const DropoutParams& p, bool vec, uint32_t blocks, bool run, cudaStream_t stream) {
-  if (p.r != nullptr) return run ? launch<T, true, kRun>(p, vec, blocks, stream) : launch<T, true, 1>(p, vec, blocks, stream);
-  return run ? launch<T, false, kRun>(p, vec, blocks, stream) : launch<T, false, 1>(p, vec, blocks, stream);
+int launch(const DropoutParams& p, bool vec, int64_t cells, cudaStream_t stream) {
+  return p.r != nullptr ? launch<T, true>(p, vec, cells, stream) : launch<T, false>(p, vec, cells, stream);
 }
 
 }  // namespace
@@ -193,7 +233,8 @@ int dropout(const DropoutCall& c, cudaStream_t stream) {
   p.inner = I;
   p.P = (uint32_t)P, p.Q = (uint32_t)Q, p.S = (uint32_t)S;
   p.s_in_mask = c.shared ? 0 : 1;
-  p.threshold = (uint32_t)c.threshold;
+  p.none = c.threshold == 65536;
+  p.border = p.none ? 0xffffffffu : (uint32_t)c.threshold << 16;
   p.scale = c.threshold < 65536 ? (float)(65536.0 / (65536 - c.threshold)) : 0.f;
   p.seed_ptr = c.seed_ptr;
   p.seed = (uint64_t)c.seed, p.offset = (uint64_t)c.offset;
@@ -203,17 +244,22 @@ int dropout(const DropoutCall& c, cudaStream_t stream) {
   for (int d = 0; d < 3; ++d)
     vec = vec && whole(c.sizes[d], c.x_strides[d]) && whole(c.sizes[d], c.out_strides[d]) &&
           (c.residual == nullptr || whole(c.sizes[d], c.residual_strides[d]));
-  const int64_t cells = vec ? (I + 7) / 8 : (I / 8 + 2 + 31) / 32;  // (a row touches at most I / 8 + 2 groups)
-  const int64_t total = P * Q * cells, per_block = vec ? kThreads : kThreads / 32;
-  TPF_REQUIRE(cells < kMost && total < kMost - kThreads, TPF_ERR_UNSUPPORTED, "dropout: too many elements");
-  p.cells = (uint32_t)cells;
-  p.div_cells = FastDiv::make((uint32_t)cells);
+  int64_t cells;
+  if (vec) {
+    const int64_t per_row = (I + 7) / 8;
+    cells = P * Q * per_row;
+    TPF_REQUIRE(cells < kMost - kThreads, TPF_ERR_UNSUPPORTED, "dropout: too many elements");
+    p.cells = (uint32_t)per_row;
+    p.div_cells = FastDiv::make((uint32_t)per_row);
+  } else {
+    cells = (P * Q * (p.s_in_mask ? S : 1) * I + 255) / 256;
+    TPF_REQUIRE(cells < 8 * (kMost - 1), TPF_ERR_UNSUPPORTED, "dropout: too many elements");
+    p.div_inner = FastDiv::make((uint32_t)(I < 32 ? I : 32));
+  }
   p.div_q = FastDiv::make((uint32_t)Q);
-  const uint32_t blocks = (uint32_t)((total + per_block - 1) / per_block);
-  const bool run = c.shared && S > 1;
-  if (c.type == kRowF32) return launch<float>(p, vec, blocks, run, stream);
-  if (c.type == kRowBF16) return launch<bf16>(p, vec, blocks, run, stream);
-  return launch<__half>(p, vec, blocks, run, stream);
+  if (c.type == kRowF32) return launch<float>(p, vec, cells, stream);
+  if (c.type == kRowBF16) return launch<bf16>(p, vec, cells, stream);
+  return launch<__half>(p, vec, cells, stream);
 }
 
 }  // namespace tpf

@@ -8,11 +8,14 @@
 // turn, exactly, and its upper 32 bits go to sincospi.  So a position of a million is as exact as position one, without a
 // table in memory and without arithmetic in 64-bit floats.
 //
-// Mapping: a team of TL lanes takes a token and a run of its heads.  A lane holds two pieces of eight elements: in the half
-// order the two that are rotated into one another, so nothing is exchanged, and its sines and cosines stay in registers for
-// all heads of the run (sincospi costs as much as a head).  What bounds it: memory (the smallest calls: the launch).
-// Head sizes that are no multiple of eight, and halves that no piece fits, take a warp per head with single elements and pass
-// partners through shared memory.
+// Mapping: a block has a stretch of tokens, as long as any other block's.  It makes their sines and cosines, in shared memory, and goes
+// through the heads of q and then through those of k: a team of TL lanes has a few of them in succession, loaded two ahead.  With the
+// sines as registers of each team they were made several times over, and took the place of loads in flight (8192 tokens, 32 + 8
+// heads of 128, bf16, forward and backward: 44 and 75 us).  A lane holds two pieces of eight elements, in the half order the two that are
+// rotated into one another, so nothing is exchanged.
+// What bounds it: memory (the smallest calls: the launch).
+// Halves that no piece of eight fits pass partners through shared memory; head sizes that are no multiple of eight and misaligned
+// tensors take a warp per head, with single elements, which do as well.
 #include "tpf_rotary.h"
 
 #include "tpf_rows.cuh"
@@ -30,32 +33,37 @@ struct RotaryParams {
     const void *x, *dy;
     void* out;
     int64_t sb, sn, sh;
-    int heads, runs, run;       // runs of `run` heads
-    int64_t first_item;         // items: (token, run)
+    int heads;
     ParamVec w;
-    bool want_dw;
   } t[2];
-  int64_t items, rows;          // rows = batch * tokens
-  int tokens, dim, rot;
+  uint32_t all;                 // tokens of all batches
+  uint32_t per_block, step;     // tokens of a block, and of a step of it
+  int tokens, dim, rot, pairs;  // pairs = rot / 2
   const int64_t* turns;
   const int64_t* positions;
   int64_t first;
   float magnitude, eps, inv_dim;
   float* terms;                 // [grid][2][dim]
+  FastDiv div_pairs;
 };
 
+// How a head is rotated, and by whom:
+//   kInterleaved, kHalf  a lane has both elements of its pairs (kHalf: rot / 16 lanes with a piece of either half)
+//   kHalfAny             halves that no piece of eight fits: pieces in order, partners through shared memory
+enum Mode : int { kInterleaved = 0, kHalf = 1, kHalfAny = 2 };
+
 // A lane's elements: VEC = 8: pieces at at[0] and at[1], eight each; VEC = 1: element lane + 32 i.
-template <int VEC, int TL, bool HALF>
+template <int VEC, int TL, int MODE>
 struct Place {
   static constexpr int E = VEC == 8 ? 16 : 8, PIECES = VEC == 8 ? 2 : 8;
   int at[PIECES];
   bool on[PIECES];
   __device__ __forceinline__ Place(int lane, const RotaryParams& p) {
     if constexpr (VEC == 8) {
-      // half order: lanes up to R / 16 hold partners, the rest of the head follows two pieces a lane
+      // kHalf: lanes up to R / 16 hold partners, the rest of the head follows two pieces a lane
       const int pairs = p.rot / 16, pieces = p.dim / 8;
-      const int a = !HALF || lane < pairs ? lane : 2 * lane;
-      const int b = !HALF ? lane + TL : lane < pairs ? lane + pairs : a + 1;
+      const int a = MODE != kHalf || lane < pairs ? lane : 2 * lane;
+      const int b = MODE != kHalf ? lane + TL : lane < pairs ? lane + pairs : a + 1;
       on[0] = a < pieces;
       on[1] = b < pieces;
       at[0] = on[0] ? 8 * a : 0;
@@ -70,72 +78,95 @@ struct Place {
   }
 };
 
-__device__ __forceinline__ void cos_sin(uint64_t turns, int64_t position, float magnitude, float& c, float& s) {
+__device__ __forceinline__ float2 cos_sin(uint64_t turns, int64_t position, float magnitude) {
   const uint64_t phase = turns * (uint64_t)position;
+  float c, s;
   sincospif((float)(int32_t)(phase >> 32) * 0x1p-31f, &s, &c);  // half turns, -1 .. 1
-  c *= magnitude;
-  s *= magnitude;
+  return make_float2(c * magnitude, s * magnitude);
 }
 
-// Cosines and sines of a lane's elements: VEC = 8: of the eight pairs it holds (HALF: element j of both pieces; else pairs 0-3 in the
-// first piece, 4-7 in the second); VEC = 1: of each element.
-template <int VEC, int TL, bool HALF>
-struct Angles {
-  float c[8], s[8];
-  uint32_t turned;  // bit j: pair (element) j is rotated
-  __device__ __forceinline__ void make(const Place<VEC, TL, HALF>& pl, const RotaryParams& p, int64_t position) {
-    turned = 0;
+// Sines and cosines of a token in shared memory: all cosines, then all sines, `pitch` numbers each.  In the half order a lane takes
+// eight pairs at once: those of even fours lie before those of odd ones, so that the 16-byte reads of neighbours meet no bank twice.
+__host__ __device__ constexpr int angle_pitch(int pairs) { return (pairs + 7) / 8 * 8; }
+template <int VEC, int MODE>
+__device__ __forceinline__ int angle_slot(int pair, int pitch) {
+  return VEC == 8 && MODE == kHalf ? (pair >> 2 & 1) * (pitch / 2) + (pair >> 3) * 4 + (pair & 3) : pair;
+}
+
+// Rotates a lane's elements; SIGN = -1: back.  `angles`: of the token; `row`: 256 floats of the team, where partners are exchanged.
+template <int VEC, int TL, int MODE, int SIGN>
+__device__ __forceinline__ void turn(float (&y)[Place<VEC, TL, MODE>::E], const Place<VEC, TL, MODE>& pl, const RotaryParams& p,
+                                     const float* angles, float* row) {
+  const int pitch = angle_pitch(p.pairs);
+  if constexpr (VEC == 8 && MODE == kHalf) {
+    if (pl.on[0] && pl.at[0] < p.pairs) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      int pair;
-      if constexpr (VEC == 8) pair = HALF ? pl.at[0] + j : (pl.at[j >> 2] >> 1) + (j & 3);
-      else pair = HALF ? (pl.at[j] < p.rot / 2 ? pl.at[j] : pl.at[j] - p.rot / 2) : pl.at[j] >> 1;
-      const bool is = VEC == 8 ? pl.on[HALF ? 0 : j >> 2] && pair < p.rot / 2 : pl.on[j] && pl.at[j] < p.rot;
-      c[j] = 1.f;
-      s[j] = 0.f;
-      if (is) {
-        turned |= 1u << j;
-        cos_sin((uint64_t)__ldg(p.turns + pair), position, p.magnitude, c[j], s[j]);
+      for (int f = 0; f < 2; ++f) {  // four pairs, two at a time
+        const int slot = angle_slot<VEC, MODE>(pl.at[0] + 4 * f, pitch);
+        const float4 c = *reinterpret_cast<const float4*>(angles + slot);
+        const float4 s = *reinterpret_cast<const float4*>(angles + pitch + slot);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float* a = y + 4 * f + 2 * j;
+          float* b = a + 8;
+          const uint64_t a2 = f2_pack(a[0], a[1]), b2 = f2_pack(b[0], b[1]);
+          const uint64_t c2 = j == 0 ? f2_pack(c.x, c.y) : f2_pack(c.z, c.w);
+          const uint64_t s2 = SIGN > 0 ? (j == 0 ? f2_pack(s.x, s.y) : f2_pack(s.z, s.w))
+                                       : (j == 0 ? f2_pack(-s.x, -s.y) : f2_pack(-s.z, -s.w));
+          const uint64_t n2 = SIGN > 0 ? (j == 0 ? f2_pack(-s.x, -s.y) : f2_pack(-s.z, -s.w))
+                                       : (j == 0 ? f2_pack(s.x, s.y) : f2_pack(s.z, s.w));
+          f2_unpack(f2_fma(b2, n2, f2_mul(a2, c2)), a[0], a[1]);
+          f2_unpack(f2_fma(a2, s2, f2_mul(b2, c2)), b[0], b[1]);
+        }
       }
     }
-  }
-};
-
-// Rotates a lane's elements; SIGN = -1: back.  `row`: 256 floats of the warp (VEC = 1 only).
-template <int VEC, int TL, bool HALF, int SIGN>
-__device__ __forceinline__ void turn(float (&y)[Place<VEC, TL, HALF>::E], const Place<VEC, TL, HALF>& pl,
-                                     const Angles<VEC, TL, HALF>& an, const RotaryParams& p, float* row) {
-  if constexpr (VEC == 8) {
+  } else if constexpr (VEC == 8 && MODE == kInterleaved) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int ia = HALF ? j : 2 * j, ib = HALF ? j + 8 : 2 * j + 1;
-      const float a = y[ia], b = y[ib], s = SIGN * an.s[j];
-      const float na = a * an.c[j] - b * s, nb = fmaf(a, s, b * an.c[j]);
-      if (an.turned >> j & 1u) {  // (an infinity next to elements that stay must not reach them)
-        y[ia] = na;
-        y[ib] = nb;
+    for (int f = 0; f < 2; ++f) {
+      const int pair = pl.at[f] >> 1;
+      if (!pl.on[f] || pair >= p.pairs) continue;
+      const float4 c4 = *reinterpret_cast<const float4*>(angles + pair);
+      const float4 s4 = *reinterpret_cast<const float4*>(angles + pitch + pair);
+      const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float &a = y[8 * f + 2 * j], &b = y[8 * f + 2 * j + 1];
+        const float na = fmaf(a, c[j], -SIGN * (b * s[j])), nb = fmaf(a, SIGN * s[j], b * c[j]);
+        if (pair + j < p.pairs) {  // (an infinity next to elements that stay must not reach them)
+          a = na;
+          b = nb;
+        }
       }
     }
   } else {
-    const int lane = threadIdx.x & 31;
+    __syncwarp();
+    if constexpr (VEC == 8) {
+#pragma unroll
+      for (int f = 0; f < 4; ++f)
+        if (pl.on[f / 2])
+          *reinterpret_cast<float4*>(row + pl.at[f / 2] + f % 2 * 4) = make_float4(y[4 * f], y[4 * f + 1], y[4 * f + 2], y[4 * f + 3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (pl.on[i]) row[pl.at[i]] = y[i];
+    }
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) row[lane + 32 * i] = y[i];
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (!(an.turned >> i & 1u)) continue;
-      const bool is_a = HALF ? pl.at[i] < p.rot / 2 : (pl.at[i] & 1) == 0;
-      const int partner = HALF ? (is_a ? pl.at[i] + p.rot / 2 : pl.at[i] - p.rot / 2) : pl.at[i] ^ 1;
-      const float o = row[partner], s = SIGN * an.s[i];
-      y[i] = is_a ? y[i] * an.c[i] - o * s : fmaf(o, s, y[i] * an.c[i]);
+    for (int i = 0; i < Place<VEC, TL, MODE>::E; ++i) {
+      const int at = pl.at[i / VEC] + i % VEC;
+      if (!pl.on[i / VEC] || at >= p.rot) continue;
+      const bool is_a = MODE == kInterleaved ? (at & 1) == 0 : at < p.pairs;
+      const int pair = MODE == kInterleaved ? at >> 1 : is_a ? at : at - p.pairs;
+      const float c = angles[pair], s = SIGN * angles[pitch + pair];
+      const float o = row[MODE == kInterleaved ? at ^ 1 : is_a ? at + p.pairs : pair];
+      y[i] = is_a ? fmaf(y[i], c, -(o * s)) : fmaf(o, s, y[i] * c);
     }
   }
 }
 
-template <typename T, int VEC, int TL, bool HALF>
+template <typename T, int VEC, int TL, int MODE>
 struct Head {  // a lane's part of a head as it lies in memory
-  using Pl = Place<VEC, TL, HALF>;
+  using Pl = Place<VEC, TL, MODE>;
   Piece<T, VEC> p[Pl::PIECES];
   __device__ __forceinline__ void load(const T* x, const Pl& pl) {
 #pragma unroll
@@ -157,146 +188,202 @@ __device__ __forceinline__ void put(T* out, const float* v, const Pl& pl) {
   for (int i = 0; i < Pl::PIECES; ++i)
     if (pl.on[i]) store_vec<T, VEC>(out + pl.at[i], v + i * VEC);
 }
+// The weights in shared memory, even fours before odd ones (as the angles of the half order).
+template <int VEC>
+__device__ __forceinline__ int weight_slot(int c) {
+  return VEC == 8 ? (c >> 2 & 1) * (kMaxDim / 2) + (c >> 3) * 4 + (c & 3) : c;
+}
 template <int VEC, class Pl>
-__device__ __forceinline__ void weights(const ParamVec& w, float (&v)[Pl::E], const Pl& pl, int dim) {
+__device__ __forceinline__ void weights(const float* mem, float (&w)[Pl::E], const Pl& pl) {
+  if constexpr (VEC == 8) {
 #pragma unroll
-  for (int i = 0; i < Pl::PIECES; ++i) {
-    param_load<VEC, 1>(w, pl.at[i], dim, 1.f, v + i * VEC);
-    if (!pl.on[i])
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) v[i * VEC + j] = 0.f;
-  }
-}
-
-struct Item {
-  int64_t row;
-  int head, heads;
-};
-__device__ __forceinline__ Item item_of(const RotaryParams::Tensor& t, int64_t i) {
-  const uint32_t row = (uint32_t)i / (uint32_t)t.runs, run = (uint32_t)i - row * t.runs;
-  const int h = (int)run * t.run;
-  return {(int64_t)row, h, min(t.run, t.heads - h)};
-}
-__device__ __forceinline__ int64_t position_of(const RotaryParams& p, int64_t row) {
-  return p.positions != nullptr ? __ldg(p.positions + row) : p.first + (int64_t)((uint32_t)row % (uint32_t)p.tokens);
-}
-
-template <typename T, int VEC, int TL, bool HALF, bool NORM>
-__global__ void __launch_bounds__(kThreads) rotary_fwd_kernel(const RotaryParams p) {
-  griddep_wait();
-  using Pl = Place<VEC, TL, HALF>;
-  __shared__ float exchange[VEC == 1 ? kThreads / 32 : 1][VEC == 1 ? 256 : 1];
-  float* row_mem = exchange[VEC == 1 ? threadIdx.x >> 5 : 0];
-  const int lane = threadIdx.x % TL;
-  const Pl pl(lane, p);
-  constexpr int TEAMS = kThreads / TL;
-  // (the teams of a warp go through the shuffles together: those without an item repeat the last one)
-  const int64_t mine = (int64_t)blockIdx.x * TEAMS + threadIdx.x / TL;
-  const bool real = mine < p.items;
-  const int64_t i = real ? mine : p.items - 1;
-  const bool second = i >= p.t[1].first_item;
-  const RotaryParams::Tensor& t = p.t[second ? 1 : 0];
-  const Item it = item_of(t, i - t.first_item);
-  const int64_t b = (int64_t)((uint32_t)it.row / (uint32_t)p.tokens), n = it.row - b * p.tokens;
-  const T* x = static_cast<const T*>(t.x) + b * t.sb + n * t.sn + it.head * t.sh;
-  T* out = static_cast<T*>(t.out) + (it.row * t.heads + it.head) * p.dim;
-  Head<T, VEC, TL, HALF> cur, next;
-  cur.load(x, pl);
-  Angles<VEC, TL, HALF> an;
-  an.make(pl, p, position_of(p, it.row));
-  float w[Pl::E];
-  if (NORM) weights<VEC, Pl>(t.w, w, pl, p.dim);
-  const int heads = __reduce_max_sync(0xffffffffu, it.heads);
-  for (int h = 0; h < heads; ++h) {
-    const bool live = h < it.heads;
-    if (h + 1 < it.heads) next.load(x + t.sh, pl);
-    float y[Pl::E];
-    cur.get(y, pl);
-    if (NORM) {
-      float ss[1] = {0.f};
-#pragma unroll
-      for (int e = 0; e < Pl::E; ++e) ss[0] = fmaf(y[e], y[e], ss[0]);
-      warp_sum(ss, TL);
-      const float r = rsqrtf(fmaf(ss[0], p.inv_dim, p.eps));
-#pragma unroll
-      for (int e = 0; e < Pl::E; ++e) y[e] = y[e] * r * w[e];
+    for (int f = 0; f < 4; ++f) {
+      const float4 x = *reinterpret_cast<const float4*>(mem + weight_slot<VEC>(pl.at[f / 2] + f % 2 * 4));
+      w[4 * f] = x.x, w[4 * f + 1] = x.y, w[4 * f + 2] = x.z, w[4 * f + 3] = x.w;
     }
-    turn<VEC, TL, HALF, 1>(y, pl, an, p, row_mem);
-    if (real && live) put<T, VEC>(out, y, pl);
-    cur = next;
-    x += t.sh;
-    out += p.dim;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = mem[pl.at[i]];
   }
 }
 
-// A block walks over the items of one tensor after the other, so that a thread's sums of dw belong to one weight at a time; the teams'
-// sums are added in shared memory in the order of the teams and leave as one term a block, which norm_fold adds up.
-template <typename T, int VEC, int TL, bool HALF, bool NORM>
-__global__ void __launch_bounds__(kThreads, NORM ? 2 : 3) rotary_bwd_kernel(const RotaryParams p) {
+__device__ __forceinline__ int64_t position_of(const RotaryParams& p, uint32_t token) {
+  return p.positions != nullptr ? __ldg(p.positions + token) : p.first + (int64_t)(token % (uint32_t)p.tokens);
+}
+
+// Where a team's rows lie in a strided tensor, one after the other.
+template <typename T>
+struct Walk {
+  const T* x;
+  int64_t row0;    // offset of the token
+  int n, head;
+  const RotaryParams::Tensor& t;
+  const int tokens;
+  __device__ __forceinline__ Walk(const RotaryParams::Tensor& t_, int tokens_, uint32_t token, int head_)
+      : head(head_), t(t_), tokens(tokens_) {
+    const uint32_t b = token / (uint32_t)tokens;
+    n = (int)(token - b * tokens);
+    row0 = (int64_t)b * t.sb + (int64_t)n * t.sn;
+    x = static_cast<const T*>(t.x) + row0 + head * t.sh;
+  }
+  __device__ __forceinline__ void next() {
+    x += t.sh;
+    if (++head < t.heads) return;
+    head = 0;
+    row0 += t.sn;
+    if (++n == tokens) {
+      n = 0;
+      row0 += t.sb - (int64_t)tokens * t.sn;
+    }
+    x = static_cast<const T*>(t.x) + row0;
+  }
+};
+
+template <typename T>
+constexpr int blocks_per_sm(bool norm) {
+  return sizeof(T) == 4 || norm ? 2 : 3;
+}
+
+// BACK, with a norm: a block's sums of dw leave as one term for each tensor (the teams' sums are added in their order), which
+// norm_fold adds up.
+template <typename T, int VEC, int TL, int MODE, bool NORM, bool BACK>
+__global__ void __launch_bounds__(kThreads, blocks_per_sm<T>(NORM)) rotary_kernel(const RotaryParams p) {
   griddep_wait();
-  using Pl = Place<VEC, TL, HALF>;
-  __shared__ float exchange[VEC == 1 ? kThreads / 32 : 1][VEC == 1 ? 256 : 1];
-  __shared__ float sums[NORM ? kThreads / 32 : 1][NORM ? kMaxDim : 1];
-  float* row_mem = exchange[VEC == 1 ? threadIdx.x >> 5 : 0];
-  const int lane = threadIdx.x % TL;
-  const Pl pl(lane, p);
+  using Pl = Place<VEC, TL, MODE>;
+  using Hd = Head<T, VEC, TL, MODE>;
   constexpr int TEAMS = kThreads / TL;
+  constexpr bool READ_X = NORM || !BACK;
+  constexpr int AHEAD = sizeof(T) == 4 || (NORM && BACK) ? 1 : 2;  // rows on their way, as many as find registers
+  extern __shared__ __align__(16) float angles[];
+  constexpr bool EXCHANGE = VEC == 1 || MODE == kHalfAny;
+  __shared__ __align__(16) float exchange[EXCHANGE ? TEAMS : 1][EXCHANGE ? (VEC == 1 ? 256 : 16 * TL) : 4];
+  __shared__ float sums[NORM && BACK ? kThreads / 32 : 1][NORM && BACK ? kMaxDim : 1];
+  __shared__ __align__(16) float wsm[NORM ? kMaxDim : 4];
+  float* row_mem = exchange[EXCHANGE ? threadIdx.x / TL : 0];
+  const int lane = threadIdx.x % TL, team = threadIdx.x / TL;
+  const Pl pl(lane, p);
+  const int pitch = angle_pitch(p.pairs);
+  const uint32_t begin = min(p.all, blockIdx.x * p.per_block), end = min(p.all, begin + p.per_block);
+#pragma unroll 1
   for (int k = 0; k < 2; ++k) {
     const RotaryParams::Tensor& t = p.t[k];
-    const int64_t items = k == 0 ? p.t[1].first_item : p.items - p.t[1].first_item;
-    float w[Pl::E], dw[Pl::E];
+    if (t.heads == 0) continue;
+    float dw[Pl::E];
 #pragma unroll
     for (int e = 0; e < Pl::E; ++e) dw[e] = 0.f;
-    if (NORM) weights<VEC, Pl>(t.w, w, pl, p.dim);
-    for (int64_t base = (int64_t)blockIdx.x * TEAMS; base < items; base += (int64_t)gridDim.x * TEAMS) {
-      const int64_t mine = base + threadIdx.x / TL;
-      const bool real = mine < items;
-      const Item it = item_of(t, real ? mine : items - 1);
-      const int64_t b = (int64_t)((uint32_t)it.row / (uint32_t)p.tokens), n = it.row - b * p.tokens;
-      const T* x = NORM ? static_cast<const T*>(t.x) + b * t.sb + n * t.sn + it.head * t.sh : nullptr;
-      const int64_t at = (it.row * t.heads + it.head) * p.dim;
-      const T* dy = static_cast<const T*>(t.dy) + at;
-      T* out = static_cast<T*>(t.out) + at;
-      Head<T, VEC, TL, HALF> cx, cg, nx, ng;
-      if (NORM) cx.load(x, pl);
-      cg.load(dy, pl);
-      Angles<VEC, TL, HALF> an;
-      an.make(pl, p, position_of(p, it.row));
-      const int heads = __reduce_max_sync(0xffffffffu, it.heads);
-      for (int h = 0; h < heads; ++h) {
-        const bool live = real && h < it.heads;
-        if (h + 1 < it.heads) {
-          if (NORM) nx.load(x + t.sh, pl);
-          ng.load(dy + p.dim, pl);
-        }
-        float g[Pl::E];
-        cg.get(g, pl);
-        turn<VEC, TL, HALF, -1>(g, pl, an, p, row_mem);
-        if (NORM) {
-          float v[Pl::E], s[2] = {0.f, 0.f};
-          cx.get(v, pl);
-#pragma unroll
-          for (int e = 0; e < Pl::E; ++e) {
-            s[0] = fmaf(v[e], v[e], s[0]);
-            s[1] = fmaf(g[e] * w[e], v[e], s[1]);
-          }
-          warp_sum(s, TL);
-          const float r = rsqrtf(fmaf(s[0], p.inv_dim, p.eps)), m = s[1] * p.inv_dim * r * r;
-#pragma unroll
-          for (int e = 0; e < Pl::E; ++e) {
-            if (live) dw[e] = fmaf(g[e], v[e] * r, dw[e]);
-            g[e] = r * fmaf(-v[e], m, g[e] * w[e]);
-          }
-        }
-        if (live) put<T, VEC>(out, g, pl);
-        if (NORM) cx = nx;
-        cg = ng;
-        if (NORM) x += t.sh;
-        dy += p.dim;
-        out += p.dim;
+    if (NORM) {
+      __syncthreads();
+      for (int c = threadIdx.x; c < p.dim; c += kThreads) {
+        float x[1];
+        param_load<1, 1>(t.w, c, p.dim, 1.f, x);
+        wsm[weight_slot<VEC>(c)] = x[0];
       }
     }
-    if constexpr (NORM) {
+#pragma unroll 1
+    for (uint32_t token0 = begin; token0 < end; token0 += p.step) {
+      const uint32_t tokens = min(end - token0, p.step), rows = tokens * t.heads;
+      const uint32_t run = (rows + TEAMS - 1) / TEAMS;  // rows of a team
+      const uint32_t mine = min(team * run, rows - 1);   // a team without rows stands at the last one
+      const int count = team * run < rows ? (int)min(run, rows - mine) : 0;
+      const uint32_t token = mine / (uint32_t)t.heads;
+      int head = (int)(mine - token * t.heads);
+      // the first rows are on their way while the angles are made
+      Walk<T> walk(t, p.tokens, token0 + token, head);
+      const int64_t at = ((int64_t)token0 * t.heads + mine) * p.dim;
+      const T* dy = BACK ? static_cast<const T*>(t.dy) + at : nullptr;
+      Hd xs[AHEAD + 1], gs[AHEAD + 1];
+      auto load = [&](Hd& x, Hd& g, int i) {
+        if (i >= count) return;
+        if (READ_X) {
+          x.load(walk.x, pl);
+          walk.next();
+        }
+        if (BACK) {
+          g.load(dy, pl);
+          dy += p.dim;
+        }
+      };
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) load(xs[i], gs[i], i);
+      if (k == 0 || p.t[0].heads == 0 || p.step < p.per_block) {  // (the angles of a block's only step serve q and k)
+        __syncthreads();                                          // those of the step before have been used
+        for (uint32_t i = threadIdx.x; i < tokens * p.pairs; i += kThreads) {
+          const uint32_t n = p.div_pairs.div(i), pair = i - n * p.pairs;
+          const float2 cs = cos_sin((uint64_t)__ldg(p.turns + pair), position_of(p, token0 + n), p.magnitude);
+          float* to = angles + n * 2 * pitch + angle_slot<VEC, MODE>(pair, pitch);
+          to[0] = cs.x;
+          to[pitch] = cs.y;
+        }
+      }
+      __syncthreads();
+      const float* an = angles + token * 2 * pitch;
+      T* out = static_cast<T*>(t.out) + at;
+      const int most = __reduce_max_sync(0xffffffffu, count);
+      auto row = [&](const Hd& x, const Hd& g, int i) {
+        float y[Pl::E];
+        if constexpr (!BACK) {
+          x.get(y, pl);
+          if (NORM) {
+            uint64_t sq = 0;
+#pragma unroll
+            for (int e = 0; e < Pl::E; e += 2) {
+              const uint64_t v = f2_pack(y[e], y[e + 1]);
+              sq = f2_fma(v, v, sq);
+            }
+            float ss[1] = {f2_sum(sq)};
+            warp_sum(ss, TL);
+            const float r = rsqrtf(fmaf(ss[0], p.inv_dim, p.eps));
+            const uint64_t r2 = f2_dup(r);
+            float w[Pl::E];
+            weights<VEC, Pl>(wsm, w, pl);
+#pragma unroll
+            for (int e = 0; e < Pl::E; e += 2)
+              f2_unpack(f2_mul(f2_mul(f2_pack(y[e], y[e + 1]), r2), f2_pack(w[e], w[e + 1])), y[e], y[e + 1]);
+          }
+          turn<VEC, TL, MODE, 1>(y, pl, p, an, row_mem);
+        } else {
+          g.get(y, pl);
+          turn<VEC, TL, MODE, -1>(y, pl, p, an, row_mem);
+          if (NORM) {
+            float v[Pl::E], w[Pl::E];
+            x.get(v, pl);
+            weights<VEC, Pl>(wsm, w, pl);
+            uint64_t sq = 0, tx = 0;
+#pragma unroll
+            for (int e = 0; e < Pl::E; e += 2) {
+              const uint64_t x2 = f2_pack(v[e], v[e + 1]);
+              sq = f2_fma(x2, x2, sq);
+              tx = f2_fma(f2_mul(f2_pack(y[e], y[e + 1]), f2_pack(w[e], w[e + 1])), x2, tx);
+            }
+            float s[2] = {f2_sum(sq), f2_sum(tx)};
+            warp_sum(s, TL);
+            const float r = rsqrtf(fmaf(s[0], p.inv_dim, p.eps)), m = s[1] * p.inv_dim * r * r;
+            const uint64_t r2 = f2_dup(r), m2 = f2_dup(-m);
+#pragma unroll
+            for (int e = 0; e < Pl::E; e += 2) {
+              const uint64_t x2 = f2_pack(v[e], v[e + 1]), g2 = f2_pack(y[e], y[e + 1]);
+              if (i < count) f2_unpack(f2_fma(g2, f2_mul(x2, r2), f2_pack(dw[e], dw[e + 1])), dw[e], dw[e + 1]);
+              f2_unpack(f2_mul(r2, f2_fma(x2, m2, f2_mul(g2, f2_pack(w[e], w[e + 1])))), y[e], y[e + 1]);
+            }
+          }
+        }
+        if (i < count) put<T, VEC>(out, y, pl);
+        out += p.dim;
+        if (++head == t.heads) {
+          head = 0;
+          if (i + 1 < count) an += 2 * pitch;
+        }
+      };
+#pragma unroll 1
+      for (int i = 0; i < most; i += AHEAD + 1) {
+#pragma unroll
+        for (int d = 0; d <= AHEAD; ++d) {
+          load(xs[(d + AHEAD) % (AHEAD + 1)], gs[(d + AHEAD) % (AHEAD + 1)], i + d + AHEAD);
+          if (d == 0 || i + d < most) row(xs[d], gs[d], i + d);
+        }
+      }
+    }
+    if constexpr (NORM && BACK) {
       if (p.terms != nullptr) {
         // teams of a warp by shuffles, then the warps
 #pragma unroll
@@ -323,48 +410,52 @@ __global__ void __launch_bounds__(kThreads, NORM ? 2 : 3) rotary_bwd_kernel(cons
   }
 }
 
-constexpr int kTermBlocks = 2 * 148;  // blocks of a backward pass with a norm
+constexpr int kTermBlocks = 2 * 148;    // blocks of a backward pass with a norm
+constexpr int kAngleBytes = 60 * 1024;  // of a step
 
-template <typename T, int VEC, int TL, bool HALF>
+template <typename T, int VEC, int TL, int MODE, bool NORM, bool BACK>
+struct Kernel {
+  static constexpr auto kernel() { return rotary_kernel<T, VEC, TL, MODE, NORM, BACK>; }
+};
+
+template <typename T, int VEC, int TL, int MODE>
 int launch(const RotaryCall& c, RotaryParams& p, bool back, cudaStream_t stream) {
   constexpr int TEAMS = kThreads / TL;
-  // Runs of heads: as long as there are about a thousand threads an SM left, so that sines and cosines are used often.
-  const int64_t want = (int64_t)sm_count() * 1024 / TL;
-  int64_t items = 0;
-  for (int k = 0; k < 2; ++k) {
-    RotaryParams::Tensor& t = p.t[k];
-    const int64_t total = c.t[0].heads + c.t[1].heads;
-    int64_t runs_all = (want + p.rows - 1) / p.rows;  // a token is cut into this many
-    if (runs_all > total) runs_all = total;
-    t.run = (int)((total + runs_all - 1) / runs_all);
-    if (t.heads > 0 && t.run > t.heads) t.run = t.heads;
-    t.runs = t.heads > 0 ? (t.heads + t.run - 1) / t.run : 1;
-    t.first_item = items;
-    items += t.heads > 0 ? p.rows * t.runs : 0;
-  }
-  p.items = items;
-  TPF_REQUIRE(items < (1ll << 31) - kThreads, TPF_ERR_UNSUPPORTED, "rotary: too many heads");
-  const int64_t blocks = (items + TEAMS - 1) / TEAMS;
+  // One wave of blocks (as many as find room on the SMs together), or fewer with a row a team.  A block takes its tokens at
+  // once, or in steps whose angles find room.
+  int most = blocks_per_sm<T>(c.norm) * sm_count();
+  if (back && c.norm && most > kTermBlocks) most = kTermBlocks;
+  const int64_t heads = c.t[0].heads + c.t[1].heads;
+  int64_t grid = ((int64_t)p.all * heads + TEAMS - 1) / TEAMS;
+  if (grid > most) grid = most;
+  if (grid > p.all) grid = p.all;
+  p.per_block = (uint32_t)((p.all + grid - 1) / grid);
+  grid = (p.all + p.per_block - 1) / p.per_block;
+  const uint32_t fit = kAngleBytes / (2 * angle_pitch(p.pairs) * 4);
+  p.step = p.per_block < fit ? p.per_block : fit;
+  const size_t smem = (size_t)p.step * 2 * angle_pitch(p.pairs) * 4;
+  auto go = [&](auto tag) {
+    auto kern = decltype(tag)::kernel();
+    static PerDeviceOnce once;  // per kernel
+    if (int rc = ensure_dynamic_smem(kern, kAngleBytes, once)) return rc;
+    launch_kernel(kern, dim3((unsigned)grid), dim3(kThreads), smem, stream, p);
+    TPF_LAUNCH_OK();
+    return TPF_OK;
+  };
   if (!back) {
-    if (c.norm) launch_kernel(rotary_fwd_kernel<T, VEC, TL, HALF, true>, dim3((unsigned)blocks), dim3(kThreads), 0, stream, p);
-    else launch_kernel(rotary_fwd_kernel<T, VEC, TL, HALF, false>, dim3((unsigned)blocks), dim3(kThreads), 0, stream, p);
-    TPF_LAUNCH_OK();
-    return TPF_OK;
+    if (c.norm) return go(Kernel<T, VEC, TL, MODE, true, false>{});
+    return go(Kernel<T, VEC, TL, MODE, false, false>{});
   }
-  if (!c.norm) {
-    launch_kernel(rotary_bwd_kernel<T, VEC, TL, HALF, false>, dim3((unsigned)blocks), dim3(kThreads), 0, stream, p);
-    TPF_LAUNCH_OK();
-    return TPF_OK;
-  }
-  const int grid = blocks < kTermBlocks ? (int)blocks : kTermBlocks;
-  launch_kernel(rotary_bwd_kernel<T, VEC, TL, HALF, true>, dim3(grid), dim3(kThreads), 0, stream, p);
-  TPF_LAUNCH_OK();
+  if (!c.norm) return go(Kernel<T, VEC, TL, MODE, false, true>{});
+  if (int rc = go(Kernel<T, VEC, TL, MODE, true, true>{})) return rc;
   if (p.terms == nullptr) return TPF_OK;
-  return norm_fold(p.terms, grid, p.dim, c.t[0].dweight, c.t[0].weight_type, c.t[1].dweight, c.t[1].weight_type, stream);
+  return norm_fold(p.terms, (int)grid, p.dim, c.t[0].dweight, c.t[0].weight_type, c.t[1].dweight, c.t[1].weight_type, stream);
 }
 template <typename T, int VEC, int TL>
 int launch(const RotaryCall& c, RotaryParams& p, bool back, cudaStream_t stream) {
-  return c.half ? launch<T, VEC, TL, true>(c, p, back, stream) : launch<T, VEC, TL, false>(c, p, back, stream);
+  if (!c.half) return launch<T, VEC, TL, kInterleaved>(c, p, back, stream);
+  if (VEC == 8 && c.rot % 16 != 0) return launch<T, VEC, TL, kHalfAny>(c, p, back, stream);
+  return launch<T, VEC, TL, kHalf>(c, p, back, stream);
 }
 template <typename T>
 int launch(const RotaryCall& c, RotaryParams& p, bool vec, bool back, cudaStream_t stream) {
@@ -404,16 +495,18 @@ int run(const RotaryCall& c, void* workspace, int64_t workspace_bytes, bool back
               TPF_ERR_UNSUPPORTED, "%s: too many tokens", who);
   TPF_REQUIRE(c.turns != nullptr, TPF_ERR_INVALID_ARGUMENT, "%s: null pointer", who);
   RotaryParams p = {};
-  p.rows = c.batch * c.tokens;
-  p.tokens = (int)c.tokens, p.dim = (int)c.dim, p.rot = (int)c.rot;
+  p.all = (uint32_t)(c.batch * c.tokens);
+  p.tokens = (int)c.tokens, p.dim = (int)c.dim, p.rot = (int)c.rot, p.pairs = (int)(c.rot / 2);
+  p.div_pairs = FastDiv::make((uint32_t)p.pairs);
   p.turns = c.turns, p.positions = c.positions, p.first = c.first;
   p.magnitude = c.magnitude, p.eps = c.eps, p.inv_dim = 1.f / (float)c.dim;
-  bool vec = c.dim % 8 == 0 && (!c.half || c.rot % 16 == 0);
+  bool vec = c.dim % 8 == 0;
   for (int k = 0; k < 2; ++k) {
     const RotaryTensor& s = c.t[k];
     RotaryParams::Tensor& t = p.t[k];
     t.heads = (int)s.heads;
     if (s.heads == 0) continue;
+    TPF_REQUIRE(c.batch * c.tokens * s.heads < (1ll << 31), TPF_ERR_UNSUPPORTED, "%s: too many heads", who);
     const bool reads_x = !back || c.norm;
     TPF_REQUIRE((s.x != nullptr || !reads_x) && s.out != nullptr && (s.dy != nullptr || !back), TPF_ERR_INVALID_ARGUMENT,
                 "%s: null pointer", who);

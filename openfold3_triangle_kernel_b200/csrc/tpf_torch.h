@@ -113,8 +113,8 @@ std::vector<Tensor> rotary_bwd_op(const std::optional<Tensor>& dq, const std::op
                                   const std::optional<Tensor>& k, const std::optional<Tensor>& qw, const std::optional<Tensor>& kw,
                                   const Tensor& turns, const std::optional<Tensor>& positions, int64_t first, double magnitude,
                                   bool half, bool norm, double eps);
-py::object py_window_attention(py::handle q, py::handle k, py::handle v, py::handle offsets, py::handle lengths, int64_t offset,
-                               int64_t left, int64_t right, int64_t sinks, double scale, bool return_lse);
+py::object py_window_attention(py::handle q, py::handle k, py::handle v, py::handle window, py::handle sinks, py::handle query_offset,
+                               py::handle key_lengths, py::handle scale, bool return_lse);
 std::tuple<Tensor, Tensor> window_fwd_op(const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& offsets,
                                          const std::optional<Tensor>& lengths, int64_t offset, int64_t left, int64_t right,
                                          int64_t sinks, double scale);

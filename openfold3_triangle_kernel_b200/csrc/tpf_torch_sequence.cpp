@@ -1,4 +1,6 @@
 // Dropout, the position rotation of heads and the window attention for eager CUDA tensors.
+#include <cmath>
+
 #include "tpf_dropout.h"
 #include "tpf_rotary.h"
 #include "tpf_torch_memory.h"
@@ -431,7 +433,8 @@ py::object py_rotary(py::handle hq, py::handle hk, py::handle hqw, py::handle hk
     return py::none();
   if (pos.defined() && (pos.scalar_type() != at::kLong || !pos.is_contiguous() || pos.sizes() != q.sizes().slice(0, q.dim() - 2)))
     return py::none();
-  if (q.numel() / D >= (1ll << 31) - 256) return py::none();
+  constexpr int64_t kMostRows = (1ll << 31) - 256;
+  if (q.numel() / D > kMostRows || (k.defined() && k.numel() / D > kMostRows)) return py::none();
   const RotaryArgs a{turns, pos, first, magnitude, half, norm, eps};
   auto wants = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
   variable_list out;
@@ -449,9 +452,24 @@ py::object py_rotary(py::handle hq, py::handle hk, py::handle hqw, py::handle hk
   return py::make_tuple(out[0], out[1]);
 }
 
-py::object py_window_attention(py::handle hq, py::handle hk, py::handle hv, py::handle ho, py::handle hl, int64_t offset, int64_t left,
-                               int64_t right, int64_t sinks, double scale, bool return_lse) {
+py::object py_window_attention(py::handle hq, py::handle hk, py::handle hv, py::handle window, py::handle hsinks, py::handle ho,
+                               py::handle hl, py::handle hscale, bool return_lse) {
   if (!plain_type(hq) || !plain_type(hk) || !plain_type(hv) || !plain_context()) return py::none();
+  auto number = [](py::handle h, int64_t lo, int64_t hi, int64_t* out) {
+    if (!PyLong_CheckExact(h.ptr())) return false;
+    int overflow = 0;
+    *out = PyLong_AsLongLongAndOverflow(h.ptr(), &overflow);
+    return overflow == 0 && *out >= lo && *out <= hi;
+  };
+  if (!PyTuple_CheckExact(window.ptr()) || PyTuple_GET_SIZE(window.ptr()) != 2) return py::none();
+  int64_t reach[2] = {-1, -1}, sinks = 0, offset = 0;
+  for (int i = 0; i < 2; ++i) {
+    const py::handle n = PyTuple_GET_ITEM(window.ptr(), i);
+    if (!n.is_none() && !number(n, 0, tpf::kWindowMost - 1, &reach[i])) return py::none();
+  }
+  if (!number(hsinks, 0, tpf::kMostSinks, &sinks)) return py::none();
+  const bool offset_is_number = number(ho, -tpf::kWindowMost, tpf::kWindowMost, &offset);
+  if (!offset_is_number) offset = 0;
   const Tensor &q = THPVariable_Unpack(hq.ptr()), &k = THPVariable_Unpack(hk.ptr()), &v = THPVariable_Unpack(hv.ptr());
   if (!plain_cuda(q) || !device_supported(q) || (q.scalar_type() != at::kBFloat16 && q.scalar_type() != at::kHalf) || q.dim() < 3)
     return py::none();
@@ -464,12 +482,19 @@ py::object py_window_attention(py::handle hq, py::handle hk, py::handle hv, py::
     batch *= q.size(d);
   }
   if (batch > 65535 || H > 65535 || q.size(nd - 3) > tpf::kWindowMost || k.size(nd - 3) > tpf::kWindowMost) return py::none();
+  double scale = 1.0 / std::sqrt((double)D);
+  if (!hscale.is_none()) {
+    if (!PyFloat_CheckExact(hscale.ptr())) return py::none();
+    scale = PyFloat_AS_DOUBLE(hscale.ptr());
+    if (!(scale >= 0x1p-100 && scale <= 0x1p100)) return py::none();
+  }
   Tensor offsets, lengths;
-  if (!unpack_optional(ho, q, offsets) || !unpack_optional(hl, q, lengths)) return py::none();
+  if (!offset_is_number && (ho.is_none() || !THPVariable_Check(ho.ptr()) || !unpack_optional(ho, q, offsets))) return py::none();
+  if (!hl.is_none() && (!THPVariable_Check(hl.ptr()) || !unpack_optional(hl, q, lengths))) return py::none();
   for (const Tensor* t : {&offsets, &lengths})
     if (t->defined() && (t->scalar_type() != at::kInt || !t->is_contiguous() || t->sizes() != q.sizes().slice(0, nd - 3)))
       return py::none();
-  const WindowArgs a{offsets, lengths, offset, left, right, sinks, scale};
+  const WindowArgs a{offsets, lengths, offset, reach[0], reach[1], sinks, scale};
   Tensor out, lse;
   {
     py::gil_scoped_release release;

@@ -8,10 +8,16 @@
 // products a tile instead of five, but every gradient is summed by one CTA in a fixed order, without atomics and without partial
 // sums of dQ in memory (at a window of 1024 keys those would be 9 times dQ in fp32, written and read).
 //
-// A CTA keeps 128 rows (keys: K and V; queries: Q and dO) in shared memory and walks over tiles of 64 columns.  S and dP are made
-// with the rows as TMEM lanes, so that P and dS, written over them as 16-bit numbers, are the A operands of the second products
-// straight from TMEM; a thread has a row.  Two groups of four warps take turns with the tiles: while one computes, the products of
-// the other run.  With the keys as rows the CTA goes through all query heads that share them.
+// An item is 128 rows (keys: K and V; queries: Q and dO), kept in shared memory while the CTA walks over their tiles of 64 columns.  S and
+// dP are made with the rows as TMEM lanes, so that P and dS, written over them as 16-bit numbers, are the A operands of the second
+// products straight from TMEM; a thread has a row.  Two groups of four warps take turns with the tiles: while one computes, the
+// products of the other run.  With the keys as rows the CTA goes through all query heads that share them.  The next item's rows are
+// loaded, and its first tiles made, while the last item's gradients are still on their way out (an item a CTA left the tensor pipe idle
+// for 4 us at its start and end: FIGURE).
+//
+// What bounds it at 128 elements a head: the tensor pipe.  An UMMA of 64 columns with both operands in shared memory reads 6 KB, 48
+// cycles, for 32 cycles of products, which makes 1280 cycles a tile with the keys as rows and 1024 with the queries (1345 and 1127
+// measured without masks, starts and ends).  Q and dO as operands in TMEM were no faster (239 us for 224).
 //
 // The sinks are seen by every later query, which would make the first keys' CTA walk over the whole sequence.  It does its window;
 // the queries beyond are split over CTAs of their own, whose sums of the sinks' rows a last kernel adds up in a fixed order.
@@ -74,25 +80,28 @@ struct BwdArgs {
   int NP;
   void *g1, *g2;               // KEYS: dV and dK; else dQ and nothing
   float* parts;                // KEYS: [B, HK, 1 + far][2][sinks][D] of the sinks' rows, or nullptr
-  int key_tiles, far, far_tiles;  // KEYS: CTAs of far queries, and query tiles of each
+  int key_tiles, far, far_tiles;  // KEYS: items of far queries (of a head), and query tiles of each
+  int row_items, heads, items;    // items: (128 rows, head, sequence), the rows fastest
+  FastDiv div_rows, div_heads, div_g;
 };
 
 template <typename T_, int DP_, bool KEYS_>
 struct BwdCfg {
   using T = T_;
   static constexpr bool KEYS = KEYS_;
-  static constexpr int DP = DP_, CHUNKS = DP / 64, NS = DP == 128 ? 4 : 6;
+  static constexpr int DP = DP_, CHUNKS = DP / 64, NACC = KEYS ? 1 : 2;
+  static constexpr int NS = DP == 64 ? 6 : 3, NR = 2;
   static constexpr int R_CHUNK = 128 * 128, C_CHUNK = kTile * 128;
   static constexpr int R_TILE = CHUNKS * R_CHUNK, C_TILE = CHUNKS * C_CHUNK;
-  static constexpr int OFF_R = 0;                              // two tiles of rows
-  static constexpr int OFF_C = OFF_R + 2 * R_TILE;             // [NS] two tiles of columns
+  static constexpr int OFF_R = 0;                              // [NR] two tiles of rows
+  static constexpr int OFF_C = OFF_R + NR * 2 * R_TILE;        // [NS] two tiles of columns
   static constexpr int OFF_VEC = OFF_C + NS * 2 * C_TILE;      // [NS] nlse and ndelta of the columns (KEYS)
   static constexpr int OFF_BAR = OFF_VEC + (KEYS ? NS * 2 * kTile * 4 : 0);
-  static constexpr int N_BAR = 2 + 2 * NS + 4;
+  static constexpr int N_BAR = 2 * NR + 4 + 2 * NS + 4;
   static constexpr int SMEM = OFF_BAR + N_BAR * 8 + 16;
   static constexpr int THREADS = 320, WARP_TMA = 8, WARP_MMA = 9;
-  static constexpr int TM_ACC1 = 256, TM_ACC2 = 256 + DP, TMEM_COLS = 512;
-  static_assert(SMEM + 1024 <= 233472 && TM_ACC2 + DP <= TMEM_COLS, "");
+  static constexpr int TM_ACC = 256, TMEM_COLS = 512;          // KEYS: dV, dK; else dQ of two items in turn
+  static_assert(SMEM + 1024 <= 233472 && TM_ACC + 2 * DP <= TMEM_COLS, "");
 };
 
 __device__ __forceinline__ void bulk_load(uint32_t elected, void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -103,10 +112,43 @@ __device__ __forceinline__ void bulk_load(uint32_t elected, void* dst, const voi
       : "memory");
 }
 
-// The column tiles of a CTA: for each of `heads` heads [extra tile 0,] lo .. hi - 1.
-struct Columns {
-  int extra, lo, hi, heads;
-  __device__ __forceinline__ int per_head() const { return extra + max(0, hi - lo); }
+// An item and its column tiles: for each of `heads` heads [a tile of the sinks,] tiles lo .. hi - 1.
+template <bool KEYS>
+struct BwdItem {
+  int r0, head, b, len, off;  // head: KEYS: a key head, else a query head
+  int part;                   // KEYS: 0, or 1 + the number of far queries' item
+  int extra, lo, heads, per_head, tiles;
+  __device__ __forceinline__ BwdItem(int item, const WindowParams& p, const BwdArgs& a) {
+    const uint32_t r = a.div_rows.div((uint32_t)item);
+    const int x = item - (int)r * a.row_items;
+    b = (int)a.div_heads.div(r);
+    head = (int)r - b * a.heads;
+    len = p.length(b), off = p.first_position(b);
+    part = KEYS && x >= a.key_tiles ? x - a.key_tiles + 1 : 0;
+    r0 = part > 0 ? 0 : x * 128;
+    extra = 0;
+    int hi;
+    if constexpr (KEYS) {
+      heads = p.G;
+      const int last = min(r0 + 127, len - 1);
+      const int first = min(max(0, r0 - p.right - off), p.N), end = max(0, min(p.N, last + p.left - off + 1));
+      lo = first / kTile;
+      hi = r0 < len ? max(lo, (end + kTile - 1) / kTile) : lo;
+      if (part > 0) {  // queries beyond the first key tile's window
+        lo = max(hi, (part - 1) * a.far_tiles);
+        hi = len > 0 ? min((p.N + kTile - 1) / kTile, part * a.far_tiles) : lo;
+      }
+    } else {
+      heads = 1;
+      const KeyRange kr = key_range(p, len, off + r0, off + min(r0 + 127, p.N - 1));
+      extra = kr.lo >= kTile && kr.sink > 0 ? 1 : 0;
+      lo = kr.sink > 0 && !extra ? 0 : kr.lo / kTile;
+      hi = (kr.hi + kTile - 1) / kTile;
+    }
+    per_head = extra + max(0, hi - lo);
+    tiles = per_head * heads;
+  }
+  __device__ __forceinline__ int column(int u) const { return u < extra ? 0 : (lo + u - extra) * kTile; }  // of tile u of a head
 };
 
 template <class Cfg>
@@ -117,12 +159,14 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
   griddep_wait();
   using T = typename Cfg::T;
   constexpr bool KEYS = Cfg::KEYS;
-  constexpr int DP = Cfg::DP, NS = Cfg::NS, CHUNKS = Cfg::CHUNKS;
+  constexpr int DP = Cfg::DP, NS = Cfg::NS, NR = Cfg::NR, NACC = Cfg::NACC, CHUNKS = Cfg::CHUNKS;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
-  uint64_t* r_full = bars;
-  uint64_t* acc_full = bars + 1;
-  uint64_t* c_full = bars + 2;           // [NS]
+  uint64_t* r_full = bars;               // [NR]
+  uint64_t* r_empty = r_full + NR;       // [NR]
+  uint64_t* acc_full = r_empty + NR;     // [2]
+  uint64_t* acc_free = acc_full + 2;     // [2]
+  uint64_t* c_full = acc_free + 2;       // [NS]
   uint64_t* c_empty = c_full + NS;
   uint64_t* sdp_full = c_empty + NS;     // [2]
   uint64_t* pds_ready = sdp_full + 2;    // [2]
@@ -132,13 +176,17 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
   const int warp = warp_index(), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    mbar_init(r_full, 1);
-    mbar_init(acc_full, 1);
+    for (int s = 0; s < NR; ++s) {
+      mbar_init(&r_full[s], 1);
+      mbar_init(&r_empty[s], 1);
+    }
     for (int s = 0; s < NS; ++s) {
       mbar_init(&c_full[s], 1);
       mbar_init(&c_empty[s], 1);
     }
     for (int g = 0; g < 2; ++g) {
+      mbar_init(&acc_full[g], 1);
+      mbar_init(&acc_free[g], 8);
       mbar_init(&sdp_full[g], 1);
       mbar_init(&pds_ready[g], 4);
     }
@@ -158,118 +206,123 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  const int b = blockIdx.z, head = blockIdx.y;  // KEYS: a key head, else a query head
-  const int len = p.length(b), off = p.first_position(b);
-  const bool far = KEYS && (int)blockIdx.x >= a.key_tiles;  // queries beyond the first key tile's window
-  const int r0 = far ? 0 : (int)blockIdx.x * 128;
-  Columns cols;
-  cols.extra = 0;
-  if constexpr (KEYS) {
-    cols.heads = p.G;
-    const int last = min(r0 + 127, len - 1);
-    const int lo = min(max(0, r0 - p.right - off), p.N), hi = max(0, min(p.N, last + p.left - off + 1));
-    cols.lo = lo / kTile;
-    cols.hi = r0 < len ? max(cols.lo, (hi + kTile - 1) / kTile) : cols.lo;
-    if (far) {
-      const int c = (int)blockIdx.x - a.key_tiles, all = (p.N + kTile - 1) / kTile;
-      cols.lo = max(cols.hi, c * a.far_tiles);
-      cols.hi = len > 0 ? min(all, (c + 1) * a.far_tiles) : cols.lo;
-    }
-  } else {
-    cols.heads = 1;
-    const KeyRange kr = key_range(p, len, off + r0, off + min(r0 + 127, p.N - 1));
-    cols.extra = kr.lo >= kTile && kr.sink > 0 ? 1 : 0;
-    cols.lo = kr.sink > 0 && !cols.extra ? 0 : kr.lo / kTile;
-    cols.hi = (kr.hi + kTile - 1) / kTile;
-  }
-  const int per_head = cols.per_head(), tiles = per_head * cols.heads;
-  // tile u of a head starts at column
-  auto first = [&](int u) { return u < cols.extra ? 0 : (cols.lo + u - cols.extra) * kTile; };
-
   if (warp == Cfg::WARP_TMA) {
     const uint32_t el = elect_one();
-    if (tiles > 0) {
-      mbar_expect_tx(el, r_full, 2 * Cfg::R_TILE);
+    int s = 0, rs = 0;
+    uint32_t ph = 1, rph = 1;
+    for (int item = blockIdx.x; item < a.items; item += gridDim.x) {
+      const BwdItem<KEYS> it(item, p, a);
+      if (it.tiles == 0) continue;
+      warp_wait(&r_empty[rs], rph, wctx);
+      mbar_expect_tx(el, &r_full[rs], 2 * Cfg::R_TILE);
+      uint8_t* rows = smem + Cfg::OFF_R + rs * 2 * Cfg::R_TILE;
 #pragma unroll
       for (int c = 0; c < CHUNKS; ++c) {
-        tma_load_4d(el, smem + Cfg::OFF_R + c * Cfg::R_CHUNK, &tmR1, r_full, 64 * c, r0, head, b);
-        tma_load_4d(el, smem + Cfg::OFF_R + Cfg::R_TILE + c * Cfg::R_CHUNK, &tmR2, r_full, 64 * c, r0, head, b);
+        tma_load_4d(el, rows + c * Cfg::R_CHUNK, &tmR1, &r_full[rs], 64 * c, it.r0, it.head, it.b);
+        tma_load_4d(el, rows + Cfg::R_TILE + c * Cfg::R_CHUNK, &tmR2, &r_full[rs], 64 * c, it.r0, it.head, it.b);
       }
-    }
-    int s = 0;
-    uint32_t ph = 1;
-    for (int hh = 0; hh < cols.heads && per_head > 0; ++hh) {
-      const int ch = KEYS ? head * p.G + hh : head / p.G;
-      const int64_t vec = ((int64_t)b * p.H + ch) * a.NP;
-      for (int u = 0; u < per_head; ++u) {
-        const int c0 = first(u);
-        warp_wait(&c_empty[s], ph, wctx);
-        mbar_expect_tx(el, &c_full[s], 2 * Cfg::C_TILE + (KEYS ? 2 * kTile * 4 : 0));
-        uint8_t* dst = smem + Cfg::OFF_C + s * 2 * Cfg::C_TILE;
+      if (++rs == NR) rs = 0, rph ^= 1;
+      for (int hh = 0; hh < it.heads; ++hh) {
+        const int ch = KEYS ? it.head * p.G + hh : (int)a.div_g.div((uint32_t)it.head);
+        const int64_t vec = ((int64_t)it.b * p.H + ch) * a.NP;
+        for (int u = 0; u < it.per_head; ++u) {
+          const int c0 = it.column(u);
+          warp_wait(&c_empty[s], ph, wctx);
+          mbar_expect_tx(el, &c_full[s], 2 * Cfg::C_TILE + (KEYS ? 2 * kTile * 4 : 0));
+          uint8_t* dst = smem + Cfg::OFF_C + s * 2 * Cfg::C_TILE;
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) {
-          tma_load_4d(el, dst + c * Cfg::C_CHUNK, &tmC1, &c_full[s], 64 * c, c0, ch, b);
-          tma_load_4d(el, dst + Cfg::C_TILE + c * Cfg::C_CHUNK, &tmC2, &c_full[s], 64 * c, c0, ch, b);
+          for (int c = 0; c < CHUNKS; ++c) {
+            tma_load_4d(el, dst + c * Cfg::C_CHUNK, &tmC1, &c_full[s], 64 * c, c0, ch, it.b);
+            tma_load_4d(el, dst + Cfg::C_TILE + c * Cfg::C_CHUNK, &tmC2, &c_full[s], 64 * c, c0, ch, it.b);
+          }
+          if constexpr (KEYS) {
+            uint8_t* v = smem + Cfg::OFF_VEC + s * 2 * kTile * 4;
+            bulk_load(el, v, a.nlse + vec + c0, kTile * 4, &c_full[s]);
+            bulk_load(el, v + kTile * 4, a.ndelta + vec + c0, kTile * 4, &c_full[s]);
+          }
+          if (++s == NS) s = 0, ph ^= 1;
         }
-        if constexpr (KEYS) {
-          uint8_t* v = smem + Cfg::OFF_VEC + s * 2 * kTile * 4;
-          bulk_load(el, v, a.nlse + vec + c0, kTile * 4, &c_full[s]);
-          bulk_load(el, v + kTile * 4, a.ndelta + vec + c0, kTile * 4, &c_full[s]);
-        }
-        if (++s == NS) s = 0, ph ^= 1;
       }
     }
   } else if (warp == Cfg::WARP_MMA) {
     const uint32_t el = elect_one();
     constexpr uint32_t idesc_s = window_idesc<T>(128, kTile, false), idesc_acc = window_idesc<T>(128, DP, true);
     constexpr uint32_t hi = smem_desc_hi(1024, swizzle_mode_for_bytes(128));
-    const uint32_t d_r1 = smem_desc_lo(smem_u32(smem + Cfg::OFF_R), 16);
-    const uint32_t d_r2 = smem_desc_lo(smem_u32(smem + Cfg::OFF_R + Cfg::R_TILE), 16);
+    const uint32_t d_r = smem_desc_lo(smem_u32(smem + Cfg::OFF_R), 16);
     const uint32_t d_c = smem_desc_lo(smem_u32(smem + Cfg::OFF_C), 16);
     const uint32_t d_cmn = smem_desc_lo(smem_u32(smem + Cfg::OFF_C), Cfg::C_CHUNK);
-    constexpr uint32_t kStage = 2 * Cfg::C_TILE >> 4, kSecond = Cfg::C_TILE >> 4;
-    int s = 0;
-    uint32_t ph = 0;
-    auto issue_sdp = [&](int t) {
+    constexpr uint32_t kRows = 2 * Cfg::R_TILE >> 4, kStage = 2 * Cfg::C_TILE >> 4, kSecond = Cfg::C_TILE >> 4;
+    // The issuing thread is what the tensor pipe waits for first: its loop over an item's tiles holds nothing but counters.  (As a walk over
+    // the tiles of all items that finds the next item by itself it made the kernel of the keys 270 us in the place of 250.)
+    int s = 0, rs = 0, bs = 0, ab = 0;
+    uint32_t ph = 0, rph = 0, pph = 0, aph = 1;
+    auto issue_sdp = [&](int buf) {
       warp_wait(&c_full[s], ph, wctx);
       tc_fence_after();
-      const uint32_t d1 = d_c + s * kStage, d2 = d1 + kSecond, to = tmem + 128 * (t & 1);
+      const uint32_t r1 = NR > 1 ? d_r + rs * kRows : d_r, r2 = r1 + (Cfg::R_TILE >> 4);
+      const uint32_t d1 = d_c + s * kStage, d2 = d1 + kSecond, to = tmem + 128 * buf;
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d)
-        umma_ss_w<hi, hi, idesc_s>(el, to, d_r1 + ((d / 4 * Cfg::R_CHUNK + d % 4 * 32) >> 4),
+        umma_ss_w<hi, hi, idesc_s>(el, to, r1 + ((d / 4 * Cfg::R_CHUNK + d % 4 * 32) >> 4),
                                    d1 + ((d / 4 * Cfg::C_CHUNK + d % 4 * 32) >> 4), d != 0);
 #pragma unroll
       for (int d = 0; d < DP / 16; ++d)
-        umma_ss_w<hi, hi, idesc_s>(el, to + 64, d_r2 + ((d / 4 * Cfg::R_CHUNK + d % 4 * 32) >> 4),
+        umma_ss_w<hi, hi, idesc_s>(el, to + 64, r2 + ((d / 4 * Cfg::R_CHUNK + d % 4 * 32) >> 4),
                                    d2 + ((d / 4 * Cfg::C_CHUNK + d % 4 * 32) >> 4), d != 0);
-      umma_commit(el, &sdp_full[t & 1]);
+      umma_commit(el, &sdp_full[buf]);
       if (++s == NS) s = 0, ph ^= 1;
     };
-    if (tiles > 0) {
-      warp_wait(r_full, 0, wctx);
-      issue_sdp(0);
-      if (tiles > 1) issue_sdp(1);
-    }
-    int bs = 0;
-    for (int t = 0; t < tiles; ++t) {
-      const int g = t & 1;
-      warp_wait(&pds_ready[g], (t >> 1) & 1, wctx);
-      tc_fence_after();
-      const uint32_t d1 = d_cmn + bs * kStage, d2 = d1 + kSecond, from = tmem + 128 * g;
-      if constexpr (KEYS) {
+    auto rows_used = [&] {  // by all S and dP of the item
+      umma_commit(el, &r_empty[rs]);
+      if (++rs == NR) rs = 0, rph ^= 1;
+    };
+    auto tiles_from = [&](int& item) {  // of the next item that has any
+      int n = 0;
+      while (item < a.items && (n = BwdItem<KEYS>(item, p, a).tiles) == 0) item += gridDim.x;
+      return __shfl_sync(0xffffffffu, n, 0);
+    };
+    int item = blockIdx.x, buf = 0, lead = 0;  // lead: tiles of the item whose S and dP were made while the one before was finished
+    int tiles = tiles_from(item);
+    while (item < a.items) {
+      if (lead == 0) warp_wait(&r_full[rs], rph, wctx);
+      for (; lead < 2 && lead < tiles; ++lead) issue_sdp((buf + lead) & 1);
+      if (tiles <= 2) rows_used();
+      int next = item + gridDim.x;
+      const int next_tiles = tiles_from(next);
+      lead = 0;
+      for (int t = 0; t < tiles; ++t) {
+        if (t == 0) warp_wait2(&pds_ready[buf], pph, &acc_free[ab], aph, wctx);
+        else warp_wait(&pds_ready[buf], pph, wctx);
+        tc_fence_after();
+        const uint32_t d1 = d_cmn + bs * kStage, d2 = d1 + kSecond, from = tmem + 128 * buf, sums = tmem + Cfg::TM_ACC + (NACC > 1 ? ab * DP : 0);
+        if constexpr (KEYS) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma_ts_w<hi, idesc_acc>(el, sums, from + 8 * k, d2 + k * 128, (k | t) != 0);
+        }
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          umma_ts_w<hi, idesc_acc>(el, tmem + Cfg::TM_ACC1, from + 8 * k, d2 + k * 128, (k | t) != 0);
+          umma_ts_w<hi, idesc_acc>(el, KEYS ? sums + DP : sums, from + 64 + 8 * k, d1 + k * 128, (k | t) != 0);
+        umma_commit(el, &c_empty[bs]);
+        if (++bs == NS) bs = 0;
+        // S and dP of two tiles ahead go over P and dS, which the products just issued have to read: the UMMAs of a thread go through the
+        // tensor pipe in order (as in the triangle attention's backward pass)
+        if (t + 2 < tiles) {
+          issue_sdp(buf);
+          if (t + 3 == tiles) rows_used();
+        } else {
+          if (t + 1 == tiles) umma_commit(el, &acc_full[ab]);
+          if (NR > 1 && tiles > 1 && lead < next_tiles) {  // of the next item (beside a single tile, its first one is not due yet)
+            if (lead == 0) warp_wait(&r_full[rs], rph, wctx);
+            issue_sdp(buf);
+            ++lead;
+          }
+        }
+        buf ^= 1;
+        pph ^= buf ^ 1;
       }
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        umma_ts_w<hi, idesc_acc>(el, tmem + (KEYS ? Cfg::TM_ACC2 : Cfg::TM_ACC1), from + 64 + 8 * k, d1 + k * 128, (k | t) != 0);
-      umma_commit(el, &c_empty[bs]);
-      if (++bs == NS) bs = 0;
-      if (t + 1 == tiles) umma_commit(el, acc_full);
-      // over P and dS, which the products just issued have to read: the UMMAs of a thread go through the tensor pipe in order (as in
-      // the triangle attention's backward pass)
-      if (t + 2 < tiles) issue_sdp(t + 2);
+      if (++ab == NACC) ab = 0, aph ^= 1;
+      item = next;
+      tiles = next_tiles;
     }
   } else {
     // ------------------------------------------------------------------ compute warps: one thread per row
@@ -277,136 +330,169 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
     const uint32_t t_s = tmem_addr(tmem, lane_base, 128 * g), t_dp = t_s + 64;
     const float c2 = p.scale * kWindowLog2e;
     const uint64_t c22 = f2_pack(c2, c2);
-    const int mine = r0 + row;
-    float nl = 0.f, nd = 0.f;
-    if (!KEYS && mine < p.N) {
-      const int64_t at = ((int64_t)b * p.H + head) * a.NP + mine;
-      nl = __ldg(a.nlse + at);
-      nd = __ldg(a.ndelta + at);
-    }
-    const uint64_t nl2 = f2_pack(nl, nl), nd2 = f2_pack(nd, nd);
-    const int w0 = r0 + lane_base, w1 = w0 + 31;  // the warp's rows
-    int u = 0;
-    auto advance = [&](int n) {
-      u += n;
-      while (u >= per_head) u -= per_head;
-    };
-    if (tiles > 0) advance(g);
-    for (int t = g; t < tiles; t += 2) {
-      const int c0 = first(u);
-      const int s = t % NS;
-      warp_wait(&sdp_full[g], (t >> 1) & 1, wctx);
-      tc_fence_after();
-      uint64_t seen;
-      bool whole;
-      if constexpr (KEYS) {
-        seen = seeing_queries(p, len, mine, off + c0);
-        whole = w1 < len && off + c0 >= w1 - p.right && off + c0 + kTile - 1 <= w0 + p.left;
-      } else {
-        seen = seen_keys(p, len, off + mine, c0);
-        whole = c0 + kTile <= min(len, off + w0 + p.right + 1) && c0 >= off + w1 - p.left;
-      }
-      const float* vec = reinterpret_cast<const float*>(smem + Cfg::OFF_VEC + s * 2 * kTile * 4);
-      auto tile = [&](auto masked) {
-        constexpr bool MASKED = decltype(masked)::value;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t rs[32], rd[32];
-          tmem_ld32(t_s + 32 * half, rs);
-          tmem_ld32(t_dp + 32 * half, rd);
+    const int rows = KEYS ? p.M : p.N, heads = KEYS ? p.HK : p.H;
+
+    // KEYS: group 0 stores dV and group 1 dK; else each a half of dQ's columns.  The sums of an item leave after the group's first tile of
+    // a later one has been handed over.
+    const int cb = KEYS ? 0 : g * (DP / 2), ce = KEYS ? DP : cb + DP / 2;
+    const float mul = KEYS && g == 0 ? 1.f : p.scale;
+    bool pending = false;
+    int d_row = 0, d_head = 0, d_b = 0, d_part = 0, ab = 0;
+    uint32_t aph = 0;
+    auto store_rows = [&](bool any) {
+      // the sinks' rows are finished by the last kernel
+      const bool part = KEYS && a.parts != nullptr && d_row == row && row < min(p.sinks, p.M);
+      T* out = static_cast<T*>(KEYS && g == 1 ? a.g2 : a.g1) + (((int64_t)d_b * rows + d_row) * heads + d_head) * p.D;
+      float* sums = nullptr;
+      if (part) sums = a.parts + (((((int64_t)d_b * p.HK + d_head) * (1 + a.far) + d_part) * 2 + g) * p.sinks + row) * p.D;
+      const uint32_t src = tmem_addr(tmem, lane_base, Cfg::TM_ACC + (KEYS ? g : ab) * DP);
+#pragma unroll 1
+      for (int c = cb; c < ce; c += 16) {
+        uint32_t r[16];
+        if (any) {
+          tmem_ld16(src + c, r);
           tmem_ld_wait();
-          const uint32_t bits = (uint32_t)(seen >> (32 * half));
+        } else {
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            uint32_t pk[8], dk[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int c = 16 * q + 2 * e;
-              uint64_t l2 = nl2, de2 = nd2;
-              if constexpr (KEYS) {
-                const float2 x = *reinterpret_cast<const float2*>(vec + 32 * half + c);
-                const float2 y = *reinterpret_cast<const float2*>(vec + kTile + 32 * half + c);
-                l2 = f2_pack(x.x, x.y);
-                de2 = f2_pack(y.x, y.y);
-              }
-              float a0, a1;
-              f2_unpack(f2_fma(f2_pack_bits(rs[c], rs[c + 1]), c22, l2), a0, a1);
-              float p0 = ex2_approx(a0), p1 = ex2_approx(a1), d0, d1;
-              f2_unpack(f2_mul(f2_pack(p0, p1), f2_add(f2_pack_bits(rd[c], rd[c + 1]), de2)), d0, d1);
-              if (MASKED) {  // (what is masked may be a NaN)
-                if (!(bits >> c & 1u)) p0 = d0 = 0.f;
-                if (!(bits >> (c + 1) & 1u)) p1 = d1 = 0.f;
-              }
-              // 16 bits, as operands of the products
-              pk[e] = pack2<T>(p0, p1);
-              dk[e] = pack2<T>(d0, d1);
-            }
-            if (KEYS) tmem_st8(t_s + 16 * half + 8 * q, pk);
-            tmem_st8(t_dp + 16 * half + 8 * q, dk);
-          }
+          for (int e = 0; e < 16; ++e) r[e] = 0u;
         }
-      };
-      if (whole) tile(std::false_type{});
-      else tile(std::true_type{});
-      if constexpr (!KEYS) {
-        // Keys behind the last one are anything, and a dS of zero times a NaN is one (S has been made from them, and masked).
-        if (c0 + kTile > len) {
-          uint8_t* kt = smem + Cfg::OFF_C + s * 2 * Cfg::C_TILE;
-          for (int e = threadIdx.x & 127; e < CHUNKS * kTile * 8; e += 128) {
-            const int r = e / 8 % kTile;
-            if (c0 + r >= len)
-              *reinterpret_cast<uint4*>(kt + e / (8 * kTile) * Cfg::C_CHUNK + r * 128 + e % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+        float v[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(r[e]) * mul;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          if (c + 8 * k >= p.D) continue;
+          if (part) {
+            *reinterpret_cast<float4*>(sums + c + 8 * k) = make_float4(v[8 * k], v[8 * k + 1], v[8 * k + 2], v[8 * k + 3]);
+            *reinterpret_cast<float4*>(sums + c + 8 * k + 4) = make_float4(v[8 * k + 4], v[8 * k + 5], v[8 * k + 6], v[8 * k + 7]);
+          } else if (d_part == 0 && d_row < rows) {
+            store_vec<T, 8>(out + c + 8 * k, v + 8 * k);
           }
-          fence_async_smem();
         }
       }
-      tmem_st_wait();
+    };
+    auto finish = [&] {
+      warp_wait(&acc_full[ab], aph, wctx);
+      tc_fence_after();
+      store_rows(true);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&pds_ready[g]);
-      advance(2);
-    }
-    if (tiles > 0) {
-      warp_wait(acc_full, 0, wctx);
-      tc_fence_after();
-    }
-    // KEYS: group 0 stores dV and group 1 dK; else each a half of dQ's columns
-    const int cb = KEYS ? 0 : g * (DP / 2), ce = KEYS ? DP : cb + DP / 2;
-    const uint32_t src = tmem_addr(tmem, lane_base, KEYS && g == 1 ? Cfg::TM_ACC2 : Cfg::TM_ACC1);
-    const float mul = KEYS && g == 0 ? 1.f : p.scale;
-    const int rows = KEYS ? p.M : p.N, heads = KEYS ? p.HK : p.H;
-    void* grad = KEYS && g == 1 ? a.g2 : a.g1;
-    // rows whose sum is finished by the last kernel
-    const bool part = KEYS && a.parts != nullptr && r0 == 0 && row < min(p.sinks, p.M);
-    T* out = static_cast<T*>(grad) + (((int64_t)b * rows + mine) * heads + head) * p.D;
-    float* sums = nullptr;
-    if (part)
-      sums = a.parts + (((((int64_t)b * p.HK + head) * (1 + a.far) + (far ? (int)blockIdx.x - a.key_tiles + 1 : 0)) * 2 + g) * p.sinks +
-                        row) * p.D;
-#pragma unroll 1
-    for (int c = cb; c < ce; c += 16) {
-      uint32_t r[16];
-      if (tiles > 0) {
-        tmem_ld16(src + c, r);
-        tmem_ld_wait();
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) r[e] = 0u;
+      if (lane == 0) mbar_arrive(&acc_free[ab]);
+      if (++ab == NACC) ab = 0, aph ^= 1;
+      pending = false;
+    };
+
+    int turn = g;   // tiles until the group's next one
+    int s = 0;      // stage of the item's first tile
+    uint32_t ph = 0;
+    for (int item = blockIdx.x; item < a.items; item += gridDim.x) {
+      const BwdItem<KEYS> it(item, p, a);
+      const int mine = it.r0 + row;
+      if (it.tiles == 0) {
+        if (pending) finish();
+        d_row = mine, d_head = it.head, d_b = it.b, d_part = it.part;
+        store_rows(false);
+        continue;
       }
-      float v[16];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) v[e] = __uint_as_float(r[e]) * mul;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        if (c + 8 * k >= p.D) continue;
-        if (part) {
-          *reinterpret_cast<float4*>(sums + c + 8 * k) = make_float4(v[8 * k], v[8 * k + 1], v[8 * k + 2], v[8 * k + 3]);
-          *reinterpret_cast<float4*>(sums + c + 8 * k + 4) = make_float4(v[8 * k + 4], v[8 * k + 5], v[8 * k + 6], v[8 * k + 7]);
-        } else if (!far && mine < rows) {
-          store_vec<T, 8>(out + c + 8 * k, v + 8 * k);
+      float nl = 0.f, nd = 0.f;
+      if (!KEYS && mine < p.N) {
+        const int64_t at = ((int64_t)it.b * p.H + it.head) * a.NP + mine;
+        nl = __ldg(a.nlse + at);
+        nd = __ldg(a.ndelta + at);
+      }
+      const uint64_t nl2 = f2_pack(nl, nl), nd2 = f2_pack(nd, nd);
+      const int w0 = it.r0 + lane_base, w1 = w0 + 31, len = it.len, off = it.off;  // the warp's rows
+      int u = turn, t = turn, st = s + turn;
+      while (u >= it.per_head && t < it.tiles) u -= it.per_head;
+      while (st >= NS) st -= NS;
+      for (; t < it.tiles; t += 2) {
+        const int c0 = it.column(u);
+        warp_wait(&sdp_full[g], ph, wctx);
+        ph ^= 1;
+        tc_fence_after();
+        uint64_t seen;
+        bool whole;
+        if constexpr (KEYS) {
+          seen = seeing_queries(p, len, mine, off + c0);
+          whole = w1 < len && off + c0 >= w1 - p.right && off + c0 + kTile - 1 <= w0 + p.left;
+        } else {
+          seen = seen_keys(p, len, off + mine, c0);
+          whole = c0 + kTile <= min(len, off + w0 + p.right + 1) && c0 >= off + w1 - p.left;
         }
+        const float* vec = reinterpret_cast<const float*>(smem + Cfg::OFF_VEC + st * 2 * kTile * 4);
+        auto tile = [&](auto masked) {
+          constexpr bool MASKED = decltype(masked)::value;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t rs[32], rd[32];
+            tmem_ld32(t_s + 32 * half, rs);
+            tmem_ld32(t_dp + 32 * half, rd);
+            tmem_ld_wait();
+            const uint32_t bits = (uint32_t)(seen >> (32 * half));
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              uint32_t pk[8], dk[8];
+              [[maybe_unused]] float4 x4, y4;  // of four columns
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const int c = 16 * q + 2 * e;
+                uint64_t l2 = nl2, de2 = nd2;
+                if constexpr (KEYS) {
+                  if (e % 2 == 0) {
+                    x4 = *reinterpret_cast<const float4*>(vec + 32 * half + c);
+                    y4 = *reinterpret_cast<const float4*>(vec + kTile + 32 * half + c);
+                  }
+                  l2 = e % 2 == 0 ? f2_pack(x4.x, x4.y) : f2_pack(x4.z, x4.w);
+                  de2 = e % 2 == 0 ? f2_pack(y4.x, y4.y) : f2_pack(y4.z, y4.w);
+                }
+                float a0, a1;
+                f2_unpack(f2_fma(f2_pack_bits(rs[c], rs[c + 1]), c22, l2), a0, a1);
+                float p0 = ex2_approx(a0), p1 = ex2_approx(a1), d0, d1;
+                f2_unpack(f2_mul(f2_pack(p0, p1), f2_add(f2_pack_bits(rd[c], rd[c + 1]), de2)), d0, d1);
+                if (MASKED) {  // (what is masked may be a NaN)
+                  if (!(bits >> c & 1u)) p0 = d0 = 0.f;
+                  if (!(bits >> (c + 1) & 1u)) p1 = d1 = 0.f;
+                }
+                // 16 bits, as operands of the products
+                pk[e] = pack2<T>(p0, p1);
+                dk[e] = pack2<T>(d0, d1);
+              }
+              if (KEYS) tmem_st8(t_s + 16 * half + 8 * q, pk);
+              tmem_st8(t_dp + 16 * half + 8 * q, dk);
+            }
+          }
+        };
+        if (whole) tile(std::false_type{});
+        else tile(std::true_type{});
+        if constexpr (!KEYS) {
+          // Keys behind the last one are anything, and a dS of zero times a NaN is one (S has been made from them, and masked).
+          if (c0 + kTile > len) {
+            uint8_t* kt = smem + Cfg::OFF_C + st * 2 * Cfg::C_TILE;
+            for (int e = threadIdx.x & 127; e < CHUNKS * kTile * 8; e += 128) {
+              const int r = e / 8 % kTile;
+              if (c0 + r >= len)
+                *reinterpret_cast<uint4*>(kt + e / (8 * kTile) * Cfg::C_CHUNK + r * 128 + e % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_async_smem();
+          }
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pds_ready[g]);
+        if (pending) finish();
+        u += 2;
+        while (u >= it.per_head) u -= it.per_head;
+        st += 2;
+        while (st >= NS) st -= NS;
       }
+      turn = t - it.tiles;
+      s = (s + it.tiles) % NS;
+      if (pending) finish();  // (the item had no tile for the group)
+      d_row = mine, d_head = it.head, d_b = it.b, d_part = it.part;
+      pending = true;
     }
+    if (pending) finish();
   }
   tc_fence_before();
   __syncthreads();
@@ -418,17 +504,29 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
 
 // ---- the sinks' rows ----------------------------------------------------------------------------------------
 template <typename T>
-__global__ void __launch_bounds__(128) window_sinks_kernel(const float* __restrict__ parts, int count, int sinks, int rows, int D, int M,
-                                                           int HK, T* __restrict__ dv, T* __restrict__ dk) {
+__global__ void __launch_bounds__(256) window_sinks_kernel(const float* __restrict__ parts, int count, int sinks, int D, int M, int HK,
+                                                           T* __restrict__ dv, T* __restrict__ dk) {
   griddep_wait();
-  const int head = blockIdx.x, b = blockIdx.y;
-  const float* from = parts + ((int64_t)b * HK + head) * count * 2 * sinks * D;
-  for (int e = threadIdx.x; e < 2 * rows * D; e += 128) {
-    const int which = e / (rows * D), rest = e - which * rows * D;
-    float s = 0.f;
-    for (int k = 0; k < count; ++k) s += from[((int64_t)k * 2 + which) * sinks * D + rest];
-    const int row = rest / D, d = rest - row * D;
-    (which == 0 ? dv : dk)[(((int64_t)b * M + row) * HK + head) * D + d] = from_f32<T>(s);
+  __shared__ float4 red[8][32];
+  const int row = blockIdx.x >> 1, which = blockIdx.x & 1, head = blockIdx.y, b = blockIdx.z;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const float* from = parts + (((int64_t)b * HK + head) * count * 2 + which) * sinks * D + row * D + 4 * lane;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (4 * lane < D)
+    for (int k = w; k < count; k += 8) {
+      const float4 x = *reinterpret_cast<const float4*>(from + (int64_t)k * 2 * sinks * D);
+      s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
+    }
+  red[w][lane] = s;
+  __syncthreads();
+  if (w == 0 && 4 * lane < D) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) {
+      const float4 x = red[k][lane];
+      s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
+    }
+    *reinterpret_cast<uint2*>((which == 0 ? dv : dk) + (((int64_t)b * M + row) * HK + head) * D + 4 * lane) =
+        make_uint2(pack2<T>(s.x, s.y), pack2<T>(s.z, s.w));
   }
 }
 
@@ -450,14 +548,23 @@ int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 
 template <class Cfg>
 int launch(const CUtensorMap& r1, const CUtensorMap& r2, const CUtensorMap& c1, const CUtensorMap& c2, const WindowParams& p,
-           const BwdArgs& a, dim3 grid, cudaStream_t stream) {
+           BwdArgs a, const WindowCall& c, cudaStream_t stream) {
+  a.row_items = Cfg::KEYS ? a.key_tiles + a.far : (int)((c.N + 127) / 128);
+  a.heads = (int)(Cfg::KEYS ? c.HK : c.H);
+  const int64_t items = (int64_t)a.row_items * a.heads * c.B;
+  TPF_REQUIRE(items < (1ll << 31) - 65536, TPF_ERR_UNSUPPORTED, "window_attn_bwd: too many rows");
+  a.items = (int)items;
+  a.div_rows = FastDiv::make((uint32_t)a.row_items);
+  a.div_heads = FastDiv::make((uint32_t)a.heads);
+  a.div_g = FastDiv::make((uint32_t)p.G);
+  const int grid = a.items < sm_count() ? a.items : sm_count();
   auto kern = window_bwd_kernel<Cfg>;
   static PerDeviceOnce once;
   if (int rc = ensure_dynamic_smem(kern, Cfg::SMEM, once, 1024)) return rc;
   int* status = nullptr;
   static PerDeviceAddress cache;
   if (int rc = device_symbol_address(g_window_bwd_status, cache, reinterpret_cast<void**>(&status))) return rc;
-  launch_kernel(kern, grid, dim3(Cfg::THREADS), Cfg::SMEM, stream, r1, r2, c1, c2, p, a, status);
+  launch_kernel(kern, dim3(grid), dim3(Cfg::THREADS), Cfg::SMEM, stream, r1, r2, c1, c2, p, a, status);
   TPF_LAUNCH_OK();
   return TPF_OK;
 }
@@ -486,12 +593,11 @@ int run(const WindowCall& c, const WindowParams& p, uint8_t* ws, cudaStream_t st
     a.key_tiles = (int)((c.M + 127) / 128);
     far_plan(c, &a.far, &a.far_tiles);
     if (a.far > 0) a.parts = reinterpret_cast<float*>(ws + 2 * stat);
-    if ((rc = launch<BwdCfg<T, DP, true>>(tk, tv, tq, tg, p, a, dim3(a.key_tiles + a.far, (unsigned)c.HK, (unsigned)c.B), stream)))
-      return rc;
+    if ((rc = launch<BwdCfg<T, DP, true>>(tk, tv, tq, tg, p, a, c, stream))) return rc;
     if (a.far > 0) {
-      launch_kernel(window_sinks_kernel<T>, dim3((unsigned)c.HK, (unsigned)c.B), dim3(128), 0, stream,
-                    static_cast<const float*>(a.parts), 1 + a.far, c.sinks, (int)(c.sinks < c.M ? c.sinks : c.M), (int)c.D, (int)c.M,
-                    (int)c.HK, static_cast<T*>(c.dv), static_cast<T*>(c.dk));
+      launch_kernel(window_sinks_kernel<T>, dim3(2 * (unsigned)(c.sinks < c.M ? c.sinks : c.M), (unsigned)c.HK, (unsigned)c.B), dim3(256),
+                    0, stream, static_cast<const float*>(a.parts), 1 + a.far, c.sinks, (int)c.D, (int)c.M, (int)c.HK,
+                    static_cast<T*>(c.dv), static_cast<T*>(c.dk));
       TPF_LAUNCH_OK();
     }
   }
@@ -503,9 +609,7 @@ int run(const WindowCall& c, const WindowParams& p, uint8_t* ws, cudaStream_t st
     if ((rc = make_window_tmap(&tv, c.v, c.type, c.B, c.M, c.HK, c.D, c.vs, kTile))) return rc;
     a.g1 = c.dq, a.g2 = nullptr;
     a.parts = nullptr;
-    if ((rc = launch<BwdCfg<T, DP, false>>(tq, tg, tk, tv, p, a, dim3((unsigned)((c.N + 127) / 128), (unsigned)c.H, (unsigned)c.B),
-                                           stream)))
-      return rc;
+    if ((rc = launch<BwdCfg<T, DP, false>>(tq, tg, tk, tv, p, a, c, stream))) return rc;
   }
   return TPF_OK;
 }

@@ -199,10 +199,12 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     for (int t = 0; t < tiles; ++t) {
       const int buf = t & 1;
       const uint32_t ph = (t >> 1) & 1;
-      warp_wait(&s_full[buf], ph, wctx);
-      tc_fence_after();
       const int j0 = first(t), n = steps(t);
       const bool whole = n == 4 && j0 + KEYS <= min(len, w0 + p.right + 1) && j0 >= w1 - p.left;
+      const uint64_t seen = whole ? 0 : seen_keys(p, len, pos, j0) & low_bits(16 * n);
+      const bool some = whole || __any_sync(0xffffffffu, seen != 0);
+      warp_wait(&s_full[buf], ph, wctx);
+      tc_fence_after();
       auto tile = [&](auto masked) {
         constexpr bool MASKED = decltype(masked)::value;
         uint32_t raw[64];
@@ -210,11 +212,14 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (!MASKED || n > 2) tmem_ld32(t_s + 64 * buf + 32, *reinterpret_cast<uint32_t(*)[32]>(raw + 32));
         tmem_ld_wait();
         if (MASKED) {
-          const uint64_t seen = seen_keys(p, len, pos, j0) & low_bits(16 * n);
-          const uint32_t lo = (uint32_t)seen, hi = (uint32_t)(seen >> 32);
 #pragma unroll
-          for (int e = 0; e < 64; ++e)
-            if (!((e < 32 ? lo : hi) >> (e & 31) & 1u)) raw[e] = 0xff800000u;
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t bits = (uint32_t)(seen >> (16 * c)) & 0xffffu;
+            if (__all_sync(0xffffffffu, bits == 0xffffu)) continue;
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (!(bits >> e & 1u)) raw[16 * c + e] = 0xff800000u;
+          }
         }
         float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
@@ -265,9 +270,15 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         f2_unpack(f2_add(sum0, sum1), r0, r1);
         l += r0 + r1;
       };
-      if (!live) {
-      } else if (whole) tile(std::false_type{});
-      else tile(std::true_type{});
+      if (live && whole) {
+        tile(std::false_type{});
+      } else if (live && some) {
+        tile(std::true_type{});
+      } else if (live) {  // none of the warp's queries sees any of them
+        const uint32_t zero[8] = {};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_st8(t_s + 64 * buf + 8 * c, zero);
+      }
       if (j0 + 16 * n > len) {
         // Values behind the last key are anything (the rest of a cache), and a probability of zero times a NaN is one.
         warp_wait(&v_full[buf], ph, wctx);

@@ -29,7 +29,7 @@ from .layer_norm import MAX_EPS, ROW_DTYPES, check_parameter
 from .trimul import SupportResult
 
 MAX_HEAD_DIM = 256
-_MAX_TOKENS = 2 ** 31 - 256
+_MOST_ROWS = 2 ** 31 - 256   # tokens of all batches times heads
 LAYOUTS = ("half", "interleaved")
 SCALINGS = (None, "linear", "ntk", "yarn")
 
@@ -102,8 +102,8 @@ def _check(named, weights, turns, magnitude, positions, layout, eps, check_devic
             return SupportResult(False, "x_dtype", f"{name} must have {first_name}'s type and device")
         if t.ndim != x.ndim or differs(t.shape[:-2] + t.shape[-1:], x.shape[:-2] + x.shape[-1:]):
             return SupportResult(False, "x_shape", f"{name} must have {first_name}'s sizes but for the heads")
-    if certain(math.prod(x.shape[:-2]) > _MAX_TOKENS):
-        return SupportResult(False, "tokens", "too many tokens")
+    if any(certain(math.prod(t.shape[:-1]) > _MOST_ROWS) for _, t in named):
+        return SupportResult(False, "tokens", "too many tokens and heads")
     for name, w in weights:
         bad = check_parameter(name, w, x.shape[-1], x)
         if bad is not None:

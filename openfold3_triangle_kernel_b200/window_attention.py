@@ -170,16 +170,21 @@ def _int32(t):
 def turbo_window_attention(q, k, v, *, window, sinks=0, query_offset=0, key_lengths=None, scale=None, return_lse=False):
     """``softmax(scale q k^T) v`` over the window and the sinks; see the module docstring for the contract."""
     tracing = torch.compiler.is_compiling()
-    res = check_window_attention_support(q, k, v, window=window, sinks=sinks, query_offset=query_offset, key_lengths=key_lengths,
-                                         scale=scale, check_device=not tracing)
-    refuse("turbo_window_attention", res)
-    left, right = (-1 if n is None else n for n in window)
-    offsets, lengths = _int32(query_offset), _int32(key_lengths)
-    offset = 0 if offsets is not None else query_offset
-    scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
     if not tracing:
-        out = C.native().window_attention(q, k, v, offsets, lengths, offset, left, right, sinks, scale, return_lse)
+        out = C.native().window_attention(q, k, v, window, sinks, query_offset, key_lengths, scale, return_lse)
         if out is not None:
             return out
-    out, lse = torch.ops.tpf_b200.window_attn_fwd(q, k, v, offsets, lengths, offset, left, right, sinks, scale)
+    refuse("turbo_window_attention", check_window_attention_support(
+        q, k, v, window=window, sinks=sinks, query_offset=query_offset, key_lengths=key_lengths, scale=scale,
+        check_device=not tracing))
+    offsets, lengths = _int32(query_offset), _int32(key_lengths)
+    scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
+    if not tracing:     # the same with numbers and tensors in the form that the native route takes
+        out = C.native().window_attention(q, k, v, tuple(window), sinks, query_offset if offsets is None else offsets, lengths, scale,
+                                          return_lse)
+        if out is not None:
+            return out
+    left, right = (-1 if n is None else n for n in window)
+    out, lse = torch.ops.tpf_b200.window_attn_fwd(q, k, v, offsets, lengths, 0 if offsets is not None else query_offset, left, right,
+                                                  sinks, scale)
     return (out, lse) if return_lse else out
