@@ -252,27 +252,24 @@ struct RotaryFn : public torch::autograd::Function<RotaryFn> {
     // (the inputs themselves where they were read in place, so that a change to them before the backward is noticed)
     ctx->save_for_backward({a.norm ? kept(q, hq) : Tensor(), a.norm && k ? kept(*k, hk) : Tensor(), qw ? *qw : Tensor(),
                             kw ? *kw : Tensor(), a.turns, a.positions});
-    ctx->saved_data["first"] = a.first;
-    ctx->saved_data["magnitude"] = a.magnitude;
-    ctx->saved_data["half"] = a.half;
-    ctx->saved_data["norm"] = a.norm;
-    ctx->saved_data["eps"] = a.eps;
-    ctx->saved_data["k"] = k.has_value();
+    // (an entry costs a microsecond)
+    ctx->saved_data["a"] = std::vector<double>{(double)(a.first >> 32), (double)(a.first & 0xffffffff), a.magnitude, (double)a.half,
+                                               (double)a.norm, a.eps, (double)k.has_value()};
     ctx->set_materialize_grads(false);
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) { return first_order(grads, gradients(ctx, grads)); }
   static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
     variable_list r(5);
-    const bool has_k = ctx->saved_data["k"].toBool();
+    const std::vector<double> v = ctx->saved_data["a"].toDoubleVector();
+    const bool has_k = v[6] != 0;
     const Tensor none;
     const Tensor& some = grads[0].defined() ? grads[0] : has_k ? grads[1] : none;
     if (!some.defined()) return r;
     c10::cuda::CUDAGuard guard(some.device());
     at::NoGradGuard no_grad;
     const auto saved = ctx->get_saved_variables();
-    const RotaryArgs a{saved[4], saved[5], ctx->saved_data["first"].toInt(), ctx->saved_data["magnitude"].toDouble(),
-                       ctx->saved_data["half"].toBool(), ctx->saved_data["norm"].toBool(), ctx->saved_data["eps"].toDouble()};
+    const RotaryArgs a{saved[4], saved[5], ((int64_t)v[0] << 32) + (int64_t)v[1], v[2], v[3] != 0, v[4] != 0, v[5]};
     const Tensor d[2] = {grads[0].defined() ? dense(grads[0]) : none, has_k && grads[1].defined() ? dense(grads[1]) : none};
     const Heads x[2] = {saved[0].defined() ? as_heads(saved[0].detach(), false) : Heads{},
                         saved[1].defined() ? as_heads(saved[1].detach(), false) : Heads{}};
@@ -355,8 +352,7 @@ struct WindowFn : public torch::autograd::Function<WindowFn> {
     const Heads hq = as_heads(q.detach(), true), hk = as_heads(k.detach(), true), hv = as_heads(v.detach(), true);
     auto [out, lse] = window_out(hq, hk, hv, a, true);
     ctx->save_for_backward({kept(q, hq), kept(k, hk), kept(v, hv), out, lse, a.offsets, a.lengths});
-    ctx->saved_data["a"] = std::vector<int64_t>{a.offset, a.left, a.right, a.sinks};
-    ctx->saved_data["scale"] = a.scale;
+    ctx->saved_data["a"] = std::vector<double>{(double)a.offset, (double)a.left, (double)a.right, (double)a.sinks, a.scale};
     ctx->mark_non_differentiable({lse});
     ctx->set_materialize_grads(false);
     return {out, lse};
@@ -368,8 +364,8 @@ struct WindowFn : public torch::autograd::Function<WindowFn> {
     c10::cuda::CUDAGuard guard(grads[0].device());
     at::NoGradGuard no_grad;
     const auto s = ctx->get_saved_variables();
-    const std::vector<int64_t> v = ctx->saved_data["a"].toIntVector();
-    const WindowArgs a{s[5], s[6], v[0], v[1], v[2], v[3], ctx->saved_data["scale"].toDouble()};
+    const std::vector<double> v = ctx->saved_data["a"].toDoubleVector();  // (whole numbers below 2^53 are exact)
+    const WindowArgs a{s[5], s[6], (int64_t)v[0], (int64_t)v[1], (int64_t)v[2], (int64_t)v[3], v[4]};
     const bool need_kv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
     const variable_list g = window_grads(dense(grads[0]), as_heads(s[0].detach(), true), as_heads(s[1].detach(), true),
                                          as_heads(s[2].detach(), true), s[3], s[4], a, ctx->needs_input_grad(0), need_kv);

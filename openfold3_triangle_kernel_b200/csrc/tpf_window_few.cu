@@ -16,6 +16,7 @@ namespace tpf {
 namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kStages = 3, kBlock = 16;
+constexpr int kMostSplits = 16;  // CTAs of a cluster
 
 template <int DP>
 struct FewCfg {
@@ -267,6 +268,15 @@ int launch(const WindowParams& p, const FewArgs& a, cudaStream_t stream) {
   auto kern = window_few_kernel<T, DP>;
   static PerDeviceOnce once;
   if (int rc = ensure_dynamic_smem(kern, Cfg::SMEM, once)) return rc;
+  if (a.splits > 8) {  // more than a cluster has everywhere
+    static PerDeviceOnce wide;
+    int dev = 0;
+    if (int rc = current_device(&dev)) return rc;
+    if (!wide.done[dev].load(std::memory_order_acquire)) {
+      TPF_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+      wide.done[dev].store(true, std::memory_order_release);
+    }
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(a.splits * a.row_tiles, p.HK, p.B);
   cfg.blockDim = dim3(kThreads);
@@ -295,13 +305,13 @@ int window_few(const WindowCall& c, const WindowParams& p, cudaStream_t stream) 
   a.rows = (int)(c.N * p.G);
   a.row_tiles = (a.rows + 15) / 16;
   a.div_g = FastDiv::make((uint32_t)p.G);
-  // Keys are split over a cluster of up to eight CTAs, while that brings more CTAs than two an SM have room for, and a split keeps
-  // at least two blocks a warp.
+  // Keys are split over a cluster of up to sixteen CTAs, while no more of them come than find room on the SMs at once (two an SM), and a
+  // split keeps at least two blocks a warp.  (One sequence of 32768 keys, 8 key heads: FIGURE us with eight, FIGURE with sixteen.)
   const int64_t ctas = c.B * c.HK * a.row_tiles;
   int64_t keys = (int64_t)c.left + c.right + c.N + c.sinks;
   if (keys > c.M) keys = c.M;
   a.splits = 1;
-  while (a.splits < 8 && ctas * a.splits * 2 <= 2 * sm_count() && keys >= a.splits * 2 * kWarps * kBlock * 2) a.splits *= 2;
+  while (a.splits < kMostSplits && ctas * a.splits * 2 <= 2 * sm_count() && keys >= a.splits * 2 * kWarps * kBlock * 2) a.splits *= 2;
   if (c.type == kRowBF16) return c.D <= 64 ? launch<bf16, 64>(p, a, stream) : launch<bf16, 128>(p, a, stream);
   return c.D <= 64 ? launch<__half, 64>(p, a, stream) : launch<__half, 128>(p, a, stream);
 }

@@ -167,11 +167,14 @@ def check_qk_norm_rotary_support(q, k, q_weight, k_weight, frequencies, position
 # custom ops: what a traced graph holds.  An eager call on plain CUDA tensors goes to `_native.rotary`.
 # --------------------------------------------------------------------------------------
 def _refuse_op(named, qw, kw, turns, positions, magnitude, half, norm, eps, check_device):
-    res = _check(named, [("q_weight", qw), ("k_weight", kw)], turns, magnitude, positions, "half" if half else "interleaved", eps,
-                 check_device)
-    refuse("turbo_qk_norm_rotary" if norm else "turbo_rotary", res)
+    name = "turbo_qk_norm_rotary" if norm else "turbo_rotary"
+    check = lambda device: _check(named, [("q_weight", qw), ("k_weight", kw)], turns, magnitude, positions,  # noqa: E731
+                                  "half" if half else "interleaved", eps, device)
+    refuse(name, check(False))
     if positions is not None and (positions.dtype != torch.int64 or differs(positions.shape, tuple(named[0][1].shape[:-2]))):
-        refuse("turbo_rotary", SupportResult(False, "positions", "the operator takes INT64 positions of q's tokens"))
+        refuse(name, SupportResult(False, "positions", "the operator takes INT64 positions of q's tokens"))
+    if check_device:
+        refuse(name, check(True))
 
 
 @torch.library.custom_op("tpf_b200::rotary_fwd", mutates_args=())
@@ -200,11 +203,11 @@ def _refuse_bwd(dq, dk, q, k, qw, kw, turns, positions, magnitude, half, norm, e
     named = [(n, t) for n, t in (("dq", dq), ("dk", dk)) if t is not None]
     if not named:
         refuse("rotary backward", SupportResult(False, "d_out", "a gradient is needed"))
-    _refuse_op(named, qw, kw, turns, positions, magnitude, half, norm, eps, check_device)
     for d, x in ((dq, q), (dk, k)):
         if norm and d is not None and (x is None or x.dtype != d.dtype or differs(x.shape, tuple(d.shape))
                                        or x.device != d.device):
             refuse("rotary backward", SupportResult(False, "x_shape", "x does not belong to this gradient"))
+    _refuse_op(named, qw, kw, turns, positions, magnitude, half, norm, eps, check_device)
 
 
 @_rotary_bwd.register_fake

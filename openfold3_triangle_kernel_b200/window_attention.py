@@ -96,11 +96,14 @@ def check_window_attention_support(q, k, v, *, window, sinks=0, query_offset=0, 
 # --------------------------------------------------------------------------------------
 def _refuse_op(q, k, v, offsets, lengths, offset, left, right, sinks, scale, check_device):
     reach = lambda n: None if n < 0 else n  # noqa: E731
-    refuse("turbo_window_attention", check_window_attention_support(
+    check = lambda device: check_window_attention_support(  # noqa: E731
         q, k, v, window=(reach(left), reach(right)), sinks=sinks, query_offset=offset if offsets is None else offsets,
-        key_lengths=lengths, scale=scale, check_device=check_device))
+        key_lengths=lengths, scale=scale, check_device=device)
+    refuse("turbo_window_attention", check(False))
     if any(t is not None and t.dtype != torch.int32 for t in (offsets, lengths)):
         refuse("turbo_window_attention", SupportResult(False, "key_lengths", "the operator takes INT32 offsets and lengths"))
+    if check_device:
+        refuse("turbo_window_attention", check(True))
 
 
 @torch.library.custom_op("tpf_b200::window_attn_fwd", mutates_args=())
@@ -129,11 +132,13 @@ def _window_bwd(d_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.
 
 
 def _refuse_bwd(d_out, q, k, v, out, lse, offsets, lengths, offset, left, right, sinks, scale, check_device):
-    _refuse_op(q, k, v, offsets, lengths, offset, left, right, sinks, scale, check_device)
+    _refuse_op(q, k, v, offsets, lengths, offset, left, right, sinks, scale, False)
     if any(t.dtype != q.dtype or t.device != q.device or differs(t.shape, tuple(q.shape)) for t in (d_out, out)):
         refuse("window attention backward", SupportResult(False, "out", "the output and its gradient must be as q"))
     if lse.dtype != torch.float32 or lse.device != q.device or differs(lse.shape, (*q.shape[:-3], q.shape[-2], q.shape[-3])):
         refuse("window attention backward", SupportResult(False, "lse", "the log-sum-exp must be FP32 [*,H,N]"))
+    if check_device:
+        _refuse_op(q, k, v, offsets, lengths, offset, left, right, sinks, scale, True)
 
 
 @_window_bwd.register_fake
