@@ -58,8 +58,13 @@ int window_attn_fwd(const WindowCall& c, cudaStream_t stream) {
   if (int rc = make_params(&p, c, "window_attn_fwd")) return rc;
   if (c.B == 0 || c.N == 0) return TPF_OK;
   if (int rc = check_inputs(c, "window_attn_fwd")) return rc;
-  // A CTA of the one kernel has 128 queries of a head, of the other 16 of all heads that share a key head.
-  return c.M > 0 && c.N >= 64 ? window_many(c, p, stream) : window_few(c, p, stream);
+  // A CTA of the one kernel has 16 rows, queries times heads of a group, of the other 128 queries of a head.  The first is quicker while
+  // its CTAs find an SM each, and beyond that where there are fewer of them by a quarter.  (Heads 32 on 8 of 128 elements, window 1024,
+  // us, few / many: 8 sequences of 8 queries 17 / 20, of 16 26 / 20, of 64 95 / 20; one sequence of 32 12 / 16, of 128 26 / 18; 64
+  // single queries 53 / more than 150.)
+  const int64_t few = c.B * c.HK * ((c.N * p.G + 15) / 16), many = c.B * c.H * ((c.N + 127) / 128);
+  if (c.M > 0 && few > sm_count() && 4 * few > 3 * many) return window_many(c, p, stream);
+  return window_few(c, p, stream);
 }
 
 int64_t window_attn_bwd_workspace_bytes(const WindowCall& c) {

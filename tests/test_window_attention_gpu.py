@@ -56,23 +56,25 @@ WINDOWS = [((None, 0), 0), ((0, 0), 0), ((5, 0), 2), ((63, 0), 0), ((64, 0), 1),
            ((None, None), 0), ((None, 5), 0), ((9, None), 5), ((200, 0), 17), ((130, 130), 33)]
 
 
+# one sequence, and enough of them for the kernel of many queries
 @pytest.mark.parametrize("window, sinks", WINDOWS)
 @pytest.mark.parametrize("n", [1, 63, 64, 65, 130, 300])
-def test_windows(window, sinks, n):
-    _check(*_inputs(1, n, n, 2, 1, 64, seed=n), window, sinks)
+@pytest.mark.parametrize("B, H", [(1, 2), (40, 6)])
+def test_windows(window, sinks, n, B, H):
+    _check(*_inputs(B, n, n, H, H // 2, 64, seed=n), window, sinks)
 
 
 @pytest.mark.parametrize("D", [8, 16, 24, 32, 40, 64, 72, 80, 96, 104, 120, 128])
 @pytest.mark.parametrize("dtype", [BF, FP16])
-@pytest.mark.parametrize("n", [20, 200])
-def test_head_sizes(D, dtype, n):
-    _check(*_inputs(2, n, n, 4, 2, D, dtype, seed=D), (50, 0), 3)
+@pytest.mark.parametrize("B, n", [(2, 20), (2, 200), (40, 200)])
+def test_head_sizes(D, dtype, B, n):
+    _check(*_inputs(B, n, n, 4, 2, D, dtype, seed=D), (50, 0), 3)
 
 
 @pytest.mark.parametrize("H, HK", [(1, 1), (3, 1), (4, 4), (8, 2), (16, 1), (24, 3), (40, 2)])
-@pytest.mark.parametrize("n", [5, 129])
-def test_shared_key_heads(H, HK, n):
-    _check(*_inputs(2, n, n, H, HK, 32, seed=H), (40, 10), 2)
+@pytest.mark.parametrize("B, n", [(2, 5), (2, 129), (40, 129)])
+def test_shared_key_heads(H, HK, B, n):
+    _check(*_inputs(B, n, n, H, HK, 32, seed=H), (40, 10), 2)
 
 
 @pytest.mark.parametrize("n", [1, 2, 5, 17])
@@ -90,27 +92,26 @@ def test_one_token(B, H, HK, M):
         _check(*_inputs(B, 1, M, H, HK, 64, seed=M), window, 4, [x - 1 for x in lengths], lengths, train=False)
 
 
-@pytest.mark.parametrize("n", [3, 100])
-def test_rows_that_see_nothing(n):
+@pytest.mark.parametrize("times, n", [(1, 3), (1, 100), (10, 100)])
+def test_rows_that_see_nothing(times, n):
     """Empty sequences, queries before the first key and behind the window."""
-    B = 5
-    q, k, v = _inputs(B, n, 150, 4, 2, 64)
-    _check(q, k, v, (10, 0), 0, [0, -n, 400, -5, 149], [0, 150, 150, 150, 150])
-    _check(q, k, v, (10, 0), 2, [0, -n, 400, -5, 149], [0, 150, 150, 150, 1])
-    _check(q, k, v, (0, 3), 64, [-200, 2 ** 29, -2 ** 29, 60, 70], [150, 150, 150, 64, 65])
+    q, k, v = _inputs(5 * times, n, 150, 4, 2, 64)
+    _check(q, k, v, (10, 0), 0, [0, -n, 400, -5, 149] * times, [0, 150, 150, 150, 150] * times)
+    _check(q, k, v, (10, 0), 2, [0, -n, 400, -5, 149] * times, [0, 150, 150, 150, 1] * times)
+    _check(q, k, v, (0, 3), 64, [-200, 2 ** 29, -2 ** 29, 60, 70] * times, [150, 150, 150, 64, 65] * times)
 
 
-@pytest.mark.parametrize("n", [70, 257])
+@pytest.mark.parametrize("times, n", [(1, 70), (1, 257), (8, 257)])
 @pytest.mark.parametrize("window, sinks", [((30, 0), 1), ((64, 64), 0), ((None, 0), 0), ((128, 128), 20)])
-def test_padded_batches(n, window, sinks):
-    _check(*_inputs(4, n, n, 4, 2, 64, seed=n), window, sinks, 0, [n, n - 1, 64, 1])
+def test_padded_batches(times, n, window, sinks):
+    _check(*_inputs(4 * times, n, n, 4, 2, 64, seed=n), window, sinks, 0, [n, n - 1, 64, 1] * times)
 
 
-@pytest.mark.parametrize("n", [1, 90])
+@pytest.mark.parametrize("times, n", [(1, 1), (1, 90), (10, 90)])
 @pytest.mark.parametrize("value", [math.nan, math.inf])
-def test_what_lies_behind_the_last_key_does_not_count(n, value):
-    q, k, v = _inputs(3, n, 200, 4, 2, 64)
-    lengths = [200, 131, 7]
+def test_what_lies_behind_the_last_key_does_not_count(times, n, value):
+    q, k, v = _inputs(3 * times, n, 200, 4, 2, 64)
+    lengths = [200, 131, 7] * times
     for b, x in enumerate(lengths):
         k[b, x:] = value
         v[b, x:] = value
@@ -118,10 +119,10 @@ def test_what_lies_behind_the_last_key_does_not_count(n, value):
     _check(q, k, v, (None, None), 0, 0, lengths)
 
 
-@pytest.mark.parametrize("n", [4, 200])
-def test_large_logits(n):
+@pytest.mark.parametrize("B, n", [(1, 4), (1, 200), (20, 200)])
+def test_large_logits(B, n):
     """Maxima that rise from tile to tile, and a scale that makes them far apart."""
-    q, k, v = _inputs(1, n, n, 2, 2, 64)
+    q, k, v = _inputs(B, n, n, 2, 2, 64)
     k = (k.float() * torch.linspace(0.1, 8, n, device="cuda")[None, :, None, None]).to(BF)
     _check(q, k, v, (None, None), 0, scale=0.25)
     _check(q, (k.float() * 0).to(BF), v, (50, 50), 2)
@@ -130,7 +131,7 @@ def test_large_logits(n):
     assert torch.isfinite(big).all()
 
 
-@pytest.mark.parametrize("n", [1, 33, 200])
+@pytest.mark.parametrize("n", [1, 33, 200, 500])
 def test_strides(n):
     """Slices of a stacked projection, head-major tensors, expanded batches, odd pitches and starts."""
     s = _rn(2, n, 8 + 2 + 2, 64, seed=n)
@@ -188,7 +189,7 @@ def test_a_cache_beyond_2_31_elements():
     k = torch.zeros(B, M, HK, D, device="cuda", dtype=BF)
     v = torch.zeros(B, M, HK, D, device="cuda", dtype=BF)
     k[-1], v[-1] = _rn(M, HK, D, seed=1), _rn(M, HK, D, seed=2)
-    for n in (1, 80):
+    for n in (1, 160):
         q = _rn(B, n, 16, D, seed=3)
         out = tk.turbo_window_attention(q, k, v, window=(500, 0), sinks=4, query_offset=M - n)
         ref = so.window_attention(q[-1:], k[-1:], v[-1:], (500, 0), 4, [M - n])
