@@ -1,5 +1,6 @@
 // Dropout, the position rotation of heads and the window attention for eager CUDA tensors.
 #include <cmath>
+#include <limits>
 
 #include "tpf_dropout.h"
 #include "tpf_rotary.h"
@@ -121,7 +122,8 @@ struct DropoutFn : public torch::autograd::Function<DropoutFn> {
     const std::vector<int64_t> v = ctx->saved_data["a"].toIntVector();
     const DropoutArgs a{ctx->get_saved_variables()[0], v[0], v[1], v[2], v[3]};
     if (ctx->needs_input_grad(0)) r[0] = dropout_out(grads[0].detach(), Tensor(), a);
-    if (v[4]) r[1] = grads[0].detach();
+    // (the very tensor: a view of it would hide from whoever accumulates gradients that others hold it, too)
+    if (v[4]) r[1] = grads[0];
     return r;
   }
 };
@@ -368,7 +370,8 @@ struct WindowFn : public torch::autograd::Function<WindowFn> {
     const WindowArgs a{s[5], s[6], (int64_t)v[0], (int64_t)v[1], (int64_t)v[2], (int64_t)v[3], v[4]};
     const bool need_kv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
     const variable_list g = window_grads(dense(grads[0]), as_heads(s[0].detach(), true), as_heads(s[1].detach(), true),
-                                         as_heads(s[2].detach(), true), s[3], s[4], a, ctx->needs_input_grad(0), need_kv);
+                                         as_heads(s[2].detach(), true), dense(s[3]), s[4].contiguous(), a, ctx->needs_input_grad(0),
+                                         need_kv);
     for (int i = 0; i < 3; ++i)
       if (ctx->needs_input_grad(i)) r[i] = g[i];
     return r;
@@ -423,7 +426,9 @@ py::object py_rotary(py::handle hq, py::handle hk, py::handle hqw, py::handle hk
     return py::none();
   const int64_t D = q.size(-1);
   if (k.defined() && (!heads_ok(k, q) || !same_but(k, q, 2))) return py::none();
-  if (!weight_ok(qw, q) || !weight_ok(kw, q) || D < 2 || D > 256 || !(eps >= 0)) return py::none();
+  if (!weight_ok(qw, q) || !weight_ok(kw, q) || D < 2 || D > 256 || !(eps >= 0) ||
+      !(std::abs(magnitude) <= std::numeric_limits<float>::max()))
+    return py::none();
   if (!plain_cuda(turns) || turns.device() != q.device() || turns.scalar_type() != at::kLong || turns.dim() != 1 ||
       !turns.is_contiguous() || turns.size(0) < 1 || 2 * turns.size(0) > D)
     return py::none();

@@ -142,6 +142,8 @@ def _check(named, weights, turns, magnitude, positions, layout, eps, check_devic
 def _parts(frequencies, positions):
     """``(turns, magnitude, positions tensor or None, first position)``."""
     turns, magnitude = frequencies if isinstance(frequencies, tuple) and len(frequencies) == 2 else (None, 1.0)
+    if not isinstance(magnitude, (int, float)):
+        turns = None
     if positions is None:
         return turns, magnitude, None, 0
     if isinstance(positions, (int, torch.SymInt)) and not isinstance(positions, bool) and -2 ** 62 <= positions <= 2 ** 62:

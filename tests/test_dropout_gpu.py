@@ -211,6 +211,29 @@ def test_gradients_are_first_order():
         g.sum().backward()
 
 
+def test_leaves_do_not_share_a_gradient():
+    x, r, w = (torch.randn(64, device="cuda").requires_grad_(True) for _ in range(3))
+    d = torch.randn(64, device="cuda")
+    tk.turbo_dropout(x, 0.5, 1, residual=r).backward(d)
+    assert len({t.data_ptr() for t in (x.grad, r.grad, d)}) == 3
+    x.grad = r.grad = None
+    ((tk.turbo_dropout(x, 0.5, 1, residual=r) + w) * 2.0).backward(d)
+    assert len({t.data_ptr() for t in (x.grad, r.grad, w.grad, d)}) == 4
+    assert torch.equal(r.grad, 2 * d) and torch.equal(w.grad, 2 * d)
+
+
+def test_one_tensor_as_both():
+    x = _rn(3, 40, seed=4).cuda().requires_grad_(True)
+    d = _rn(3, 40, seed=5).cuda()
+    kept = so.dropout_mask(x.shape, 0.25, 1).cuda()
+    out = tk.turbo_dropout(x, 0.25, 1, residual=x)
+    # two fp32 roundings of the forward, three of the gradient and its sum
+    expected = lambda t: t.double() + torch.where(kept, t.double() / 0.75, 0.0)  # noqa: E731
+    assert ((out.double() - expected(x.detach())).abs() <= 4 * 2.0 ** -24 * expected(x.detach()).abs()).all()
+    g, = torch.autograd.grad(out, x, d)
+    assert ((g.double() - expected(d)).abs() <= 4 * 2.0 ** -24 * expected(d).abs()).all()
+
+
 @pytest.mark.parametrize("seed", [17, (17, 2), "tensor"])
 def test_pair_block_trains_with_dropout(seed):
     """The block with dropout is its four updates, each dropped with the mask of its site and added."""

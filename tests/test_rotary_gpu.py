@@ -166,6 +166,26 @@ def test_nothing():
     assert (w.grad == 0).all()
 
 
+def test_keys_without_heads():
+    q, k = _rn(2, 9, 4, 64).requires_grad_(True), _rn(2, 9, 0, 64).requires_grad_(True)
+    qw, kw = (_rn(64, seed=2) + 1).requires_grad_(True), (_rn(64, seed=3) + 1).requires_grad_(True)
+    fill = [torch.full((1 << 18,), float("nan"), device="cuda") for _ in range(4)]   # what workspaces then hold
+    del fill
+    a, b = tk.turbo_qk_norm_rotary(q, k, qw, kw, _freq(64))
+    g = torch.autograd.grad([a, b], [q, k, qw, kw], [torch.ones_like(a), torch.ones_like(b)])
+    assert torch.equal(g[3], torch.zeros_like(kw)) and g[1].shape == k.shape and g[2].isfinite().all()
+
+
+def test_magnitudes_that_are_no_numbers_are_refused():
+    x = _rn(1, 3, 2, 64)
+    for magnitude in (float("nan"), float("inf"), 1e300, "one", torch.ones((), device="cuda")):
+        f = tk.RotaryFrequencies(_freq(64).turns, magnitude)
+        with pytest.raises(ValueError, match="frequencies"):
+            tk.turbo_rotary(x, f)
+        with pytest.raises(ValueError, match="frequencies"):
+            tk.turbo_qk_norm_rotary(x, x, None, None, f)
+
+
 def test_one_output_used():
     """A gradient that never came counts as zeros."""
     q, k = _rn(1, 9, 4, 64).requires_grad_(True), _rn(1, 9, 2, 64, seed=1).requires_grad_(True)

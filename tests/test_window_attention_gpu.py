@@ -286,6 +286,55 @@ def test_some_gradients_only_and_no_second_ones():
         g.float().sum().backward()
 
 
+def test_gradients_from_packed_activations():
+    """Inside `int8_activations` the backward pass runs on what the format holds of q, k, v and the output."""
+    leaves = [t.requires_grad_(True) for t in _inputs(2, 300, 300, 8, 2, 64)]
+    q, k, v = (t * 1 for t in leaves)
+    d = _rn(2, 300, 8, 64, seed=3)
+    with tk.int8_activations(min_elements=1):
+        out, lse = tk.turbo_window_attention(q, k, v, window=(50, 0), sinks=2, return_lse=True)
+    back = [tk.unpack_activation(*tk.pack_activation(t.detach().view(-1, 128)), t.dtype).view(t.shape) for t in (q, k, v, out)]
+    got = torch.autograd.grad(out, leaves, d)
+    want = torch.ops.tpf_b200.window_attn_bwd(d, *back, lse, None, None, 0, 50, 0, 2, 64 ** -0.5)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_saved_tensors_of_other_layouts():
+    """A hook of the caller's may hand back any strides."""
+    q, k, v = (t.requires_grad_(True) for t in _inputs(2, 100, 100, 4, 2, 64))
+    d = _rn(2, 100, 4, 64, seed=3)
+    ref = torch.autograd.grad(tk.turbo_window_attention(q, k, v, window=(50, 0)), [q, k, v], d)
+    turned = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1) if t.ndim > 1 else t  # noqa: E731
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), turned):
+        out = tk.turbo_window_attention(q, k, v, window=(50, 0))
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, [q, k, v], d), ref))
+
+
+def test_threads_at_once():
+    import threading
+    ins = [_inputs(2, 500, 500, 4, 2, 64, seed=s) for s in (0, 10)]
+    d = _rn(2, 500, 4, 64, seed=3)
+
+    def step(t):
+        leaves = [x.detach().requires_grad_(True) for x in t]
+        out = tk.turbo_window_attention(*leaves, window=(100, 0), sinks=4)
+        return [out.detach(), *torch.autograd.grad(out, leaves, d)]
+
+    expected = [step(t) for t in ins]
+    torch.cuda.synchronize()
+    results = [None, None]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            results[i] = [step(ins[i]) for _ in range(20)]
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert all(torch.equal(a, b) for i in range(2) for r in results[i] for a, b in zip(r, expected[i]))
+
+
 def test_a_layer_of_them():
     """What a sequence layer does: stacked projection, norm and rotation, attention, projection, dropout with the residual."""
     g = torch.Generator(device="cuda").manual_seed(0)
