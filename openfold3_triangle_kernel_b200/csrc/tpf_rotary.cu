@@ -11,7 +11,7 @@
 // Mapping: a block has a stretch of tokens, as long as any other block's.  It makes their sines and cosines, in shared memory, and goes
 // through the heads of q and then through those of k: a team of TL lanes has a few of them in succession, loaded two ahead.  With the
 // sines as registers of each team they were made several times over, and took the place of loads in flight (8192 tokens, 32 + 8
-// heads of 128, bf16, forward and backward: 44 and 75 us).  A lane holds two pieces of eight elements, in the half order the two that are
+// heads of 128, bf16, with norms, forward and backward: 44 and 75 us, now 36 and 51; 32 heads without norms 32, now 23).  A lane holds two pieces of eight elements, in the half order the two that are
 // rotated into one another, so nothing is exchanged.
 // What bounds it: memory (the smallest calls: the launch).
 // Halves that no piece of eight fits pass partners through shared memory; head sizes that are no multiple of eight and misaligned
@@ -467,7 +467,7 @@ int launch(const RotaryCall& c, RotaryParams& p, bool vec, bool back, cudaStream
   return launch<T, 8, 16>(c, p, back, stream);
 }
 
-int run(const RotaryCall& c, void* workspace, int64_t workspace_bytes, bool back, cudaStream_t stream) {
+int run(RotaryCall c, void* workspace, int64_t workspace_bytes, bool back, cudaStream_t stream) {
   const char* who = back ? "rotary_bwd" : "rotary_fwd";
   TPF_REQUIRE(row_type_ok(c.type), TPF_ERR_INVALID_ARGUMENT, "%s: unknown element type %d", who, c.type);
   TPF_REQUIRE(c.batch >= 0 && c.tokens >= 0 && c.t[0].heads >= 0 && c.t[1].heads >= 0, TPF_ERR_INVALID_ARGUMENT,
@@ -505,7 +505,12 @@ int run(const RotaryCall& c, void* workspace, int64_t workspace_bytes, bool back
     const RotaryTensor& s = c.t[k];
     RotaryParams::Tensor& t = p.t[k];
     t.heads = (int)s.heads;
-    if (s.heads == 0) continue;
+    if (s.heads == 0) {
+      if (s.dweight != nullptr)
+        TPF_CUDA_OK(cudaMemsetAsync(s.dweight, 0, (size_t)c.dim * row_type_size(s.weight_type), stream));
+      c.t[k].dweight = nullptr;
+      continue;
+    }
     TPF_REQUIRE(c.batch * c.tokens * s.heads < (1ll << 31), TPF_ERR_UNSUPPORTED, "%s: too many heads", who);
     const bool reads_x = !back || c.norm;
     TPF_REQUIRE((s.x != nullptr || !reads_x) && s.out != nullptr && (s.dy != nullptr || !back), TPF_ERR_INVALID_ARGUMENT,

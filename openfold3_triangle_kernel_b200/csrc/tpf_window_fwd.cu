@@ -6,7 +6,11 @@
 // Two CTAs share an SM, so that one computes exponentials while the other's products run.
 // Tiles that every query of a warp sees whole take a way without masks.  The sinks, when they lie before the window, are a
 // tile of their own, of as many steps of 16 keys as there are sinks.
-// What bounds it: at 128 elements a head the products (512 cycles a tile) and the exponentials (16 a clock and SM, 512 cycles) alike.
+// What bounds it at 128 elements a head: the tensor pipe.  S = Q K^T is made 64 columns at a time, of 6 KB from shared memory, 48
+// cycles for 32 cycles of products, so a tile takes it 640 cycles; the two CTAs of an SM need 1600 for a tile each, which leaves it
+// 80 % busy.  The exponentials (16 a clock and SM) are 1024 of them, beside the products.
+// Measured (B200, bf16, 32 heads on 8 of 128, 8192 queries, window 1024, 4 sinks): 154 us, 0.84 PFLOP/s.  Tiles of 128 keys with one S at a
+// time (187 us), two threads a row (188), a part of the exponentials as polynomials (160) and a persistent walk (154) gained nothing.
 #include "tpf_window_kernels.h"
 
 namespace tpf {
