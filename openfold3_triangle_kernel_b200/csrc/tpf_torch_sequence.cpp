@@ -81,7 +81,7 @@ bool dropout_layout(const Tensor& x, const Tensor& residual, int64_t shared, tpf
     c.out_strides[i] = order[i].o;
   }
   c.sizes[3] = inner;
-  c.shared = shared >= 0;
+  c.shared = s.shared;  // (not where the shared dimension is a single element, whose place another one may have taken)
   return true;
 }
 

@@ -74,6 +74,16 @@ def test_strides(shared, cols):
     _check(one.contiguous(), shared=shared, x_cuda=x[:, :1].cuda().expand(2, 10, 12, cols))
 
 
+@pytest.mark.parametrize("shape, shared, order", [((8, 1, 2, 2, 3), 1, (2, 0, 3, 1, 4)), ((17, 1, 8, 5, 16), 1, (3, 2, 0, 1, 4)),
+                                                  ((1, 2, 3, 40, 16), 0, (3, 2, 1, 0, 4)), ((2, 8, 1, 17, 3), -3, (3, 1, 0, 2, 4))])
+def test_a_shared_dimension_of_one_element(shape, shared, order):
+    """Among dimensions that do not lie one behind the other."""
+    back = [order.index(i) for i in range(5)]
+    x = _rn(*shape, seed=1)
+    _check(x, shared=shared, x_cuda=x.permute(order).contiguous().cuda().permute(back))
+    _check(x, shared=None, x_cuda=x.permute(order).contiguous().cuda().permute(back))
+
+
 @pytest.mark.parametrize("p", [0.0, 1e-6, 0.1, 1 / 3, 0.9999, 1.0])
 def test_probabilities(p):
     _check(_rn(3, 1000, seed=5).bfloat16(), p=p, residual=_rn(3, 1000, seed=6).bfloat16())
@@ -168,6 +178,24 @@ def test_captured_replays_read_the_seed():
         expected = step()
         assert torch.equal(out, expected[0]) and torch.equal(grad, expected[1])
         assert not torch.equal(out, r)
+
+
+def test_captured_replays_draw_new_seeds():
+    x = torch.ones(1 << 14, device="cuda", requires_grad=True)
+
+    def step():
+        out = tk.turbo_dropout(x, 0.5)
+        return out.detach(), torch.autograd.grad(out, x, torch.ones_like(x))[0]
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, g = step()
+    seen = []
+    for _ in range(3):
+        graph.replay()
+        assert torch.equal(out, g) and not any(torch.equal(out, s) for s in seen)
+        seen.append(out.clone())
 
 
 def test_a_changed_seed_is_noticed():
