@@ -17,7 +17,7 @@ Operator contract:
   fp32.  The same inputs give the same bits.
 
 A single token over its cache is ``N = 1`` with ``query_offset = key_lengths - 1``.  Probabilities and their gradients are rounded
-to q's type as operands of the products; sums and the softmax are fp32.  A key or value inside the sequence that is infinite or NaN
+to q's type as operands of the products; sums and the softmax are fp32 (a probability below 2^-126 is zero).  A key or value inside the sequence that is infinite or NaN
 reaches every query whose 128 neighbours see it, as a product of zero with it does elsewhere.
 
 Unsupported inputs raise ``ValueError("turbo_window_attention unsupported [code]: reason")``, in a traced call when it is traced or,

@@ -151,7 +151,8 @@ def window_attention(q, k, v, window, sinks=0, offsets=None, lengths=None, scale
 
     e: half a step of the type, once for P (and dS) as an operand.  A logit is off by D roundings of its products' magnitudes (the order
     of a product's sum is not known) and 3 of its own, and an exponential by 2^-22; a row's probabilities are off by twice the
-    largest of these, with the sum's 64 roundings.
+    largest of these, with the sum's 64 roundings.  An exponential below 2^-126 is zero in fp32 without subnormal numbers, which its
+    product with dP - delta (or dO), of any size, shows.
     """
     B, N, H, D = q.shape
     M, HK = k.shape[1:3]
@@ -184,10 +185,11 @@ def window_attention(q, k, v, window, sinks=0, offsets=None, lengths=None, scale
     rel = rel + 4 * U * torch.where(lse == -math.inf, 0.0, lse).abs()[..., None]
     dp_off = (g.abs() @ v.abs().transpose(-1, -2)) * D * U
     delta_off = (g.abs() * (e * out.abs() + (1 + e) * out_off + D * U * out.abs())).sum(-1, keepdim=True)
-    ds_off = p * (dp_off + delta_off) + ds.abs() * (e + rel + 4 * U)
+    least = torch.where(ok, 2.0 ** -126, 0.0)
+    ds_off = p * (dp_off + delta_off) + ds.abs() * (e + rel + 4 * U) + least * (dp - delta).abs()
     fold = lambda t: back(t.unflatten(1, (HK, H // HK)).sum(2))  # noqa: E731
     sums = 512 * U     # of a gradient over the rows of its tiles
     res.update(dq=back(ds @ k) * scale, dq_off=back((ds_off + sums * ds.abs()) @ k.abs()) * scale,
                dk=fold(ds.transpose(-1, -2) @ q) * scale, dk_off=fold((ds_off + sums * ds.abs()).transpose(-1, -2) @ q.abs()) * scale,
-               dv=fold(p.transpose(-1, -2) @ g), dv_off=fold((p * (e + rel + sums)).transpose(-1, -2) @ g.abs()))
+               dv=fold(p.transpose(-1, -2) @ g), dv_off=fold((p * (e + rel + sums) + least).transpose(-1, -2) @ g.abs()))
     return res
