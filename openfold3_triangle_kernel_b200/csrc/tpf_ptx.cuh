@@ -229,6 +229,15 @@ __device__ __forceinline__ void tma_store_3d(uint32_t elected, const CUtensorMap
       ::"l"(map), "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(elected)
       : "memory");
 }
+__device__ __forceinline__ void tma_store_4d(uint32_t elected, const CUtensorMap* map, const void* src, int c0, int c1, int c2,
+                                             int c3) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "@q cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];\n\t"
+      "@q cp.async.bulk.commit_group;\n\t}"
+      ::"l"(map), "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(elected)
+      : "memory");
+}
 __device__ __forceinline__ void tma_store_5d(uint32_t elected, const CUtensorMap* map, const void* src, int c0, int c1,
                                              int c2, int c3, int c4) {
   asm volatile(

@@ -81,8 +81,8 @@ struct BwdArgs {
   void *g1, *g2;               // KEYS: dV and dK; else dQ and nothing
   float* parts;                // KEYS: [B, HK, 1 + far][2][sinks][D] of the sinks' rows, or nullptr
   int key_tiles, far, far_tiles;  // KEYS: items of far queries (of a head), and query tiles of each
-  int row_items, heads, items;    // items: (128 rows, head, sequence), the rows fastest
-  FastDiv div_rows, div_heads, div_g;
+  int row_items, heads, lists, items;    // items: (head, sequence, 128 rows), the heads fastest
+  FastDiv div_heads, div_lists, div_g;  // (lists: heads of all sequences)
 };
 
 template <typename T_, int DP_, bool KEYS_>
@@ -112,6 +112,17 @@ __device__ __forceinline__ void bulk_load(uint32_t elected, void* dst, const voi
       : "memory");
 }
 
+// The items of a CTA: one of every gridDim.x, from the front and from the back of them in turn, so that with the longest items first the
+// CTAs get like sums.  (One stride for all: 8192 queries, causal, 16 heads on 4 of 128: 1090 us, now 770.)
+struct BwdWalk {
+  int item, step;
+  __device__ __forceinline__ BwdWalk() : item(blockIdx.x), step(2 * (gridDim.x - 1 - blockIdx.x) + 1) {}
+  __device__ __forceinline__ void next() {
+    item += step;
+    step = 2 * gridDim.x - step;
+  }
+};
+
 // An item and its column tiles: for each of `heads` heads [a tile of the sinks,] tiles lo .. hi - 1.
 template <bool KEYS>
 struct BwdItem {
@@ -119,10 +130,11 @@ struct BwdItem {
   int part;                   // KEYS: 0, or 1 + the number of far queries' item
   int extra, lo, heads, per_head, tiles;
   __device__ __forceinline__ BwdItem(int item, const WindowParams& p, const BwdArgs& a) {
-    const uint32_t r = a.div_rows.div((uint32_t)item);
-    const int x = item - (int)r * a.row_items;
-    b = (int)a.div_heads.div(r);
-    head = (int)r - b * a.heads;
+    const int turn = (int)a.div_lists.div((uint32_t)item), list = item - turn * a.lists;
+    b = (int)a.div_heads.div((uint32_t)list);
+    head = list - b * a.heads;
+    // the longest items first: the first keys, or the last queries, where the window is longer on the left
+    const int x = (p.left > p.right) == KEYS ? turn : a.row_items - 1 - turn;
     len = p.length(b), off = p.first_position(b);
     part = KEYS && x >= a.key_tiles ? x - a.key_tiles + 1 : 0;
     r0 = part > 0 ? 0 : x * 128;
@@ -210,8 +222,8 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
     const uint32_t el = elect_one();
     int s = 0, rs = 0;
     uint32_t ph = 1, rph = 1;
-    for (int item = blockIdx.x; item < a.items; item += gridDim.x) {
-      const BwdItem<KEYS> it(item, p, a);
+    for (BwdWalk walk; walk.item < a.items; walk.next()) {
+      const BwdItem<KEYS> it(walk.item, p, a);
       if (it.tiles == 0) continue;
       warp_wait(&r_empty[rs], rph, wctx);
       mbar_expect_tx(el, &r_full[rs], 2 * Cfg::R_TILE);
@@ -276,19 +288,20 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
       umma_commit(el, &r_empty[rs]);
       if (++rs == NR) rs = 0, rph ^= 1;
     };
-    auto tiles_from = [&](int& item) {  // of the next item that has any
+    auto tiles_from = [&](BwdWalk& w) {  // of the next item that has any
       int n = 0;
-      while (item < a.items && (n = BwdItem<KEYS>(item, p, a).tiles) == 0) item += gridDim.x;
+      while (w.item < a.items && (n = BwdItem<KEYS>(w.item, p, a).tiles) == 0) w.next();
       return __shfl_sync(0xffffffffu, n, 0);
     };
-    int item = blockIdx.x, buf = 0, lead = 0;  // lead: tiles of the item whose S and dP were made while the one before was finished
-    int tiles = tiles_from(item);
-    while (item < a.items) {
+    BwdWalk walk;
+    int buf = 0, lead = 0;  // lead: tiles of the item whose S and dP were made while the one before was finished
+    int tiles = tiles_from(walk);
+    while (walk.item < a.items) {
       if (lead == 0) warp_wait(&r_full[rs], rph, wctx);
       for (; lead < 2 && lead < tiles; ++lead) issue_sdp((buf + lead) & 1);
       if (tiles <= 2) rows_used();
-      int next = item + gridDim.x;
-      const int next_tiles = tiles_from(next);
+      walk.next();
+      const int next_tiles = tiles_from(walk);
       lead = 0;
       for (int t = 0; t < tiles; ++t) {
         if (t == 0) warp_wait2(&pds_ready[buf], pph, &acc_free[ab], aph, wctx);
@@ -321,7 +334,6 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
         pph ^= buf ^ 1;
       }
       if (++ab == NACC) ab = 0, aph ^= 1;
-      item = next;
       tiles = next_tiles;
     }
   } else {
@@ -385,8 +397,8 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
     int turn = g;   // tiles until the group's next one
     int s = 0;      // stage of the item's first tile
     uint32_t ph = 0;
-    for (int item = blockIdx.x; item < a.items; item += gridDim.x) {
-      const BwdItem<KEYS> it(item, p, a);
+    for (BwdWalk walk; walk.item < a.items; walk.next()) {
+      const BwdItem<KEYS> it(walk.item, p, a);
       const int mine = it.r0 + row;
       if (it.tiles == 0) {
         if (pending) finish();
@@ -554,7 +566,9 @@ int launch(const CUtensorMap& r1, const CUtensorMap& r2, const CUtensorMap& c1, 
   const int64_t items = (int64_t)a.row_items * a.heads * c.B;
   TPF_REQUIRE(items < (1ll << 31) - 65536, TPF_ERR_UNSUPPORTED, "window_attn_bwd: too many rows");
   a.items = (int)items;
-  a.div_rows = FastDiv::make((uint32_t)a.row_items);
+  TPF_REQUIRE((int64_t)a.heads * c.B < (1ll << 31), TPF_ERR_UNSUPPORTED, "window_attn_bwd: too many heads");
+  a.lists = a.heads * (int)c.B;
+  a.div_lists = FastDiv::make((uint32_t)a.lists);
   a.div_heads = FastDiv::make((uint32_t)a.heads);
   a.div_g = FastDiv::make((uint32_t)p.G);
   const int grid = a.items < sm_count() ? a.items : sm_count();
