@@ -17,7 +17,8 @@
 //
 // What bounds it at 128 elements a head: the tensor pipe.  An UMMA of 64 columns with both operands in shared memory reads 6 KB, 48
 // cycles, for 32 cycles of products, which makes 1280 cycles a tile with the keys as rows and 1024 with the queries (1345 and 1127
-// measured without masks, starts and ends).  Q and dO as operands in TMEM were no faster (239 us for 224).
+// measured without masks, starts and ends).  Q and dO as operands in TMEM were no faster (239 us for 224),
+// nor were gradients that leave by TMA through the place of the item's rows (dQ 184 us for 186, at 64 elements a head 152 for 146).
 //
 // The sinks are seen by every later query, which would make the first keys' CTA walk over the whole sequence.  It does its window;
 // the queries beyond are split over CTAs of their own, whose sums of the sinks' rows a last kernel adds up in a fixed order.
@@ -41,36 +42,60 @@ constexpr int kTile = 64;  // columns of a tile
 
 // ---- stats ------------------------------------------------------------------------------------------------
 // [B, H, NP] of -lse log2(e) (-inf: the row sees nothing, or lies behind the last one) and of -delta.
-template <typename T>
+// A team of lanes, one for every eight elements of a head, has eight queries of a head (a query at a time it took 33 us at 8192 queries of
+// 32 heads of 128 and 31 at 64, now 26 and 14; the bytes are 20 and 10).
+template <typename T, int LANES>
 __global__ void __launch_bounds__(256) window_stats_kernel(const T* __restrict__ out, const T* __restrict__ d_out,
                                                            const float* __restrict__ lse, float* __restrict__ nlse,
-                                                           float* __restrict__ ndelta, int N, int NP, int H, int D, int64_t rows) {
+                                                           float* __restrict__ ndelta, int N, int NP, int H, int D, int64_t teams) {
   griddep_wait();
-  const int lane = threadIdx.x & 15;
-  const int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);  // (b, i of NP, h)
-  const int64_t bi = r / H;
-  const int h = (int)(r - bi * H);
-  const int64_t b = bi / NP;
-  const int i = (int)(bi - b * NP);
-  float s[1] = {0.f};
-  const bool on = r < rows && i < N;
-  if (on && lane * 8 < D) {
-    const int64_t at = ((b * N + i) * H + h) * D + lane * 8;
-    Piece<T, 8> x, y;
-    x.load(out + at);
-    y.load(d_out + at);
-    float u[8], v[8];
-    x.get(u);
-    y.get(v);
+  const int lane = threadIdx.x % LANES;
+  const int64_t team = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;  // (b, eight queries, h)
+  const int64_t bi = team / H;
+  const int h = (int)(team - bi * H);
+  const int64_t b = bi / (NP / 8);
+  const int i0 = (int)(bi - b * (NP / 8)) * 8;
+  const bool on = team < teams && lane * 8 < D;
+  const int64_t at = ((b * N + i0) * H + h) * D + lane * 8, pitch = (int64_t)H * D;
+  float s[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s[0] = fmaf(u[e], v[e], s[0]);
+  for (int half = 0; half < 8; half += 4) {
+    Piece<T, 8> x[4], y[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (on && i0 + half + k < N) {
+        x[k].load(out + at + (half + k) * pitch);
+        y[k].load(d_out + at + (half + k) * pitch);
+      } else {
+        x[k].zero();
+        y[k].zero();
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float u[8], v[8], t = 0.f;
+      x[k].get(u);
+      y[k].get(v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) t = fmaf(u[e], v[e], t);
+      s[half + k] = t;
+    }
   }
-  warp_sum(s, 16);
-  if (lane == 0 && r < rows) {
-    const int64_t at = (b * H + h) * NP + i;
-    const float l = on ? lse[(b * H + h) * N + i] : -INFINITY;
-    nlse[at] = l == -INFINITY ? -INFINITY : -l * kWindowLog2e;
-    ndelta[at] = -s[0];
+  // eight sums over the team: the lanes share the queries out while they add
+#pragma unroll
+  for (int n = 4; n > 0; n >>= 1)
+#pragma unroll
+    for (int k = 0; k < n; ++k) {
+      const bool upper = (lane & n) != 0;
+      s[k] = (upper ? s[k + n] : s[k]) + __shfl_xor_sync(0xffffffffu, upper ? s[k] : s[k + n], n);
+    }
+  if (LANES == 16) s[0] += __shfl_xor_sync(0xffffffffu, s[0], 8);
+  if (lane < 8 && team < teams) {
+    const int i = i0 + lane;
+    const int64_t to = (b * H + h) * NP + i;
+    const float l = i < N ? lse[(b * H + h) * N + i] : -INFINITY;
+    nlse[to] = l == -INFINITY ? -INFINITY : -l * kWindowLog2e;
+    ndelta[to] = -s[0];
   }
 }
 
@@ -591,9 +616,11 @@ int run(const WindowCall& c, const WindowParams& p, uint8_t* ws, cudaStream_t st
   float* ndelta = reinterpret_cast<float*>(ws + stat);
   a.nlse = nlse, a.ndelta = ndelta;
   a.NP = (int)NP;
-  const int64_t rows = c.B * NP * c.H;
-  launch_kernel(window_stats_kernel<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, stream, static_cast<const T*>(c.out),
-                static_cast<const T*>(c.d_out), c.lse, nlse, ndelta, (int)c.N, (int)NP, (int)c.H, (int)c.D, rows);
+  constexpr int LANES = DP / 8;
+  const int64_t teams = c.B * c.H * (NP / 8);
+  launch_kernel(window_stats_kernel<T, LANES>, dim3((unsigned)((teams + 256 / LANES - 1) / (256 / LANES))), dim3(256), 0, stream,
+                static_cast<const T*>(c.out), static_cast<const T*>(c.d_out), static_cast<const float*>(c.lse), nlse, ndelta, (int)c.N,
+                (int)NP, (int)c.H, (int)c.D, teams);
   TPF_LAUNCH_OK();
   const int64_t os[3] = {c.N * c.H * c.D, c.H * c.D, c.D};
   int rc;
