@@ -10,8 +10,8 @@
 //
 // An item is 128 rows (keys: K and V; queries: Q and dO), kept in shared memory while the CTA walks over their tiles of 64 columns.  S and
 // dP are made with the rows as TMEM lanes, so that P and dS, written over them as 16-bit numbers, are the A operands of the second
-// products straight from TMEM; a thread has a row.  Two groups of four warps take turns with the tiles: while one computes, the
-// products of the other run.  With the keys as rows the CTA goes through all query heads that share them.  The next item's rows are
+// products straight from TMEM; a thread has a row.  Two groups of four warps take turns with the tiles, three where heads of 64 elements
+// leave room for a third S and dP in TMEM: while one computes, the products of the others run.  With the keys as rows the CTA goes through all query heads that share them.  The next item's rows are
 // loaded, and its first tiles made, while the last item's gradients are still on their way out (an item a CTA left the tensor pipe idle
 // for 4 us at its start and end: 8192 queries, 32 heads on 8 of 128, window 1024: dQ 224 us, now 195, dK and dV 250).
 //
@@ -116,16 +116,19 @@ struct BwdCfg {
   static constexpr bool KEYS = KEYS_;
   static constexpr int DP = DP_, CHUNKS = DP / 64, NACC = KEYS ? 1 : 2;
   static constexpr int NS = DP == 64 ? 6 : 3, NR = 2;
+  // Groups of compute warps, each with an S and a dP.  (Heads of 64, 8192 queries, 32 on 8 heads, window 1024: dQ 145 us with two, 118 with
+  // three, dK and dV 193 and 169.)
+  static constexpr int NG = DP == 64 ? 3 : 2;
   static constexpr int R_CHUNK = 128 * 128, C_CHUNK = kTile * 128;
   static constexpr int R_TILE = CHUNKS * R_CHUNK, C_TILE = CHUNKS * C_CHUNK;
   static constexpr int OFF_R = 0;                              // [NR] two tiles of rows
   static constexpr int OFF_C = OFF_R + NR * 2 * R_TILE;        // [NS] two tiles of columns
   static constexpr int OFF_VEC = OFF_C + NS * 2 * C_TILE;      // [NS] nlse and ndelta of the columns (KEYS)
   static constexpr int OFF_BAR = OFF_VEC + (KEYS ? NS * 2 * kTile * 4 : 0);
-  static constexpr int N_BAR = 2 * NR + 4 + 2 * NS + 4;
+  static constexpr int N_BAR = 2 * NR + 4 + 2 * NS + 2 * NG;
   static constexpr int SMEM = OFF_BAR + N_BAR * 8 + 16;
-  static constexpr int THREADS = 320, WARP_TMA = 8, WARP_MMA = 9;
-  static constexpr int TM_ACC = 256, TMEM_COLS = 512;          // KEYS: dV, dK; else dQ of two items in turn
+  static constexpr int THREADS = 128 * NG + 64, WARP_TMA = 4 * NG, WARP_MMA = WARP_TMA + 1;
+  static constexpr int TM_ACC = 128 * NG, TMEM_COLS = 512;          // KEYS: dV, dK; else dQ of two items in turn
   static_assert(SMEM + 1024 <= 233472 && TM_ACC + 2 * DP <= TMEM_COLS, "");
 };
 
@@ -196,7 +199,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
   griddep_wait();
   using T = typename Cfg::T;
   constexpr bool KEYS = Cfg::KEYS;
-  constexpr int DP = Cfg::DP, NS = Cfg::NS, NR = Cfg::NR, NACC = Cfg::NACC, CHUNKS = Cfg::CHUNKS;
+  constexpr int DP = Cfg::DP, NS = Cfg::NS, NR = Cfg::NR, NG = Cfg::NG, NACC = Cfg::NACC, CHUNKS = Cfg::CHUNKS;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
   uint64_t* r_full = bars;               // [NR]
@@ -205,8 +208,8 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
   uint64_t* acc_free = acc_full + 2;     // [2]
   uint64_t* c_full = acc_free + 2;       // [NS]
   uint64_t* c_empty = c_full + NS;
-  uint64_t* sdp_full = c_empty + NS;     // [2]
-  uint64_t* pds_ready = sdp_full + 2;    // [2]
+  uint64_t* sdp_full = c_empty + NS;     // [NG]
+  uint64_t* pds_ready = sdp_full + NG;   // [NG]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + Cfg::N_BAR);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const WaitCtx wctx{abort_flag, status};
@@ -224,6 +227,8 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
     for (int g = 0; g < 2; ++g) {
       mbar_init(&acc_full[g], 1);
       mbar_init(&acc_free[g], 8);
+    }
+    for (int g = 0; g < NG; ++g) {
       mbar_init(&sdp_full[g], 1);
       mbar_init(&pds_ready[g], 4);
     }
@@ -323,8 +328,8 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
     int tiles = tiles_from(walk);
     while (walk.item < a.items) {
       if (lead == 0) warp_wait(&r_full[rs], rph, wctx);
-      for (; lead < 2 && lead < tiles; ++lead) issue_sdp((buf + lead) & 1);
-      if (tiles <= 2) rows_used();
+      for (; lead < NG && lead < tiles; ++lead) issue_sdp(buf + lead < NG ? buf + lead : buf + lead - NG);
+      if (tiles <= NG) rows_used();
       walk.next();
       const int next_tiles = tiles_from(walk);
       lead = 0;
@@ -342,21 +347,20 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
           umma_ts_w<hi, idesc_acc>(el, KEYS ? sums + DP : sums, from + 64 + 8 * k, d1 + k * 128, (k | t) != 0);
         umma_commit(el, &c_empty[bs]);
         if (++bs == NS) bs = 0;
-        // S and dP of two tiles ahead go over P and dS, which the products just issued have to read: the UMMAs of a thread go through the
+        // S and dP of NG tiles ahead go over P and dS, which the products just issued have to read: the UMMAs of a thread go through the
         // tensor pipe in order (as in the triangle attention's backward pass)
-        if (t + 2 < tiles) {
+        if (t + NG < tiles) {
           issue_sdp(buf);
-          if (t + 3 == tiles) rows_used();
+          if (t + NG + 1 == tiles) rows_used();
         } else {
           if (t + 1 == tiles) umma_commit(el, &acc_full[ab]);
-          if (NR > 1 && tiles > 1 && lead < next_tiles) {  // of the next item (beside a single tile, its first one is not due yet)
+          if (NR > 1 && tiles >= NG && lead < next_tiles) {  // of the next item (beside fewer tiles, its first one is not due yet)
             if (lead == 0) warp_wait(&r_full[rs], rph, wctx);
             issue_sdp(buf);
             ++lead;
           }
         }
-        buf ^= 1;
-        pph ^= buf ^ 1;
+        if (++buf == NG) buf = 0, pph ^= 1;
       }
       if (++ab == NACC) ab = 0, aph ^= 1;
       tiles = next_tiles;
@@ -369,9 +373,11 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
     const uint64_t c22 = f2_pack(c2, c2);
     const int rows = KEYS ? p.M : p.N, heads = KEYS ? p.HK : p.H;
 
-    // KEYS: group 0 stores dV and group 1 dK; else each a half of dQ's columns.  The sums of an item leave after the group's first tile of
-    // a later one has been handed over.
+    // KEYS: group 0 stores dV and group 1 dK; else each a half of dQ's columns (a third group nothing).  The sums of an item leave after
+    // the group's first tile of a later one has been handed over.
     const int cb = KEYS ? 0 : g * (DP / 2), ce = KEYS ? DP : cb + DP / 2;
+    const bool stores = g < 2;
+    constexpr int PART = KEYS && NG == 3 ? 16 : 32;  // columns in registers at a time
     const float mul = KEYS && g == 0 ? 1.f : p.scale;
     bool pending = false;
     int d_row = 0, d_head = 0, d_b = 0, d_part = 0, ab = 0;
@@ -428,7 +434,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
       if (it.tiles == 0) {
         if (pending) finish();
         d_row = mine, d_head = it.head, d_b = it.b, d_part = it.part;
-        store_rows(false);
+        if (stores) store_rows(false);
         continue;
       }
       float nl = 0.f, nd = 0.f;
@@ -442,7 +448,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
       int u = turn, t = turn, st = s + turn;
       while (u >= it.per_head && t < it.tiles) u -= it.per_head;
       while (st >= NS) st -= NS;
-      for (; t < it.tiles; t += 2) {
+      for (; t < it.tiles; t += NG) {
         const int c0 = it.column(u);
         warp_wait(&sdp_full[g], ph, wctx);
         ph ^= 1;
@@ -460,14 +466,19 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
         auto tile = [&](auto masked) {
           constexpr bool MASKED = decltype(masked)::value;
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t rs[32], rd[32];
-            tmem_ld32(t_s + 32 * half, rs);
-            tmem_ld32(t_dp + 32 * half, rd);
+          for (int half = 0; half < kTile / PART; ++half) {
+            uint32_t rs[PART], rd[PART];
+            if constexpr (PART == 32) {
+              tmem_ld32(t_s + 32 * half, rs);
+              tmem_ld32(t_dp + 32 * half, rd);
+            } else {
+              tmem_ld16(t_s + 16 * half, rs);
+              tmem_ld16(t_dp + 16 * half, rd);
+            }
             tmem_ld_wait();
-            const uint32_t bits = (uint32_t)(seen >> (32 * half));
+            const uint32_t bits = (uint32_t)(seen >> (PART * half));
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
+            for (int q = 0; q < PART / 16; ++q) {
               uint32_t pk[8], dk[8];
               [[maybe_unused]] float4 x4, y4;  // of four columns
 #pragma unroll
@@ -476,8 +487,8 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
                 uint64_t l2 = nl2, de2 = nd2;
                 if constexpr (KEYS) {
                   if (e % 2 == 0) {
-                    x4 = *reinterpret_cast<const float4*>(vec + 32 * half + c);
-                    y4 = *reinterpret_cast<const float4*>(vec + kTile + 32 * half + c);
+                    x4 = *reinterpret_cast<const float4*>(vec + PART * half + c);
+                    y4 = *reinterpret_cast<const float4*>(vec + kTile + PART * half + c);
                   }
                   l2 = e % 2 == 0 ? f2_pack(x4.x, x4.y) : f2_pack(x4.z, x4.w);
                   de2 = e % 2 == 0 ? f2_pack(y4.x, y4.y) : f2_pack(y4.z, y4.w);
@@ -494,8 +505,8 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
                 pk[e] = pack2<T>(p0, p1);
                 dk[e] = pack2<T>(d0, d1);
               }
-              if (KEYS) tmem_st8(t_s + 16 * half + 8 * q, pk);
-              tmem_st8(t_dp + 16 * half + 8 * q, dk);
+              if (KEYS) tmem_st8(t_s + PART / 2 * half + 8 * q, pk);
+              tmem_st8(t_dp + PART / 2 * half + 8 * q, dk);
             }
           }
         };
@@ -518,16 +529,16 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
         __syncwarp();
         if (lane == 0) mbar_arrive(&pds_ready[g]);
         if (pending) finish();
-        u += 2;
+        u += NG;
         while (u >= it.per_head) u -= it.per_head;
-        st += 2;
+        st += NG;
         while (st >= NS) st -= NS;
       }
       turn = t - it.tiles;
       s = (s + it.tiles) % NS;
       if (pending) finish();  // (the item had no tile for the group)
       d_row = mine, d_head = it.head, d_b = it.b, d_part = it.part;
-      pending = true;
+      pending = stores;
     }
     if (pending) finish();
   }
