@@ -3,10 +3,10 @@
 //   P = exp(S - lse) where a key is seen (0 elsewhere, and in rows that see nothing),  dP = dO V^T,  dS = P (dP - delta)
 //   dV = P^T dO,  dK = scale dS^T Q,  dQ = scale dS K,       delta = rowsum(dO out)
 //
-// Three kernels: `stats` makes -lse log2(e) and -delta of every query, padded to whole tiles; `window_bwd_kernel` then runs
-// twice, once with the keys as rows (dK and dV) and once with the queries (dQ).  It makes S and dP again for each: seven
-// products a tile instead of five, but every gradient is summed by one CTA in a fixed order, without atomics and without partial
-// sums of dQ in memory (at a window of 1024 keys those would be 9 times dQ in fp32, written and read).
+// `window_stats_kernel` makes -lse log2(e) and -delta of every query, padded to whole tiles; `window_bwd_kernel` then runs with the keys as
+// rows (dK and dV), with the queries (dQ), and before these, for the queries that see few keys, to make delta again from P and dP.
+// It makes S and dP each time: seven products a tile instead of five, but every gradient is summed by one CTA in a fixed order,
+// without atomics and without partial sums of dQ in memory (at a window of 1024 keys those would be 9 times dQ in fp32).
 //
 // An item is 128 rows (keys: K and V; queries: Q and dO), kept in shared memory while the CTA walks over their tiles of 64 columns.  S and
 // dP are made with the rows as TMEM lanes, so that P and dS, written over them as 16-bit numbers, are the A operands of the second
@@ -39,6 +39,10 @@ int window_bwd_status_fetch_and_clear(int* out) {
 namespace {
 
 constexpr int kTile = 64;  // columns of a tile
+// delta from the stored output has the roundings of that and of the probabilities in it.  Beside a dS of many keys they do not show; where a
+// query sees fewer than this, delta is made as the sum of P dP in fp32, tile by tile.  (Error of dQ and dK relative to their
+// norms, bf16, roundings of dS and of the results alone 0.0023: with two keys 0.0043, nine 0.0028, 31 0.0025, 128 0.0024.)
+constexpr int kFewKeys = 128;
 
 // ---- stats ------------------------------------------------------------------------------------------------
 // [B, H, NP] of -lse log2(e) (-inf: the row sees nothing, or lies behind the last one) and of -delta.
@@ -102,6 +106,7 @@ __global__ void __launch_bounds__(256) window_stats_kernel(const T* __restrict__
 // ---- gradients --------------------------------------------------------------------------------------------
 struct BwdArgs {
   const float *nlse, *ndelta;  // [B, H, NP]
+  float* exact;                // ndelta, to be written
   int NP;
   void *g1, *g2;               // KEYS: dV and dK; else dQ and nothing
   float* parts;                // KEYS: [B, HK, 1 + far][2][sinks][D] of the sinks' rows, or nullptr
@@ -110,10 +115,12 @@ struct BwdArgs {
   FastDiv div_heads, div_lists, div_g;  // (lists: heads of all sequences)
 };
 
-template <typename T_, int DP_, bool KEYS_>
+enum BwdRole { kKeyRows, kQueryRows, kDeltas };
+
+template <typename T_, int DP_, BwdRole ROLE>
 struct BwdCfg {
   using T = T_;
-  static constexpr bool KEYS = KEYS_;
+  static constexpr bool KEYS = ROLE == kKeyRows, DELTA = ROLE == kDeltas;
   static constexpr int DP = DP_, CHUNKS = DP / 64, NACC = KEYS ? 1 : 2;
   static constexpr int NS = DP == 64 ? 6 : 3, NR = 2;
   // Groups of compute warps, each with an S and a dP.  (Heads of 64, 8192 queries, 32 on 8 heads, window 1024: dQ 145 us with two, 118 with
@@ -124,7 +131,8 @@ struct BwdCfg {
   static constexpr int OFF_R = 0;                              // [NR] two tiles of rows
   static constexpr int OFF_C = OFF_R + NR * 2 * R_TILE;        // [NS] two tiles of columns
   static constexpr int OFF_VEC = OFF_C + NS * 2 * C_TILE;      // [NS] nlse and ndelta of the columns (KEYS)
-  static constexpr int OFF_BAR = OFF_VEC + (KEYS ? NS * 2 * kTile * 4 : 0);
+  static constexpr int OFF_SUM = OFF_VEC + (KEYS ? NS * 2 * kTile * 4 : 0);  // [2][NG][128] fp32 (DELTA)
+  static constexpr int OFF_BAR = OFF_SUM + (DELTA ? 2 * NG * 128 * 4 : 0);
   static constexpr int N_BAR = 2 * NR + 4 + 2 * NS + 2 * NG;
   static constexpr int SMEM = OFF_BAR + N_BAR * 8 + 16;
   static constexpr int THREADS = 128 * NG + 64, WARP_TMA = 4 * NG, WARP_MMA = WARP_TMA + 1;
@@ -152,8 +160,9 @@ struct BwdWalk {
 };
 
 // An item and its column tiles: for each of `heads` heads [a tile of the sinks,] tiles lo .. hi - 1.
-template <bool KEYS>
+template <class Cfg>
 struct BwdItem {
+  static constexpr bool KEYS = Cfg::KEYS;
   int r0, head, b, len, off;  // head: KEYS: a key head, else a query head
   int part;                   // KEYS: 0, or 1 + the number of far queries' item
   int extra, lo, heads, per_head, tiles;
@@ -185,6 +194,10 @@ struct BwdItem {
       lo = kr.sink > 0 && !extra ? 0 : kr.lo / kTile;
       hi = (kr.hi + kTile - 1) / kTile;
     }
+    if (Cfg::DELTA) {  // (the fewest keys are those of a query at one of the ends)
+      auto count = [&](int pos) { return __popcll(seen_keys(p, min(len, 64), pos, 0)) + max(0, min(len, pos + p.right + 1) - max(64, pos - p.left)); };
+      if (min(count(off + r0), count(off + min(r0 + 127, p.N - 1))) >= kFewKeys) hi = lo, extra = 0;
+    }
     per_head = extra + max(0, hi - lo);
     tiles = per_head * heads;
   }
@@ -198,7 +211,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
                   const BwdArgs a, int* __restrict__ status) {
   griddep_wait();
   using T = typename Cfg::T;
-  constexpr bool KEYS = Cfg::KEYS;
+  constexpr bool KEYS = Cfg::KEYS, DELTA = Cfg::DELTA;
   constexpr int DP = Cfg::DP, NS = Cfg::NS, NR = Cfg::NR, NG = Cfg::NG, NACC = Cfg::NACC, CHUNKS = Cfg::CHUNKS;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
@@ -253,7 +266,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
     int s = 0, rs = 0;
     uint32_t ph = 1, rph = 1;
     for (BwdWalk walk; walk.item < a.items; walk.next()) {
-      const BwdItem<KEYS> it(walk.item, p, a);
+      const BwdItem<Cfg> it(walk.item, p, a);
       if (it.tiles == 0) continue;
       warp_wait(&r_empty[rs], rph, wctx);
       mbar_expect_tx(el, &r_full[rs], 2 * Cfg::R_TILE);
@@ -320,7 +333,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
     };
     auto tiles_from = [&](BwdWalk& w) {  // of the next item that has any
       int n = 0;
-      while (w.item < a.items && (n = BwdItem<KEYS>(w.item, p, a).tiles) == 0) w.next();
+      while (w.item < a.items && (n = BwdItem<Cfg>(w.item, p, a).tiles) == 0) w.next();
       return __shfl_sync(0xffffffffu, n, 0);
     };
     BwdWalk walk;
@@ -334,7 +347,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
       const int next_tiles = tiles_from(walk);
       lead = 0;
       for (int t = 0; t < tiles; ++t) {
-        if (t == 0) warp_wait2(&pds_ready[buf], pph, &acc_free[ab], aph, wctx);
+        if (t == 0 && !DELTA) warp_wait2(&pds_ready[buf], pph, &acc_free[ab], aph, wctx);
         else warp_wait(&pds_ready[buf], pph, wctx);
         tc_fence_after();
         const uint32_t d1 = d_cmn + bs * kStage, d2 = d1 + kSecond, from = tmem + 128 * buf, sums = tmem + Cfg::TM_ACC + (NACC > 1 ? ab * DP : 0);
@@ -342,9 +355,11 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
 #pragma unroll
           for (int k = 0; k < 4; ++k) umma_ts_w<hi, idesc_acc>(el, sums, from + 8 * k, d2 + k * 128, (k | t) != 0);
         }
+        if constexpr (!DELTA) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          umma_ts_w<hi, idesc_acc>(el, KEYS ? sums + DP : sums, from + 64 + 8 * k, d1 + k * 128, (k | t) != 0);
+          for (int k = 0; k < 4; ++k)
+            umma_ts_w<hi, idesc_acc>(el, KEYS ? sums + DP : sums, from + 64 + 8 * k, d1 + k * 128, (k | t) != 0);
+        }
         umma_commit(el, &c_empty[bs]);
         if (++bs == NS) bs = 0;
         // S and dP of NG tiles ahead go over P and dS, which the products just issued have to read: the UMMAs of a thread go through the
@@ -376,7 +391,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
     // KEYS: group 0 stores dV and group 1 dK; else each a half of dQ's columns (a third group nothing).  The sums of an item leave after
     // the group's first tile of a later one has been handed over.
     const int cb = KEYS ? 0 : g * (DP / 2), ce = KEYS ? DP : cb + DP / 2;
-    const bool stores = g < 2;
+    const bool stores = g < 2 && !DELTA;
     constexpr int PART = KEYS && NG == 3 ? 16 : 32;  // columns in registers at a time
     const float mul = KEYS && g == 0 ? 1.f : p.scale;
     bool pending = false;
@@ -426,10 +441,11 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
     };
 
     int turn = g;   // tiles until the group's next one
+    [[maybe_unused]] int which = 0;
     int s = 0;      // stage of the item's first tile
     uint32_t ph = 0;
     for (BwdWalk walk; walk.item < a.items; walk.next()) {
-      const BwdItem<KEYS> it(walk.item, p, a);
+      const BwdItem<Cfg> it(walk.item, p, a);
       const int mine = it.r0 + row;
       if (it.tiles == 0) {
         if (pending) finish();
@@ -441,9 +457,10 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
       if (!KEYS && mine < p.N) {
         const int64_t at = ((int64_t)it.b * p.H + it.head) * a.NP + mine;
         nl = __ldg(a.nlse + at);
-        nd = __ldg(a.ndelta + at);
+        if (!DELTA) nd = __ldg(a.ndelta + at);
       }
       const uint64_t nl2 = f2_pack(nl, nl), nd2 = f2_pack(nd, nd);
+      [[maybe_unused]] uint64_t delta2 = 0;
       const int w0 = it.r0 + lane_base, w1 = w0 + 31, len = it.len, off = it.off;  // the warp's rows
       int u = turn, t = turn, st = s + turn;
       while (u >= it.per_head && t < it.tiles) u -= it.per_head;
@@ -501,18 +518,22 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
                   if (!(bits >> c & 1u)) p0 = d0 = 0.f;
                   if (!(bits >> (c + 1) & 1u)) p1 = d1 = 0.f;
                 }
-                // 16 bits, as operands of the products
-                pk[e] = pack2<T>(p0, p1);
-                dk[e] = pack2<T>(d0, d1);
+                if constexpr (DELTA) {
+                  delta2 = f2_add(delta2, f2_pack(d0, d1));
+                } else {
+                  // 16 bits, as operands of the products
+                  pk[e] = pack2<T>(p0, p1);
+                  dk[e] = pack2<T>(d0, d1);
+                }
               }
               if (KEYS) tmem_st8(t_s + PART / 2 * half + 8 * q, pk);
-              tmem_st8(t_dp + PART / 2 * half + 8 * q, dk);
+              if (!DELTA) tmem_st8(t_dp + PART / 2 * half + 8 * q, dk);
             }
           }
         };
         if (whole) tile(std::false_type{});
         else tile(std::true_type{});
-        if constexpr (!KEYS) {
+        if constexpr (!KEYS && !DELTA) {
           // Keys behind the last one are anything, and a dS of zero times a NaN is one (S has been made from them, and masked).
           if (c0 + kTile > len) {
             uint8_t* kt = smem + Cfg::OFF_C + st * 2 * Cfg::C_TILE;
@@ -536,6 +557,19 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
       }
       turn = t - it.tiles;
       s = (s + it.tiles) % NS;
+      if constexpr (DELTA) {
+        // the groups' parts of the rows' sums, added in their order
+        float* sums = reinterpret_cast<float*>(smem + Cfg::OFF_SUM) + which * NG * 128;
+        which ^= 1;  // (so that what the first group reads stays until everybody has come here again)
+        sums[g * 128 + row] = f2_sum(delta2);
+        asm volatile("bar.sync 1, %0;" ::"n"(NG * 128) : "memory");
+        if (g == 0 && mine < p.N) {
+          float sum = sums[row];
+#pragma unroll
+          for (int k = 1; k < NG; ++k) sum += sums[k * 128 + row];
+          a.exact[((int64_t)it.b * p.H + it.head) * a.NP + mine] = -sum;
+        }
+      }
       if (pending) finish();  // (the item had no tile for the group)
       d_row = mine, d_head = it.head, d_b = it.b, d_part = it.part;
       pending = stores;
@@ -635,6 +669,16 @@ int run(const WindowCall& c, const WindowParams& p, uint8_t* ws, cudaStream_t st
   TPF_LAUNCH_OK();
   const int64_t os[3] = {c.N * c.H * c.D, c.H * c.D, c.D};
   int rc;
+  // (without a bound on either side, and with enough keys, every query sees enough of them)
+  if (c.lengths != nullptr || c.left != kWindowUnlimited || c.right != kWindowUnlimited || c.M < kFewKeys) {
+    CUtensorMap tk, tv, tq, tg;
+    if ((rc = make_window_tmap(&tq, c.q, c.type, c.B, c.N, c.H, c.D, c.qs, 128))) return rc;
+    if ((rc = make_window_tmap(&tg, c.d_out, c.type, c.B, c.N, c.H, c.D, os, 128))) return rc;
+    if ((rc = make_window_tmap(&tk, c.k, c.type, c.B, c.M, c.HK, c.D, c.ks, kTile))) return rc;
+    if ((rc = make_window_tmap(&tv, c.v, c.type, c.B, c.M, c.HK, c.D, c.vs, kTile))) return rc;
+    a.exact = ndelta;
+    if ((rc = launch<BwdCfg<T, DP, kDeltas>>(tq, tg, tk, tv, p, a, c, stream))) return rc;
+  }
   if (c.dk != nullptr) {
     CUtensorMap tk, tv, tq, tg;
     if ((rc = make_window_tmap(&tk, c.k, c.type, c.B, c.M, c.HK, c.D, c.ks, 128))) return rc;
@@ -645,7 +689,7 @@ int run(const WindowCall& c, const WindowParams& p, uint8_t* ws, cudaStream_t st
     a.key_tiles = (int)((c.M + 127) / 128);
     far_plan(c, &a.far, &a.far_tiles);
     if (a.far > 0) a.parts = reinterpret_cast<float*>(ws + 2 * stat);
-    if ((rc = launch<BwdCfg<T, DP, true>>(tk, tv, tq, tg, p, a, c, stream))) return rc;
+    if ((rc = launch<BwdCfg<T, DP, kKeyRows>>(tk, tv, tq, tg, p, a, c, stream))) return rc;
     if (a.far > 0) {
       launch_kernel(window_sinks_kernel<T>, dim3(2 * (unsigned)(c.sinks < c.M ? c.sinks : c.M), (unsigned)c.HK, (unsigned)c.B), dim3(256),
                     0, stream, static_cast<const float*>(a.parts), 1 + a.far, c.sinks, (int)c.D, (int)c.M, (int)c.HK,
@@ -661,7 +705,7 @@ int run(const WindowCall& c, const WindowParams& p, uint8_t* ws, cudaStream_t st
     if ((rc = make_window_tmap(&tv, c.v, c.type, c.B, c.M, c.HK, c.D, c.vs, kTile))) return rc;
     a.g1 = c.dq, a.g2 = nullptr;
     a.parts = nullptr;
-    if ((rc = launch<BwdCfg<T, DP, false>>(tq, tg, tk, tv, p, a, c, stream))) return rc;
+    if ((rc = launch<BwdCfg<T, DP, kQueryRows>>(tq, tg, tk, tv, p, a, c, stream))) return rc;
   }
   return TPF_OK;
 }

@@ -286,6 +286,20 @@ def test_some_gradients_only_and_no_second_ones():
         g.float().sum().backward()
 
 
+@pytest.mark.parametrize("B, n, D, window, sinks", [(200, 4, 80, (800, 0), 0), (8, 300, 128, (1, 0), 0), (8, 300, 64, (3, 3), 1), (8, 300, 64, (8, 0), 0),
+                                                    (4, 400, 128, (None, 0), 0), (300, 2, 32, (5, 0), 0), (3, 700, 96, (0, 40), 7)])
+@pytest.mark.parametrize("dtype", [BF, FP16])
+def test_few_keys_cost_no_precision(B, n, D, window, sinks, dtype):
+    """dS and the result are rounded once each: in the norm 2 / sqrt(3) half steps at the most where the two never cancel, 1.5 with the
+    spread of some hundred numbers.  Roundings of the output in delta would be beside a dS that is small where a query sees few keys."""
+    q, k, v = (t.requires_grad_(True) for t in _inputs(B, n, n, 4, 2, D, dtype))
+    d = _rn(B, n, 4, D, seed=8, dtype=dtype)
+    ref = so.window_attention(q.detach(), k.detach(), v.detach(), window, sinks, d_out=d)
+    grads = torch.autograd.grad(tk.turbo_window_attention(q, k, v, window=window, sinks=sinks), [q, k, v], d)
+    for name, g in zip(("dq", "dk", "dv"), grads):
+        assert (g.double() - ref[name]).norm() <= 1.5 * so.half_step(dtype) * ref[name].norm(), name
+
+
 def test_gradients_from_packed_activations():
     """Inside `int8_activations` the backward pass runs on what the format holds of q, k, v and the output."""
     leaves = [t.requires_grad_(True) for t in _inputs(2, 300, 300, 8, 2, 64)]
