@@ -13,7 +13,7 @@
 // products straight from TMEM; a thread has a row.  Two groups of four warps take turns with the tiles, three where heads of 64 elements
 // leave room for a third S and dP in TMEM: while one computes, the products of the others run.  With the keys as rows the CTA goes through all query heads that share them.  The next item's rows are
 // loaded, and its first tiles made, while the last item's gradients are still on their way out (an item a CTA left the tensor pipe idle
-// for 4 us at its start and end: 8192 queries, 32 heads on 8 of 128, window 1024: dQ 224 us, now 195, dK and dV 250).
+// for 4 us at its start and end: 8192 queries, 32 heads on 8 of 128, window 1024: dQ 224 us, now 187, dK and dV 250 to 267).
 //
 // What bounds it at 128 elements a head: the tensor pipe.  An UMMA of 64 columns with both operands in shared memory reads 6 KB, 48
 // cycles, for 32 cycles of products, which makes 1280 cycles a tile with the keys as rows and 1024 with the queries (1345 and 1127
@@ -117,9 +117,11 @@ struct BwdArgs {
 
 enum BwdRole { kKeyRows, kQueryRows, kDeltas };
 
-template <typename T_, int DP_, BwdRole ROLE>
+template <typename T_, int DP_, BwdRole ROLE, bool TWICE_ = false>
 struct BwdCfg {
   using T = T_;
+  static constexpr bool TWICE = TWICE_;
+  static constexpr int STEP = TWICE ? 16 : 8;                  // columns of TMEM from one 16 of an operand to the next
   static constexpr bool KEYS = ROLE == kKeyRows, DELTA = ROLE == kDeltas;
   static constexpr int DP = DP_, CHUNKS = DP / 64, NACC = KEYS ? 1 : 2;
   static constexpr int NS = DP == 64 ? 6 : 3, NR = 2;
@@ -211,7 +213,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
                   const BwdArgs a, int* __restrict__ status) {
   griddep_wait();
   using T = typename Cfg::T;
-  constexpr bool KEYS = Cfg::KEYS, DELTA = Cfg::DELTA;
+  constexpr bool KEYS = Cfg::KEYS, DELTA = Cfg::DELTA, TWICE = Cfg::TWICE;
   constexpr int DP = Cfg::DP, NS = Cfg::NS, NR = Cfg::NR, NG = Cfg::NG, NACC = Cfg::NACC, CHUNKS = Cfg::CHUNKS;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cfg::OFF_BAR);
@@ -353,12 +355,18 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
         const uint32_t d1 = d_cmn + bs * kStage, d2 = d1 + kSecond, from = tmem + 128 * buf, sums = tmem + Cfg::TM_ACC + (NACC > 1 ? ab * DP : 0);
         if constexpr (KEYS) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) umma_ts_w<hi, idesc_acc>(el, sums, from + 8 * k, d2 + k * 128, (k | t) != 0);
+          for (int k = 0; k < 4; ++k) {
+            umma_ts_w<hi, idesc_acc>(el, sums, from + Cfg::STEP * k, d2 + k * 128, (k | t) != 0);
+            if constexpr (TWICE) umma_ts_w<hi, idesc_acc>(el, sums, from + Cfg::STEP * k + 8, d2 + k * 128, true);
+          }
         }
         if constexpr (!DELTA) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_ts_w<hi, idesc_acc>(el, KEYS ? sums + DP : sums, from + 64 + 8 * k, d1 + k * 128, (k | t) != 0);
+          for (int k = 0; k < 4; ++k) {
+            umma_ts_w<hi, idesc_acc>(el, KEYS ? sums + DP : sums, from + 64 + Cfg::STEP * k, d1 + k * 128, (k | t) != 0);
+            if constexpr (TWICE)
+              umma_ts_w<hi, idesc_acc>(el, KEYS ? sums + DP : sums, from + 64 + Cfg::STEP * k + 8, d1 + k * 128, true);
+          }
         }
         umma_commit(el, &c_empty[bs]);
         if (++bs == NS) bs = 0;
@@ -497,6 +505,7 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
 #pragma unroll
             for (int q = 0; q < PART / 16; ++q) {
               uint32_t pk[8], dk[8];
+              [[maybe_unused]] uint32_t pl[8], dl[8];  // what the rounding of these leaves over
               [[maybe_unused]] float4 x4, y4;  // of four columns
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
@@ -524,10 +533,20 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tmR1, const __grid_constan
                   // 16 bits, as operands of the products
                   pk[e] = pack2<T>(p0, p1);
                   dk[e] = pack2<T>(d0, d1);
+                  if constexpr (TWICE) {
+                    const float2 ph = unpack2<T>(pk[e]), dh = unpack2<T>(dk[e]);
+                    pl[e] = pack2<T>(p0 - ph.x, p1 - ph.y);
+                    dl[e] = pack2<T>(d0 - dh.x, d1 - dh.y);
+                  }
                 }
               }
-              if (KEYS) tmem_st8(t_s + PART / 2 * half + 8 * q, pk);
-              if (!DELTA) tmem_st8(t_dp + PART / 2 * half + 8 * q, dk);
+              const int at = (PART * half + 16 * q) / 16 * Cfg::STEP;
+              if (KEYS) tmem_st8(t_s + at, pk);
+              if (!DELTA) tmem_st8(t_dp + at, dk);
+              if constexpr (TWICE) {
+                if (KEYS) tmem_st8(t_s + at + 8, pl);
+                tmem_st8(t_dp + at + 8, dl);
+              }
             }
           }
         };
@@ -669,6 +688,10 @@ int run(const WindowCall& c, const WindowParams& p, uint8_t* ws, cudaStream_t st
   TPF_LAUNCH_OK();
   const int64_t os[3] = {c.N * c.H * c.D, c.H * c.D, c.D};
   int rc;
+  // Short sequences take P and dS in two parts, which together have 16 bits of mantissa (22 in fp16): a gradient that is the sum of a few
+  // products shows the rounding of each.  (Three of 4 tokens: error of dK relative to its norm 0.0026, now 0.0017, 16.9 us, now 18.5; 256 of
+  // 128 tokens, 16 heads of 128: 303 us, now 324.)  In longer ones the errors are those of the mean, sqrt(2) of the result's rounding.
+  const bool twice = c.N <= 128 && c.M <= 128;
   // (without a bound on either side, and with enough keys, every query sees enough of them)
   if (c.lengths != nullptr || c.left != kWindowUnlimited || c.right != kWindowUnlimited || c.M < kFewKeys) {
     CUtensorMap tk, tv, tq, tg;
@@ -689,7 +712,9 @@ int run(const WindowCall& c, const WindowParams& p, uint8_t* ws, cudaStream_t st
     a.key_tiles = (int)((c.M + 127) / 128);
     far_plan(c, &a.far, &a.far_tiles);
     if (a.far > 0) a.parts = reinterpret_cast<float*>(ws + 2 * stat);
-    if ((rc = launch<BwdCfg<T, DP, kKeyRows>>(tk, tv, tq, tg, p, a, c, stream))) return rc;
+    if ((rc = twice ? launch<BwdCfg<T, DP, kKeyRows, true>>(tk, tv, tq, tg, p, a, c, stream)
+                    : launch<BwdCfg<T, DP, kKeyRows>>(tk, tv, tq, tg, p, a, c, stream)))
+      return rc;
     if (a.far > 0) {
       launch_kernel(window_sinks_kernel<T>, dim3(2 * (unsigned)(c.sinks < c.M ? c.sinks : c.M), (unsigned)c.HK, (unsigned)c.B), dim3(256),
                     0, stream, static_cast<const float*>(a.parts), 1 + a.far, c.sinks, (int)c.D, (int)c.M, (int)c.HK,
@@ -705,7 +730,9 @@ int run(const WindowCall& c, const WindowParams& p, uint8_t* ws, cudaStream_t st
     if ((rc = make_window_tmap(&tv, c.v, c.type, c.B, c.M, c.HK, c.D, c.vs, kTile))) return rc;
     a.g1 = c.dq, a.g2 = nullptr;
     a.parts = nullptr;
-    if ((rc = launch<BwdCfg<T, DP, kQueryRows>>(tq, tg, tk, tv, p, a, c, stream))) return rc;
+    if ((rc = twice ? launch<BwdCfg<T, DP, kQueryRows, true>>(tq, tg, tk, tv, p, a, c, stream)
+                    : launch<BwdCfg<T, DP, kQueryRows>>(tq, tg, tk, tv, p, a, c, stream)))
+      return rc;
   }
   return TPF_OK;
 }
