@@ -17,8 +17,9 @@ Operator contract:
   fp32.  The same inputs give the same bits.
 
 A single token over its cache is ``N = 1`` with ``query_offset = key_lengths - 1``.  Probabilities and their gradients are rounded
-to q's type as operands of the products; sums and the softmax are fp32 (a probability below 2^-126 is zero).  A key or value inside the sequence that is infinite or NaN
-reaches every query whose 128 neighbours see it, as a product of zero with it does elsewhere.
+to q's type as operands of the products (short calls take them in two parts); sums and the softmax are fp32, and a probability below
+2^-126 is zero.  A key or value inside the sequence that is infinite or NaN reaches every query whose 128 neighbours see it, as a
+product of zero with it does elsewhere.
 
 Unsupported inputs raise ``ValueError("turbo_window_attention unsupported [code]: reason")``, in a traced call when it is traced or,
 for sizes that are free there, when it runs.  The reference has no counterpart.
