@@ -19,6 +19,9 @@ Tensor dense(const Tensor& t) {
   return aligned(c, 32) ? c : c.clone();
 }
 
+// A saved tensor that a kernel reads from its first element on.  (A hook of the caller's may have handed back other strides.)
+Tensor in_order(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+
 MaybeTensor maybe(const Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); }
 
 // An optional tensor argument: false if it needs the Python route.
@@ -120,7 +123,7 @@ struct DropoutFn : public torch::autograd::Function<DropoutFn> {
     c10::cuda::CUDAGuard guard(grads[0].device());
     at::NoGradGuard no_grad;
     const std::vector<int64_t> v = ctx->saved_data["a"].toIntVector();
-    const DropoutArgs a{ctx->get_saved_variables()[0], v[0], v[1], v[2], v[3]};
+    const DropoutArgs a{in_order(ctx->get_saved_variables()[0]), v[0], v[1], v[2], v[3]};
     if (ctx->needs_input_grad(0)) r[0] = dropout_out(grads[0].detach(), Tensor(), a);
     // (the very tensor: a view of it would hide from whoever accumulates gradients that others hold it, too)
     if (v[4]) r[1] = grads[0];
@@ -271,7 +274,8 @@ struct RotaryFn : public torch::autograd::Function<RotaryFn> {
     c10::cuda::CUDAGuard guard(some.device());
     at::NoGradGuard no_grad;
     const auto saved = ctx->get_saved_variables();
-    const RotaryArgs a{saved[4], saved[5], ((int64_t)v[0] << 32) + (int64_t)v[1], v[2], v[3] != 0, v[4] != 0, v[5]};
+    const RotaryArgs a{in_order(saved[4]), in_order(saved[5]), ((int64_t)v[0] << 32) + (int64_t)v[1], v[2], v[3] != 0, v[4] != 0,
+                       v[5]};
     const Tensor d[2] = {grads[0].defined() ? dense(grads[0]) : none, has_k && grads[1].defined() ? dense(grads[1]) : none};
     const Heads x[2] = {saved[0].defined() ? as_heads(saved[0].detach(), false) : Heads{},
                         saved[1].defined() ? as_heads(saved[1].detach(), false) : Heads{}};
@@ -367,7 +371,7 @@ struct WindowFn : public torch::autograd::Function<WindowFn> {
     at::NoGradGuard no_grad;
     const auto s = ctx->get_saved_variables();
     const std::vector<double> v = ctx->saved_data["a"].toDoubleVector();  // (whole numbers below 2^53 are exact)
-    const WindowArgs a{s[5], s[6], (int64_t)v[0], (int64_t)v[1], (int64_t)v[2], (int64_t)v[3], v[4]};
+    const WindowArgs a{in_order(s[5]), in_order(s[6]), (int64_t)v[0], (int64_t)v[1], (int64_t)v[2], (int64_t)v[3], v[4]};
     const bool need_kv = ctx->needs_input_grad(1) || ctx->needs_input_grad(2);
     const variable_list g = window_grads(dense(grads[0]), as_heads(s[0].detach(), true), as_heads(s[1].detach(), true),
                                          as_heads(s[2].detach(), true), dense(s[3]), s[4].contiguous(), a, ctx->needs_input_grad(0),

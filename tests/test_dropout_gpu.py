@@ -292,3 +292,14 @@ def test_pair_block_trains_with_dropout(seed):
     got, want = torch.autograd.grad(out, z, d)[0].float(), torch.autograd.grad(expected, z, d)[0].float()
     # the same kernels, and sums of bf16 gradients: a handful of roundings of each
     assert (got - want).norm() <= 2.0 ** -7 * want.norm()
+
+
+def test_a_saved_seed_of_another_layout():
+    """A hook of the caller's may hand back any strides."""
+    x, seed = _rn(3, 500, seed=4).cuda().requires_grad_(True), torch.tensor([5, 9], device="cuda")
+    d = _rn(3, 500, seed=5).cuda()
+    want = torch.autograd.grad(tk.turbo_dropout(x, 0.5, seed), x, d)[0]
+    spread = lambda t: torch.stack([t, t + 1], -1)[..., 0]  # noqa: E731
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), spread):
+        out = tk.turbo_dropout(x, 0.5, seed)
+    assert torch.equal(torch.autograd.grad(out, x, d)[0], want)

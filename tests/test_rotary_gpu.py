@@ -291,3 +291,27 @@ def test_second_derivatives_and_changed_inputs_raise():
     x.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         a.sum().backward()
+
+
+@pytest.mark.parametrize("norm", [False, True])
+def test_saved_tensors_of_other_layouts(norm):
+    """A hook of the caller's may hand back any strides of the positions and the frequencies, too: transposed, spread out, expanded."""
+    q, k = (_rn(3, 50, h, 64, seed=h, dtype=torch.bfloat16).requires_grad_(True) for h in (4, 2))
+    fr = _freq(32)
+    row = torch.randint(0, 10 ** 6, (1, 50), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    positions = torch.cat([row, row, row])
+    d = [_rn(3, 50, h, 64, seed=h + 10, dtype=torch.bfloat16) for h in (4, 2)]
+
+    def call():
+        if norm:
+            return tk.turbo_qk_norm_rotary(q, k, None, None, fr, positions)
+        return tk.turbo_rotary(q, fr, positions), tk.turbo_rotary(k, fr, positions)
+
+    want = torch.autograd.grad(call(), [q, k], d)
+    turned = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1) if t.ndim > 1 else t  # noqa: E731
+    spread = lambda t: torch.stack([t, t + 1], -1)[..., 0]  # noqa: E731
+    once = lambda t: t[:1].clone().expand(t.shape) if t.ndim == 2 else t  # noqa: E731
+    for hook in (turned, spread, once):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), hook):
+            outs = call()
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(outs, [q, k], d), want))

@@ -402,3 +402,23 @@ def test_a_layer_of_them():
     assert (out.double() - ref).norm() <= room * ref.norm()
     for a, b in zip(grads, want):
         assert (a.double() - b).norm() <= room * b.norm()
+
+
+def test_saved_offsets_and_lengths_of_other_layouts():
+    """A hook of the caller's may hand back any strides of these, too: transposed, spread out, expanded."""
+    q, k, v = (t.unflatten(0, (2, 3)).contiguous().requires_grad_(True) for t in _inputs(6, 40, 100, 4, 2, 64))
+    d = _rn(2, 3, 40, 4, 64, seed=3)
+    some = torch.tensor([[60, 10, 33]], dtype=torch.int32, device="cuda")
+    offsets, lengths = torch.cat([some, some]), torch.cat([some + 40, some + 40])
+
+    def call():
+        return tk.turbo_window_attention(q, k, v, window=(20, 0), sinks=2, query_offset=offsets, key_lengths=lengths)
+
+    want = torch.autograd.grad(call(), [q, k, v], d)
+    turned = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)  # noqa: E731
+    spread = lambda t: torch.stack([t, t + 1], -1)[..., 0]  # noqa: E731
+    once = lambda t: t[:1].clone().expand(t.shape) if t.ndim == 2 else t  # noqa: E731
+    for hook in (turned, spread, once):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), hook):
+            out = call()
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, [q, k, v], d), want))
