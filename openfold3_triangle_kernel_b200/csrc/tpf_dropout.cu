@@ -75,6 +75,11 @@ __device__ __forceinline__ uint32_t kept_bits(const uint32_t (&w)[4], uint32_t b
 }
 
 constexpr int kThreads = 256;
+// The first index along S of a block's run.  (Runs lie along the grid's y, and along z where there are more of them than y takes.)
+template <int RUN>
+__device__ __forceinline__ uint32_t run_start() {
+  return (blockIdx.z * gridDim.y + blockIdx.y) * RUN;
+}
 template <typename T, bool RES>
 __device__ __forceinline__ void drop_vec(const Piece<T, 8>& x, const Piece<T, 8>& r, const bool (&kept)[8], float scale, T* out) {
   float v[8], w[8];
@@ -97,8 +102,8 @@ __global__ void __launch_bounds__(kThreads) dropout_vec_kernel(const DropoutPara
   const uint32_t cell = blockIdx.x * kThreads + threadIdx.x;
   const uint32_t row = p.div_cells.div(cell), vec = cell - row * p.cells;
   const uint32_t pi = p.div_q.div(row), qi = row - pi * p.Q;
-  if (pi >= p.P) return;
-  const uint32_t s0 = blockIdx.y * RUN;
+  const uint32_t s0 = run_start<RUN>();
+  if (pi >= p.P || s0 >= p.S) return;
   const int64_t e = (int64_t)vec * 8;
   const T* x = static_cast<const T*>(p.x) + pi * p.xp + qi * p.xq + s0 * p.xs + e;
   const T* r = RES ? static_cast<const T*>(p.r) + pi * p.rp + qi * p.rq + s0 * p.rs + e : nullptr;
@@ -138,9 +143,10 @@ template <typename T, bool RES, int RUN>
 __global__ void __launch_bounds__(kThreads) dropout_any_kernel(const DropoutParams p) {
   griddep_wait();
   const int lane = threadIdx.x & 31;
+  const uint32_t s0 = run_start<RUN>();  // (of a shared dimension; else 0)
+  if (s0 >= p.S) return;
   const uint64_t m0 = ((uint64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * 256;
   const uint64_t row0 = m0 / (uint64_t)p.inner, e0 = m0 - row0 * p.inner;
-  const uint32_t s0 = blockIdx.y * RUN;  // (of a shared dimension; else 0)
   const int n = RUN == 1 ? 1 : min(RUN, (int)(p.S - s0));
   T v[RUN][8], w[RUN][8];
   T* out[8];
@@ -190,8 +196,8 @@ __global__ void __launch_bounds__(kThreads) dropout_any_kernel(const DropoutPara
 template <typename T, bool RES, int RUN>
 int launch(const DropoutParams& p, bool vec, int64_t cells, cudaStream_t stream) {
   const int64_t per_block = vec ? kThreads : kThreads / 32;
-  const dim3 grid((unsigned)((cells + per_block - 1) / per_block), p.s_in_mask && !vec ? 1 : (p.S + RUN - 1) / RUN);
-  TPF_REQUIRE(grid.y <= 65535, TPF_ERR_UNSUPPORTED, "dropout: the shared dimension is too long");
+  const uint32_t runs = p.s_in_mask && !vec ? 1 : (p.S + RUN - 1) / RUN, z = (runs + 65534) / 65535;
+  const dim3 grid((unsigned)((cells + per_block - 1) / per_block), (runs + z - 1) / z, z);
   if (vec) launch_kernel(dropout_vec_kernel<T, RES, RUN>, grid, dim3(kThreads), 0, stream, p);
   else if constexpr (RUN <= 4) launch_kernel(dropout_any_kernel<T, RES, RUN>, grid, dim3(kThreads), 0, stream, p);
   TPF_LAUNCH_OK();
@@ -201,7 +207,8 @@ template <typename T, bool RES>
 int launch(const DropoutParams& p, bool vec, int64_t cells, cudaStream_t stream) {
   // Long runs make few masks, and few threads: a run is shortened while there would be fewer blocks than eight an SM (two, where
   // a thread has eight elements of every row).
-  const int64_t enough = (vec ? 8ll : 2ll) * sm_count(), blocks = cells / (vec ? kThreads : kThreads / 32);
+  const int64_t enough = (vec ? 8ll : 2ll) * sm_count(), per_block = vec ? kThreads : kThreads / 32;
+  const int64_t blocks = (cells + per_block - 1) / per_block;
   const int64_t s = p.s_in_mask ? 1 : p.S;
   if (s >= 8 && vec && blocks * (s / 8) >= enough) return launch<T, RES, 8>(p, vec, cells, stream);
   if (s >= 4 && blocks * (s / 4) >= enough) return launch<T, RES, 4>(p, vec, cells, stream);

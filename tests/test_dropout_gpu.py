@@ -303,3 +303,11 @@ def test_a_saved_seed_of_another_layout():
     with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), spread):
         out = tk.turbo_dropout(x, 0.5, seed)
     assert torch.equal(torch.autograd.grad(out, x, d)[0], want)
+
+
+@pytest.mark.parametrize("shape, shared", [((131070, 16), 0), ((131071, 16), 0), ((200000, 64), 0), ((600000, 8), 0), ((131071, 5), 0),
+                                           ((300001, 3), 0), ((2, 140001, 24), 1), ((2, 140001, 3, 3), 1), ((1, 530000, 2, 8), -3)])
+def test_a_long_shared_dimension(shape, shared):
+    """One mask for all tokens: more runs than a dimension of a grid takes."""
+    x = _rn(*shape, seed=3).bfloat16()
+    _check(x, shared=shared, residual=_rn(*shape, seed=4).bfloat16())
