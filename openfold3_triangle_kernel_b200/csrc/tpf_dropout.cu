@@ -252,6 +252,7 @@ int dropout(const DropoutCall& c, cudaStream_t stream) {
   for (int d = 0; d < 3; ++d)
     vec = vec && whole(c.sizes[d], c.x_strides[d]) && whole(c.sizes[d], c.out_strides[d]) &&
           (c.residual == nullptr || whole(c.sizes[d], c.residual_strides[d]));
+  TPF_REQUIRE(!(vec && p.s_in_mask) || S <= 65535, TPF_ERR_UNSUPPORTED, "dropout: the third dimension is too long without a shared mask");
   int64_t cells;
   if (vec) {
     const int64_t per_row = (I + 7) / 8;
