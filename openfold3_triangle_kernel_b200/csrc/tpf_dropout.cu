@@ -253,16 +253,14 @@ int dropout(const DropoutCall& c, cudaStream_t stream) {
     vec = vec && whole(c.sizes[d], c.x_strides[d]) && whole(c.sizes[d], c.out_strides[d]) &&
           (c.residual == nullptr || whole(c.sizes[d], c.residual_strides[d]));
   TPF_REQUIRE(!(vec && p.s_in_mask) || S <= 65535, TPF_ERR_UNSUPPORTED, "dropout: the third dimension is too long without a shared mask");
-  int64_t cells;
+  int64_t cells = P * Q * ((I + 7) / 8);
+  vec = vec && cells < kMost - kThreads;  // (more of them have indices beyond 32 bits, which the kernel of any rows has)
   if (vec) {
-    const int64_t per_row = (I + 7) / 8;
-    cells = P * Q * per_row;
-    TPF_REQUIRE(cells < kMost - kThreads, TPF_ERR_UNSUPPORTED, "dropout: too many elements");
-    p.cells = (uint32_t)per_row;
-    p.div_cells = FastDiv::make((uint32_t)per_row);
+    p.cells = (uint32_t)((I + 7) / 8);
+    p.div_cells = FastDiv::make(p.cells);
   } else {
     cells = (P * Q * (p.s_in_mask ? S : 1) * I + 255) / 256;
-    TPF_REQUIRE(cells < 8 * (kMost - 1), TPF_ERR_UNSUPPORTED, "dropout: too many elements");
+    TPF_REQUIRE(cells < (1ll << 36) / 256, TPF_ERR_UNSUPPORTED, "dropout: too many elements");  // (two such tensors fit no device)
     p.div_inner = FastDiv::make((uint32_t)(I < 32 ? I : 32));
   }
   p.div_q = FastDiv::make((uint32_t)Q);

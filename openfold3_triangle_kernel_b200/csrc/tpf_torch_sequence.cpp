@@ -76,6 +76,8 @@ bool dropout_layout(const Tensor& x, const Tensor& residual, int64_t shared, tpf
     rest[0] = rest[1];
     rest[1] = rest[2];
   }
+  constexpr int64_t kMostRows = 1ll << 31;
+  if (rest[1].size >= kMostRows || rest[0].size >= kMostRows || rest[1].size * rest[0].size >= kMostRows) return false;
   const Dim order[3] = {rest[1], rest[0], s};  // p, q, s
   for (int i = 0; i < 3; ++i) {
     c.sizes[i] = order[i].size;
@@ -404,7 +406,11 @@ py::object py_dropout(py::handle hx, py::handle hr, py::handle hs, int64_t seed,
   if (!unpack_optional(hr, x, r) || !unpack_optional(hs, x, s)) return py::none();
   if (r.defined() && (r.scalar_type() != x.scalar_type() || r.sizes() != x.sizes())) return py::none();
   if (s.defined() && (s.scalar_type() != at::kLong || s.dim() != 1 || s.size(0) != 2 || !s.is_contiguous())) return py::none();
-  if (shared >= 0 && shared >= x.dim() - 1) return py::none();
+  if (x.numel() >= 1ll << 36) return py::none();
+  if (shared >= 0) {
+    constexpr int64_t kMost = 1ll << 31;
+    if (shared >= x.dim() - 1 || x.size(shared) >= kMost || c10::multiply_integers(x.sizes().slice(0, shared)) >= kMost) return py::none();
+  }
   const DropoutArgs a{s, seed, offset, threshold, shared};
   Tensor out;
   {

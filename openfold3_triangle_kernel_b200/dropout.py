@@ -3,14 +3,15 @@
 Operator contract:
 
 * ``x``: bf16, fp16 or fp32 ``[*]``.  Dimensions that lie at few strides (slices, transposed pair tensors) are read in place, other
-  layouts through a contiguous copy.  The result does not depend on strides.
+  layouts through a contiguous copy.  The result does not depend on strides.  Fewer than 2^36 elements.
 * ``p``: probability of an element to be dropped, held as ``round(65536 p) / 65536``.  ``out = residual + (kept ? x / (1 - p) : 0)``, one
   rounding; a dropped infinity or NaN is a zero.
 * ``seed``: an ``int``, a pair ``(seed, offset)`` of them, an int64 tensor ``[2]`` on x's device that holds the pair (a captured
   graph reads it at every replay; do not change it between a forward and its backward), or ``None``: drawn from torch's
   generator of the device.  The same seed gives the same mask.  Take another seed, or another offset, for every call.
 * ``shared_dim``: a dimension, not the last one, along which all elements share one mask (the row-wise dropout of a pair
-  tensor ``[*, N, N, C]`` has -3); ``None``: every element has its own.
+  tensor ``[*, N, N, C]`` has -3); ``None``: every element has its own.  It has fewer than 2^31 elements, and so have the dimensions
+  before it together.
 * ``residual``: added, of x's shape and type.  ``training=False``: nothing is dropped.
 * returns x's type and shape, contiguous; autograd for x and the residual, first order, reverse mode only.  Between the passes
   nothing is kept but the seed.
@@ -25,6 +26,7 @@ sizes that are free there, when it runs.  The reference's counterpart is the dro
 """
 from __future__ import annotations
 
+import math
 from typing import Optional
 
 import torch
@@ -35,6 +37,8 @@ from .layer_norm import ROW_DTYPES
 from .trimul import SupportResult
 
 _STEPS = 65536
+_MOST_ELEMENTS = 2 ** 36
+_MOST = 2 ** 31     # of a shared dimension, and of those before it
 
 
 def _is_int(n):
@@ -59,6 +63,8 @@ def check_dropout_support(x, p, seed=None, shared_dim=None, residual=None, *, ch
         return SupportResult(False, "x_shape", "x must have a dimension")
     if x.dtype not in ROW_DTYPES:
         return SupportResult(False, "x_dtype", "x must be BF16, FP16 or FP32")
+    if certain(x.numel() >= _MOST_ELEMENTS):
+        return SupportResult(False, "x_shape", "x must have fewer than 2^36 elements")
     if not (isinstance(p, (int, float)) and 0 <= p <= 1):
         return SupportResult(False, "p", "p must be a number in 0 .. 1")
     if isinstance(seed, torch.Tensor):
@@ -71,6 +77,10 @@ def check_dropout_support(x, p, seed=None, shared_dim=None, residual=None, *, ch
     if shared_dim is not None and not (_is_int(shared_dim) and -x.ndim <= shared_dim < x.ndim
                                        and shared_dim % x.ndim != x.ndim - 1):
         return SupportResult(False, "shared_dim", "shared_dim must be a dimension of x but the last one")
+    if shared_dim is not None:
+        shared = shared_dim % x.ndim
+        if certain(x.shape[shared] >= _MOST) or certain(math.prod(x.shape[:shared]) >= _MOST):
+            return SupportResult(False, "shared_dim", "a shared dimension, and those before it together, must be below 2^31")
     if residual is not None:
         if not isinstance(residual, torch.Tensor) or differs(residual.shape, tuple(x.shape)):
             return SupportResult(False, "residual_shape", "residual must have x's shape")

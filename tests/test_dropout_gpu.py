@@ -311,3 +311,14 @@ def test_a_long_shared_dimension(shape, shared):
     """One mask for all tokens: more runs than a dimension of a grid takes."""
     x = _rn(*shape, seed=3).bfloat16()
     _check(x, shared=shared, residual=_rn(*shape, seed=4).bfloat16())
+
+
+@pytest.mark.parametrize("cols", [2 ** 34 + 4096, 2 ** 34 + 4099])
+def test_groups_beyond_32_bits(cols):
+    """Elements of a tensor that has more than 2^31 groups of eight, from its middle and from its end."""
+    out = tk.turbo_dropout(torch.ones(cols, device="cuda", dtype=torch.bfloat16), 0.5, 21)
+    for first in (cols // 16 * 8, (cols - 4096) // 8 * 8):
+        bits = [h >= 32768 for g in range(first // 8, first // 8 + 512) for w in so.philox(21, 0, g) for h in (w & 0xFFFF, w >> 16)]
+        assert torch.equal(out[first:first + 4096].cpu() != 0, torch.tensor(bits))
+    del out
+    torch.cuda.empty_cache()

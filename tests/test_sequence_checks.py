@@ -382,3 +382,14 @@ def test_a_sharded_block_with_dropout_wants_a_seed():
         pair_stack_block(E(1, 4, 4, 32, dt=BF), E(1, 4, 4), {}, 2, group=object(), dropout=0.1)
     assert _site_seeds(7) == [(7, i) for i in range(4)] and _site_seeds((7, 3)) == [(7, 12 + i) for i in range(4)] and _site_seeds(None) == [None] * 4
     assert [t.tolist() for t in _site_seeds(torch.tensor([7, 3]))] == [[7, 12 + i] for i in range(4)]
+
+
+def test_dropout_sizes():
+    """What no launch takes is refused by the check.  (Expanded tensors of any size need no memory.)"""
+    big = lambda *s: E(1, dt=BF).expand(*s)  # noqa: E731
+    code = lambda x, **kw: tk.check_dropout_support(x, 0.5, 1, **kw, check_device=False).code  # noqa: E731
+    assert code(big(2 ** 36 - 1)) == code(big(2 ** 31, 16)) == code(big(2 ** 31 - 1, 4), shared_dim=0) == "ok"
+    assert code(big(2 ** 31 - 1, 4, 2), shared_dim=1) == code(big(200000, 64), shared_dim=0) == "ok"
+    assert code(big(2 ** 36)) == code(big(2 ** 18, 2 ** 18)) == "x_shape"
+    assert code(big(2 ** 31, 4), shared_dim=0) == code(big(2 ** 31, 2, 2), shared_dim=1) == "shared_dim"
+    assert code(big(2 ** 16, 2 ** 15, 1, 2), shared_dim=-2) == "shared_dim"
