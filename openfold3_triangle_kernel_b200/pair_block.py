@@ -23,9 +23,10 @@ import torch.nn.functional as F
 
 from . import _cabi as C
 from . import dap
+from ._checks import refuse
 from .attention import count_invocations, turbo_attention
-from .dropout import turbo_dropout
-from .trimul import native_weight_order, turbo_trimul
+from .dropout import _seed_numbers, turbo_dropout
+from .trimul import SupportResult, native_weight_order, turbo_trimul
 
 _attention_order = operator.itemgetter("ln_w", "ln_b", "w_z", "w_q", "w_k", "w_v", "w_g", "w_o")
 
@@ -92,13 +93,16 @@ def triangle_attention_update(z, mask, p, heads, transpose_bias=False, inf=1e9, 
 
 
 def _site_seeds(seed):
-    """Seeds of the block's four dropouts from the caller's one: the offsets 4 n .. 4 n + 3 of its offset n."""
+    """Seeds of the block's four dropouts from the caller's one: the offsets 4 n .. 4 n + 3 of its offset n, modulo 2^64."""
     if seed is None:
         return [None] * 4
-    if isinstance(seed, torch.Tensor):
+    if isinstance(seed, torch.Tensor) and seed.dtype == torch.int64 and seed.shape == (2,):
         return list(torch.stack([seed[:1].expand(4), 4 * seed[1:] + torch.arange(4, device=seed.device)], 1))
-    number, offset = seed if isinstance(seed, (tuple, list)) else (seed, 0)
-    return [(number, 4 * offset + i) for i in range(4)]
+    pair = None if isinstance(seed, torch.Tensor) else _seed_numbers(seed)
+    if pair is None:
+        refuse("pair_stack_block", SupportResult(False, "seed", "seed must be a 64-bit int, a pair of them, an INT64 tensor [2], or None"))
+    number, offset = pair
+    return [_seed_numbers((number, (4 * offset + i) % 2 ** 64)) for i in range(4)]
 
 
 def pair_stack_block(z, mask, params, heads, group=None, trimul_backend=None, attention_fn=None, dropout=0.0, seed=None,

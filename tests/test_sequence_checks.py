@@ -393,3 +393,21 @@ def test_dropout_sizes():
     assert code(big(2 ** 36)) == code(big(2 ** 18, 2 ** 18)) == "x_shape"
     assert code(big(2 ** 31, 4), shared_dim=0) == code(big(2 ** 31, 2, 2), shared_dim=1) == "shared_dim"
     assert code(big(2 ** 16, 2 ** 15, 1, 2), shared_dim=-2) == "shared_dim"
+
+
+@pytest.mark.parametrize("offset", [0, 3, -1, 2 ** 61, 2 ** 62, -2 ** 61 - 1, 2 ** 63 - 1, -2 ** 63, 2 ** 64 - 1])
+def test_site_seeds_of_any_offset(offset):
+    """Numbers and the tensor that holds them give the same seeds: four in a row, modulo 2^64."""
+    from openfold3_triangle_kernel_b200.pair_block import _site_seeds
+    signed = lambda n: (n + 2 ** 63) % 2 ** 64 - 2 ** 63  # noqa: E731
+    expected = [(7, signed(4 * offset + i)) for i in range(4)]
+    assert _site_seeds((7, offset)) == expected
+    assert [tuple(t.tolist()) for t in _site_seeds(torch.tensor([7, signed(offset)]))] == expected
+    assert all(tk.check_dropout_support(E(4), 0.5, s, check_device=False).supported for s in expected)
+
+
+@pytest.mark.parametrize("seed", [(1, 2, 3), "seed", 1.5, (1, 2 ** 64), (1, None), E(2), E(3, dt=I64), E(2, dt=I32), True])
+def test_a_block_refuses_a_bad_seed(seed):
+    from openfold3_triangle_kernel_b200.pair_block import pair_stack_block
+    with pytest.raises(ValueError, match=r"pair_stack_block unsupported \[seed\]"):
+        pair_stack_block(E(1, 4, 4, 32, dt=BF), E(1, 4, 4), {}, 2, dropout=0.1, seed=seed)
