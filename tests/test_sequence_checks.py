@@ -411,3 +411,11 @@ def test_a_block_refuses_a_bad_seed(seed):
     from openfold3_triangle_kernel_b200.pair_block import pair_stack_block
     with pytest.raises(ValueError, match=r"pair_stack_block unsupported \[seed\]"):
         pair_stack_block(E(1, 4, 4, 32, dt=BF), E(1, 4, 4), {}, 2, dropout=0.1, seed=seed)
+
+
+def test_public_names():
+    """What the documents call is there; blocks of a stack that share a seed and count their offsets share no mask."""
+    from openfold3_triangle_kernel_b200 import pair_block
+    assert all(hasattr(tk, name) for name in tk.__all__) and tk.pair_stack_block is pair_block.pair_stack_block
+    assert "pair_stack_block" in tk.__all__
+    assert len({s for n in range(48) for s in pair_block._site_seeds((5, n))}) == 4 * 48
