@@ -5,8 +5,8 @@
 //   backward: g = the inverse rotation of dz (times m);  t = g w;  dx = r (t - x r^2 sum(t x) / D);  dw = sum of g x r
 //
 // Angles: f_i comes as turns a position in 64-bit fixed point, the product with the position modulo 2^64 is the phase modulo a
-// turn, exactly, and its upper 32 bits go to sincospi.  So a position of a million is as exact as position one, without a
-// table in memory and without arithmetic in 64-bit floats.
+// turn, exactly, and its upper 32 bits, rounded to fp32 (by 2^-26 of a turn at most), go to sincospi.  So a position of a million is as
+// exact as position one, without a table in memory and without arithmetic in 64-bit floats.
 //
 // Mapping: a block has a stretch of tokens, as long as any other block's.  It makes their sines and cosines, in shared memory, and goes
 // through the heads of q and then through those of k: a team of TL lanes has a few of them in succession, loaded two ahead.  With the

@@ -10,8 +10,11 @@ Operator contract:
 * ``layout``: ``"half"`` rotates element i with i + R / 2, ``"interleaved"`` 2 i with 2 i + 1.
 * the norm: ``x / sqrt(mean(x^2) + eps) * weight``, ``weight`` ``[D]`` of any of the three types or ``None`` (ones).
 * returns x's type, contiguous; autograd for x, q, k and the weights (a gradient has its parameter's type), first order,
-  reverse mode only.  The norm keeps q and k for the backward pass, the rotation alone nothing.  All arithmetic is fp32, angles
-  are exact to 2^-32 of a turn at any position, sums have a fixed order: the same inputs give the same bits.
+  reverse mode only.  The norm keeps q and k for the backward pass, the rotation alone nothing.  All arithmetic is fp32, sums have a
+  fixed order: the same inputs give the same bits.
+* angles: position times ``turns`` is exact modulo a turn, at any position; what goes to the sine and cosine is that number rounded to
+  fp32, off by 2^-26 of a turn at most.  The ``turns`` that :func:`rotary_frequencies` makes are off by what it computes in 64-bit
+  floats, about 2^-51 of themselves, which a position multiplies (below 2^-26 of a turn up to position 2^26).
 
 Unsupported inputs raise ``ValueError("turbo_rotary unsupported [code]: reason")`` (``turbo_qk_norm_rotary`` likewise), in a traced
 call when it is traced or, for sizes that are free there, when it runs.  The reference has no counterpart.

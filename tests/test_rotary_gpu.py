@@ -315,3 +315,22 @@ def test_saved_tensors_of_other_layouts(norm):
         with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), hook):
             outs = call()
         assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(outs, [q, k], d), want))
+
+
+@pytest.mark.parametrize("dim", [2, 64])
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_angles_of_any_position(dim, layout):
+    """Sines and cosines of the exact phase, by whole numbers: an angle off by 2^-26 of a turn for its rounding to fp32 and 2^-32 for the
+    bits that are cut off, and 2^-23 for sincospi (two steps of a number below one)."""
+    import random
+    rng = random.Random(5)
+    rates = [rng.randrange(-2 ** 63, 2 ** 63) for _ in range(dim // 2 - 1)] + [2 ** 32 + 1]
+    at = [0, 1, -1, 2 ** 62, -2 ** 62, 2 ** 63 - 1, -2 ** 63] + [rng.randrange(-2 ** 63, 2 ** 63) for _ in range(300)]
+    fr = tk.RotaryFrequencies(torch.tensor(rates, device="cuda"))
+    x = torch.zeros(1, len(at), 1, dim, device="cuda")
+    first, second = so.pairs(dim, layout == "half")
+    x[..., first] = 1.0
+    out = tk.turbo_rotary(x, fr, torch.tensor([at], device="cuda"), layout=layout)[0, :, 0].double().cpu()
+    t = torch.tensor([[(r * p % 2 ** 64) / 2 ** 64 for r in rates] for p in at], dtype=torch.float64) * 2 * math.pi
+    room = 2 * math.pi * (2.0 ** -26 + 2.0 ** -32) + 2.0 ** -23
+    assert (out[:, first] - t.cos()).abs().max() <= room and (out[:, second] - t.sin()).abs().max() <= room
