@@ -422,3 +422,37 @@ def test_saved_offsets_and_lengths_of_other_layouts():
         with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), hook):
             out = call()
         assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, [q, k, v], d), want))
+
+
+# Rounding to the nearest is off by up to half a step of a number's power of two, 1 / sqrt(3) of that in the mean square; over numbers of a
+# normal distribution, whose mean square is 1.9 times that of their powers of two, 0.42 half steps of their norm.  Two such roundings,
+# independent of one another, 0.42 sqrt(2).  A tenth on top for the spread (of some 70000 numbers: below a hundredth) and for what is in fp32.
+ONE_ROUNDING = 1.1 * 0.42
+TWO_ROUNDINGS = 1.1 * 0.42 * math.sqrt(2)
+
+
+@pytest.mark.parametrize("B, n, D, window, sinks, bound", [
+    (8, 300, 128, (1, 0), 0, TWO_ROUNDINGS), (8, 300, 64, (3, 3), 1, TWO_ROUNDINGS), (8, 300, 64, (8, 0), 0, TWO_ROUNDINGS),
+    (16, 129, 64, (1, 0), 0, TWO_ROUNDINGS), (16, 128, 64, (1, 0), 0, ONE_ROUNDING), (200, 4, 80, (800, 0), 0, ONE_ROUNDING),
+    (300, 2, 32, (5, 0), 0, ONE_ROUNDING)])
+@pytest.mark.parametrize("dtype", [BF, FP16])
+def test_roundings_of_gradients(B, n, D, window, sinks, bound, dtype):
+    """dS and P are rounded once as operands (up to 128 tokens and keys in two parts: not at all, at this scale), and the results once.
+    The roundings of the stored output in delta would make 0.72 to 1.15 half steps of these."""
+    q, k, v = (t.requires_grad_(True) for t in _inputs(B, n, n, 4, 2, D, dtype))
+    d = _rn(B, n, 4, D, seed=8, dtype=dtype)
+    ref = so.window_attention(q.detach(), k.detach(), v.detach(), window, sinks, d_out=d)
+    grads = torch.autograd.grad(tk.turbo_window_attention(q, k, v, window=window, sinks=sinks), [q, k, v], d)
+    for name, g in zip(("dq", "dk", "dv"), grads):
+        assert (g.double() - ref[name]).norm() <= bound * so.half_step(dtype) * ref[name].norm(), name
+
+
+@pytest.mark.parametrize("B, n, M, bound", [(200, 1, 9, ONE_ROUNDING), (200, 1, 200, ONE_ROUNDING), (60, 3, 400, ONE_ROUNDING),
+                                            (8, 300, 300, TWO_ROUNDINGS)])
+@pytest.mark.parametrize("dtype", [BF, FP16])
+def test_roundings_of_the_output(B, n, M, bound, dtype):
+    """Few queries take P in two parts, many in one."""
+    q, k, v = _inputs(B, n, M, 4, 2, 64, dtype)
+    ref = so.window_attention(q, k, v, (None, 0), 0, [M - n] * B)
+    out = tk.turbo_window_attention(q, k, v, window=(None, 0), query_offset=M - n)
+    assert (out.double() - ref["out"]).norm() <= bound * so.half_step(dtype) * ref["out"].norm()
