@@ -446,6 +446,7 @@ py::object py_rotary(py::handle hq, py::handle hk, py::handle hqw, py::handle hk
     return py::none();
   constexpr int64_t kMostRows = (1ll << 31) - 256;
   if (q.numel() / D > kMostRows || (k.defined() && k.numel() / D > kMostRows)) return py::none();
+  if (q.size(-2) + (k.defined() ? k.size(-2) : 0) >= 1 << 24) return py::none();
   const RotaryArgs a{turns, pos, first, magnitude, half, norm, eps};
   auto wants = [](const Tensor& t) { return t.defined() && t.requires_grad(); };
   variable_list out;

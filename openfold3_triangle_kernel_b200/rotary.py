@@ -33,6 +33,7 @@ from .trimul import SupportResult
 
 MAX_HEAD_DIM = 256
 _MOST_ROWS = 2 ** 31 - 256   # tokens of all batches times heads
+_MOST_HEADS = 2 ** 24 - 1    # of q and k together
 LAYOUTS = ("half", "interleaved")
 SCALINGS = (None, "linear", "ntk", "yarn")
 
@@ -105,7 +106,7 @@ def _check(named, weights, turns, magnitude, positions, layout, eps, check_devic
             return SupportResult(False, "x_dtype", f"{name} must have {first_name}'s type and device")
         if t.ndim != x.ndim or differs(t.shape[:-2] + t.shape[-1:], x.shape[:-2] + x.shape[-1:]):
             return SupportResult(False, "x_shape", f"{name} must have {first_name}'s sizes but for the heads")
-    if any(certain(math.prod(t.shape[:-1]) > _MOST_ROWS) for _, t in named):
+    if any(certain(math.prod(t.shape[:-1]) > _MOST_ROWS) for _, t in named) or certain(sum(t.shape[-2] for _, t in named) > _MOST_HEADS):
         return SupportResult(False, "tokens", "too many tokens and heads")
     for name, w in weights:
         bad = check_parameter(name, w, x.shape[-1], x)

@@ -419,3 +419,12 @@ def test_public_names():
     assert all(hasattr(tk, name) for name in tk.__all__) and tk.pair_stack_block is pair_block.pair_stack_block
     assert "pair_stack_block" in tk.__all__
     assert len({s for n in range(48) for s in pair_block._site_seeds((5, n))}) == 4 * 48
+
+
+def test_rotary_sizes():
+    """What no launch takes is refused by the check.  (Expanded tensors of any size need no memory.)"""
+    big = lambda *s: E(1, dt=BF).expand(*s)  # noqa: E731
+    one = lambda *s: tk.check_rotary_support(big(*s), _fr(2), check_device=False).code  # noqa: E731
+    both = lambda n, h, hk: tk.check_qk_norm_rotary_support(big(n, h, 2), big(n, hk, 2), None, None, _fr(2), check_device=False).code  # noqa: E731
+    assert one(2 ** 24, 127, 2) == one(1, 2 ** 24 - 1, 2) == both(1, 2 ** 24 - 2, 1) == both(100, 8, 2) == "ok"
+    assert one(2 ** 24, 128, 2) == one(1, 2 ** 24, 2) == both(1, 2 ** 23, 2 ** 23) == "tokens"
