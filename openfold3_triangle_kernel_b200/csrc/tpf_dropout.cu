@@ -9,10 +9,14 @@
 // depend neither on strides nor on the launch, and eight elements share one evaluation (a 32-bit word each would double its
 // cost; 16 bits resolve p to 2^-16, and the scale uses the probability that is really used).
 //
-// What bounds it: memory.  Ten rounds are twenty 32 x 32 -> 64 bit products, about 90 instructions for eight elements; a
-// shared mask is made once by a thread that then walks along the shared dimension.
+// What bounds it: memory where the mask is shared: it is made once by a thread that then walks along the shared dimension.  Instructions
+// where every element has its own: 225 of them for eight elements without a residual (ten rounds are twenty 32 x 32 -> 64 bit
+// products, with their keys about 90), and 72 % of all issue slots are taken, with the ALU and the multiplier at 57 and 58 %.
 // Measured (B200, bf16, 1 x 384 x 384 x 128, with a residual and without): 17.0 and 10.9 us with a mask shared along the rows (6.7 and
-// 6.9 TB/s, the rate of a copy), 23.1 and 21.1 us with bits for every element.
+// 6.9 TB/s, the rate of a copy), 23.1 and 21.1 us with bits for every element.  Rows at any address are slower, most of all with a shared
+// mask, where a thread has two-byte loads of up to four rows (257 x 257 x 97 with a residual: 9.9 us for every element, 19.7 shared, 5.9 at
+// the rate of a copy), and so are short mask rows over a long shared dimension, where a run has a block to itself (200000 x 64:
+// 51 us for 11.7; 300001 x 33: 1390 for 9.1).
 #include "tpf_dropout.h"
 
 #include "tpf_rows.cuh"
@@ -94,8 +98,7 @@ __device__ __forceinline__ void drop_vec(const Piece<T, 8>& x, const Piece<T, 8>
 }
 
 // Rows that start on vector boundaries and on groups of the mask: a thread per vector of the mask and run of the shared dimension.
-// (Without a shared dimension the products and the selections bound it, 21 us for 11.5 at the copy rate; four vectors a thread, with
-// their keys made once, took as long, and with a residual 28 for 23.)
+// (Without a shared dimension: four vectors a thread, with their keys made once, took as long, 21 us, and with a residual 28 for 23.)
 template <typename T, bool RES, int RUN>
 __global__ void __launch_bounds__(kThreads) dropout_vec_kernel(const DropoutParams p) {
   griddep_wait();

@@ -61,7 +61,9 @@ int window_attn_fwd(const WindowCall& c, cudaStream_t stream) {
   // A CTA of the one kernel has 16 rows, queries times heads of a group, of the other 128 queries of a head.  The first is quicker while
   // its CTAs find an SM each, and beyond that where there are fewer of them by a quarter.  (Heads 32 on 8 of 128 elements, window 1024,
   // us, few / many: 8 sequences of 8 queries 17 / 20, of 16 26 / 20, of 64 95 / 20; one sequence of 32 12 / 16, of 128 26 / 18; 64
-  // single queries 53 / more than 150.)
+  // single queries 55 / 116.  As many key heads as heads, where both have as many CTAs: 32 of 128, single queries of 4 sequences 18.5 /
+  // 19.5, of 16 56 / 49, of 64 191 / 175; 16 of 64: of 16 20.6 / 20.8, of 64 61 / 64, 2 to 8 queries of 64 61 / 69, the rule's worst; 8 of
+  // 64: of 64 39 / 34.  Heads 64 on 8: 16 sequences of 8 queries 53 / 71, of 16 102 / 71; 32 on 1: of 8 28 / 39, of 16 52 / 38.)
   const int64_t few = c.B * c.HK * ((c.N * p.G + 15) / 16), many = c.B * c.H * ((c.N + 127) / 128);
   if (c.M > 0 && few > sm_count() && 4 * few > 3 * many) return window_many(c, p, stream);
   return window_few(c, p, stream);

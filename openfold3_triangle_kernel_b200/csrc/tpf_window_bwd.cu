@@ -42,6 +42,9 @@ constexpr int kTile = 64;  // columns of a tile
 // delta from the stored output has the roundings of that and of the probabilities in it.  Beside a dS of many keys they do not show; where a
 // query sees fewer than this, delta is made as the sum of P dP in fp32, tile by tile.  (Error of dQ and dK relative to their
 // norms, bf16, roundings of dS and of the results alone 0.0023: with two keys 0.0043, nine 0.0028, 31 0.0025, 128 0.0024.)
+// It costs a third S and dP of the items that have such a query (backward, us, without it and with it: 8192 tokens, 32 heads on 8 of 128,
+// windows of 64, 100 and 127 keys 155 and 199, 183 and 232, 180 and 229, of 128, where only the first queries see fewer, 176 and 187; of 64
+// elements a head, 64 keys 91 and 123; causal, 256 of 128 tokens 257 and 323).
 constexpr int kFewKeys = 128;
 
 // ---- stats ------------------------------------------------------------------------------------------------
@@ -688,9 +691,11 @@ int run(const WindowCall& c, const WindowParams& p, uint8_t* ws, cudaStream_t st
   TPF_LAUNCH_OK();
   const int64_t os[3] = {c.N * c.H * c.D, c.H * c.D, c.D};
   int rc;
-  // Short sequences take P and dS in two parts, which together have 16 bits of mantissa (22 in fp16): a gradient that is the sum of a few
-  // products shows the rounding of each.  (Three of 4 tokens: error of dK relative to its norm 0.0026, now 0.0017, 16.9 us, now 18.5; 256 of
-  // 128 tokens, 16 heads of 128: 303 us, now 324.)  In longer ones the errors are those of the mean, sqrt(2) of the result's rounding.
+  // Short sequences take P and dS in two parts, which together have 16 bits of mantissa (22 in fp16), so that the result's own rounding is
+  // what is left of the error: 0.42 half steps of the gradient's norm for 0.60 with one part, at any length.  What differs is the
+  // price, since longer sequences wait for the tensor pipe (backward, us, one part and two: 16.9 and 18.5 for three of 4
+  // tokens, 303 and 322 for 256 of 128, 16 heads on 4 of 128, 71 and 82 for 64 of 128, 16 heads of 64; beyond: 327 and 359 for 128 of
+  // 256, 63 and 75 for two of 2053, 128 on both sides, 480 and 597 for 8192, 32 heads on 8, window 1024).
   const bool twice = c.N <= 128 && c.M <= 128;
   // (without a bound on either side, and with enough keys, every query sees enough of them)
   if (c.lengths != nullptr || c.left != kWindowUnlimited || c.right != kWindowUnlimited || c.M < kFewKeys) {

@@ -12,8 +12,9 @@ Operator contract:
 * ``shared_dim``: a dimension, not the last one, along which all elements share one mask (the row-wise dropout of a pair
   tensor ``[*, N, N, C]`` has -3); ``None``: every element has its own.  It has fewer than 2^31 elements, and so have the dimensions
   before it together.
-* ``residual``: added, of x's shape and type.  ``training=False``: nothing is dropped.
-* returns x's type and shape, contiguous; autograd for x and the residual, first order, reverse mode only.  Between the passes
+* ``residual``: added, of x's shape and type.  ``training=False``: nothing is dropped, and the result is ``x``
+  itself or ``residual + x``.
+* returns x's type and shape, contiguous in training; autograd for x and the residual, first order, reverse mode only.  Between the passes
   nothing is kept but the seed.
 
 The random bits: element m of the mask (row-major in x's shape with 1 in the place of the shared dimension) is dropped where half word

@@ -17,8 +17,9 @@ Operator contract:
   fp32.  The same inputs give the same bits.
 
 A single token over its cache is ``N = 1`` with ``query_offset = key_lengths - 1``.  Probabilities and their gradients are rounded
-to q's type as operands of the products (short calls take them in two parts); sums and the softmax are fp32, and a probability below
-2^-126 is zero.  A key or value inside the sequence that is infinite or NaN reaches every query whose 128 neighbours see it, as a
+to q's type as operands of the products, in fp16 within its range as well (a loss scale keeps them there).  Calls of few queries, and
+gradients of at most 128 queries and 128 keys, take them in two parts: their results are off by 0.42 half steps of their norm, others
+by 0.60.  Sums and the softmax are fp32, and a probability below 2^-126 is zero.  The log-sum-exp has no gradient.  A key or value inside the sequence that is infinite or NaN reaches every query whose 128 neighbours see it, as a
 product of zero with it does elsewhere.
 
 Unsupported inputs raise ``ValueError("turbo_window_attention unsupported [code]: reason")``, in a traced call when it is traced or,
