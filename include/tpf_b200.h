@@ -297,6 +297,7 @@ int tpf_norm_linear_bwd(const void* d_out, const void* x, int64_t x_pitch, const
  * are not below `threshold` (0 .. 65536): half word m & 7 (the low half of a word first) of Philox 4x32-10 with key = seed and
  * counter = (m >> 3, offset).  The backward pass is the same call with x = the output's gradient and no residual.
  *   sizes    elements (p, q, s, e); e is contiguous in all tensors, the strides (in elements) are those of p, q and s
+ *            (p, q, s and p q below 2^31, s up to 65535 without a shared mask, the mask below 2^36 elements)
  *   shared   1: the mask is shared along s, m = (p Q + q) E + e; 0: m = ((p Q + q) S + s) E + e
  *   residual NULL: none
  *   seed_offset  (seed, offset) in device memory, or NULL: the two numbers that follow */
